@@ -6,7 +6,7 @@ The library is the only compute path of this package: if it is missing or fails 
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libflashsvd_hip.so"
@@ -115,6 +115,13 @@ WBITS_FP16 = -16
 WBITS_Q4_FP16 = -4
 
 # name -> (restype, argtypes); mirrors include/flashsvd_hip.h declaration by declaration
+class Kv8Cache(ctypes.Structure):
+    """fsvd_kv8_cache: codes and scales of a KV cache in 8 bits."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("sc_b", c_int64), ("sc_s", c_int64), ("sc_h", c_int64),
+                ("ss_b", c_int64), ("ss_n", c_int64), ("ss_h", c_int64), ("S", ctypes.c_int32), ("Hk", ctypes.c_int32), ("Dh", ctypes.c_int32),
+                ("block", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "fsvd_version": (c_int, []),
     "fsvd_last_error": (c_char_p, []),
@@ -180,6 +187,15 @@ SIGNATURES = {
     "fsvd_decode_step_validate": (c_int, [c_void_p, c_int, c_int]),
     "fsvd_decode_step_set_state": (c_int, [c_void_p, c_int64, ctypes.c_int32, c_void_p]),
     "fsvd_greedy_token": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "fsvd_sample_token": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_double, c_void_p, c_int, c_void_p, c_double, c_void_p,
+                                  c_double, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "fsvd_kv8_append": (c_int, [ctypes.POINTER(Kv8Cache)] + [c_void_p, c_int64, c_int64, c_int64] * 2 + [c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                c_int, c_int, c_int, c_void_p]),
+    "fsvd_attn_decode_kv8_scratch_bytes": (c_size_t, [c_int] * 6),
+    "fsvd_attn_decode_kv8": (c_int, [ctypes.POINTER(Kv8Cache)] + [c_void_p, c_int64, c_int64] * 3 + [c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                     c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "fsvd_attn_prefill_kv8": (c_int, [ctypes.POINTER(Kv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "fsvd_set_token_rows": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int32, c_int, c_void_p]),
     "fsvd_mlp_block_scratch_bytes": (c_size_t, [ctypes.POINTER(MlpBlock)]),
     "fsvd_attn_block_scratch_bytes": (c_size_t, [ctypes.POINTER(AttnBlock)]),

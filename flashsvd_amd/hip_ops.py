@@ -3,6 +3,7 @@ the current torch stream handed to libflashsvd_hip.  PyTorch only provides devic
 streams here; every arithmetic step runs in the HIP library."""
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 from typing import Optional
@@ -43,6 +44,14 @@ def _elem(t: torch.Tensor, name: str):
     if code is None:
         raise ValueError(f"{name} must be torch.bfloat16 or torch.float16, got {t.dtype}")
     return t.dtype, code
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The context of a call whose tensors are on ``device``: nothing where that is the current one."""
+    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -514,6 +523,45 @@ def _greedy_token_impl(logits, tokens, positions):
     _lib.check("fsvd_greedy_token", rc)
 
 
+def sample_token_(logits: torch.Tensor, uniforms: torch.Tensor, tokens: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
+                  temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> None:
+    """``tokens[b]`` = a draw from the filtered logits of row b and ``positions[b] += 1`` in one launch; logits [B, V] with unit inner stride,
+    uniforms float32 [B] in [0, 1), tokens int64 [B, 1] or [B], positions int32 [B].
+
+    In descending order of the logits (equal ones by index), with weights ``w = exp((l - max) / temperature)`` and running sums C: ``top_k`` keeps
+    the first k (0: all), ``top_p`` those up to the first whose C exceeds ``top_p`` times the sum of these (1: all), ``min_p`` those with
+    ``w >= min_p``; the token is the first of what all three keep whose C exceeds ``uniforms[b]`` times the kept sum.  Each of the four is a number or a
+    contiguous tensor [B] (float32, ``top_k`` int32).  ``temperature <= 0`` and rows whose largest logit is not finite give the greedy
+    token.  Custom operator flashsvd_hip::sample_token_ (tokens and positions are mutated arguments)."""
+    number = lambda v, other: (other, v) if isinstance(v, torch.Tensor) else (v, None)      # noqa: E731
+    (t, ts), (k, ks), (p, ps), (m, ms) = number(temperature, 1.0), number(top_k, 0), number(top_p, 1.0), number(min_p, 0.0)
+    _OPS.sample_token_.default(logits, uniforms, tokens, positions, float(t), int(k), float(p), float(m), ts, ks, ps, ms)
+
+
+def _sample_token_impl(logits, uniforms, tokens, positions, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps):
+    _, code = _elem(logits, "logits")
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError(f"logits must be [B, V] with unit inner stride, got {tuple(logits.shape)} strides {logits.stride()}")
+    B, V = logits.shape
+    _need(tokens, "tokens", dtype=torch.long)
+    if tokens.numel() != B or tokens.shape[0] != B:
+        raise ValueError(f"tokens must hold {B} rows of one id, got {tuple(tokens.shape)}")
+    dev = logits.device
+    if tokens.device != dev:
+        raise ValueError(f"logits and tokens must be on one device, got {dev} and {tokens.device}")
+    for t, nm, dt in ((uniforms, "uniforms", torch.float32), (positions, "positions", torch.int32), (temperatures, "temperature", torch.float32),
+                      (top_ks, "top_k", torch.int32), (top_ps, "top_p", torch.float32), (min_ps, "min_p", torch.float32)):
+        if t is None:
+            continue
+        if t.dtype != dt or t.shape != (B,) or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{nm} must be a contiguous {dt} [{B}] tensor on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    with _on(dev):
+        rc = _lib.load().fsvd_sample_token(logits.data_ptr(), logits.stride(0), uniforms.data_ptr(), tokens.data_ptr(), tokens.stride(0), _ptr(positions),
+                                           temperature, _ptr(temperatures), top_k, _ptr(top_ks), top_p, _ptr(top_ps), min_p, _ptr(min_ps), B, V, code,
+                                           _stream())
+    _lib.check("fsvd_sample_token", rc)
+
+
 def set_token_rows_(tokens: torch.Tensor, src: torch.Tensor, positions: torch.Tensor, position: int) -> None:
     """``tokens.copy_(src)`` and ``positions.fill_(position)`` in one launch (contiguous int64 / int64 / int32 of the same
     number of rows on one device).  Custom operator flashsvd_hip::set_token_rows_ (tokens and positions are mutated arguments)."""
@@ -897,4 +945,162 @@ def _attn_prefill_impl(q, k, v, q_pos0, causal, pad_mask, add_mask, out, softmax
                                out.data_ptr(), out.stride(0), out.stride(1), out.stride(2), B, M, H, Hk, Dh, S, int(bool(causal)),
                                float(softmax_scale) if softmax_scale else 0.0, code, _stream())
     _lib.check("fsvd_attn_prefill", rc)
+    return out
+
+
+# ------------------------------------------------------------------ KV cache in 8 bits
+def kv8_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               positions: torch.Tensor, *, block: int, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+               rows: Optional[torch.Tensor] = None) -> None:
+    """Rows of keys and values [B, T, Hk, Dh] into a cache in 8 bits at positions[b] .. positions[b] + T - 1 (``rows`` int32 [B]: that many of
+    sequence b), keys rotated there when ``cos`` / ``sin`` [len, Dh / 2] are given.  Caches float8_e4m3fn [>=B, S, Hk, Dh], scales float32
+    [>=B, ceil(S / block), Hk], ``value = code * scale`` with one power of two for each ``block`` (16, 32, 64 or 128) tokens of a head; a block that is open
+    takes further rows, and where they need a larger scale, the rows that it holds move to it.  Rows outside the cache are dropped.
+    Custom operator flashsvd_hip::kv8_append (caches and scales are mutated arguments); see fsvd_kv8_append."""
+    _OPS.kv8_append.default(k, v, k_cache, v_cache, k_scale, v_scale, positions, int(block), cos, sin, rows)
+
+
+def attn_decode_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    cache_seqlens: torch.Tensor, *, block: int, k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
+                    cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, seqlen_add: int = 0, nsplit: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """:func:`attn_decode_densekv` over a cache in 8 bits (operands as :func:`kv8_append`): q [B, H, Dh] over cache_seqlens[b] + seqlen_add keys; with
+    ``k_new`` / ``v_new`` [B, Hk, Dh] these are appended at cache_seqlens[b] first and cache_seqlens[b] + 1 keys are seen.  ``cos`` / ``sin`` rotate q (and
+    k_new) at cache_seqlens[b].  A sequence without keys gives zeros.  Custom operator flashsvd_hip::attn_decode_kv8."""
+    a = (q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, int(block), k_new, v_new, cos, sin, int(seqlen_add),
+         None if nsplit is None else int(nsplit), None if not softmax_scale else float(softmax_scale))
+    return _OPS.attn_decode_kv8.default(*a) if out is None else _OPS.attn_decode_kv8.out(*a, out=out)
+
+
+def attn_prefill_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, q_pos0: torch.Tensor, *,
+                     block: int, rows: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """Causal attention of a chunk over a cache in 8 bits that holds the chunk's rows already: q [B, M, H, Dh], row m of sequence b at position
+    q_pos0[b] + m over the keys up to that, rotated there when ``cos`` / ``sin`` are given.  ``rows`` int32 [B]: so many rows of sequence b are
+    real; the others of ``out`` are left as they were (zeros when the call makes it).  Custom operator flashsvd_hip::attn_prefill_kv8."""
+    a = (q, k_cache, v_cache, k_scale, v_scale, q_pos0, int(block), rows, cos, sin, None if not softmax_scale else float(softmax_scale))
+    return _OPS.attn_prefill_kv8.default(*a) if out is None else _OPS.attn_prefill_kv8.out(*a, out=out)
+
+
+def _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block):
+    """Checks of a cache in 8 bits; its descriptor for the C ABI."""
+    _need(k_cache, "k_cache", dtype=torch.float8_e4m3fn); _need(v_cache, "v_cache", dtype=torch.float8_e4m3fn)
+    _need(k_scale, "k_scale", dtype=torch.float32); _need(v_scale, "v_scale", dtype=torch.float32)
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or strides != v_cache.stride() or shape[0] < B or strides[3] != 1:
+        raise ValueError(f"caches must be matching [B>={B}, S, Hk, Dh] tensors with unit inner stride, got {tuple(shape)} / {tuple(v_cache.shape)}")
+    nb, S, Hk, Dh = shape
+    if block not in (16, 32, 64, 128):
+        raise ValueError(f"block must be 16, 32, 64 or 128 tokens, got {block}")
+    want = (nb, -(-S // block), Hk)
+    if k_scale.shape != want or v_scale.shape != want or k_scale.stride() != v_scale.stride():
+        raise ValueError(f"scales must be matching {want} tensors, got {tuple(k_scale.shape)} / {tuple(v_scale.shape)}")
+    dev = k_cache.device
+    if not (dev == v_cache.device == k_scale.device == v_scale.device):
+        raise ValueError("caches and scales must be on one device")
+    return _lib.Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), strides[0], strides[1], strides[2],
+                         *k_scale.stride(), S, Hk, Dh, block)
+
+
+def _apart(B, k_cache, k_scale) -> None:
+    """Rows that a call writes must not lie in each other: no expanded caches."""
+    if (B > 1 and (k_cache.stride(0) == 0 or k_scale.stride(0) == 0)) or (k_cache.shape[2] > 1 and (k_cache.stride(2) == 0 or k_scale.stride(2) == 0)) \
+            or k_scale.stride(1) == 0 and k_scale.shape[1] > 1:
+        raise ValueError("a cache that is written to must not be expanded over its sequences, blocks or heads")
+
+
+def _kv8_vector(t, B, dev, nm):
+    if t is None:
+        return None
+    _need(t, nm, dtype=torch.int32)
+    if t.numel() != B or not t.is_contiguous() or t.device != dev:
+        raise ValueError(f"{nm} must be a contiguous int32 [{B}] tensor on {dev}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _kv8_rope(cos, sin, Dh, dt, dev):
+    if (cos is None) != (sin is None) or (cos is not None and (cos.device != dev or sin.device != dev)):
+        raise ValueError(f"cos and sin go together, on {dev}")
+    return _rope_tables(cos, sin, Dh, dt)
+
+
+def _kv8_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, block, cos, sin, rows):
+    dt, code = _elem(k, "k")
+    _need(v, "v", dtype=dt)
+    B = k.shape[0]
+    c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
+    dev = k_cache.device
+    if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != (c.Hk, c.Dh) or k.stride(3) != 1 or v.stride(3) != 1 or k.device != dev or v.device != dev:
+        raise ValueError(f"k and v must be [B, T, {c.Hk}, {c.Dh}] tensors with unit inner stride on {dev}, got {tuple(k.shape)} / {tuple(v.shape)}")
+    _apart(B, k_cache, k_scale)
+    rope_len = _kv8_rope(cos, sin, c.Dh, dt, dev)
+    pos, n = _kv8_vector(positions, B, dev, "positions"), _kv8_vector(rows, B, dev, "rows")
+    if B == 0:
+        return
+    with _on(dev):
+        rc = _lib.load().fsvd_kv8_append(c, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), pos, n,
+                                         _ptr(cos), _ptr(sin), rope_len, B, k.shape[1], code, _stream())
+    _lib.check("fsvd_kv8_append", rc)
+
+
+def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out):
+    dt, code = _elem(q, "q")
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError(f"q must be [B,H,Dh] with unit inner stride, got {tuple(q.shape)}")
+    B, H, Dh = q.shape
+    c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
+    dev = k_cache.device
+    if c.Dh != Dh or H % c.Hk or q.device != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {dev}")
+    rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    lens = _kv8_vector(cache_seqlens, B, dev, "cache_seqlens")
+    sk_b = sk_h = sv_b = sv_h = 0
+    if (k_new is None) != (v_new is None):
+        raise ValueError("k_new and v_new go together")
+    if k_new is not None:
+        _need(k_new, "k_new", dtype=dt); _need(v_new, "v_new", dtype=dt)
+        if k_new.shape != (B, c.Hk, Dh) or v_new.shape != (B, c.Hk, Dh) or k_new.stride(2) != 1 or v_new.stride(2) != 1 or k_new.device != dev \
+                or v_new.device != dev:
+            raise ValueError(f"k_new/v_new must be [B,Hk,Dh] tensors with unit inner stride on {dev}, got {tuple(k_new.shape)} / {tuple(v_new.shape)}")
+        _apart(B, k_cache, k_scale)
+        sk_b, sk_h, sv_b, sv_h = k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1)
+    if out is None:
+        out = torch.empty(B, H, Dh, device=dev, dtype=dt)
+    elif out.shape != (B, H, Dh) or out.stride(2) != 1 or out.dtype != dt or out.device != dev:
+        raise ValueError(f"out must be {dt} [B,H,Dh] with unit inner stride on {dev}")
+    if B == 0:
+        return out
+    lib = _lib.load()
+    nsplit = 0 if nsplit is None else nsplit
+    nbytes = lib.fsvd_attn_decode_kv8_scratch_bytes(B, H, c.Hk, Dh, c.S, nsplit)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None       # of this call and stream
+    with _on(dev):
+        rc = lib.fsvd_attn_decode_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), _ptr(k_new), sk_b, sk_h, _ptr(v_new), sv_b, sv_h, lens, seqlen_add,
+                                      _ptr(cos), _ptr(sin), rope_len, out.data_ptr(), out.stride(0), out.stride(1), _ptr(scratch), nbytes, B, H, nsplit,
+                                      softmax_scale or 0.0, code, _stream())
+    _lib.check("fsvd_attn_decode_kv8", rc)
+    return out
+
+
+def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block, rows, cos, sin, softmax_scale, out):
+    dt, code = _elem(q, "q")
+    if q.dim() != 4 or q.stride(3) != 1:
+        raise ValueError(f"q must be [B,M,H,Dh] with unit inner stride, got {tuple(q.shape)}")
+    B, M, H, Dh = q.shape
+    c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
+    dev = k_cache.device
+    if c.Dh != Dh or H % c.Hk or q.device != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {dev}")
+    rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    pos, n = _kv8_vector(q_pos0, B, dev, "q_pos0"), _kv8_vector(rows, B, dev, "rows")
+    if out is None:
+        out = (torch.empty if rows is None else torch.zeros)(B, M, H, Dh, device=dev, dtype=dt)
+    elif out.shape != (B, M, H, Dh) or out.stride(3) != 1 or out.dtype != dt or out.device != dev:
+        raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on {dev}")
+    if B == 0:
+        return out
+    with _on(dev):
+        rc = _lib.load().fsvd_attn_prefill_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pos, n, _ptr(cos), _ptr(sin), rope_len, out.data_ptr(),
+                                               out.stride(0), out.stride(1), out.stride(2), B, M, H, softmax_scale or 0.0, code, _stream())
+    _lib.check("fsvd_attn_prefill_kv8", rc)
     return out

@@ -13,6 +13,7 @@ tensors.  ``flashsvd_amd.hip_ops`` and the modules under ``flashsvd_amd.kernels`
   rope_tables, rope_tables_mask       fsvd_rope_tables, fsvd_rope_tables_mask   the latter with the padding mask as bytes
   greedy_token_                       fsvd_greedy_token      argmax of every row + position increment
   set_token_rows_                     fsvd_set_token_rows    token and position of every row
+  sample_token_                       fsvd_sample_token      a draw from filtered logits + position increment
   qkv_rope_append / .out              fsvd_qkv_rope_append   head expansion + RoPE + dense-cache append
   attn_decode_densekv / .out          fsvd_attn_decode_densekv(_static)   the flash_attn_with_kvcache role
   attn_decode_rankkv / .out           fsvd_attn_decode_rankkv             decode over the rank-space cache
@@ -20,6 +21,9 @@ tensors.  ``flashsvd_amd.hip_ops`` and the modules under ``flashsvd_amd.kernels`
   rankkv_fill                         fsvd_rankkv_fill
   lowrank_expand_heads                fsvd_lowrank_expand_heads           prompt-pass head expansion (+ RoPE)
   rope_attn_prefill / .out            fsvd_attn_prefill                   causal prompt attention
+  kv8_append                          fsvd_kv8_append                     rows into a KV cache in 8 bits
+  attn_decode_kv8 / .out              fsvd_attn_decode_kv8                single-query attention over it, with append
+  attn_prefill_kv8 / .out             fsvd_attn_prefill_kv8               a chunk of a prompt over it
   reconstruct_qkv_token               fsvd_reconstruct_qkv_token          reference-layout current-token q / k / v
   xw_linear                           fsvd_xw_linear                      reference-layout x @ W
   mlp_dual_split                      fsvd_mlp_dual_split                 reference-layout dual-split MLP
@@ -166,6 +170,15 @@ def _set_token_rows(tokens, src, positions, position):
 _define("set_token_rows_(Tensor(a!) tokens, Tensor src, Tensor(b!) positions, int position) -> ()", _set_token_rows, lambda *a, **k: None)
 
 
+def _sample_token(logits, uniforms, tokens, positions, temperature, top_k, top_p, min_p, temperatures=None, top_ks=None, top_ps=None, min_ps=None):
+    from . import hip_ops
+    hip_ops._sample_token_impl(logits, uniforms, tokens, positions, temperature, top_k, top_p, min_p, temperatures, top_ks, top_ps, min_ps)
+
+
+_define("sample_token_(Tensor logits, Tensor uniforms, Tensor(a!) tokens, Tensor(b!)? positions, float temperature, int top_k, float top_p, float min_p, "
+        "Tensor? temperatures=None, Tensor? top_ks=None, Tensor? top_ps=None, Tensor? min_ps=None) -> ()", _sample_token, lambda *a, **k: None)
+
+
 # ------------------------------------------------------------------ q / k / v expansion + RoPE + cache append
 def _qkv(p, q_u, k_u, v_u, cos, sin, positions, k_cache, v_cache, num_heads, num_kv_heads, head_dim, cfg=0):
     from . import hip_ops
@@ -288,6 +301,37 @@ _define(f"rope_attn_prefill({_PF_ARGS}) -> Tensor", _prefill, lambda q, *a, **k:
 _define(f"rope_attn_prefill.out({_PF_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_out, lambda *a, out, **k: out)
 
 
+# ------------------------------------------------------------------ KV cache in 8 bits
+def _kv8_append(k, v, k_cache, v_cache, k_scale, v_scale, positions, block, cos=None, sin=None, rows=None):
+    from . import hip_ops
+    hip_ops._kv8_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, block, cos, sin, rows)
+
+
+def _attn_kv8(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block, k_new=None, v_new=None, cos=None, sin=None, seqlen_add=0, nsplit=None,
+              softmax_scale=None, *, out=None):
+    from . import hip_ops
+    return hip_ops._attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block, k_new, v_new, cos, sin, seqlen_add, nsplit,
+                                         softmax_scale, out)
+
+
+def _prefill_kv8(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block, rows=None, cos=None, sin=None, softmax_scale=None, *, out=None):
+    from . import hip_ops
+    return hip_ops._attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block, rows, cos, sin, softmax_scale, out)
+
+
+_KV8_HELD = "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, Tensor(d!) v_scale"
+_define(f"kv8_append(Tensor k, Tensor v, {_KV8_HELD}, Tensor positions, int block, Tensor? cos=None, Tensor? sin=None, Tensor? rows=None) -> ()",
+        _kv8_append, lambda *a, **k: None)
+_KD_ARGS = (f"Tensor q, {_KV8_HELD}, Tensor cache_seqlens, int block, Tensor? k_new=None, Tensor? v_new=None, Tensor? cos=None, Tensor? sin=None, "
+            "int seqlen_add=0, int? nsplit=None, float? softmax_scale=None")
+_define(f"attn_decode_kv8({_KD_ARGS}) -> Tensor", _attn_kv8, lambda q, *a, **k: q.new_empty(q.shape))
+_define(f"attn_decode_kv8.out({_KD_ARGS}, *, Tensor(e!) out) -> Tensor(e!)", _attn_kv8, lambda *a, out, **k: out)
+_KP_ARGS = ("Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor q_pos0, int block, Tensor? rows=None, Tensor? cos=None, "
+            "Tensor? sin=None, float? softmax_scale=None")
+_define(f"attn_prefill_kv8({_KP_ARGS}) -> Tensor", _prefill_kv8, lambda q, *a, **k: q.new_empty(q.shape))
+_define(f"attn_prefill_kv8.out({_KP_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_kv8, lambda *a, out, **k: out)
+
+
 # ------------------------------------------------------------------ reference operand layouts
 def _reconstruct(Pq, Pk, Pv, Vq, Vk, Vv, bq=None, bk=None, bv=None):
     from .kernels import densekv_reconstruct as DR
@@ -323,5 +367,5 @@ _define("mlp_dual_split(Tensor PUp, Tensor PGate, Tensor GateU, Tensor UpU, Tens
         PUp.new_empty((PUp.shape[0], DownU.shape[1])))
 
 ops = getattr(torch.ops, NS)
-OP_NAMES = ("linear", "swiglu_linear", "rmsnorm", "greedy_token_", "set_token_rows_", "lowrank_mlp", "lowrank_attn_prefill", "rope_tables", "rope_tables_mask", "qkv_rope_append", "attn_decode_densekv", "attn_decode_rankkv", "rankkv_append", "rankkv_fill", "linear_rankkv_append",
+OP_NAMES = ("linear", "swiglu_linear", "rmsnorm", "greedy_token_", "set_token_rows_", "sample_token_", "kv8_append", "attn_decode_kv8", "attn_prefill_kv8", "lowrank_mlp", "lowrank_attn_prefill", "rope_tables", "rope_tables_mask", "qkv_rope_append", "attn_decode_densekv", "attn_decode_rankkv", "rankkv_append", "rankkv_fill", "linear_rankkv_append",
             "lowrank_expand_heads", "rope_attn_prefill", "reconstruct_qkv_token", "xw_linear", "mlp_dual_split")

@@ -176,6 +176,56 @@ int fsvd_greedy_token(const void* logits, int64_t ld, int64_t* tokens, int64_t l
                       void* stream);
 /* tokens[b] = src[b], positions[b] = position for b < B, in one launch. */
 int fsvd_set_token_rows(int64_t* tokens, const int64_t* src, int32_t* positions, int32_t position, int B, void* stream);
+/* The next token of every row drawn from its filtered logits [B, V] (rows ld elements apart, at any element's address).  With the logits in descending
+ * order, equal ones by index, w_i = exp((l_i - l_0) / T) and C_n the sum of the first n: top_k (0: off) keeps n_k of them, top_p those up to the smallest n
+ * with C_n > top_p C_{n_k} (1 and more: off), min_p (0: off) those with w >= min_p; N is the least of the three, one at least, and the token the first
+ * with C > u C_N, u = uniforms[b] in [0, 1).  Sums in 64 bits.  T <= 0, and a row whose largest logit is not finite, give the greedy token.
+ * temperatures / top_ks / top_ps / min_ps, when given, hold B values in place of the numbers.  positions, when given: positions[b] += 1.
+ * The draw of _sample_next_token (scripts/demo_support/api.py:192), which sorts the row, from given random numbers. */
+int fsvd_sample_token(const void* logits, int64_t ld, const float* uniforms, int64_t* tokens, int64_t ldt, int32_t* positions, double temperature,
+                      const float* temperatures, int top_k, const int32_t* top_ks, double top_p, const float* top_ps, double min_p,
+                      const float* min_ps, int B, int V, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * KV cache in 8 bits.  Codes [B, S, Hk, Dh] in e4m3 (finite form, largest 448), keys after their rotation; one fp32 scale for each sequence, block of
+ * `block` tokens and kv head, value = code * scale.  fsvd_kv8_append makes every scale a power of two, 2^e with the smallest e >= -126 for which
+ * 448 * 2^e covers what is held.  k and v share their strides (elements; multiples of 16, as the addresses of 16 bytes), k_scale and v_scale theirs.
+ * head_dim 64 and 128; blocks of 16, 32, 64 and 128 tokens.  No counterpart in the reference, whose caches are of 16 bits. */
+typedef struct fsvd_kv8_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t sc_b, sc_s, sc_h;              /* codes: sequence, token, head */
+  int64_t ss_b, ss_n, ss_h;              /* scales: sequence, block, head */
+  int32_t S, Hk, Dh, block;
+} fsvd_kv8_cache;
+
+/* Row t < rows[b] (rows NULL: T) of k and v [B, T, Hk, Dh] goes to cache position positions[b] + t of sequence b; k is rotated there (cos and sin
+ * [rope_len, Dh / 2], NULL: not; halves of a head are the pairs, fp32) and rounded once.  A block's scale covers its new rows; a block with rows before the
+ * first new one keeps the larger of that and its old scale, and those rows move to it.  The rows behind the last written one of a block are not valid
+ * from then on.  Rows outside [0, S) are dropped.  A NaN stays one, an infinity becomes the largest code; neither decides a scale. */
+int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t,
+                    int64_t sv_h, const int32_t* positions, const int32_t* rows, const void* cos, const void* sin, int rope_len, int B, int T, int dtype,
+                    void* stream);
+
+/* fsvd_attn_decode_densekv over a cache in 8 bits: one query token per sequence, q [B, H, Dh] over cache_seqlens[b] + seqlen_add keys; with
+ * k_new / v_new [B, Hk, Dh] these are appended at cache_seqlens[b] first (fsvd_kv8_append) and cache_seqlens[b] + 1 keys are seen.  cos / sin also
+ * rotate q at cache_seqlens[b].  scratch: fsvd_attn_decode_kv8_scratch_bytes, of this call and stream alone, of any content.  nsplit <= 0: chosen here, as
+ * the size of the scratch is. */
+size_t fsvd_attn_decode_kv8_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit);
+int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
+                         const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
+                         int rope_len, void* out, int64_t so_b, int64_t so_h, void* scratch, size_t scratch_bytes, int B, int H, int nsplit, float scale,
+                         int dtype, void* stream);
+
+/* Causal attention of a chunk of a prompt over a cache in 8 bits that holds the chunk's own rows already: q [B, M, H, Dh], row m of sequence b stands
+ * at position q_pos0[b] + m (rotated there with cos / sin, NULL: q comes rotated) and sees the keys up to that.  Rows m >= rows[b] (NULL: M) of out
+ * [B, M, H, Dh] are left as they were.  Softmax scale 1 / sqrt(Dh) when scale <= 0. */
+int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
+                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, int B, int M, int H,
+                          float scale, int dtype, void* stream);
+
 
 
 /* ---------------------------------------------------------------------------------------------
