@@ -162,6 +162,23 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(a, b), fmaxf(c, d));
 }
 
+// the other lanes' values of a column (lane % 16) by register swaps: the largest of the four, and their sum
+__device__ __forceinline__ float column_max(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float w = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const uint32_t x = __float_as_uint(w);
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t x = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
 // Workgroup `part` of `parts` reads its share of them, whole 16-byte pieces inside the range, and keeps nothing.
 template <int THREADS>
 __device__ __forceinline__ void request_ahead(const Ahead& a, int part, int parts, int tid) {

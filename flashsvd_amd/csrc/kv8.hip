@@ -116,7 +116,10 @@ int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, in
   return launch_kv8_append(fn, a, static_cast<hipStream_t>(stream));
 }
 
-size_t fsvd_attn_decode_kv8_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) { return 0; }
+size_t fsvd_attn_decode_kv8_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0) return 0;
+  return kv8_scratch_bytes(B, H, Dh, kv8_ranges(B, H, Hk, S, nsplit));
+}
 
 int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
                          const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
@@ -128,6 +131,12 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
   if (q == nullptr || out == nullptr || cache_seqlens == nullptr || (k_new == nullptr) != (v_new == nullptr)) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (H <= 0 || H % cache->Hk) { set_last_error("%s: %d query heads over %d", fn, H, cache->Hk); return kErrBadShape; }
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int ranges = kv8_ranges(B, H, cache->Hk, cache->S, nsplit);
+  const size_t need = kv8_scratch_bytes(B, H, cache->Dh, ranges);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 3))) {
+    set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, ranges, need);
+    return kErrWorkspace;
+  }
   if (k_new) {
     const Kv8AppendArgs n{*cache, in16(k_new), sk_b, 0, sk_h, in16(v_new), sv_b, 0, sv_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, B, 1, dtype};
     if (const int rc = launch_kv8_append(fn, n, st)) return rc;
@@ -135,7 +144,7 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
   }
   const Kv8AttnArgs a{*cache, in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
                       B, 1, H, seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
-  return launch_kv8_attend(fn, a, st);
+  return launch_kv8_decode(fn, a, ranges, static_cast<float*>(scratch), st);
 }
 
 int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,

@@ -30,6 +30,19 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }     // -126 <= e <= 127
 
+// a pair of codes (low or high half of a word) as a pair of 16-bit elements, exact in both types
+template <int DT> struct Code16;
+template <> struct Code16<0> {
+  template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
+  }
+};
+template <> struct Code16<1> {
+  template <bool HI> static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+  }
+};
+
 struct Kv8AppendArgs {
   fsvd_kv8_cache c;
   const uint16_t* k; int64_t sk_b, sk_t, sk_h;         // [B, T, Hk, Dh]
@@ -53,6 +66,10 @@ struct Kv8AttnArgs {
 };
 int check_kv8_cache(const char* fn, const fsvd_kv8_cache* c);
 int launch_kv8_append(const char* fn, const Kv8AppendArgs& a, hipStream_t st);
+// ranges of keys that a sequence may be cut into, and the scratch for their partial results
+int kv8_ranges(int B, int H, int Hk, int S, int nsplit);
+size_t kv8_scratch_bytes(int B, int H, int Dh, int ranges);
+int launch_kv8_decode(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st);
 int launch_kv8_attend(const char* fn, const Kv8AttnArgs& a, hipStream_t st);
 
 }  // namespace fsvd

@@ -138,22 +138,6 @@ __global__ __launch_bounds__(kPfThreads) void lowrank_expand_kernel(ExpandArgs a
 //     priority around the products and scalar address parts were built and gave nothing: two workgroups share a compute
 //     unit, and each covers the other's waits.
 // ---------------------------------------------------------------------------------------------
-// the other lanes' values of a column (lane % 16) by register swaps: the largest of the four, and their sum
-__device__ __forceinline__ float column_max(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float w = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  const uint32_t x = __float_as_uint(w);
-  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-}
-__device__ __forceinline__ float column_sum(float v) {
-  const uint32_t u = __float_as_uint(v);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const uint32_t x = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-  const auto q = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __uint_as_float(q[0]) + __uint_as_float(q[1]);
-}
 // exp(s * scale - m), every step rounded by itself
 __device__ __forceinline__ float weight_of(float s, float scale, float m) {
 #pragma clang fp contract(off)
