@@ -195,7 +195,8 @@ SIGNATURES = {
     "fsvd_attn_decode_kv8": (c_int, [ctypes.POINTER(Kv8Cache)] + [c_void_p, c_int64, c_int64] * 3 + [c_void_p, c_int, c_void_p, c_void_p, c_int,
                                      c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "fsvd_attn_prefill_kv8": (c_int, [ctypes.POINTER(Kv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-                                      c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+                                      c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "fsvd_attn_prefill_kv8_scratch_bytes": (c_size_t, [c_int] * 6),
     "fsvd_set_token_rows": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int32, c_int, c_void_p]),
     "fsvd_mlp_block_scratch_bytes": (c_size_t, [ctypes.POINTER(MlpBlock)]),
     "fsvd_attn_block_scratch_bytes": (c_size_t, [ctypes.POINTER(AttnBlock)]),

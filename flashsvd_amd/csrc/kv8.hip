@@ -118,7 +118,7 @@ int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, in
 
 size_t fsvd_attn_decode_kv8_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) {
   if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0) return 0;
-  return kv8_scratch_bytes(B, H, Dh, kv8_ranges(B, H, Hk, S, nsplit));
+  return kv8_decode_scratch_bytes(B, H, Dh, kv8_ranges(B, H, Hk, S, nsplit));
 }
 
 int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
@@ -132,8 +132,8 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
   if (H <= 0 || H % cache->Hk) { set_last_error("%s: %d query heads over %d", fn, H, cache->Hk); return kErrBadShape; }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int ranges = kv8_ranges(B, H, cache->Hk, cache->S, nsplit);
-  const size_t need = kv8_scratch_bytes(B, H, cache->Dh, ranges);
-  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 3))) {
+  const size_t need = kv8_decode_scratch_bytes(B, H, cache->Dh, ranges);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
     set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, ranges, need);
     return kErrWorkspace;
   }
@@ -147,9 +147,14 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
   return launch_kv8_decode(fn, a, ranges, static_cast<float*>(scratch), st);
 }
 
+size_t fsvd_attn_prefill_kv8_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
+  if (B <= 0 || M <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0) return 0;
+  return kv8_prompt_scratch_bytes(B, M, H, Hk, Dh, S);
+}
+
 int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
-                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, int B, int M, int H,
-                          float scale, int dtype, void* stream) {
+                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
+                          size_t scratch_bytes, int B, int M, int H, float scale, int dtype, void* stream) {
   const char* fn = "fsvd_attn_prefill_kv8";
   if (const int rc = check_kv8_cache(fn, cache)) return rc;
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
@@ -157,7 +162,7 @@ int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq
   if (M < 0 || H <= 0 || H % cache->Hk) { set_last_error("%s: %d rows of %d query heads over %d", fn, M, H, cache->Hk); return kErrBadShape; }
   const Kv8AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
                       B, M, H, 1, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
-  return M == 0 ? kOk : launch_kv8_attend(fn, a, static_cast<hipStream_t>(stream));
+  return M == 0 ? kOk : launch_kv8_prompt(fn, a, static_cast<float*>(scratch), scratch_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

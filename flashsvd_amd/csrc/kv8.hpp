@@ -68,8 +68,9 @@ int check_kv8_cache(const char* fn, const fsvd_kv8_cache* c);
 int launch_kv8_append(const char* fn, const Kv8AppendArgs& a, hipStream_t st);
 // ranges of keys that a sequence may be cut into, and the scratch for their partial results
 int kv8_ranges(int B, int H, int Hk, int S, int nsplit);
-size_t kv8_scratch_bytes(int B, int H, int Dh, int ranges);
+size_t kv8_decode_scratch_bytes(int B, int H, int Dh, int ranges);
+size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S);
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st);
-int launch_kv8_attend(const char* fn, const Kv8AttnArgs& a, hipStream_t st);
+int launch_kv8_prompt(const char* fn, const Kv8AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st);
 
 }  // namespace fsvd

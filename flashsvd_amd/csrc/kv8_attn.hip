@@ -3,6 +3,113 @@
 
 namespace fsvd {
 
+// Partial results of key ranges: values [rows][ranges][Dh], not divided by their sums, and behind them (maximum, sum) [rows][ranges].
+struct Kv8Parts {
+  float* base;
+  int64_t rows;
+  int ranges, dh;
+  static size_t bytes(int64_t rows, int ranges, int dh) { return (size_t)rows * ranges * (dh + 2) * sizeof(float); }
+  __device__ __forceinline__ float* values(int64_t row, int s) const { return base + (row * ranges + s) * dh; }
+  __device__ __forceinline__ f32x2_t* stats(int64_t row, int s) const { return reinterpret_cast<f32x2_t*>(base + rows * ranges * dh) + row * ranges + s; }
+};
+
+// eight elements x at dimension d of a query row, rotated in fp32 and rounded to the type of the products; d and its partner are half a head apart
+template <class E, int HALF>
+__device__ __forceinline__ u32x4_t rotated(u32x4_t x, const uint16_t* row, const uint16_t* cos, const uint16_t* sin, int d) {
+  const bool up = d >= HALF;
+  const int pair = up ? d - HALF : d + HALF, at = up ? d - HALF : d;
+  const u32x4_t y = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(row + pair));
+  const u32x4_t cw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(cos + at));
+  const u32x4_t sw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(sin + at));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float sl = up ? E::lo(sw[i]) : -E::lo(sw[i]), sh = up ? E::hi(sw[i]) : -E::hi(sw[i]);
+    x[i] = E::pack2(E::lo(x[i]) * E::lo(cw[i]) + E::lo(y[i]) * sl, E::hi(x[i]) * E::hi(cw[i]) + E::hi(y[i]) * sh);
+  }
+  return x;
+}
+
+constexpr int kMinRange = 256;                            // keys of a decode range, but for the last
+__host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
+  const int per = (keys + ranges - 1) / ranges;
+  return per < kMinRange ? kMinRange : (per + 127) / 128 * 128;
+}
+
+// The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
+// token, head of the group).
+template <int DT, int DH, int WPR>
+__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges, bool decode, float* scratch) {
+  typedef E16<DT> E;
+  constexpr int D = DH / kWave, U = 8;
+  __shared__ float vs[4][DH];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part_of = wave % WPR, G = a.H / a.c.Hk;
+  const int64_t rows = (int64_t)a.B * a.M * a.H, row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;
+  const int64_t at = row < rows ? row : rows - 1;
+  const int b = (int)(at / ((int64_t)a.M * a.H)), in = (int)(at - (int64_t)b * a.M * a.H);
+  int m, h, used = ranges;
+  bool live = row < rows;
+  if (decode) {
+    m = 0; h = in;
+    const int keys = max(0, min(a.positions[b] + a.key_add, a.c.S)), per = kv8_range(keys, ranges);
+    used = (keys + per - 1) / per;
+    live = live && per < keys;                             // else written by its only workgroup
+  } else {
+    const int hk = in / (a.M * G), r = in - hk * a.M * G;
+    m = r / G;
+    h = hk * G + r - m * G;
+    live = live && (!a.rows || m < a.rows[b]);
+  }
+  const Kv8Parts part{scratch, rows, ranges, DH};
+  float v[D], sum = 0.f, top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < D; ++i) v[i] = 0.f;
+  if (live) {
+    for (int s0 = 0; s0 < used; s0 += kWave) top = fmaxf(top, s0 + lane < used ? (*part.stats(at, s0 + lane))[0] : -INFINITY);
+    top = wave_max(top);
+    for (int s0 = 0; s0 < used; s0 += kWave) {
+      const f32x2_t st = *part.stats(at, min(s0 + lane, used - 1));
+      const float w = s0 + lane < used && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
+      sum += w * st[1];
+      const int n = min(kWave, used - s0);
+      for (int s = part_of; s < n; s += WPR * U) {
+        float x[U][D];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : 0.f;
+#pragma unroll
+          for (int i = 0; i < D; ++i) v[i] += f > 0.f ? f * x[u][i] : 0.f;      // a range without a visible key has written no values
+        }
+      }
+    }
+    sum = wave_sum(sum);
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) vs[wave][lane * D + i] = v[i];
+    __syncthreads();
+    if (part_of == 0) {
+#pragma unroll
+      for (int i = 0; i < D; ++i)
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) v[i] += vs[wave + w][lane * D + i];
+    }
+  }
+  if (!live || part_of) return;
+  uint16_t* o = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + lane * D;
+#pragma unroll
+  for (int i = 0; i < D; ++i) o[i] = (uint16_t)E::bits(sum > 0.f ? v[i] / sum : 0.f);
+}
+template <int DT, int DH>
+static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* scratch, hipStream_t st) {
+  const int64_t rows = (int64_t)a.B * a.M * a.H;
+  if (ranges > 8) hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ranges, decode, scratch);
+  else hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ranges, decode, scratch);
+}
+
 // ---------------------------------------------------------------------------------------------
 // One query token per sequence.  A workgroup takes a range of the keys of one kv head for up to 16 of its query heads, a wave every fourth step of 32
 // keys, on the matrix cores: S^T = K Q^T, O^T = V^T P^T (16 x 16 x 32).
@@ -11,11 +118,6 @@ namespace fsvd {
 //   V: lane (n, g) loads those eight keys' dimensions DH / 16 n .. of the row, and byte permutes put two keys of a dimension next to each other.
 // Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.
 // ---------------------------------------------------------------------------------------------
-constexpr int kMinRange = 256;                            // keys of a range, but for the last
-__host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
-  const int per = (keys + ranges - 1) / ranges;
-  return per < kMinRange ? kMinRange : (per + 127) / 128 * 128;
-}
 constexpr int kDecWaves = 4, kDecStep = 32, kDecGroup = 16;
 
 template <int DT, int DH>
@@ -80,18 +182,7 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
     for (int st = 0; st < ST; ++st) {
       const int d = 64 * (st >> 1) + 16 * g + 8 * (st & 1);
       u32x4_t x = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(qp + d));
-      if (a.cos) {
-        const bool up = d >= HALF;
-        const int dt = up ? d - HALF : d;
-        const u32x4_t y = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(qp + (up ? d - HALF : d + HALF)));
-        const u32x4_t cw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.cos + tp + dt));
-        const u32x4_t sw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.sin + tp + dt));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float sl = up ? E::lo(sw[i]) : -E::lo(sw[i]), sh = up ? E::hi(sw[i]) : -E::hi(sw[i]);
-          x[i] = E::pack2(E::lo(x[i]) * E::lo(cw[i]) + E::lo(y[i]) * sl, E::hi(x[i]) * E::hi(cw[i]) + E::hi(y[i]) * sh);
-        }
-      }
+      if (a.cos) x = rotated<E, HALF>(x, qp, a.cos + tp, a.sin + tp, d);
       if (n >= heads) x = u32x4_t{0u, 0u, 0u, 0u};
       qf[st] = __builtin_bit_cast(frag_t, x);
     }
@@ -190,30 +281,12 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
     if (whole) {
       a.out[(int64_t)b * a.so_b + (int64_t)(h0 + q) * a.so_h + d] = (uint16_t)E::bits(sum > 0.f ? v / sum : 0.f);
     } else {
-      float* part = scratch + ((int64_t)(b * a.H + h0 + q) * ranges + s) * (DH + 2);
-      part[d] = v;
-      if (d == 0) { part[DH] = top; part[DH + 1] = sum; }
+      const Kv8Parts part{scratch, (int64_t)a.B * a.H, ranges, DH};
+      const int64_t row = (int64_t)b * a.H + h0 + q;
+      part.values(row, s)[d] = v;
+      if (d == 0) *part.stats(row, s) = f32x2_t{top, sum};
     }
   }
-}
-
-// The ranges of a head joined, in their order.
-template <int DT, int DH>
-__global__ __launch_bounds__(DH) void kv8_join_kernel(Kv8AttnArgs a, int ranges, const float* scratch) {
-  typedef E16<DT> E;
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x;
-  const int keys = max(0, min(a.positions[b] + a.key_add, a.c.S)), per = kv8_range(keys, ranges);
-  if (per >= keys) return;                                 // written by its only workgroup
-  const int used = (keys + per - 1) / per;
-  const float* part = scratch + (int64_t)(b * a.H + h) * ranges * (DH + 2);
-  float top = -INFINITY, sum = 0.f, v = 0.f;
-  for (int s = 0; s < used; ++s) top = fmaxf(top, part[s * (DH + 2) + DH]);
-  for (int s = 0; s < used; ++s) {
-    const float f = __builtin_amdgcn_exp2f(part[s * (DH + 2) + DH] - top);
-    sum += f * part[s * (DH + 2) + DH + 1];
-    v += f * part[s * (DH + 2) + d];
-  }
-  a.out[(int64_t)b * a.so_b + (int64_t)h * a.so_h + d] = (uint16_t)E::bits(sum > 0.f ? v / sum : 0.f);
 }
 
 int kv8_ranges(int B, int H, int Hk, int S, int nsplit) {
@@ -224,15 +297,16 @@ int kv8_ranges(int B, int H, int Hk, int S, int nsplit) {
   }
   return max(1, min(nsplit, most));
 }
-size_t kv8_scratch_bytes(int B, int H, int Dh, int ranges) { return ranges > 1 ? (size_t)B * H * ranges * (Dh + 2) * sizeof(float) : 0; }
+size_t kv8_decode_scratch_bytes(int B, int H, int Dh, int ranges) { return ranges > 1 ? Kv8Parts::bytes((int64_t)B * H, ranges, Dh) : 0; }
 
 template <int DT, int DH>
 static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   const int groups = (a.H / a.c.Hk + kDecGroup - 1) / kDecGroup;
   hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave), 0, st, a, ranges, scratch);
-  if (ranges > 1) hipLaunchKernelGGL((kv8_join_kernel<DT, DH>), dim3(a.H, a.B), dim3(DH), 0, st, a, ranges, scratch);
+  if (ranges > 1) launch_join<DT, DH>(a, ranges, true, scratch, st);
 }
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+  if ((int64_t)a.B * a.H * ranges > 0x7fffffff) { set_last_error("%s: %d sequences of %d heads in %d ranges", fn, a.B, a.H, ranges); return kErrBadShape; }
   if (a.dt == 1) a.c.Dh == 128 ? decode_form<1, 128>(a, ranges, scratch, st) : decode_form<1, 64>(a, ranges, scratch, st);
   else a.c.Dh == 128 ? decode_form<0, 128>(a, ranges, scratch, st) : decode_form<0, 64>(a, ranges, scratch, st);
   const hipError_t e = hipGetLastError();
@@ -240,57 +314,318 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& a, int ranges, float* s
   return kOk;
 }
 
-// One wave for a query row of one head: every key's score by a sum over the lanes, the running maximum and sum of the softmax.
-template <int DT>
-__global__ __launch_bounds__(64) void kv8_attend_kernel(Kv8AttnArgs a) {
-  typedef E16<DT> E;
-  const int m = blockIdx.x, h = blockIdx.y, b = blockIdx.z, lane = threadIdx.x, half = a.c.Dh >> 1;
-  if (a.rows && m >= a.rows[b]) return;
-  const int hk = h / (a.H / a.c.Hk), pos = a.positions[b] + m;
-  const int keys = max(0, min(pos + a.key_add, a.c.S));
-  const uint16_t* q = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
-  // dimensions lane and lane + half of this lane (the first half lanes alone where half is 32)
-  float q0 = 0.f, q1 = 0.f;
-  const bool in = lane < half;
-  if (in) {
-    q0 = E::val(q[lane]); q1 = E::val(q[lane + half]);
-    if (a.cos) {
-      const int64_t tp = min(max(pos, 0), a.rope_len - 1);
-      const float c = E::val(a.cos[tp * half + lane]), n = E::val(a.sin[tp * half + lane]);
-      const float y0 = q0 * c - q1 * n, y1 = q0 * n + q1 * c;
-      q0 = y0; q1 = y1;
-    }
-  }
-  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + (in ? lane : 0);
-  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h + (in ? lane : 0);
-  const float* ks = a.c.k_scale + b * a.c.ss_b + hk * a.c.ss_h;
-  const float* vs = a.c.v_scale + b * a.c.ss_b + hk * a.c.ss_h;
-  float top = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int n = 0; n < keys; ++n) {
-    const uint8_t* k = kb + (int64_t)n * a.c.sc_s;
-    const auto kk = codes_lo((uint32_t)k[0] | (uint32_t)k[half] << 8);
-    const float s = wave_sum(q0 * kk[0] + q1 * kk[1]) * ks[(int64_t)(n / a.c.block) * a.c.ss_n] * a.scale;
-    const float now = fmaxf(top, s), w = __expf(s - now), keep = __expf(top - now);
-    const uint8_t* v = vb + (int64_t)n * a.c.sc_s;
-    const auto vv = codes_lo((uint32_t)v[0] | (uint32_t)v[half] << 8);
-    const float f = w * vs[(int64_t)(n / a.c.block) * a.c.ss_n];
-    o0 = o0 * keep + f * vv[0];
-    o1 = o1 * keep + f * vv[1];
-    sum = sum * keep + w;
-    top = now;
-  }
-  if (!in) return;
-  uint16_t* o = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h;
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  o[lane] = (uint16_t)E::bits(o0 * inv);
-  o[lane + half] = (uint16_t)E::bits(o1 * inv);
+// ---------------------------------------------------------------------------------------------
+// A chunk of a prompt.  The query rows of the heads that share a kv head are one list, row r = query token r / G of head r % G, so that grouped heads share
+// the tiles of keys too.  A workgroup of NW waves takes 16 MI rows for each wave; tiles of 64 keys go through LDS as 16-bit elements, converted once for
+// the workgroup: K row by row, V transposed (two keys of a dimension next to each other by byte permutes), two buffers and one barrier a tile.
+//   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
+//   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
+//   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
+//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.
+// V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
+// writes off each other's banks (found by enumeration).
+// ---------------------------------------------------------------------------------------------
+constexpr int kTile = 64;
+__device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
+// four codes as two pairs of bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, bool hi, float scale, bool power) {
+  if (power) return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+  const f32x2_t x = hi ? codes_hi(w) : codes_lo(w);
+  return pack_bf16x2(x[0] * scale, x[1] * scale);
 }
 
-int launch_kv8_attend(const char* fn, const Kv8AttnArgs& a, hipStream_t st) {
-  if (a.H > 65535) { set_last_error("%s: %d query heads", fn, a.H); return kErrBadShape; }
-  const dim3 grid(a.M, a.H, a.B);
-  if (a.dt == 1) hipLaunchKernelGGL(kv8_attend_kernel<1>, grid, dim3(64), 0, st, a);
-  else hipLaunchKernelGGL(kv8_attend_kernel<0>, grid, dim3(64), 0, st, a);
+template <int DT, int DH, int MI, int NW>
+__global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
+  typedef E16<DT> E;
+  typedef typename E::frag_t frag_t;
+  typedef E16<0>::frag_t pfrag_t;
+  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * NW, QW = 16 * MI, BM = QW * NW;
+  constexpr int KL = DH / 16, KP = (kTile * KL + TH - 1) / TH;              // lanes of a key row; passes of the workgroup over the tile's keys
+  constexpr int VL = DH / 4, VP = (kTile / 4 * VL + TH - 1) / TH;
+  constexpr bool kRest = DT == 1;
+  extern __shared__ __align__(16) unsigned char smem[];
+  uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile][KSTR]
+  uint16_t* Vt = Ks + 2 * kTile * KSTR;                                     // [2][DH][kTile]
+
+  const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
+  int mt, hb;
+  // the row tiles of a kv head on one XCD, the ones with the most keys first
+  if (HB % 8 == 0) {
+    const int per = HB >> 3, r = blockIdx.x >> 3;
+    mt = r / per;
+    hb = (blockIdx.x & 7) * per + r - mt * per;
+  } else {
+    const int t = xcd_run_index(blockIdx.x, MT * HB);
+    hb = t / MT;
+    mt = t - hb * MT;
+  }
+  mt = MT - 1 - mt;
+  const int hk = hb / a.B, b = hb - hk * a.B, range = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
+  const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
+  if (row0 >= rows) return;
+  const int pos = a.positions[b];
+  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
+  const int all_end = seen_by(min(row0 + BM, rows) - 1);
+  const int tiles = (all_end + kTile - 1) / kTile, per = (tiles + ranges - 1) / ranges;
+  const int n_begin = range * per * kTile, n_end = min(all_end, (range + 1) * per * kTile);
+  const int w0 = row0 + wave * QW;
+  const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
+
+  frag_t qf[MI][ST];
+  int seen[MI];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r = min(w0 + 16 * mi + lr, rows - 1), m = r / G, h = hk * G + r - m * G;
+    seen[mi] = seen_by(r);
+    const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
+    constexpr int HALF = DH / 2;
+    const int64_t tp = a.cos ? (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF : 0;
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
+      const int d = 32 * st + 8 * lg;
+      u32x4_t x = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(qp + d));
+      if (a.cos) x = rotated<E, HALF>(x, qp, a.cos + tp, a.sin + tp, d);
+      qf[mi][st] = __builtin_bit_cast(frag_t, x);
+    }
+  }
+  const float scale = a.scale * 1.4426950408889634f;
+  float m_run[MI], l_run[MI];
+  f32x4_t o[MI][NT];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    m_run[mi] = -INFINITY; l_run[mi] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[mi][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
+  const float* ksp = a.c.k_scale + b * a.c.ss_b + hk * a.c.ss_h;
+  const float* vsp = a.c.v_scale + b * a.c.ss_b + hk * a.c.ss_h;
+  const int shift = 31 - __builtin_clz(a.c.block);
+  // K: KL lanes with 16 codes each for a row; V: VL lanes with 4 codes each for four adjacent keys
+  const int krow = tid / KL, kd = tid % KL * 16, vrow = tid / VL, vd = tid % VL * 4;
+  u32x4_t kreg[KP];
+  uint32_t vreg[VP][4];
+  float vscale[VP], kscale[4];
+  const auto request = [&](int n0) {
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int row = krow + p * (TH / KL);
+      if (kTile * KL % TH == 0 || row < kTile) kreg[p] = *reinterpret_cast<const u32x4_t*>(kb + (int64_t)min(n0 + row, n_end - 1) * a.c.sc_s + kd);
+    }
+#pragma unroll
+    for (int p = 0; p < VP; ++p) {
+      const int row = 4 * (vrow + p * (TH / VL));
+      if (kTile / 4 * VL % TH == 0 || row < kTile) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vb + (int64_t)min(n0 + row + e, n_end - 1) * a.c.sc_s + vd);
+        vscale[p] = vsp[(int64_t)(min(n0 + row, n_end - 1) >> shift) * a.c.ss_n];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kscale[j] = ksp[(int64_t)(min(n0 + 16 * j, n_end - 1) >> shift) * a.c.ss_n];
+  };
+  const auto stage = [&](int buf) {
+    uint16_t* ks = Ks + buf * kTile * KSTR;
+    uint16_t* vt = Vt + buf * DH * kTile;
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+      const int row = krow + p * (TH / KL);
+      if (kTile * KL % TH == 0 || row < kTile) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t x = kreg[p][2 * h], y = kreg[p][2 * h + 1];
+          *reinterpret_cast<u32x4_t*>(ks + row * KSTR + kd + 8 * h) = u32x4_t{Code16<DT>::template pair<false>(x), Code16<DT>::template pair<true>(x),
+                                                                              Code16<DT>::template pair<false>(y), Code16<DT>::template pair<true>(y)};
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < VP; ++p) {
+      const int row4 = vrow + p * (TH / VL);
+      if (kTile / 4 * VL % TH == 0 || row4 < kTile / 4) {
+        const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
+        const bool power = (__float_as_uint(vscale[p]) & 0x7fffffu) == 0;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
+          const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = vd + 2 * c + e;
+            *reinterpret_cast<u32x2_t*>(vt + d * kTile + (col ^ (8 * v_piece(d)))) = u32x2_t{scaled_pair(lo, e, vscale[p], power), scaled_pair(hi, e, vscale[p], power)};
+          }
+        }
+      }
+    }
+  };
+
+  if (n_begin < n_end) request(n_begin);
+  int buf = 0;
+  for (int n0 = n_begin; n0 < n_end; n0 += kTile, buf ^= 1) {
+    stage(buf);
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = kscale[j] * scale;
+    if (n0 + kTile < n_end) request(n0 + kTile);
+    __syncthreads();                     // this buffer is written; the other one is read by nobody any more
+    if (n0 >= wave_end) continue;
+    const uint16_t* ks = Ks + buf * kTile * KSTR;
+    const uint16_t* vt = Vt + buf * DH * kTile;
+    f32x4_t s[MI][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      frag_t kf[ST];
+#pragma unroll
+      for (int st = 0; st < ST; ++st) kf[st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (16 * j + lr) * KSTR + 32 * st + 8 * lg));
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) {
+        s[mi][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < ST; ++st) s[mi][j] = E::mfma(kf[st], qf[mi][st], s[mi][j]);
+      }
+    }
+    const bool plain = n0 + kTile <= seen_by(w0);                  // every row of the wave sees the whole tile (rows see more from one to the next)
+    pfrag_t ph[MI][2], pl[MI][2];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      float top = -INFINITY;
+      if (plain) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, f[j] * fmaxf(fmaxf(s[mi][j][0], s[mi][j][1]), fmaxf(s[mi][j][2], s[mi][j][3])));
+      } else {
+        const int vis = seen[mi] - n0 - 4 * lg;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[mi][j][i] = 16 * j + i < vis ? s[mi][j][i] * f[j] : -INFINITY;
+            top = fmaxf(top, s[mi][j][i]);
+          }
+      }
+      top = fmaxf(m_run[mi], column_max(top));
+      if (__any(top > m_run[mi])) {
+        const float keep = top > m_run[mi] ? __builtin_amdgcn_exp2f(m_run[mi] - top) : 1.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[mi][t] *= keep;
+        l_run[mi] *= keep;
+        m_run[mi] = top;
+      }
+      const float base = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet: exp2(-inf - 0)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[mi][j][i] = __builtin_amdgcn_exp2f(plain ? fmaf(s[mi][j][i], f[j], -base) : s[mi][j][i] - base);
+          l_run[mi] += s[mi][j][i];
+        }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        uint32_t hw[4], lw[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x0 = s[mi][2 * st + (c >> 1)][2 * (c & 1)], x1 = s[mi][2 * st + (c >> 1)][2 * (c & 1) + 1];
+          hw[c] = pack_bf16x2(x0, x1);
+          if (kRest) lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+        }
+        ph[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
+        if (kRest) pl[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+      }
+    }
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int d = 16 * t + lr;
+        const pfrag_t vf = __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + d * kTile + ((32 * st + 8 * lg) ^ (8 * v_piece(d)))));
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+          o[mi][t] = E16<0>::mfma(vf, ph[mi][st], o[mi][t]);
+          if (kRest) o[mi][t] = E16<0>::mfma(vf, pl[mi][st], o[mi][t]);
+        }
+      }
+  }
+  // element i of tile t is dimension 16 t + 4 lg + i of row lr
+  const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r = w0 + 16 * mi + lr;
+    const float l = column_sum(l_run[mi]);
+    if (r >= rows) continue;
+    if (ranges > 1) {
+      const Kv8Parts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+      const int64_t row = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
+      if (lg == 0) *part.stats(row, range) = f32x2_t{m_run[mi], l};
+      float* v = part.values(row, range) + 4 * lg;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t*>(v + 16 * t) = o[mi][t];
+      continue;
+    }
+    const int m = r / G, h = hk * G + r - m * G;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + 4 * lg;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const u32x2_t w{E::pack2(o[mi][t][0] * inv, o[mi][t][1] * inv), E::pack2(o[mi][t][2] * inv, o[mi][t][3] * inv)};
+      if (out8) {
+        *reinterpret_cast<u32x2_t*>(op + 16 * t) = w;
+      } else {
+        op[16 * t] = (uint16_t)w.x; op[16 * t + 1] = (uint16_t)(w.x >> 16);
+        op[16 * t + 2] = (uint16_t)w.y; op[16 * t + 3] = (uint16_t)(w.y >> 16);
+      }
+    }
+  }
+}
+
+// Rows of a workgroup and key ranges of a chunk: 256 rows where they fill the chip, fewer below, and where 64 rows leave part of it idle, the keys in ranges.
+struct PromptForm { int rows, ranges; };
+static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
+  const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
+  const auto groups = [&](int bm) { return (list + bm - 1) / bm * pairs; };
+  if (groups(256) * 2 >= cu * 3) return {256, 1};
+  if (groups(128) >= cu) return {128, 1};
+  const int64_t n = groups(64);
+  if (n * 2 > cu) return {64, 1};
+  return {64, (int)max((int64_t)1, min((2 * cu + n - 1) / n, (int64_t)(S + 4 * kTile - 1) / (4 * kTile)))};
+}
+size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
+  const PromptForm f = prompt_form(B, M, H, Hk, S);
+  return f.ranges > 1 ? Kv8Parts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
+}
+
+template <int DT, int DH, int MI, int NW>
+static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+  constexpr size_t lds = 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
+  static bool granted = lds <= 65536;
+  if (!granted) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) { set_last_error("%s: cannot reserve %zu bytes of LDS: %s", fn, lds, hipGetErrorString(e)); return kErrLaunch; }
+    granted = true;
+  }
+  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * NW - 1) / (16 * MI * NW) * a.B * a.c.Hk;
+  if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
+  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, NW>), dim3((unsigned)groups, ranges), dim3(NW * kWave), lds, st, a, ranges, scratch);
+  if (ranges > 1) launch_join<DT, DH>(a, ranges, false, scratch, st);
+  return kOk;
+}
+template <int DT, int DH>
+static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
+  if (f.rows == 256) return prompt_launch<DT, DH, 2, 8>(fn, a, f.ranges, scratch, st);
+  if (f.rows == 128) return prompt_launch<DT, DH, 2, 4>(fn, a, f.ranges, scratch, st);
+  return prompt_launch<DT, DH, 1, 4>(fn, a, f.ranges, scratch, st);
+}
+int launch_kv8_prompt(const char* fn, const Kv8AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
+  const PromptForm f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);
+  const size_t need = kv8_prompt_scratch_bytes(a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.c.S);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
+    set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, f.ranges, need);
+    return kErrWorkspace;
+  }
+  const int rc = a.dt == 1 ? (a.c.Dh == 128 ? prompt_launch_rows<1, 128>(fn, a, f, scratch, st) : prompt_launch_rows<1, 64>(fn, a, f, scratch, st))
+                           : (a.c.Dh == 128 ? prompt_launch_rows<0, 128>(fn, a, f, scratch, st) : prompt_launch_rows<0, 64>(fn, a, f, scratch, st));
+  if (rc != kOk) return rc;
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
   return kOk;

@@ -1099,8 +1099,11 @@ def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block,
         raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on {dev}")
     if B == 0:
         return out
+    lib = _lib.load()
+    nbytes = lib.fsvd_attn_prefill_kv8_scratch_bytes(B, M, H, c.Hk, Dh, c.S)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None       # of this call and stream
     with _on(dev):
-        rc = _lib.load().fsvd_attn_prefill_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pos, n, _ptr(cos), _ptr(sin), rope_len, out.data_ptr(),
-                                               out.stride(0), out.stride(1), out.stride(2), B, M, H, softmax_scale or 0.0, code, _stream())
+        rc = lib.fsvd_attn_prefill_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pos, n, _ptr(cos), _ptr(sin), rope_len, out.data_ptr(),
+                                       out.stride(0), out.stride(1), out.stride(2), _ptr(scratch), nbytes, B, M, H, softmax_scale or 0.0, code, _stream())
     _lib.check("fsvd_attn_prefill_kv8", rc)
     return out

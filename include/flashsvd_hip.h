@@ -221,10 +221,11 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
 
 /* Causal attention of a chunk of a prompt over a cache in 8 bits that holds the chunk's own rows already: q [B, M, H, Dh], row m of sequence b stands
  * at position q_pos0[b] + m (rotated there with cos / sin, NULL: q comes rotated) and sees the keys up to that.  Rows m >= rows[b] (NULL: M) of out
- * [B, M, H, Dh] are left as they were.  Softmax scale 1 / sqrt(Dh) when scale <= 0. */
+ * [B, M, H, Dh] are left as they were.  Softmax scale 1 / sqrt(Dh) when scale <= 0.  scratch as for fsvd_attn_decode_kv8. */
+size_t fsvd_attn_prefill_kv8_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S);
 int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
-                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, int B, int M, int H,
-                          float scale, int dtype, void* stream);
+                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
+                          size_t scratch_bytes, int B, int M, int H, float scale, int dtype, void* stream);
 
 
 

@@ -120,7 +120,7 @@ def test_refusals_of_the_c_abi():
     assert append(cache(), T=0) == 0                      # nothing to write
     decode = lambda H=2, out=p, v=None, c=cache(): lib.fsvd_attn_decode_kv8(c, p, 128, 64, p if v else None, 64, 64, None, 64, 64, p, 0, None, None, 0, out, 128, 64, None, 0, 1, H, 0, 0.0, 0, None)      # noqa: E731
     assert decode(H=3) == -1 and decode(out=None) == -4 and decode(v=True) == -4 and decode(c=cache(Dh=32)) == -1
-    chunk = lambda H=2, M=1, q=p: lib.fsvd_attn_prefill_kv8(cache(), q, 128, 128, 64, p, None, None, None, 0, p, 128, 128, 64, 1, M, H, 0.0, 0, None)      # noqa: E731
+    chunk = lambda H=2, M=1, q=p: lib.fsvd_attn_prefill_kv8(cache(), q, 128, 128, 64, p, None, None, None, 0, p, 128, 128, 64, None, 0, 1, M, H, 0.0, 0, None)      # noqa: E731
     assert chunk(H=3) == -1 and chunk(M=-1) == -1 and chunk(q=None) == -4 and chunk(M=0) == 0
     draw = lambda x=p, B=1, V=8, dt=0: lib.fsvd_sample_token(x, 8, p, p, 1, None, 1.0, None, 0, None, 1.0, None, 0.0, None, B, V, dt, None)      # noqa: E731
     assert draw(x=None) == -4 and draw(B=0) == -1 and draw(V=0) == -1 and draw(V=(1 << 24) + 1) == -1 and draw(dt=2) == -3 and draw(x=p + 1) == -2
