@@ -11,7 +11,7 @@
 namespace fsvd {
 
 constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / kWave, kDrawRow = 1 << 24;
-constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64;      // two 16-bit counts a word; bins of one wave's look
+constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64;      // a word counts a negative value (low half) and a positive one; bins of one wave's look
 constexpr int kMostExtra = kDrawRow / 32768;
 
 struct SampleArgs {
@@ -24,49 +24,60 @@ struct SampleArgs {
   int V;
 };
 
-// patterns as whole numbers in the order of their values, NaN above everything, the two zeros equal; and back
-template <int DT>
-__device__ __forceinline__ uint32_t draw_key(uint32_t p) {
-  constexpr uint32_t kInf = DT == 1 ? 0x7c00u : 0x7f80u;
-  const uint32_t mag = p & 0x7fffu;
-  if (mag > kInf) return 0xffffu;                       // above the key of the infinity
-  if (mag == 0) return 0x8000u;
-  return (p & 0x8000u) ? 0x7fffu - mag : 0x8000u + mag;
+// 16-bit patterns as unsigned numbers in the order of their values, two to a word: a negative pattern inverted, a positive one above all of them.  -0 comes
+// out next below +0 (its count is moved there), a NaN beyond the infinity of its sign.
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+constexpr uint32_t kMinusZero = 0x7fffu, kZero = 0x8000u;
+__device__ __forceinline__ uint32_t order_pair(uint32_t w) {
+  const i16x2_t p = __builtin_bit_cast(i16x2_t, w);
+  return __builtin_bit_cast(uint32_t, (i16x2_t)(p ^ ((p >> 15) | (short)0x8000)));
 }
 template <int DT>
-__device__ __forceinline__ float key_value(uint32_t k) {
-  return E16<DT>::val(k >= 0x8000u ? k - 0x8000u : 0xffffu - k);          // 0x7fff - k is the magnitude, the sign bit above it
-}
+__device__ __forceinline__ float key_value(uint32_t k) { return E16<DT>::val(k >= kZero ? k - kZero : 0xffffu - k); }
 
-template <class T>
-__device__ __forceinline__ T wave_scan(T v, int lane) {                   // inclusive, towards higher lanes
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const T x = __shfl_up(v, o);
-    if (lane >= o) v += x;
-  }
-  return v;
+// running sums over the lanes of a wave (each lane with all before it), by register moves
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) { return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
+  return v + __builtin_bit_cast(double, u32x2_t{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, ROWS, 0xf, false),
+                                                (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, ROWS, 0xf, false)});
 }
 template <class T>
-__device__ __forceinline__ T wave_total(T v) {
+__device__ __forceinline__ T wave_scan(T v) {
+  v = dpp_add<0x111, 0xf>(v);      // row_shr 1, 2, 4, 8, then the last lane of a row into the next rows
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);
+  return dpp_add<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ double lane_value(double v, int l) {
+  const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
+  return __builtin_bit_cast(double, u32x2_t{(uint32_t)__builtin_amdgcn_readlane(w.x, l), (uint32_t)__builtin_amdgcn_readlane(w.y, l)});
+}
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
   return v;
 }
 
-template <int DT>
+// R: 16-byte pieces of the row that a thread keeps in registers; 0: longer rows, read once for each pass.
+template <int DT, int R>
 __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a) {
-  constexpr uint32_t kInf = DT == 1 ? 0x7c00u : 0x7f80u, kLowest = 0x7fffu - kInf + 1, kHighest = 0x8000u + kInf - 1;     // keys of the finite values
+  constexpr uint32_t kInf = DT == 1 ? 0x7c00u : 0x7f80u, kNegInf = kMinusZero - kInf, kLowest = kNegInf + 1, kHighest = kZero + kInf - 1;
   extern __shared__ __align__(16) uint32_t hist[];                       // [kHistWords]
-  __shared__ double seg_mass[kSegs], wave_mass[kDrawWaves], at_mass;
-  __shared__ uint32_t seg_count[kSegs], wave_count[kDrawWaves], wave_most[kDrawWaves], wave_kept[kDrawWaves], at_seg, at_count, rank_key, rank_in, rank_n;
+  __shared__ double seg_mass[kSegs], group_mass[kDrawWaves];             // from the largest values down
+  __shared__ uint32_t seg_count[kSegs], group_count[kDrawWaves], wave_a[kDrawWaves], wave_b[kDrawWaves], wave_kept[kDrawWaves], drawn_key, drawn_rank;
   __shared__ uint16_t extra[kMostExtra];                                  // keys that hold 32768 more than their bin says, once for each
   __shared__ uint32_t n_extra;
-  __shared__ double rank_mass;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint16_t* row = a.logits + (int64_t)b * a.ld;
-  const int V = a.V, pieces = (V + 7) >> 3;
-  // eight logits; behind the row's end stands -inf, which is never counted
+  const int V = a.V, pieces = (V + 7) >> 3, rounds = R > 0 ? R : (pieces + kDrawThreads - 1) / kDrawThreads;
+  // eight logits as ordered numbers; behind the row's end stands -inf, which is never counted
   const auto fetch = [&](int c) {
     if (c * 8 + 8 <= V) return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(row + (int64_t)c * 8));
     uint32_t w[4];
@@ -77,211 +88,246 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
     }
     return u32x4_t{w[0], w[1], w[2], w[3]};
   };
-  const auto each = [&](u32x4_t v, auto f) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const auto ordered = [](u32x4_t v) { return u32x4_t{order_pair(v.x), order_pair(v.y), order_pair(v.z), order_pair(v.w)}; };
+  u32x4_t held[R > 0 ? R : 1];
+  if constexpr (R > 0) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f(draw_key<DT>((w[e >> 1] >> (16 * (e & 1))) & 0xffffu), e);
+    for (int r = 0; r < R; ++r) held[r] = fetch(r * kDrawThreads + tid);
+  }
+  const auto all_pieces = [&](auto f) {                                   // f(round, piece)
+    if constexpr (R > 0) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) f(r, held[r]);
+    } else {
+      for (int r = 0; r < rounds; ++r) f(r, ordered(fetch(r * kDrawThreads + tid)));
+    }
   };
-
-  // the largest
-  uint32_t most = 0;
-  for (int c = tid; c < pieces; c += kDrawThreads) each(fetch(c), [&](uint32_t k, int) { most = max(most, k); });
-#pragma unroll
-  for (int o = 32; o; o >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
-  if (lane == 0) wave_most[wave] = most;
-  for (int i = tid; i < kHistWords; i += kDrawThreads) hist[i] = 0;
+  for (int i = tid; i < kHistWords / 4; i += kDrawThreads) reinterpret_cast<u32x4_t*>(hist)[i] = u32x4_t{0u, 0u, 0u, 0u};
+  for (int i = tid; i < kSegs; i += kDrawThreads) { seg_mass[i] = 0.; seg_count[i] = 0; }
   if (tid == 0) n_extra = 0;
-  __syncthreads();
+  if constexpr (R > 0) {
 #pragma unroll
-  for (int i = 0; i < kDrawWaves; ++i) most = max(most, wave_most[i]);
+    for (int r = 0; r < R; ++r) held[r] = ordered(held[r]);
+  }
+
+  // the largest, and the smallest: a NaN lies beyond the infinity of its sign
+  u16x2_t up = {0, 0}, down = {0xffff, 0xffff};
+  all_pieces([&](int, u32x4_t v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = v[i];                          // a bit cast of an element of a vector would take the first one
+      up = __builtin_elementwise_max(up, __builtin_bit_cast(u16x2_t, w));
+      down = __builtin_elementwise_min(down, __builtin_bit_cast(u16x2_t, w));
+    }
+  });
+  {
+    const uint32_t x = wave_most(max((uint32_t)up.x, (uint32_t)up.y)), y = wave_most(0xffffu - min((uint32_t)down.x, (uint32_t)down.y));
+    if (lane == 0) { wave_a[wave] = x; wave_b[wave] = y; }
+  }
+  __syncthreads();
+  uint32_t most = 0, deep = 0;
+#pragma unroll
+  for (int i = 0; i < kDrawWaves; ++i) { most = max(most, wave_a[i]); deep = max(deep, wave_b[i]); }
+  const bool nan = most > kHighest + 1 || 0xffffu - deep < kNegInf;
+  if (most == kMinusZero) most = kZero;
 
   const double temp = a.temperatures ? (double)a.temperatures[b] : a.temperature;
   uint32_t key = most, rank = 0;                        // the token: this occurrence of this key
-  if (temp > 0. && most >= kLowest && most <= kHighest) {
-    const double top_p = a.top_ps ? (double)a.top_ps[b] : a.top_p, min_p = a.min_ps ? (double)a.min_ps[b] : a.min_p;
+  if (temp > 0. && !nan && most >= kLowest && most <= kHighest) {
+    const double top_p = a.top_ps ? (double)a.top_ps[b] : a.top_p, min_p = a.min_ps ? (double)a.min_ps[b] : a.min_p, u = (double)a.uniforms[b];
     const int top_k = a.top_ks ? a.top_ks[b] : a.top_k;
-    const float high = key_value<DT>(most);
+    const double high = (double)key_value<DT>(most);
     // what is below e^-80 of the largest changes no sum of 64 bits and is not counted
-    const double floor_ = (double)high - 80. * temp;
+    const double floor_ = high - 80. * temp;
     uint32_t least = kLowest;
-    if (floor_ > (double)key_value<DT>(kLowest)) least = max(kLowest, draw_key<DT>(E16<DT>::bits((float)floor_)));
-    const auto count_up = [&](int c) {
-      each(fetch(c), [&](uint32_t k, int) { if (k >= least) atomicAdd(&hist[k >> 1], 1u << (16 * (k & 1))); });
+    if (floor_ > (double)key_value<DT>(kLowest)) least = max(kLowest, order_pair(E16<DT>::bits((float)floor_)) & 0xffffu);
+    uint32_t mine = 0;                                  // counted by this thread
+    const auto count_up = [&](u32x4_t v) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t k = h ? v[i] >> 16 : v[i] & 0xffffu;
+          const bool in = k >= least;
+          if (in) atomicAdd(&hist[k & 0x7fffu], k >> 15 ? 0x10000u : 1u);
+          if (R == 0 || R > 8) mine += in;
+        }
     };
-    uint32_t mine = 0;
-    for (int c = tid; c < pieces; c += kDrawThreads) {
-      count_up(c);
-      each(fetch(c), [&](uint32_t k, int) { mine += k >= least; });
+    all_pieces([&](int, u32x4_t v) { count_up(v); });
+    if (R == 0 || R > 8) {
+      mine = wave_scan(mine);
+      if (lane == 63) wave_a[wave] = mine;
     }
+    __syncthreads();
     const auto bin = [&](uint32_t k) {
-      uint32_t n = (hist[k >> 1] >> (16 * (k & 1))) & 0xffffu;
+      uint32_t n = (hist[k & 0x7fffu] >> (k >> 15 ? 16 : 0)) & 0xffffu;
       for (uint32_t i = 0; i < n_extra; ++i) n += extra[i] == k ? 32768u : 0u;
       return n;
     };
-    const auto weight = [&](uint32_t k) { return exp(((double)key_value<DT>(k) - (double)high) / temp); };
-    mine = wave_total(mine);
-    uint32_t counted = 0, in_all = 0;
-    for (int round = 0; round < 2; ++round) {
+    const auto merged = [&](uint32_t k) { return k == kMinusZero ? 0u : k == kZero ? bin(kZero) + bin(kMinusZero) : bin(k); };
+    const auto weight = [&](uint32_t k) { return exp(((double)key_value<DT>(k) - high) / temp); };
+    if (R == 0 || R > 8) {
+      // A 16-bit count runs over where more than 65535 logits are equal, and all of them come to less then than there are.  The row is counted again in
+      // steps that cannot, and after each what exceeds 32767 is set aside.
+      uint32_t there = 0, sum = 0, counted = 0;
+      for (int i = tid; i < kHistWords; i += kDrawThreads) sum += (hist[i] & 0xffffu) + (hist[i] >> 16);
+      sum = lane_value(wave_scan(sum), 63);
+      if (lane == 0) wave_b[wave] = sum;
       __syncthreads();
-      for (int s = tid; s < kSegs; s += kDrawThreads) { seg_mass[s] = 0.; seg_count[s] = 0; }
-      if (lane == 0) wave_count[wave] = mine;
-      __syncthreads();
-      uint32_t kept = 0;
-      for (int s = (int)(least / kSegBins) + wave; s <= (int)(most / kSegBins); s += kDrawWaves) {
-        const uint32_t k = s * kSegBins + lane, n = k <= most ? bin(k) : 0;
-        if (!__any(n != 0)) continue;
-        const double w = n ? weight(k) : 0.;
-        const double m = wave_total(n * w);
-        const uint32_t c = wave_total(n);
-        kept += w >= min_p ? n : 0;
-        if (lane == 0) { seg_mass[s] = m; seg_count[s] = c; }
-      }
-      kept = wave_total(kept);
-      if (lane == 0) wave_kept[wave] = kept;
-      __syncthreads();
-      counted = 0;
-      in_all = 0;
-      for (int i = 0; i < kDrawWaves; ++i) counted += wave_count[i];
-      uint32_t c = wave_total(seg_count[tid]);
-      __syncthreads();
-      if (lane == 0) wave_most[wave] = c;
-      __syncthreads();
-      for (int i = 0; i < kDrawWaves; ++i) in_all += wave_most[i];
-      if (in_all == counted) break;
-      // A 16-bit count has run over (more than 65535 equal logits): the row is counted again in steps that cannot, and after each what exceeds 32767 is
-      // set aside.
-      __syncthreads();
-      for (int i = tid; i < kHistWords; i += kDrawThreads) hist[i] = 0;
-      for (int c0 = 0; c0 < pieces; c0 += 4095) {
-        __syncthreads();
-        for (int c = c0 + tid; c < min(c0 + 4095, pieces); c += kDrawThreads) count_up(c);
-        __syncthreads();
-        for (int i = tid; i < kHistWords; i += kDrawThreads) {
-          const uint32_t w = hist[i];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (w & (0x8000u << (16 * h))) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)(2 * i + h);
-          hist[i] = w & 0x7fff7fffu;
+      for (int i = 0; i < kDrawWaves; ++i) { there += wave_b[i]; counted += wave_a[i]; }
+      if (there != counted) {
+        for (int i = tid; i < kHistWords; i += kDrawThreads) hist[i] = 0;
+        for (int c0 = 0; c0 < pieces; c0 += 4095) {
+          __syncthreads();
+          for (int c = c0 + tid; c < min(c0 + 4095, pieces); c += kDrawThreads) count_up(ordered(fetch(c)));
+          __syncthreads();
+          for (int i = tid; i < kHistWords; i += kDrawThreads) {
+            const uint32_t w = hist[i];
+            if (w & 0x8000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)i;
+            if (w & 0x80000000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)(i + 0x8000);
+            hist[i] = w & 0x7fff7fffu;
+          }
         }
+        __syncthreads();
       }
     }
-    // running sums over the segments, from the largest values down: thread t has segment kSegs - 1 - t
-    const int seg = kSegs - 1 - tid;
-    double mass = seg_mass[seg];
-    uint32_t count = seg_count[seg];
-    const double own_mass = mass;
-    const uint32_t own_count = count;
-    mass = wave_scan(mass, lane);
-    count = wave_scan(count, lane);
-    if (lane == 63) { wave_mass[wave] = mass; wave_count[wave] = count; }
+    // sums over segments of 64 keys
+    uint32_t kept = 0;
+    for (int s = (int)(least / kSegBins) + wave; s <= (int)(most / kSegBins); s += kDrawWaves) {
+      const uint32_t k = s * kSegBins + lane, n = merged(k);
+      if (!__any(n != 0)) continue;
+      const double w = n ? weight(k) : 0.;
+      const double m = wave_scan(n * w);
+      const uint32_t c = wave_scan(n);
+      kept += w >= min_p ? n : 0;
+      if (lane == 63) { seg_mass[kSegs - 1 - s] = m; seg_count[kSegs - 1 - s] = c; }
+    }
+    kept = wave_scan(kept);
+    if (lane == 63) wave_kept[wave] = kept;
     __syncthreads();
-    double mass0 = 0., all = 0.;
-    uint32_t count0 = 0;
-    for (int i = 0; i < kDrawWaves; ++i) {
-      if (i < wave) { mass0 += wave_mass[i]; count0 += wave_count[i]; }
-      all += wave_mass[i];
+    // running sums of groups of 64 segments, a wave each
+    const double gm = wave_scan(seg_mass[tid]);
+    const uint32_t gc = wave_scan(seg_count[tid]);
+    seg_mass[tid] = gm;
+    seg_count[tid] = gc;
+    if (lane == 63) { group_mass[wave] = gm; group_count[wave] = gc; }
+    __syncthreads();
+    if (wave == 0) {
+      double run_m = 0., to_m = 0.;                     // lane i: up to group i
+      uint32_t run_c = 0, to_c = 0, likely = 0;
+#pragma unroll
+      for (int i = 0; i < kDrawWaves; ++i) {
+        run_m += group_mass[i];
+        run_c += group_count[i];
+        likely += wave_kept[i];
+        if (lane == i) { to_m = run_m; to_c = run_c; }
+      }
+      // The n-th of the order, where n is the smallest with C_n > target (by_mass) or given: its key, how many of its key are up to it, n and C_n.  Where
+      // rounding leaves no C above the target, the last that there is.
+      uint32_t at_key = 0, at_rank = 0, at_n = 0;
+      double at_mass = 0.;
+      const auto locate = [&](bool by_mass, double target, uint32_t n) {
+        const auto first = [&](bool in, double m, uint32_t c, uint32_t before) {
+          const uint64_t hit = __ballot(in && (by_mass ? m > target : c >= n)), some = __ballot(in && c > before);
+          return hit ? __builtin_ctzll(hit) : some ? 63 - __builtin_clzll(some) : 0;
+        };
+        const auto shifted = [&](uint32_t c) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x138, 0xf, 0xf, false); };      // from the lane before
+        const int g = first(lane < kDrawWaves, to_m, to_c, shifted(to_c));
+        const double m0 = g ? lane_value(to_m, g - 1) : 0.;
+        const uint32_t c0 = g ? lane_value(to_c, g - 1) : 0;
+        const double ms = m0 + seg_mass[g * kWave + lane];
+        const uint32_t cs = c0 + seg_count[g * kWave + lane], cp = shifted(cs);
+        const int t = first(true, ms, cs, lane ? cp : c0);
+        const double m1 = t ? lane_value(ms, t - 1) : m0;
+        const uint32_t c1 = t ? lane_value(cs, t - 1) : c0;
+        const uint32_t k = (kSegs - 1 - (g * kWave + t)) * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(k) : 0;
+        const double w = c ? weight(k) : 0., m = c * w, mk = m1 + wave_scan(m);
+        const uint32_t ck = c1 + wave_scan(c);
+        const bool found = __any(c && (by_mass ? mk > target : ck >= n));
+        const int l = first(c != 0, mk, ck, ck - c);
+        uint32_t j = c;
+        if (found) j = by_mass ? (uint32_t)fmin(fmax(floor((target - (mk - m)) / w), 0.) + 1., (double)c) : n - (ck - c);
+        at_key = lane_value(k, l);
+        at_rank = lane_value(j, l);
+        at_n = lane_value(ck - c + j, l);
+        at_mass = lane_value(mk - m + j * w, l);
+      };
+      uint32_t keep = top_k > 0 && (uint32_t)top_k < run_c ? (uint32_t)top_k : run_c;
+      double z = run_m;
+      if (keep < run_c) { locate(false, 0., keep); z = at_mass; }
+      uint32_t n = keep;
+      if (top_p < 1.) { locate(true, top_p * z, 0); n = min(n, at_n); }
+      if (min_p > 0.) n = min(n, likely);
+      n = max(n, 1u);
+      if (n < run_c) { if (n != at_n) locate(false, 0., n); z = at_mass; }
+      locate(true, u * z, 0);
+      if (at_n > n) locate(false, 0., n);
+      if (lane == 0) { drawn_key = at_key; drawn_rank = at_rank - 1; }
     }
-    mass += mass0;
-    count += count0;
-    // The n-th of the order, where n is the smallest with C_n > target (by_mass) or given: its key, how many of its key are up to it, n and C_n
-    const auto locate = [&](bool by_mass, double target, uint32_t n) {
-      __syncthreads();
-      const bool here = by_mass ? mass > target && mass - own_mass <= target : count >= n && count - own_count < n;
-      if (tid == 0) at_seg = 0xffffffffu;
-      __syncthreads();
-      if (here && own_count) atomicMin(&at_seg, (uint32_t)tid);           // rounding may leave two neighbours, or none
-      __syncthreads();
-      uint32_t t = at_seg;
-      __syncthreads();
-      if (t == 0xffffffffu) {                                            // none: the last that has any
-        if (tid == 0) at_seg = 0;
-        __syncthreads();
-        if (own_count) atomicMax(&at_seg, (uint32_t)tid);
-        __syncthreads();
-        t = at_seg;
-      }
-      if ((uint32_t)tid == t) { at_mass = mass - own_mass; at_count = count - own_count; }
-      __syncthreads();
-      if (wave == 0) {
-        const uint32_t k = (kSegs - 1 - t) * kSegBins + kSegBins - 1 - lane, c = k <= most && k >= least ? bin(k) : 0;
-        const double w = c ? weight(k) : 0., m = c * w;
-        const double ms = at_mass + wave_scan(m, lane);
-        const uint32_t cs = at_count + wave_scan(c, lane);
-        const uint64_t hit = __ballot(c && (by_mass ? ms > target : cs >= n)), some = __ballot(c != 0);
-        const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
-        if (lane == l) {
-          uint32_t j = c;
-          const double before = ms - m;
-          if (hit) j = by_mass ? (uint32_t)fmin(fmax(floor((target - before) / w), 0.) + 1., (double)c) : n - (cs - c);
-          rank_key = k;
-          rank_in = j;
-          rank_n = cs - c + j;
-          rank_mass = before + j * w;
-        }
-      }
-      __syncthreads();
-    };
-    uint32_t keep = top_k > 0 && (uint32_t)top_k < in_all ? (uint32_t)top_k : in_all;
-    double z = all;
-    if (keep < in_all) { locate(false, 0., keep); z = rank_mass; }
-    uint32_t n = keep;
-    if (top_p < 1.) { locate(true, top_p * z, 0); n = min(n, rank_n); }
-    uint32_t likely = 0;
-    for (int i = 0; i < kDrawWaves; ++i) likely += wave_kept[i];
-    if (min_p > 0.) n = min(n, likely);
-    n = max(n, 1u);
-    if (n < in_all) { locate(false, 0., n); z = rank_mass; }
-    locate(true, (double)a.uniforms[b] * z, 0);
-    if (rank_n > n) locate(false, 0., n);
-    key = rank_key;
-    rank = rank_in - 1;
+    __syncthreads();
+    key = drawn_key;
+    rank = drawn_rank;
   }
 
   // that occurrence, by index: how many a wave has in each of its pieces, then the piece, then the element
   __syncthreads();
-  const int rounds = (pieces + kDrawThreads - 1) / kDrawThreads;
-  for (int r = 0; r < rounds; ++r) {
-    const int c = r * kDrawThreads + tid;
+  const uint32_t lo = nan ? kHighest + 2 : key == kZero ? kMinusZero : key, span = nan ? 0xffffu - (kHighest + 2) + kNegInf : key == kZero ? 1 : 0;
+  const auto hits = [&](u32x4_t v, auto f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (((v[i] - lo) & 0xffffu) <= span) f(2 * i);
+      if ((((v[i] >> 16) - lo) & 0xffffu) <= span) f(2 * i + 1);
+    }
+  };
+  all_pieces([&](int r, u32x4_t v) {
     uint32_t n = 0;
-    if (c < pieces) each(fetch(c), [&](uint32_t k, int) { n += k == key; });
-    n = wave_total(n);
-    if (lane == 0) hist[r * kDrawWaves + wave] = n;
-  }
+    hits(v, [&](int) { ++n; });
+    n = wave_scan(n);
+    if (lane == 63) hist[r * kDrawWaves + wave] = n;
+  });
   __syncthreads();
   if (wave != 0) return;
   uint32_t before = 0;
   for (int i0 = 0; i0 < rounds * kDrawWaves; i0 += kWave) {
-    const uint32_t n = i0 + lane < rounds * kDrawWaves ? hist[i0 + lane] : 0, s = before + wave_scan(n, lane);
+    const uint32_t n = i0 + lane < rounds * kDrawWaves ? hist[i0 + lane] : 0, s = before + wave_scan(n);
     const uint64_t hit = __ballot(s > rank);
-    if (hit == 0) { before = __shfl(s, 63); continue; }
+    if (hit == 0) { before = lane_value(s, 63); continue; }
     const int l = __builtin_ctzll(hit), c = (i0 + l) * kWave + lane;
-    before = __shfl(s - n, l);
-    const u32x4_t v = fetch(min(c, pieces - 1));
+    before = lane_value(s - n, l);
+    const u32x4_t v = ordered(fetch(c));
     uint32_t m = 0;
-    if (c < pieces) each(v, [&](uint32_t k, int) { m += k == key; });
-    uint32_t at = before + wave_scan(m, lane) - m;
-    if (c < pieces && at <= rank && rank < at + m) {
-      each(v, [&](uint32_t k, int e) {
-        if (k == key) { if (at == rank) a.tokens[(int64_t)b * a.ldt] = c * 8 + e; ++at; }
-      });
+    hits(v, [&](int) { ++m; });
+    uint32_t at = before + wave_scan(m) - m;
+    if (at <= rank && rank < at + m) {
+      hits(v, [&](int e) { if (at++ == rank) a.tokens[(int64_t)b * a.ldt] = (int64_t)c * 8 + e; });
       if (a.positions) a.positions[b] += 1;
     }
     return;
   }
 }
 
-template <int DT>
+template <int DT, int R>
 static int launch_sample(const char* fn, const SampleArgs& a, int B, hipStream_t st) {
   static bool granted = false;
   if (!granted) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sample_token_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, kHistWords * 4);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sample_token_kernel<DT, R>), hipFuncAttributeMaxDynamicSharedMemorySize, kHistWords * 4);
     if (e != hipSuccess) { set_last_error("%s: cannot reserve %d bytes of LDS: %s", fn, kHistWords * 4, hipGetErrorString(e)); return kErrLaunch; }
     granted = true;
   }
-  hipLaunchKernelGGL(sample_token_kernel<DT>, dim3(B), dim3(kDrawThreads), kHistWords * 4, st, a);
+  hipLaunchKernelGGL((sample_token_kernel<DT, R>), dim3(B), dim3(kDrawThreads), kHistWords * 4, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
   return kOk;
+}
+
+template <int DT>
+static int launch_sample_row(const char* fn, const SampleArgs& a, int B, hipStream_t st) {
+  constexpr int kRound = kDrawThreads * 8;
+  if (a.V <= 2 * kRound) return launch_sample<DT, 2>(fn, a, B, st);
+  if (a.V <= 4 * kRound) return launch_sample<DT, 4>(fn, a, B, st);
+  if (a.V < 8 * kRound) return launch_sample<DT, 8>(fn, a, B, st);       // at most 65535: no count can run over
+  if (a.V <= 16 * kRound) return launch_sample<DT, 16>(fn, a, B, st);
+  return launch_sample<DT, 0>(fn, a, B, st);
 }
 
 }  // namespace fsvd
@@ -298,5 +344,5 @@ extern "C" int fsvd_sample_token(const void* logits, int64_t ld, const float* un
   if ((reinterpret_cast<uintptr_t>(logits) & 1) != 0) { set_last_error("%s: logits must be 2-byte aligned", fn); return kErrBadAlign; }
   const SampleArgs a{static_cast<const uint16_t*>(logits), ld, uniforms, tokens, ldt, positions, temperature, top_p, min_p, top_k,
                      temperatures, top_ps, min_ps, top_ks, V};
-  return dtype == 1 ? launch_sample<1>(fn, a, B, static_cast<hipStream_t>(stream)) : launch_sample<0>(fn, a, B, static_cast<hipStream_t>(stream));
+  return dtype == 1 ? launch_sample_row<1>(fn, a, B, static_cast<hipStream_t>(stream)) : launch_sample_row<0>(fn, a, B, static_cast<hipStream_t>(stream));
 }
