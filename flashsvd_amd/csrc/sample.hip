@@ -11,7 +11,7 @@
 namespace fsvd {
 
 constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / kWave, kDrawRow = 1 << 24;
-constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64;      // a word counts a negative value (low half) and a positive one; bins of one wave's look
+constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64;      // two 16-bit counts a word; keys of a segment
 constexpr int kMostExtra = kDrawRow / 32768;
 
 struct SampleArgs {
@@ -26,6 +26,7 @@ struct SampleArgs {
 
 // 16-bit patterns as unsigned numbers in the order of their values, two to a word: a negative pattern inverted, a positive one above all of them.  -0 comes
 // out next below +0 (its count is moved there), a NaN beyond the infinity of its sign.
+typedef double f64x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 constexpr uint32_t kMinusZero = 0x7fffu, kZero = 0x8000u;
@@ -58,6 +59,17 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int l) { return __bui
 __device__ __forceinline__ double lane_value(double v, int l) {
   const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
   return __builtin_bit_cast(double, u32x2_t{(uint32_t)__builtin_amdgcn_readlane(w.x, l), (uint32_t)__builtin_amdgcn_readlane(w.y, l)});
+}
+// e^x for -746 < x <= 0, to a few 2^-53: x = n ln 2 + r, the series of e^r to r^13 (|r| <= 0.347: the next term is 4e-18)
+__device__ __forceinline__ double exp_below(double x) {
+  const double n = rint(x * 1.4426950408889634074);
+  double r = fma(n, -6.93147180369123816490e-01, x);      // ln 2 in two parts, the first of 32 bits
+  r = fma(n, -1.90821492927058770002e-10, r);
+  double y = 1. / 6227020800.;
+#pragma unroll
+  for (const double c : {1. / 479001600., 1. / 39916800., 1. / 3628800., 1. / 362880., 1. / 40320., 1. / 5040., 1. / 720., 1. / 120., 1. / 24., 1. / 6., .5, 1., 1.})
+    y = fma(y, r, c);
+  return ldexp(y, (int)n);
 }
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
 #pragma unroll
@@ -143,15 +155,24 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
     if (floor_ > (double)key_value<DT>(kLowest)) least = max(kLowest, order_pair(E16<DT>::bits((float)floor_)) & 0xffffu);
     uint32_t mine = 0;                                  // counted by this thread
     const auto count_up = [&](u32x4_t v) {
+      u16x2_t low = {0xffff, 0xffff};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = v[i];
+        low = __builtin_elementwise_min(low, __builtin_bit_cast(u16x2_t, w));
+      }
+      const auto add = [&](uint32_t k) { atomicAdd(&hist[k >> 1], 1u + (k & 1u) * 0xffffu); };
+      if (__all(min((uint32_t)low.x, (uint32_t)low.y) >= least)) {        // nothing of the wave's pieces is left out
+        mine += 8;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t k = h ? v[i] >> 16 : v[i] & 0xffffu;
-          const bool in = k >= least;
-          if (in) atomicAdd(&hist[k & 0x7fffu], k >> 15 ? 0x10000u : 1u);
-          if (R == 0 || R > 8) mine += in;
+        for (int i = 0; i < 4; ++i) { add(v[i] & 0xffffu); add(v[i] >> 16); }
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t w = e < 4 ? (e < 2 ? v[0] : v[1]) : (e < 6 ? v[2] : v[3]), k = e & 1 ? w >> 16 : w & 0xffffu;
+          if (k >= least) { add(k); ++mine; }
         }
+      }
     };
     all_pieces([&](int, u32x4_t v) { count_up(v); });
     if (R == 0 || R > 8) {
@@ -159,18 +180,30 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
       if (lane == 63) wave_a[wave] = mine;
     }
     __syncthreads();
-    const auto bin = [&](uint32_t k) {
-      uint32_t n = (hist[k & 0x7fffu] >> (k >> 15 ? 16 : 0)) & 0xffffu;
-      for (uint32_t i = 0; i < n_extra; ++i) n += extra[i] == k ? 32768u : 0u;
+    constexpr bool kMayRunOver = R == 0 || R > 8;        // rows of more than 65535
+    uint32_t extras = 0;
+    const auto counts = [&](uint32_t k, uint32_t n) {     // of key k whose bin holds n
+      for (uint32_t i = 0; kMayRunOver && i < extras; ++i) n += extra[i] == k ? 32768u : 0u;
       return n;
     };
-    const auto merged = [&](uint32_t k) { return k == kMinusZero ? 0u : k == kZero ? bin(kZero) + bin(kMinusZero) : bin(k); };
-    const auto weight = [&](uint32_t k) { return exp(((double)key_value<DT>(k) - high) / temp); };
-    if (R == 0 || R > 8) {
+    const auto bin = [&](uint32_t k) { return counts(k, (hist[k >> 1] >> (16 * (k & 1))) & 0xffffu); };
+    // the count of -0 belongs to 0
+    const auto merged = [&](uint32_t s, uint32_t k, uint32_t n) {
+      if (s == kMinusZero / kSegBins) return k == kMinusZero ? 0u : n;
+      if (s == kZero / kSegBins) return k == kZero ? n + bin(kMinusZero) : n;
+      return n;
+    };
+    const double per = 1. / fmax(temp, 1e-280);
+    const auto weight = [&](uint32_t k) { return exp_below(((double)key_value<DT>(k) - high) * per); };
+    if (kMayRunOver) {
       // A 16-bit count runs over where more than 65535 logits are equal, and all of them come to less then than there are.  The row is counted again in
       // steps that cannot, and after each what exceeds 32767 is set aside.
       uint32_t there = 0, sum = 0, counted = 0;
-      for (int i = tid; i < kHistWords; i += kDrawThreads) sum += (hist[i] & 0xffffu) + (hist[i] >> 16);
+#pragma unroll
+      for (int i = 0; i < kHistWords / 4; i += kDrawThreads) {
+        const u32x4_t w = reinterpret_cast<const u32x4_t*>(hist)[i + tid];
+        sum += (w.x & 0xffffu) + (w.x >> 16) + (w.y & 0xffffu) + (w.y >> 16) + (w.z & 0xffffu) + (w.z >> 16) + (w.w & 0xffffu) + (w.w >> 16);
+      }
       sum = lane_value(wave_scan(sum), 63);
       if (lane == 0) wave_b[wave] = sum;
       __syncthreads();
@@ -183,24 +216,57 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
           __syncthreads();
           for (int i = tid; i < kHistWords; i += kDrawThreads) {
             const uint32_t w = hist[i];
-            if (w & 0x8000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)i;
-            if (w & 0x80000000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)(i + 0x8000);
+            if (w & 0x8000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)(2 * i);
+            if (w & 0x80000000u) extra[atomicAdd(&n_extra, 1u)] = (uint16_t)(2 * i + 1);
             hist[i] = w & 0x7fff7fffu;
           }
         }
         __syncthreads();
+        extras = n_extra;
       }
     }
-    // sums over segments of 64 keys
+    // Sums over segments of 64 keys.  A wave asks for the counts of every 16th of 256 segments at once (those that hold something stand side by side, so
+    // the waves share them); the sums over the lanes come from the matrix cores, in 64 bits: a segment's masses are the rows, and a column of ones puts
+    // their sums into the segment's own column.
     uint32_t kept = 0;
-    for (int s = (int)(least / kSegBins) + wave; s <= (int)(most / kSegBins); s += kDrawWaves) {
-      const uint32_t k = s * kSegBins + lane, n = merged(k);
-      if (!__any(n != 0)) continue;
-      const double w = n ? weight(k) : 0.;
-      const double m = wave_scan(n * w);
-      const uint32_t c = wave_scan(n);
-      kept += w >= min_p ? n : 0;
-      if (lane == 63) { seg_mass[kSegs - 1 - s] = m; seg_count[kSegs - 1 - s] = c; }
+    constexpr int kAsk = 16, kStep = kAsk * kDrawWaves;
+    const int last_seg = (int)(most / kSegBins);
+    for (int s0 = (int)(least / kSegBins) / kStep * kStep + wave; s0 <= last_seg; s0 += kStep) {
+      const uint16_t* counts16 = reinterpret_cast<const uint16_t*>(hist) + s0 * kSegBins + lane;
+      constexpr int kNext = kDrawWaves * kSegBins;
+      uint32_t raw[kAsk];
+#pragma unroll
+      for (int i = 0; i < kAsk; ++i) raw[i] = counts16[i * kNext];
+      uint32_t some = 0;                                  // segments with a count, and those whose counts are not all in their bins
+#pragma unroll
+      for (int i = 0; i < kAsk; ++i) some |= __any(raw[i] != 0) ? 1u << i : 0u;
+      const auto also = [&](int s) {
+        s -= s0;
+        if (s >= 0 && s < kStep && s % kDrawWaves == 0) some |= 1u << (s / kDrawWaves);
+      };
+      also(kZero / kSegBins);
+      for (uint32_t i = 0; kMayRunOver && i < extras; ++i) also(extra[i] / kSegBins);
+      f64x4_t mass = {0., 0., 0., 0.};
+      f32x4_t count = {0.f, 0.f, 0.f, 0.f};               // whole numbers up to 2^24
+      while (some) {
+        const int i = __builtin_ctz(some), s = s0 + i * kDrawWaves;
+        some &= some - 1;
+        const uint32_t k = s * kSegBins + lane, n = merged(s, k, counts(k, counts16[i * kNext]));
+        const bool own = (lane & 15) == i;
+        const double w = n ? weight(k) : 0.;
+        if (min_p > 0.) kept += w >= min_p ? n : 0;
+        mass = __builtin_amdgcn_mfma_f64_16x16x4f64(n * w, own ? 1. : 0., mass, 0, 0, 0);
+        count = __builtin_amdgcn_mfma_f32_16x16x4f32((float)n, own ? 1.f : 0.f, count, 0, 0, 0);
+      }
+      double m = (mass[0] + mass[1]) + (mass[2] + mass[3]);
+      float c = (count[0] + count[1]) + (count[2] + count[3]);
+      m += __shfl_xor(m, 16); c += __shfl_xor(c, 16);
+      m += __shfl_xor(m, 32); c += __shfl_xor(c, 32);
+      if (lane < kAsk) {
+        const int at = kSegs - 1 - (s0 + lane * kDrawWaves);
+        seg_mass[at] = m;
+        seg_count[at] = (uint32_t)c;
+      }
     }
     kept = wave_scan(kept);
     if (lane == 63) wave_kept[wave] = kept;
@@ -240,7 +306,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
         const int t = first(true, ms, cs, lane ? cp : c0);
         const double m1 = t ? lane_value(ms, t - 1) : m0;
         const uint32_t c1 = t ? lane_value(cs, t - 1) : c0;
-        const uint32_t k = (kSegs - 1 - (g * kWave + t)) * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(k) : 0;
+        const uint32_t k = (kSegs - 1 - (g * kWave + t)) * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(k / kSegBins, k, bin(k)) : 0;
         const double w = c ? weight(k) : 0., m = c * w, mk = m1 + wave_scan(m);
         const uint32_t ck = c1 + wave_scan(c);
         const bool found = __any(c && (by_mass ? mk > target : ck >= n));
@@ -279,11 +345,24 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
       if ((((v[i] >> 16) - lo) & 0xffffu) <= span) f(2 * i + 1);
     }
   };
+  const u16x2_t first = {(unsigned short)lo, (unsigned short)lo};
+  uint32_t sums = 0;                                      // of up to three rounds, ten bits each (512 of a wave at most)
   all_pieces([&](int r, u32x4_t v) {
     uint32_t n = 0;
-    hits(v, [&](int) { ++n; });
-    n = wave_scan(n);
-    if (lane == 63) hist[r * kDrawWaves + wave] = n;
+    u16x2_t least_off = {0xffff, 0xffff};                 // distance from the key, two elements to an instruction
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = v[i];
+      least_off = __builtin_elementwise_min(least_off, (u16x2_t)(__builtin_bit_cast(u16x2_t, w) - first));
+    }
+    if (__any(min((uint32_t)least_off.x, (uint32_t)least_off.y) <= span)) hits(v, [&](int) { ++n; });
+    sums |= n << (10 * (r % 3));
+    if (r % 3 == 2 || r == rounds - 1) {
+      sums = wave_scan(sums);
+      if (lane == 63)
+        for (int q = r - r % 3; q <= r; ++q) hist[q * kDrawWaves + wave] = (sums >> (10 * (q % 3))) & 0x3ffu;
+      sums = 0;
+    }
   });
   __syncthreads();
   if (wave != 0) return;
