@@ -3,73 +3,117 @@
 
 namespace fsvd {
 
-// One workgroup for a block of one kv head of one sequence, keys and values one after the other.  The scale of a block comes from the new rows, and
-// where rows stand before the first of them, from the scale that those have: they are moved to the larger one.
-template <int DT>
+// Rows of a call in registers: a lane holds dimensions d .. d + 7 and the eight half a head further of a row (the pairs of the rotation), LPR lanes a row; a
+// workgroup has P times 256 / LPR rows of the keys or the values of one kv head, that is one block or, of small blocks, several.  The scale of a block is the
+// largest magnitude of its new rows, and where rows stand before the first of them, that of the scale that those have: they are moved to the larger one.
+template <int DT, int DH, int P>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   typedef E16<DT> E;
-  const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x;
-  const int p = a.positions[b], rows = a.rows ? min(a.rows[b], a.T) : a.T;
+  constexpr int HALF = DH / 2, LPR = HALF / 8;
+  __shared__ float red[4];
+  const int part = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, tid = threadIdx.x;
+  const int p = a.positions[b], rows = a.rows ? min(a.rows[b], a.T) : a.T, block = a.c.block;
   const int64_t end = (int64_t)p + rows;
   const int first = max(p, 0), last = (int)(end < a.c.S ? end : a.c.S);          // the rows that are written
-  const int64_t blk = (int64_t)(first / a.c.block) + blockIdx.x, r0 = blk * a.c.block;
-  if (first >= last || r0 >= last) return;
-  const int n0 = (int)(r0 > first ? r0 : first), n1 = (int)(r0 + a.c.block < last ? r0 + a.c.block : last);
-  const int half = a.c.Dh >> 1;
-  __shared__ float red[4];
-  for (int part = 0; part < 2; ++part) {
-    const uint16_t* src = part ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h;
-    const int64_t st = part ? a.sv_t : a.sk_t;
-    uint8_t* dst = static_cast<uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
-    float* scale = (part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + blk * a.c.ss_n + hk * a.c.ss_h;
-    const auto pair = [&](int row, int d, float& x0, float& x1) {
-      const uint16_t* s = src + (int64_t)(row - p) * st;
-      x0 = E::val(s[d]); x1 = E::val(s[d + half]);
-      if (part == 0 && a.cos) {
-        const int64_t tp = min(row, a.rope_len - 1);
-        const float c = E::val(a.cos[tp * half + d]), n = E::val(a.sin[tp * half + d]);
-        const float y0 = x0 * c - x1 * n, y1 = x0 * n + x1 * c;
-        x0 = y0; x1 = y1;
-      }
-    };
-    float amax = 0.f;
-    for (int i = tid; i < (n1 - n0) * half; i += 256) {
-      float x0, x1;
-      pair(n0 + i / half, i % half, x0, x1);
-      amax = fmaxf(amax, fmaxf(finite_mag(x0), finite_mag(x1)));
+  const int64_t row0 = (int64_t)(first / block) * block + (int64_t)blockIdx.y * (P * 256 / LPR);
+  if (first >= last || row0 >= last) return;
+  const uint16_t* src = part ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h;
+  const int64_t st = part ? a.sv_t : a.sk_t;
+  uint8_t* dst = static_cast<uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  float* scales = (part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const int d = tid % LPR * 8;
+  const bool turn = part == 0 && a.cos != nullptr;
+  u32x4_t lo[P], hi[P], cw[P], sw[P];
+  int64_t row[P];
+  bool in[P];
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    row[i] = row0 + (i * 256 + tid) / LPR;
+    in[i] = row[i] >= first && row[i] < last;
+    const int64_t r = in[i] ? row[i] : first;
+    const uint16_t* x = src + (r - p) * st + d;
+    lo[i] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x));
+    hi[i] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x + HALF));
+    if (turn) {
+      const int64_t tp = (r < a.rope_len ? r : a.rope_len - 1) * HALF + d;
+      cw[i] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.cos + tp));
+      sw[i] = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.sin + tp));
     }
-    amax = wave_max(amax);
-    if ((tid & 63) == 0) red[tid >> 6] = amax;
-    const float old = n0 > r0 ? *scale : 0.f;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float fresh = power_of_two(scale_exponent(amax)), now = fmaxf(old, fresh), inv = 1.f / now;
-    if (n0 > r0 && now > old) {
-      const float move = old * inv;
-      for (int i = tid; i < (int)(n0 - r0) * (a.c.Dh / 4); i += 256) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(dst + (r0 + i / (a.c.Dh / 4)) * a.c.sc_s) + i % (a.c.Dh / 4);
-        const auto lo = codes_lo(*w), hi = codes_hi(*w);
-        *w = codes_of(lo[0] * move, lo[1] * move, hi[0] * move, hi[1] * move);
-      }
-    }
-    for (int i = tid; i < (n1 - n0) * half; i += 256) {
-      float x0, x1;
-      const int row = n0 + i / half, d = i % half;
-      pair(row, d, x0, x1);
-      const uint32_t w = codes_of(in_code_range(x0 * inv), in_code_range(x1 * inv), 0.f, 0.f);
-      dst[row * a.c.sc_s + d] = (uint8_t)w;
-      dst[row * a.c.sc_s + d + half] = (uint8_t)(w >> 8);
-    }
-    __syncthreads();
-    if (tid == 0) *scale = now;
   }
+  const int64_t blk = row[0] / block;                     // of this thread's rows: one block, whatever P (more than one pass means a larger block)
+  const bool open = blk * block < first;                  // rows stand before the first new one
+  const float old = open ? scales[blk * a.c.ss_n] : 0.f;
+  float x0[P][8], x1[P][8], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t wl = lo[i][e >> 1], wh = hi[i][e >> 1];
+      float u = e & 1 ? E::hi(wl) : E::lo(wl), v = e & 1 ? E::hi(wh) : E::lo(wh);
+      if (turn) {
+        const uint32_t wc = cw[i][e >> 1], ws = sw[i][e >> 1];
+        const float c = e & 1 ? E::hi(wc) : E::lo(wc), s = e & 1 ? E::hi(ws) : E::lo(ws), y0 = u * c - v * s, y1 = u * s + v * c;
+        u = y0; v = y1;
+      }
+      x0[i][e] = u; x1[i][e] = v;
+      amax = fmaxf(amax, in[i] ? fmaxf(finite_mag(u), finite_mag(v)) : 0.f);
+    }
+  amax = wave_max(amax);
+  if ((tid & 63) == 0) red[tid >> 6] = amax;
+  __syncthreads();
+  const int waves = min(4, block * LPR / kWave), w0 = (tid >> 6) / waves * waves;        // that hold the block
+  for (int i = 0; i < waves; ++i) amax = fmaxf(amax, red[w0 + i]);
+  if (blk * block >= last || (blk + 1) * block <= first) return;
+  const float now = fmaxf(old, power_of_two(scale_exponent(amax))), inv = 1.f / now;
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    uint8_t* y = dst + row[i] * a.c.sc_s + d;
+    if (in[i]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { x0[i][e] = in_code_range(x0[i][e] * inv); x1[i][e] = in_code_range(x1[i][e] * inv); }
+      *reinterpret_cast<u32x2_t*>(y) = u32x2_t{codes_of(x0[i][0], x0[i][1], x0[i][2], x0[i][3]), codes_of(x0[i][4], x0[i][5], x0[i][6], x0[i][7])};
+      *reinterpret_cast<u32x2_t*>(y + HALF) = u32x2_t{codes_of(x1[i][0], x1[i][1], x1[i][2], x1[i][3]), codes_of(x1[i][4], x1[i][5], x1[i][6], x1[i][7])};
+    } else if (row[i] < first && now > old) {
+      u32x2_t held[2] = {*reinterpret_cast<const u32x2_t*>(y), *reinterpret_cast<const u32x2_t*>(y + HALF)};
+      const float move = old * inv;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) held[h][q] = moved(held[h][q], move);
+      *reinterpret_cast<u32x2_t*>(y) = held[0];
+      *reinterpret_cast<u32x2_t*>(y + HALF) = held[1];
+    }
+  }
+  if (row[0] == blk * block && d == 0) scales[blk * a.c.ss_n] = now;
 }
 
+// One row for each sequence: one wave for a kv head, its lanes 0 to 15 with the key's dimensions, 16 to 31 with the value's.
+template <int DT, int DH>
+__global__ __launch_bounds__(kWave) void kv8_append_one_kernel(Kv8AppendArgs a) {
+  const int b = blockIdx.x / a.c.Hk, hk = blockIdx.x % a.c.Hk, pos = a.positions[b];
+  if (pos < 0 || pos >= a.c.S || (a.rows && a.rows[b] <= 0)) return;
+  append_row<DT, DH>(a.c, a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin, a.rope_len, b, hk, pos,
+                     threadIdx.x);
+}
+
+template <int DT, int DH>
+static void append_form(const Kv8AppendArgs& a, hipStream_t st) {
+  if (a.T == 1) {
+    hipLaunchKernelGGL((kv8_append_one_kernel<DT, DH>), dim3((unsigned)(a.B * a.c.Hk)), dim3(kWave), 0, st, a);
+    return;
+  }
+  constexpr int LPR = DH / 16;
+  const int passes = max(1, a.c.block * LPR / 256), rows = passes * 256 / LPR;       // rows of a workgroup: whole blocks
+  const dim3 grid(2 * a.c.Hk, (unsigned)((a.T + a.c.block - 1 + (int64_t)rows - 1) / rows), a.B);
+  if (passes == 1) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 1>), grid, dim3(256), 0, st, a);
+  else if (passes == 2) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 2>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 4>), grid, dim3(256), 0, st, a);
+}
 int launch_kv8_append(const char* fn, const Kv8AppendArgs& a, hipStream_t st) {
   if (a.T == 0) return kOk;
-  const dim3 grid((a.T + a.c.block - 2) / a.c.block + 1, a.c.Hk, a.B);
-  if (a.dt == 1) hipLaunchKernelGGL(kv8_append_kernel<1>, grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL(kv8_append_kernel<0>, grid, dim3(256), 0, st, a);
+  if ((int64_t)a.B * a.c.Hk > 0x7fffffff || a.T > (1 << 20)) { set_last_error("%s: %d rows of %d heads for %d sequences", fn, a.T, a.c.Hk, a.B); return kErrBadShape; }
+  if (a.dt == 1) a.c.Dh == 128 ? append_form<1, 128>(a, st) : append_form<1, 64>(a, st);
+  else a.c.Dh == 128 ? append_form<0, 128>(a, st) : append_form<0, 64>(a, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
   return kOk;
@@ -137,13 +181,9 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
     set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, ranges, need);
     return kErrWorkspace;
   }
-  if (k_new) {
-    const Kv8AppendArgs n{*cache, in16(k_new), sk_b, 0, sk_h, in16(v_new), sv_b, 0, sv_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, B, 1, dtype};
-    if (const int rc = launch_kv8_append(fn, n, st)) return rc;
-    seqlen_add = 1;
-  }
   const Kv8AttnArgs a{*cache, in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
-                      B, 1, H, seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
+                      B, 1, H, k_new ? 1 : seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype,
+                      in16(k_new), sk_b, sk_h, in16(v_new), sv_b, sv_h};
   return launch_kv8_decode(fn, a, ranges, static_cast<float*>(scratch), st);
 }
 

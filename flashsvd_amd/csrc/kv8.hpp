@@ -63,7 +63,66 @@ struct Kv8AttnArgs {
   int key_add;                                         // query row m sees the keys below positions[b] + m + key_add
   float scale;
   int dt;
+  // decode: the rows [B, Hk, Dh] that the call appends at positions[b], or null
+  const uint16_t* k_new = nullptr; int64_t sk_b = 0, sk_h = 0;
+  const uint16_t* v_new = nullptr; int64_t sv_b = 0, sv_h = 0;
 };
+// four held codes at another scale, `move` times their own
+__device__ __forceinline__ uint32_t moved(uint32_t w, float move) {
+  const f32x2_t lo = codes_lo(w), hi = codes_hi(w);
+  return codes_of(lo[0] * move, lo[1] * move, hi[0] * move, hi[1] * move);
+}
+
+// One row of a kv head (k, v [Dh]) into its place at position pos, 0 <= pos < S, by one wave: lanes 0 to 15 hold the key, 16 to 31 the value, each lane DH / 32
+// dimensions of either half of the head.  The rows of the block before it are moved where the row needs a larger scale.
+template <int DT, int DH>
+__device__ __forceinline__ void append_row(const fsvd_kv8_cache& c, const uint16_t* k, const uint16_t* v, const uint16_t* cos, const uint16_t* sin, int rope_len,
+                                           int b, int hk, int pos, int lane) {
+  typedef E16<DT> E;
+  constexpr int HALF = DH / 2, N = HALF / 16;
+  const int part = (lane >> 4) & 1, d = (lane & 15) * N, at = pos % c.block;
+  const int64_t base = b * c.sc_b + hk * c.sc_h;
+  uint8_t* codes = static_cast<uint8_t*>(part ? c.v : c.k) + base;
+  float* scale = (part ? c.v_scale : c.k_scale) + b * c.ss_b + (int64_t)(pos / c.block) * c.ss_n + hk * c.ss_h;
+  const uint16_t* x = (part ? v : k) + d;
+  const float old = at > 0 ? *scale : 0.f;
+  float x0[N], x1[N], amax = 0.f;
+  const bool turn = part == 0 && cos != nullptr;
+  const int64_t tp = (int64_t)min(pos, rope_len - 1) * HALF + d;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    x0[e] = E::val(x[e]); x1[e] = E::val(x[e + HALF]);
+    if (turn) {
+      const float cc = E::val(cos[tp + e]), s = E::val(sin[tp + e]), y0 = x0[e] * cc - x1[e] * s, y1 = x0[e] * s + x1[e] * cc;
+      x0[e] = y0; x1[e] = y1;
+    }
+    amax = fmaxf(amax, fmaxf(finite_mag(x0[e]), finite_mag(x1[e])));
+  }
+  amax = row16_max(amax);
+  const float now = fmaxf(old, power_of_two(scale_exponent(amax))), inv = 1.f / now;
+  if (lane < 32) {
+    uint8_t* y = codes + (int64_t)pos * c.sc_s + d;
+#pragma unroll
+    for (int e = 0; e < N; ++e) { x0[e] = in_code_range(x0[e] * inv); x1[e] = in_code_range(x1[e] * inv); }
+    if constexpr (N == 4) {
+      *reinterpret_cast<uint32_t*>(y) = codes_of(x0[0], x0[1], x0[2], x0[3]);
+      *reinterpret_cast<uint32_t*>(y + HALF) = codes_of(x1[0], x1[1], x1[2], x1[3]);
+    } else {
+      *reinterpret_cast<uint16_t*>(y) = (uint16_t)codes_of(x0[0], x0[1], 0.f, 0.f);
+      *reinterpret_cast<uint16_t*>(y + HALF) = (uint16_t)codes_of(x1[0], x1[1], 0.f, 0.f);
+    }
+    if ((lane & 15) == 0) *scale = now;
+  }
+  // rare: lanes 0 to 31 go over the rows before it, each word by word of its part
+  if (__any(at > 0 && now > old) && lane < 32 && now > old) {
+    const float move = old * inv;
+    for (int i = lane & 15; i < at * (DH / 4); i += 16) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(codes + (int64_t)(pos - at + i / (DH / 4)) * c.sc_s) + i % (DH / 4);
+      *w = moved(*w, move);
+    }
+  }
+}
+
 int check_kv8_cache(const char* fn, const fsvd_kv8_cache* c);
 int launch_kv8_append(const char* fn, const Kv8AppendArgs& a, hipStream_t st);
 // ranges of keys that a sequence may be cut into, and the scratch for their partial results

@@ -170,7 +170,20 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
     for (int t = 0; t < 2; ++t) vs[t] = vsp[(int64_t)(min(c0 + 16 * t, k1 - 1) >> shift) * a.c.ss_n];
   };
   int c0 = k0 + wave * kDecStep;
-  if (c0 < k1) { fetch_k(c0); fetch_v(c0); }
+  // The new row is the last key.  Ranges are whole blocks, so this workgroup alone reads the block that the row may change: it writes the row before it reads
+  // that block, with what stands in front of it on its way.
+  const bool appends = a.k_new != nullptr && pos >= k0 && pos < k1;
+  const bool late = appends && c0 + kDecStep > (pos >> shift << shift);
+  if (c0 < k1 && !late) { fetch_k(c0); fetch_v(c0); }
+  if (appends) {
+    if (wave == 0) {
+      append_row<DT, DH>(a.c, a.k_new + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v_new + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin,
+                         a.rope_len, b, hk, pos, lane);
+      wait_stores_acked();
+    }
+    __syncthreads();
+    if (c0 < k1 && late) { fetch_k(c0); fetch_v(c0); }
+  }
 
   // q: element e of piece (j, h) is dimension 64 j + 16 g + 8 h + e of query n, rotated in fp32 and rounded to the type of the products
   frag_t qf[ST];
@@ -305,7 +318,13 @@ static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStr
   hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave), 0, st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, true, scratch, st);
 }
-int launch_kv8_decode(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float* scratch, hipStream_t st) {
+  Kv8AttnArgs a = args;
+  if (a.k_new != nullptr && a.H / a.c.Hk > kDecGroup) {    // several workgroups read the keys of a kv head: the rows in a launch before them
+    const Kv8AppendArgs n{a.c, a.k_new, a.sk_b, 0, a.sk_h, a.v_new, a.sv_b, 0, a.sv_h, a.positions, nullptr, a.cos, a.sin, a.rope_len, a.B, 1, a.dt};
+    if (const int rc = launch_kv8_append(fn, n, st)) return rc;
+    a.k_new = nullptr;
+  }
   if ((int64_t)a.B * a.H * ranges > 0x7fffffff) { set_last_error("%s: %d sequences of %d heads in %d ranges", fn, a.B, a.H, ranges); return kErrBadShape; }
   if (a.dt == 1) a.c.Dh == 128 ? decode_form<1, 128>(a, ranges, scratch, st) : decode_form<1, 64>(a, ranges, scratch, st);
   else a.c.Dh == 128 ? decode_form<0, 128>(a, ranges, scratch, st) : decode_form<0, 64>(a, ranges, scratch, st);

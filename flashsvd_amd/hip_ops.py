@@ -13,7 +13,7 @@ import torch
 from . import _lib
 from .torch_ops import ops as _OPS
 
-_BF16 = torch.bfloat16
+_BF16, _F8, _F32, _I32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
 
 
 def _stream() -> int:
@@ -49,9 +49,9 @@ def _elem(t: torch.Tensor, name: str):
 _HERE = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
-    """The context of a call whose tensors are on ``device``: nothing where that is the current one."""
-    return _HERE if device.index == torch._C._cuda_getDevice() else torch.cuda.device(device)
+def _on(index: int):
+    """The context of a call whose tensors are on device ``index``: nothing where that is the current one."""
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -546,19 +546,18 @@ def _sample_token_impl(logits, uniforms, tokens, positions, temperature, top_k, 
     _need(tokens, "tokens", dtype=torch.long)
     if tokens.numel() != B or tokens.shape[0] != B:
         raise ValueError(f"tokens must hold {B} rows of one id, got {tuple(tokens.shape)}")
-    dev = logits.device
-    if tokens.device != dev:
-        raise ValueError(f"logits and tokens must be on one device, got {dev} and {tokens.device}")
-    for t, nm, dt in ((uniforms, "uniforms", torch.float32), (positions, "positions", torch.int32), (temperatures, "temperature", torch.float32),
-                      (top_ks, "top_k", torch.int32), (top_ps, "top_p", torch.float32), (min_ps, "min_p", torch.float32)):
-        if t is None:
-            continue
-        if t.dtype != dt or t.shape != (B,) or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{nm} must be a contiguous {dt} [{B}] tensor on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    dev = logits.get_device()
+    if tokens.get_device() != dev:
+        raise ValueError(f"logits and tokens must be on one device, got {logits.device} and {tokens.device}")
+    ptrs = []
+    for t, nm, dt in ((uniforms, "uniforms", _F32), (positions, "positions", _I32), (temperatures, "temperature", _F32), (top_ks, "top_k", _I32),
+                      (top_ps, "top_p", _F32), (min_ps, "min_p", _F32)):
+        if t is not None and (t.dtype is not dt or tuple(t.shape) != (B,) or t.get_device() != dev or not t.is_contiguous()):
+            raise ValueError(f"{nm} must be a contiguous {dt} [{B}] tensor on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        ptrs.append(None if t is None else t.data_ptr())
     with _on(dev):
-        rc = _lib.load().fsvd_sample_token(logits.data_ptr(), logits.stride(0), uniforms.data_ptr(), tokens.data_ptr(), tokens.stride(0), _ptr(positions),
-                                           temperature, _ptr(temperatures), top_k, _ptr(top_ks), top_p, _ptr(top_ps), min_p, _ptr(min_ps), B, V, code,
-                                           _stream())
+        rc = _lib.load().fsvd_sample_token(logits.data_ptr(), logits.stride(0), ptrs[0], tokens.data_ptr(), tokens.stride(0), ptrs[1], temperature, ptrs[2],
+                                           top_k, ptrs[3], top_p, ptrs[4], min_p, ptrs[5], B, V, code, _stream())
     _lib.check("fsvd_sample_token", rc)
 
 
@@ -982,128 +981,152 @@ def attn_prefill_kv8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return _OPS.attn_prefill_kv8.default(*a) if out is None else _OPS.attn_prefill_kv8.out(*a, out=out)
 
 
-def _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block):
-    """Checks of a cache in 8 bits; its descriptor for the C ABI."""
-    _need(k_cache, "k_cache", dtype=torch.float8_e4m3fn); _need(v_cache, "v_cache", dtype=torch.float8_e4m3fn)
-    _need(k_scale, "k_scale", dtype=torch.float32); _need(v_scale, "v_scale", dtype=torch.float32)
-    shape, strides = k_cache.shape, k_cache.stride()
-    if len(shape) != 4 or shape != v_cache.shape or strides != v_cache.stride() or shape[0] < B or strides[3] != 1:
-        raise ValueError(f"caches must be matching [B>={B}, S, Hk, Dh] tensors with unit inner stride, got {tuple(shape)} / {tuple(v_cache.shape)}")
-    nb, S, Hk, Dh = shape
+def _kv8_cache(B, kc, vc, ks, vs, block):
+    """Checks of a cache in 8 bits; its descriptor for the C ABI.  One pass over what a good call has, in few lookups (a decode step takes it per layer)."""
+    shape, st, ss = kc.shape, kc.stride(), ks.stride()
+    dev = kc.get_device()
+    if not (kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and kc.is_cuda and vc.is_cuda and ks.is_cuda and vs.is_cuda
+            and len(shape) == 4 and vc.shape == shape and vc.stride() == st and shape[0] >= B and st[3] == 1 and vs.shape == ks.shape and vs.stride() == ss
+            and block in (16, 32, 64, 128) and tuple(ks.shape) == (shape[0], -(-shape[1] // block), shape[2])
+            and vc.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
+        _refuse_kv8_cache(B, kc, vc, ks, vs, block)
+    return _lib.Kv8Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], shape[1], shape[2], shape[3], block)
+
+
+def _refuse_kv8_cache(B, kc, vc, ks, vs, block):
+    _need(kc, "k_cache", dtype=_F8); _need(vc, "v_cache", dtype=_F8)
+    _need(ks, "k_scale", dtype=_F32); _need(vs, "v_scale", dtype=_F32)
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride() or kc.shape[0] < B or kc.stride(3) != 1:
+        raise ValueError(f"caches must be matching [B>={B}, S, Hk, Dh] tensors with unit inner stride, got {tuple(kc.shape)} / {tuple(vc.shape)}")
     if block not in (16, 32, 64, 128):
         raise ValueError(f"block must be 16, 32, 64 or 128 tokens, got {block}")
-    want = (nb, -(-S // block), Hk)
-    if k_scale.shape != want or v_scale.shape != want or k_scale.stride() != v_scale.stride():
-        raise ValueError(f"scales must be matching {want} tensors, got {tuple(k_scale.shape)} / {tuple(v_scale.shape)}")
-    dev = k_cache.device
-    if not (dev == v_cache.device == k_scale.device == v_scale.device):
-        raise ValueError("caches and scales must be on one device")
-    return _lib.Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), strides[0], strides[1], strides[2],
-                         *k_scale.stride(), S, Hk, Dh, block)
+    want = (kc.shape[0], -(-kc.shape[1] // block), kc.shape[2])
+    if tuple(ks.shape) != want or ks.shape != vs.shape or ks.stride() != vs.stride():
+        raise ValueError(f"scales must be matching {want} tensors, got {tuple(ks.shape)} / {tuple(vs.shape)}")
+    raise ValueError("caches and scales must be on one device")
 
 
-def _apart(B, k_cache, k_scale) -> None:
-    """Rows that a call writes must not lie in each other: no expanded caches."""
-    if (B > 1 and (k_cache.stride(0) == 0 or k_scale.stride(0) == 0)) or (k_cache.shape[2] > 1 and (k_cache.stride(2) == 0 or k_scale.stride(2) == 0)) \
-            or k_scale.stride(1) == 0 and k_scale.shape[1] > 1:
+def _apart(B, c) -> None:
+    """Rows that a call writes must not lie in each other: no caches expanded over their sequences, blocks or heads."""
+    if (B > 1 and (c.sc_b == 0 or c.ss_b == 0)) or (c.Hk > 1 and (c.sc_h == 0 or c.ss_h == 0)) or (c.ss_n == 0 and c.S > c.block) or (c.sc_s == 0 and c.S > 1):
         raise ValueError("a cache that is written to must not be expanded over its sequences, blocks or heads")
 
 
 def _kv8_vector(t, B, dev, nm):
     if t is None:
         return None
-    _need(t, nm, dtype=torch.int32)
-    if t.numel() != B or not t.is_contiguous() or t.device != dev:
-        raise ValueError(f"{nm} must be a contiguous int32 [{B}] tensor on {dev}, got {tuple(t.shape)} on {t.device}")
+    if t.dtype is not _I32 or t.get_device() != dev or t.numel() != B or not t.is_contiguous():
+        _need(t, nm, dtype=_I32)
+        raise ValueError(f"{nm} must be a contiguous int32 [{B}] tensor on cuda:{dev}, got {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _kv8_rope(cos, sin, Dh, dt, dev):
-    if (cos is None) != (sin is None) or (cos is not None and (cos.device != dev or sin.device != dev)):
-        raise ValueError(f"cos and sin go together, on {dev}")
-    return _rope_tables(cos, sin, Dh, dt)
+    """Addresses and rows of the rotation tables."""
+    if cos is None and sin is None:
+        return None, None, 0
+    if cos is None or sin is None or cos.get_device() != dev or sin.get_device() != dev:
+        raise ValueError(f"cos and sin go together, on cuda:{dev}")
+    shape = cos.shape
+    if not (cos.dtype is dt and sin.dtype is dt and sin.shape == shape and len(shape) == 2 and 2 * shape[1] == Dh and cos.is_contiguous() and sin.is_contiguous()):
+        _need(cos, "cos", dtype=dt); _need(sin, "sin", dtype=dt)
+        raise ValueError(f"cos/sin must be contiguous [len, {Dh // 2}] tables")
+    return cos.data_ptr(), sin.data_ptr(), shape[0]
 
 
 def _kv8_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, block, cos, sin, rows):
     dt, code = _elem(k, "k")
-    _need(v, "v", dtype=dt)
-    B = k.shape[0]
+    shape, st, sv = k.shape, k.stride(), v.stride()
+    B = shape[0]
     c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
-    dev = k_cache.device
-    if k.dim() != 4 or k.shape != v.shape or k.shape[2:] != (c.Hk, c.Dh) or k.stride(3) != 1 or v.stride(3) != 1 or k.device != dev or v.device != dev:
-        raise ValueError(f"k and v must be [B, T, {c.Hk}, {c.Dh}] tensors with unit inner stride on {dev}, got {tuple(k.shape)} / {tuple(v.shape)}")
-    _apart(B, k_cache, k_scale)
-    rope_len = _kv8_rope(cos, sin, c.Dh, dt, dev)
+    dev = k_cache.get_device()
+    if not (v.dtype is dt and len(shape) == 4 and v.shape == shape and shape[2] == c.Hk and shape[3] == c.Dh and st[3] == 1 and sv[3] == 1
+            and k.get_device() == dev and v.get_device() == dev):
+        _need(v, "v", dtype=dt)
+        raise ValueError(f"k and v must be [B, T, {c.Hk}, {c.Dh}] tensors with unit inner stride on cuda:{dev}, got {tuple(shape)} / {tuple(v.shape)}")
+    _apart(B, c)
+    cp, sp, rope_len = _kv8_rope(cos, sin, c.Dh, dt, dev)
     pos, n = _kv8_vector(positions, B, dev, "positions"), _kv8_vector(rows, B, dev, "rows")
     if B == 0:
         return
     with _on(dev):
-        rc = _lib.load().fsvd_kv8_append(c, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), pos, n,
-                                         _ptr(cos), _ptr(sin), rope_len, B, k.shape[1], code, _stream())
-    _lib.check("fsvd_kv8_append", rc)
+        rc = _lib.load().fsvd_kv8_append(c, k.data_ptr(), st[0], st[1], st[2], v.data_ptr(), sv[0], sv[1], sv[2], pos, n, cp, sp, rope_len, B, shape[1], code,
+                                         _stream())
+    if rc:
+        _lib.check("fsvd_kv8_append", rc)
 
 
 def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out):
     dt, code = _elem(q, "q")
-    if q.dim() != 3 or q.stride(2) != 1:
+    sq = q.stride()
+    if len(sq) != 3 or sq[2] != 1:
         raise ValueError(f"q must be [B,H,Dh] with unit inner stride, got {tuple(q.shape)}")
     B, H, Dh = q.shape
     c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
-    dev = k_cache.device
-    if c.Dh != Dh or H % c.Hk or q.device != dev:
-        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {dev}")
-    rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    dev, Hk = k_cache.get_device(), c.Hk
+    if c.Dh != Dh or H % Hk or q.get_device() != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")
+    cp, sp, rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
     lens = _kv8_vector(cache_seqlens, B, dev, "cache_seqlens")
-    sk_b = sk_h = sv_b = sv_h = 0
-    if (k_new is None) != (v_new is None):
+    kp = vp = None
+    sk = sv = (0, 0)
+    if k_new is not None and v_new is not None:
+        sk, sv = k_new.stride(), v_new.stride()
+        new = (B, Hk, Dh)
+        if not (k_new.dtype is dt and v_new.dtype is dt and tuple(k_new.shape) == new and tuple(v_new.shape) == new and sk[2] == 1 and sv[2] == 1
+                and k_new.get_device() == dev and v_new.get_device() == dev):
+            _need(k_new, "k_new", dtype=dt); _need(v_new, "v_new", dtype=dt)
+            raise ValueError(f"k_new/v_new must be [B,Hk,Dh] tensors with unit inner stride on cuda:{dev}, got {tuple(k_new.shape)} / {tuple(v_new.shape)}")
+        _apart(B, c)
+        kp, vp = k_new.data_ptr(), v_new.data_ptr()
+    elif k_new is not None or v_new is not None:
         raise ValueError("k_new and v_new go together")
-    if k_new is not None:
-        _need(k_new, "k_new", dtype=dt); _need(v_new, "v_new", dtype=dt)
-        if k_new.shape != (B, c.Hk, Dh) or v_new.shape != (B, c.Hk, Dh) or k_new.stride(2) != 1 or v_new.stride(2) != 1 or k_new.device != dev \
-                or v_new.device != dev:
-            raise ValueError(f"k_new/v_new must be [B,Hk,Dh] tensors with unit inner stride on {dev}, got {tuple(k_new.shape)} / {tuple(v_new.shape)}")
-        _apart(B, k_cache, k_scale)
-        sk_b, sk_h, sv_b, sv_h = k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1)
     if out is None:
-        out = torch.empty(B, H, Dh, device=dev, dtype=dt)
-    elif out.shape != (B, H, Dh) or out.stride(2) != 1 or out.dtype != dt or out.device != dev:
-        raise ValueError(f"out must be {dt} [B,H,Dh] with unit inner stride on {dev}")
+        out = torch.empty((B, H, Dh), device=q.device, dtype=dt)
+    elif out.shape != q.shape or out.stride(2) != 1 or out.dtype is not dt or out.get_device() != dev:
+        raise ValueError(f"out must be {dt} [B,H,Dh] with unit inner stride on cuda:{dev}")
     if B == 0:
         return out
-    lib = _lib.load()
+    lib, so = _lib.load(), out.stride()
     nsplit = 0 if nsplit is None else nsplit
-    nbytes = lib.fsvd_attn_decode_kv8_scratch_bytes(B, H, c.Hk, Dh, c.S, nsplit)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None       # of this call and stream
+    nbytes, scratch, ptr = lib.fsvd_attn_decode_kv8_scratch_bytes(B, H, Hk, Dh, c.S, nsplit), None, None
+    if nbytes:
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # of this call and stream
+        ptr = scratch.data_ptr()
     with _on(dev):
-        rc = lib.fsvd_attn_decode_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), _ptr(k_new), sk_b, sk_h, _ptr(v_new), sv_b, sv_h, lens, seqlen_add,
-                                      _ptr(cos), _ptr(sin), rope_len, out.data_ptr(), out.stride(0), out.stride(1), _ptr(scratch), nbytes, B, H, nsplit,
-                                      softmax_scale or 0.0, code, _stream())
-    _lib.check("fsvd_attn_decode_kv8", rc)
+        rc = lib.fsvd_attn_decode_kv8(c, q.data_ptr(), sq[0], sq[1], kp, sk[0], sk[1], vp, sv[0], sv[1], lens, seqlen_add, cp, sp, rope_len, out.data_ptr(),
+                                      so[0], so[1], ptr, nbytes, B, H, nsplit, softmax_scale or 0.0, code, _stream())
+    if rc:
+        _lib.check("fsvd_attn_decode_kv8", rc)
     return out
 
 
 def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block, rows, cos, sin, softmax_scale, out):
     dt, code = _elem(q, "q")
-    if q.dim() != 4 or q.stride(3) != 1:
+    sq = q.stride()
+    if len(sq) != 4 or sq[3] != 1:
         raise ValueError(f"q must be [B,M,H,Dh] with unit inner stride, got {tuple(q.shape)}")
     B, M, H, Dh = q.shape
     c = _kv8_cache(B, k_cache, v_cache, k_scale, v_scale, block)
-    dev = k_cache.device
-    if c.Dh != Dh or H % c.Hk or q.device != dev:
-        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {dev}")
-    rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    dev = k_cache.get_device()
+    if c.Dh != Dh or H % c.Hk or q.get_device() != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")
+    cp, sp, rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
     pos, n = _kv8_vector(q_pos0, B, dev, "q_pos0"), _kv8_vector(rows, B, dev, "rows")
     if out is None:
-        out = (torch.empty if rows is None else torch.zeros)(B, M, H, Dh, device=dev, dtype=dt)
-    elif out.shape != (B, M, H, Dh) or out.stride(3) != 1 or out.dtype != dt or out.device != dev:
-        raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on {dev}")
+        out = (torch.empty if rows is None else torch.zeros)((B, M, H, Dh), device=q.device, dtype=dt)
+    elif out.shape != q.shape or out.stride(3) != 1 or out.dtype is not dt or out.get_device() != dev:
+        raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on cuda:{dev}")
     if B == 0:
         return out
-    lib = _lib.load()
-    nbytes = lib.fsvd_attn_prefill_kv8_scratch_bytes(B, M, H, c.Hk, Dh, c.S)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None       # of this call and stream
+    lib, so = _lib.load(), out.stride()
+    nbytes, scratch, ptr = lib.fsvd_attn_prefill_kv8_scratch_bytes(B, M, H, c.Hk, Dh, c.S), None, None
+    if nbytes:
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # of this call and stream
+        ptr = scratch.data_ptr()
     with _on(dev):
-        rc = lib.fsvd_attn_prefill_kv8(c, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), pos, n, _ptr(cos), _ptr(sin), rope_len, out.data_ptr(),
-                                       out.stride(0), out.stride(1), out.stride(2), _ptr(scratch), nbytes, B, M, H, softmax_scale or 0.0, code, _stream())
-    _lib.check("fsvd_attn_prefill_kv8", rc)
+        rc = lib.fsvd_attn_prefill_kv8(c, q.data_ptr(), sq[0], sq[1], sq[2], pos, n, cp, sp, rope_len, out.data_ptr(), so[0], so[1], so[2], ptr, nbytes, B, M, H,
+                                       softmax_scale or 0.0, code, _stream())
+    if rc:
+        _lib.check("fsvd_attn_prefill_kv8", rc)
     return out
