@@ -86,14 +86,21 @@ __device__ __forceinline__ void append_row(const fsvd_kv8_cache& c, const uint16
   float* scale = (part ? c.v_scale : c.k_scale) + b * c.ss_b + (int64_t)(pos / c.block) * c.ss_n + hk * c.ss_h;
   const uint16_t* x = (part ? v : k) + d;
   const float old = at > 0 ? *scale : 0.f;
-  float x0[N], x1[N], amax = 0.f;
+  uint32_t w0[N], w1[N], wc[N], ws[N];                   // everything is asked for at once
   const bool turn = part == 0 && cos != nullptr;
   const int64_t tp = (int64_t)min(pos, rope_len - 1) * HALF + d;
 #pragma unroll
+  for (int e = 0; e < N; ++e) { w0[e] = x[e]; w1[e] = x[e + HALF]; }
+  if (turn) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) { wc[e] = cos[tp + e]; ws[e] = sin[tp + e]; }
+  }
+  float x0[N], x1[N], amax = 0.f;
+#pragma unroll
   for (int e = 0; e < N; ++e) {
-    x0[e] = E::val(x[e]); x1[e] = E::val(x[e + HALF]);
+    x0[e] = E::val(w0[e]); x1[e] = E::val(w1[e]);
     if (turn) {
-      const float cc = E::val(cos[tp + e]), s = E::val(sin[tp + e]), y0 = x0[e] * cc - x1[e] * s, y1 = x0[e] * s + x1[e] * cc;
+      const float c1 = E::val(wc[e]), s1 = E::val(ws[e]), y0 = x0[e] * c1 - x1[e] * s1, y1 = x0[e] * s1 + x1[e] * c1;
       x0[e] = y0; x1[e] = y1;
     }
     amax = fmaxf(amax, fmaxf(finite_mag(x0[e]), finite_mag(x1[e])));

@@ -13,21 +13,18 @@ struct Kv8Parts {
   __device__ __forceinline__ f32x2_t* stats(int64_t row, int s) const { return reinterpret_cast<f32x2_t*>(base + rows * ranges * dh) + row * ranges + s; }
 };
 
-// eight elements x at dimension d of a query row, rotated in fp32 and rounded to the type of the products; d and its partner are half a head apart
-template <class E, int HALF>
-__device__ __forceinline__ u32x4_t rotated(u32x4_t x, const uint16_t* row, const uint16_t* cos, const uint16_t* sin, int d) {
-  const bool up = d >= HALF;
-  const int pair = up ? d - HALF : d + HALF, at = up ? d - HALF : d;
-  const u32x4_t y = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(row + pair));
-  const u32x4_t cw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(cos + at));
-  const u32x4_t sw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(sin + at));
+// eight elements x of a query row in the lower or upper half of the head, rotated with their partners y half a head away, in fp32 and rounded to the type of
+// the products
+template <class E>
+__device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float sl = up ? E::lo(sw[i]) : -E::lo(sw[i]), sh = up ? E::hi(sw[i]) : -E::hi(sw[i]);
-    x[i] = E::pack2(E::lo(x[i]) * E::lo(cw[i]) + E::lo(y[i]) * sl, E::hi(x[i]) * E::hi(cw[i]) + E::hi(y[i]) * sh);
+    const float sl = upper ? E::lo(sin[i]) : -E::lo(sin[i]), sh = upper ? E::hi(sin[i]) : -E::hi(sin[i]);
+    x[i] = E::pack2(E::lo(x[i]) * E::lo(cos[i]) + E::lo(y[i]) * sl, E::hi(x[i]) * E::hi(cos[i]) + E::hi(y[i]) * sh);
   }
   return x;
 }
+__device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 
 constexpr int kMinRange = 256;                            // keys of a decode range, but for the last
 __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
@@ -36,7 +33,7 @@ __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
 }
 
 // The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
-// token, head of the group).
+// token, head of the group).  Nothing that a load needs comes from another load: what it takes is a round trip to memory and its launch.
 template <int DT, int DH, int WPR>
 __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges, bool decode, float* scratch) {
   typedef E16<DT> E;
@@ -44,49 +41,42 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges
   __shared__ float vs[4][DH];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part_of = wave % WPR, G = a.H / a.c.Hk;
   const int64_t rows = (int64_t)a.B * a.M * a.H, row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;
-  const int64_t at = row < rows ? row : rows - 1;
-  const int b = (int)(at / ((int64_t)a.M * a.H)), in = (int)(at - (int64_t)b * a.M * a.H);
-  int m, h, used = ranges;
-  bool live = row < rows;
-  if (decode) {
-    m = 0; h = in;
-    const int keys = max(0, min(a.positions[b] + a.key_add, a.c.S)), per = kv8_range(keys, ranges);
-    used = (keys + per - 1) / per;
-    live = live && per < keys;                             // else written by its only workgroup
-  } else {
-    const int hk = in / (a.M * G), r = in - hk * a.M * G;
-    m = r / G;
-    h = hk * G + r - m * G;
-    live = live && (!a.rows || m < a.rows[b]);
-  }
+  const bool live = row < rows;
+  const int64_t at = live ? row : rows - 1;
   const Kv8Parts part{scratch, rows, ranges, DH};
   float v[D], sum = 0.f, top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < D; ++i) v[i] = 0.f;
-  if (live) {
-    for (int s0 = 0; s0 < used; s0 += kWave) top = fmaxf(top, s0 + lane < used ? (*part.stats(at, s0 + lane))[0] : -INFINITY);
-    top = wave_max(top);
-    for (int s0 = 0; s0 < used; s0 += kWave) {
-      const f32x2_t st = *part.stats(at, min(s0 + lane, used - 1));
-      const float w = s0 + lane < used && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
-      sum += w * st[1];
-      const int n = min(kWave, used - s0);
-      for (int s = part_of; s < n; s += WPR * U) {
-        float x[U][D];
+  if (ranges > kWave)
+    for (int s0 = 0; s0 < ranges; s0 += kWave) top = fmaxf(top, s0 + lane < ranges ? (*part.stats(at, s0 + lane))[0] : -INFINITY);
+  for (int s0 = 0; s0 < ranges; s0 += kWave) {
+    const int n = min(kWave, ranges - s0);
+    const f32x2_t st = *part.stats(at, s0 + min(lane, n - 1));
+    float w = 0.f;
+    for (int s = part_of; s < n; s += WPR * U) {
+      float x[U][D];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
+        for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
+      if (s == part_of) {                                  // the weights, with the first values on their way
+        if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
+        w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
+      }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : 0.f;
+      for (int u = 0; u < U; ++u) {
+        const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : 0.f;
 #pragma unroll
-          for (int i = 0; i < D; ++i) v[i] += f > 0.f ? f * x[u][i] : 0.f;      // a range without a visible key has written no values
-        }
+        for (int i = 0; i < D; ++i) v[i] += f > 0.f ? f * x[u][i] : 0.f;        // a range without keys has written no values
       }
     }
-    sum = wave_sum(sum);
+    if (part_of >= n) {                                    // more waves than ranges: the sum all the same
+      if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
+      w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
+    }
+    sum += w * st[1];
   }
+  sum = wave_sum(sum);
   if (WPR > 1) {
 #pragma unroll
     for (int i = 0; i < D; ++i) vs[wave][lane * D + i] = v[i];
@@ -98,7 +88,9 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges
         for (int w = 1; w < WPR; ++w) v[i] += vs[wave + w][lane * D + i];
     }
   }
-  if (!live || part_of) return;
+  const int b = (int)(at / ((int64_t)a.M * a.H)), in = (int)(at - (int64_t)b * a.M * a.H), hk = in / (a.M * G), r = in - hk * a.M * G;
+  const int m = decode ? 0 : r / G, h = decode ? in : hk * G + r - m * G;
+  if (!live || part_of || (a.rows && m >= a.rows[b])) return;
   uint16_t* o = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + lane * D;
 #pragma unroll
   for (int i = 0; i < D; ++i) o[i] = (uint16_t)E::bits(sum > 0.f ? v[i] / sum : 0.f);
@@ -121,25 +113,33 @@ static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* sc
 constexpr int kDecWaves = 4, kDecStep = 32, kDecGroup = 16;
 
 template <int DT, int DH>
-__global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
+__global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef typename E::frag_t frag_t;
   typedef E16<0>::frag_t pfrag_t;
   constexpr int J = DH / 64, ST = DH / 32, NT = DH / 16, VW = DH / 64;      // 16-byte pieces of a key; products a tile; output tiles; words of a value piece
-  __shared__ float os[kDecWaves][kDecGroup][DH + 4], ms[kDecWaves][kDecGroup], ls[kDecWaves][kDecGroup];
+  extern __shared__ __align__(16) float os[];                               // [kDecWaves][heads of a workgroup][DH + 4]
+  __shared__ float ms[kDecWaves][kDecGroup], ls[kDecWaves][kDecGroup];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   const int G = a.H / a.c.Hk, GG = (G + kDecGroup - 1) / kDecGroup;
-  int id = blockIdx.x;
-  const int s = id % ranges; id /= ranges;
+  // The heads of a sequence, whose ranges are alike, on different XCDs; the last range of every sequence, which may hold the new row, first.
+  const int pairs = a.B * a.c.Hk * GG, turn = blockIdx.x / pairs;
+  int id = blockIdx.x - turn * pairs;
   const int gg = id % GG; id /= GG;
-  const int hk = id % a.c.Hk, b = id / a.c.Hk;
+  const int b = id / a.c.Hk, hk = id - b * a.c.Hk;
   const int pos = a.positions[b], keys = max(0, min(pos + a.key_add, a.c.S));
-  const int per = kv8_range(keys, ranges), k0 = min(s * per, keys), k1 = min(k0 + per, keys);
-  if (k0 >= k1 && s > 0) return;
+  const int per = kv8_range(keys, ranges), used = max(1, (keys + per - 1) / per), s = turn < used ? used - 1 - turn : turn;
+  const int k0 = min(s * per, keys), k1 = min(k0 + per, keys);
   const int h0 = hk * G + gg * kDecGroup, heads = min(kDecGroup, G - gg * kDecGroup);
+  const Kv8Parts part{scratch, (int64_t)a.B * a.H, ranges, DH};
+  if (s >= used) {
+    if (tid < heads) *part.stats((int64_t)b * a.H + h0 + tid, s) = f32x2_t{-INFINITY, 0.f};
+    return;
+  }
 
-  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + g * 16;
-  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h + n * NT;
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint32_t row = (uint32_t)a.c.sc_s;                                  // a step's first row is the wave's, 64 bits; from there on 32 do
   const float* ksp = a.c.k_scale + b * a.c.ss_b + hk * a.c.ss_h;
   const float* vsp = a.c.v_scale + b * a.c.ss_b + hk * a.c.ss_h;
   const int shift = 31 - __builtin_clz(a.c.block);
@@ -149,16 +149,16 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
   const auto fetch_k = [&](int c0) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint8_t* p = kb + (int64_t)min(c0 + 16 * t + n, k1 - 1) * a.c.sc_s;
+      const uint32_t off = (uint32_t)min(16 * t + n, k1 - 1 - c0) * row + 16 * g;
 #pragma unroll
-      for (int j = 0; j < J; ++j) kr[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(p + 64 * j));
+      for (int j = 0; j < J; ++j) kr[t][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + (int64_t)c0 * a.c.sc_s + off + 64 * j));
       ks[t] = ksp[(int64_t)(min(c0 + 16 * t, k1 - 1) >> shift) * a.c.ss_n];
     }
   };
   const auto fetch_v = [&](int c0) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint8_t* p = vb + (int64_t)min(c0 + 16 * (e >> 2) + 4 * g + (e & 3), k1 - 1) * a.c.sc_s;
+      const uint8_t* p = vb + (int64_t)c0 * a.c.sc_s + ((uint32_t)min(16 * (e >> 2) + 4 * g + (e & 3), k1 - 1 - c0) * row + n * NT);
       if constexpr (VW == 2) {
         const u32x2_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t*>(p));
         vr[e][0] = w.x; vr[e][1] = w.y;
@@ -170,35 +170,45 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
     for (int t = 0; t < 2; ++t) vs[t] = vsp[(int64_t)(min(c0 + 16 * t, k1 - 1) >> shift) * a.c.ss_n];
   };
   int c0 = k0 + wave * kDecStep;
-  // The new row is the last key.  Ranges are whole blocks, so this workgroup alone reads the block that the row may change: it writes the row before it reads
-  // that block, with what stands in front of it on its way.
+  // The new row is the last key.  Ranges are whole blocks, so this workgroup alone reads the block that the row may change; one wave writes the row while the
+  // others begin, and the steps that touch its block come behind a barrier.
   const bool appends = a.k_new != nullptr && pos >= k0 && pos < k1;
-  const bool late = appends && c0 + kDecStep > (pos >> shift << shift);
-  if (c0 < k1 && !late) { fetch_k(c0); fetch_v(c0); }
-  if (appends) {
-    if (wave == 0) {
-      append_row<DT, DH>(a.c, a.k_new + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v_new + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin,
-                         a.rope_len, b, hk, pos, lane);
-      wait_stores_acked();
-    }
-    __syncthreads();
-    if (c0 < k1 && late) { fetch_k(c0); fetch_v(c0); }
-  }
+  const int before = appends ? (pos >> shift << shift) - (kDecStep - 1) : k1;
+  if (appends && wave == kDecWaves - 1)
+    append_row<DT, DH>(a.c, a.k_new + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v_new + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin, a.rope_len,
+                       b, hk, pos, lane);
+  if (c0 < before) { fetch_k(c0); fetch_v(c0); }
 
   // q: element e of piece (j, h) is dimension 64 j + 16 g + 8 h + e of query n, rotated in fp32 and rounded to the type of the products
   frag_t qf[ST];
   {
     const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)(h0 + min(n, heads - 1)) * a.sq_h;
     constexpr int HALF = DH / 2;
-    const int64_t tp = a.cos ? (int64_t)min(max(pos, 0), a.rope_len - 1) * HALF : 0;
+    const auto dim = [&](int st) { return 64 * (st >> 1) + 16 * g + 8 * (st & 1); };
+    u32x4_t x[ST], y[2], cw[2], sw[2];
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
-      const int d = 64 * (st >> 1) + 16 * g + 8 * (st & 1);
-      u32x4_t x = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(qp + d));
-      if (a.cos) x = rotated<E, HALF>(x, qp, a.cos + tp, a.sin + tp, d);
-      if (n >= heads) x = u32x4_t{0u, 0u, 0u, 0u};
-      qf[st] = __builtin_bit_cast(frag_t, x);
+    for (int st = 0; st < ST; ++st) x[st] = eight(qp + dim(st));
+    if (a.cos) {
+      const int64_t tp = (int64_t)min(max(pos, 0), a.rope_len - 1) * HALF;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {                       // of 128 dimensions the partner is the lane's own, of 64 another lane has it
+        if constexpr (DH == 64) y[h] = eight(qp + (dim(h) ^ HALF));
+        cw[h] = eight(a.cos + tp + dim(h) % HALF);
+        sw[h] = eight(a.sin + tp + dim(h) % HALF);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (DH == 64) {
+          x[h] = rotated<E>(x[h], y[h], cw[h], sw[h], dim(h) >= HALF);
+        } else {
+          const u32x4_t low = x[h];
+          x[h] = rotated<E>(low, x[h + 2], cw[h], sw[h], false);
+          x[h + 2] = rotated<E>(x[h + 2], low, cw[h], sw[h], true);
+        }
+      }
     }
+#pragma unroll
+    for (int st = 0; st < ST; ++st) qf[st] = __builtin_bit_cast(frag_t, n < heads ? x[st] : u32x4_t{0u, 0u, 0u, 0u});
   }
 
   const float scale = a.scale * 1.4426950408889634f;      // weights are powers of two of the scores' differences
@@ -206,7 +216,8 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
   f32x4_t o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (; c0 < k1; c0 += kDecWaves * kDecStep) {
+  const auto walk = [&](int stop) {
+  for (; c0 < stop; c0 += kDecWaves * kDecStep) {
     const int next = c0 + kDecWaves * kDecStep;
     float x[2][4], f[2];
 #pragma unroll
@@ -226,7 +237,7 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
       for (int i = 0; i < 4; ++i) x[t][i] = acc[i] * by;
       f[t] = vs[t];
     }
-    if (next < k1) fetch_k(next);
+    if (next < stop) fetch_k(next);
     if (c0 + kDecStep > k1) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -269,17 +280,27 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
         o[t + 1] = E16<0>::mfma(__builtin_bit_cast(pfrag_t, v1), hi, o[t + 1]);
         o[t + 1] = E16<0>::mfma(__builtin_bit_cast(pfrag_t, v1), lo, o[t + 1]);
       }
-    if (next < k1) fetch_v(next);
+    if (next < stop) fetch_v(next);
+  }
+  };
+  walk(before);
+  if (appends) {
+    wait_stores_acked();
+    __syncthreads();
+    if (c0 < k1) { fetch_k(c0); fetch_v(c0); }
+    walk(k1);
   }
   // the waves' results through LDS: element i of tile t is dimension NT (4 g + i) + t of query n
   l = column_sum(l);
   if (g == 0) { ms[wave][n] = m; ls[wave][n] = l; }
+  if (n < heads) {
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) os[wave][n][NT * (4 * g + i) + t] = o[t][i];
+      for (int t = 0; t < NT; t += 4)
+        *reinterpret_cast<f32x4_t*>(os + (wave * heads + n) * (DH + 4) + NT * (4 * g + i) + t) = f32x4_t{o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]};
+  }
   __syncthreads();
-  const bool whole = per >= keys;                          // a single range
   for (int e = tid; e < heads * DH; e += kDecWaves * kWave) {
     const int q = e / DH, d = e % DH;
     float top = -INFINITY, sum = 0.f, v = 0.f;
@@ -289,12 +310,11 @@ __global__ __launch_bounds__(kDecWaves * kWave) void kv8_decode_kernel(Kv8AttnAr
     for (int w = 0; w < kDecWaves; ++w) {
       const float f = ms[w][q] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[w][q] - top);
       sum += f * ls[w][q];
-      v += f * os[w][q][d];
+      v += f * os[(w * heads + q) * (DH + 4) + d];
     }
-    if (whole) {
+    if (ranges == 1) {
       a.out[(int64_t)b * a.so_b + (int64_t)(h0 + q) * a.so_h + d] = (uint16_t)E::bits(sum > 0.f ? v / sum : 0.f);
     } else {
-      const Kv8Parts part{scratch, (int64_t)a.B * a.H, ranges, DH};
       const int64_t row = (int64_t)b * a.H + h0 + q;
       part.values(row, s)[d] = v;
       if (d == 0) *part.stats(row, s) = f32x2_t{top, sum};
@@ -315,7 +335,8 @@ size_t kv8_decode_scratch_bytes(int B, int H, int Dh, int ranges) { return range
 template <int DT, int DH>
 static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   const int groups = (a.H / a.c.Hk + kDecGroup - 1) / kDecGroup;
-  hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave), 0, st, a, ranges, scratch);
+  hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave),
+                     kDecWaves * min(a.H / a.c.Hk, kDecGroup) * (DH + 4) * sizeof(float), st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, true, scratch, st);
 }
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float* scratch, hipStream_t st) {
@@ -398,15 +419,23 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
     const int r = min(w0 + 16 * mi + lr, rows - 1), m = r / G, h = hk * G + r - m * G;
     seen[mi] = seen_by(r);
     const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
-    constexpr int HALF = DH / 2;
-    const int64_t tp = a.cos ? (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF : 0;
+    constexpr int HALF = DH / 2, SH = ST / 2;
+    u32x4_t x[ST], cw[SH], sw[SH];
 #pragma unroll
-    for (int st = 0; st < ST; ++st) {
-      const int d = 32 * st + 8 * lg;
-      u32x4_t x = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(qp + d));
-      if (a.cos) x = rotated<E, HALF>(x, qp, a.cos + tp, a.sin + tp, d);
-      qf[mi][st] = __builtin_bit_cast(frag_t, x);
+    for (int st = 0; st < ST; ++st) x[st] = eight(qp + 32 * st + 8 * lg);
+    if (a.cos) {
+      const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lg;
+#pragma unroll
+      for (int st = 0; st < SH; ++st) { cw[st] = eight(a.cos + tp + 32 * st); sw[st] = eight(a.sin + tp + 32 * st); }
+#pragma unroll
+      for (int st = 0; st < SH; ++st) {
+        const u32x4_t low = x[st];
+        x[st] = rotated<E>(low, x[st + SH], cw[st], sw[st], false);
+        x[st + SH] = rotated<E>(x[st + SH], low, cw[st], sw[st], true);
+      }
     }
+#pragma unroll
+    for (int st = 0; st < ST; ++st) qf[mi][st] = __builtin_bit_cast(frag_t, x[st]);
   }
   const float scale = a.scale * 1.4426950408889634f;
   float m_run[MI], l_run[MI];
