@@ -173,17 +173,28 @@ def _manual_llama_decode_step(model, input_ids: torch.Tensor, *, past_key_values
     return SimpleNamespace(logits=logits, past_key_values=past_key_values)
 
 
-def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batch_size: int, device):
+def _draw_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, top_p: float, min_p: float, generator) -> torch.Tensor:
+    """hip_ops.sample_token_ on logits [B, V] with uniform numbers from ``generator``; ids [B, 1]."""
+    from . import hip_ops
+    tokens = torch.empty(logits.shape[0], 1, dtype=torch.long, device=logits.device)
+    u = torch.rand(logits.shape[0], generator=generator, device=logits.device)
+    hip_ops.sample_token_(logits, u, tokens, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+    return tokens
+
+
+def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batch_size: int, device, kv8_cache: bool = False):
     """(cache, use_manual_decode).  The dense FlashSVD cache is used when the dense-attention decode
     route or the dense-KV baseline is switched on; the package has no other cache for its modules."""
-    from .runtime.cache import FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
+    from .runtime.cache import FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
     dtype = next(iter(model.parameters())).dtype
     use_flash = _env_truthy("FLASH_SVD_ENABLE_DENSE_ATTN_DECODE") and not _env_truthy("SVDLLM_FLASH_FALLBACK")
     # the rank-space cache when the checkpoint asks for it (config side channel written by the loader,
     # utils/model_utils.py:438-439) or the rank-space baseline switch is on (utils/evaluator.py:418-456)
     use_rank = (bool(getattr(model.config, "flash_svd_use_lowrank_cache", False)) or _env_truthy("FLASH_SVD_BASELINE_LR_KVCACHE")) \
         and not use_flash
-    kind = FlashSVDLegacySparseKVCache if use_rank else FlashSVDV15DenseKVCache
+    if kv8_cache and use_rank:
+        raise ValueError("kv8_cache and the rank-space cache are mutually exclusive.")
+    kind = FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if use_rank else FlashSVDV15DenseKVCache
     cache = kind(model.config, max_batch_size=int(batch_size), max_cache_len=int(prompt_len) + int(max_new_tokens) + 4,
                  device=device, dtype=dtype)
     return cache, bool(use_flash)
@@ -191,8 +202,13 @@ def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batc
 
 @torch.no_grad()
 def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, device=None, do_sample: bool = False,
-                  temperature: float = 0.8, top_p: float = 0.95, use_graph: Optional[bool] = None) -> dict[str, Any]:
-    """Single-prompt generation; returns text and token ids like the reference's generate_text."""
+                  temperature: float = 0.8, top_p: float = 0.95, use_graph: Optional[bool] = None, top_k: int = 0, min_p: float = 0.0,
+                  seed: Optional[int] = None, kv8_cache: bool = False) -> dict[str, Any]:
+    """Single-prompt generation; returns text and token ids like the reference's generate_text.
+
+    ``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are additions to its arguments: with any of them sampling takes
+    ``hip_ops.sample_token_`` with uniform numbers of a generator of its own (seeded with ``seed``), captured graph included.
+    ``kv8_cache`` keeps keys and values in 8 bits (FlashSVDKV8Cache)."""
     if device is None:
         try:
             device = next(model.parameters()).device
@@ -212,24 +228,31 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
         raise ValueError("generate_text currently supports batch_size=1 only.")
     prompt_len = int(input_ids.shape[1])
     cache, _ = _build_generation_cache(model, prompt_len=prompt_len, max_new_tokens=int(max_new_tokens), batch_size=1,
-                                       device=device)
+                                       device=device, kv8_cache=bool(kv8_cache))
     out = model(input_ids=input_ids, past_key_values=cache, cache_position=torch.arange(prompt_len), logits_to_keep=1)
     output_ids = input_ids[0].tolist()
     eos = getattr(tokenizer, "eos_token_id", None)
     sample = dict(do_sample=bool(do_sample), temperature=float(temperature), top_p=float(top_p))
-    next_token = _sample_next_token(out.logits[:, -1, :], **sample)
+    pick = lambda logits: _sample_next_token(logits, **sample)      # noqa: E731
+    draws = generator = None
+    if do_sample and (top_k > 0 or min_p > 0 or seed is not None):
+        draws = dict(temperature=float(temperature), top_k=int(top_k), top_p=float(top_p), min_p=float(min_p))
+        generator = torch.Generator(device=out.logits.device)
+        generator.seed() if seed is None else generator.manual_seed(int(seed))
+        pick = lambda logits: _draw_next_token(logits, generator=generator, **draws)      # noqa: E731
+    next_token = pick(out.logits[:, -1, :])
     if use_graph is None:
         use_graph = _env_truthy("FLASH_SVD_DENSE_DECODE_GRAPH") or _env_truthy("FLASH_SVD_MLP_CUDA_GRAPH")
     dec = None
     pdec = None
-    if use_graph and not do_sample and hasattr(model, "decode_step"):
+    if use_graph and (not do_sample or draws is not None) and hasattr(model, "decode_step"):
         from .graphs import GraphedDecoder
         from .step import make_persistent_decoder
-        pdec = make_persistent_decoder(model, cache, 1, max_new_tokens=int(max_new_tokens) + 1)
+        pdec = make_persistent_decoder(model, cache, 1, max_new_tokens=int(max_new_tokens) + 1) if draws is None else None
         if pdec is not None:
             pdec.set_state(next_token, prompt_len)
         else:
-            dec = GraphedDecoder(model, cache, 1)
+            dec = GraphedDecoder(model, cache, 1, sampling=draws, generator=generator)
             dec.set_state(next_token, prompt_len)
             dec.capture()
     for step in range(int(max_new_tokens)):
@@ -244,7 +267,7 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
         else:
             out = _manual_llama_decode_step(model, next_token, past_key_values=cache,
                                             cache_position=torch.tensor([prompt_len + step]))
-            next_token = _sample_next_token(out.logits[:, -1, :], **sample)
+            next_token = pick(out.logits[:, -1, :])
     if pdec is not None:
         pdec.check()      # a step that gave up waiting leaves stale token ids behind: raise instead of returning them
     completion = output_ids[prompt_len:]
@@ -257,18 +280,20 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
 def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128, batch_size: int = 1, device: str = "cuda",
                         warmup: int = 5, max_cache_len: Optional[int] = None, lowrank_cache: bool = False,
                         flashsvd_dense_cache: Optional[bool] = None, baseline_dense_kvcache: bool = False, use_graph: bool = True,
-                        profile_decode: bool = False, profile_decode_steps: int = 20) -> dict:
+                        profile_decode: bool = False, profile_decode_steps: int = 20, kv8_cache: bool = False) -> dict:
     """Prefill a random prompt, run `warmup` untimed decode tokens, then time `new_tokens` tokens
     between two device synchronisations.  Result keys follow the reference's dict.
 
     Cache choice as in utils/evaluator.py:352-388: ``lowrank_cache`` decodes over the rank-space cache
     (FlashSVDLegacySparseKVCache: per-layer, possibly unequal q/k/v ranks, shaped at the first write), otherwise the
     dense cache (the package has no third, HF-static one, so ``flashsvd_dense_cache`` left unset means "dense unless
-    lowrank_cache").  Two modes switched on together raise, as there."""
+    lowrank_cache").  ``kv8_cache`` decodes over keys and values in 8 bits (FlashSVDKV8Cache).  Two modes switched on together raise, as there."""
     from .graphs import GraphedDecoder
-    from .runtime.cache import FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
+    from .runtime.cache import FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
     if flashsvd_dense_cache is None:
-        flashsvd_dense_cache = not (lowrank_cache or baseline_dense_kvcache)
+        flashsvd_dense_cache = not (lowrank_cache or baseline_dense_kvcache or kv8_cache)
+    if kv8_cache and (lowrank_cache or flashsvd_dense_cache or baseline_dense_kvcache):
+        raise ValueError("kv8_cache and the other caches are mutually exclusive.")
     if lowrank_cache and flashsvd_dense_cache:
         raise ValueError("lowrank_cache and flashsvd_dense_cache are mutually exclusive.")
     if lowrank_cache and baseline_dense_kvcache:
@@ -282,7 +307,7 @@ def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128,
     dtype = next(iter(model.parameters())).dtype
     vocab = int(getattr(model.config, "vocab_size", 32000))
     input_ids = torch.randint(0, vocab, (int(batch_size), int(prompt_len)), device=dev, dtype=torch.long)
-    kind = FlashSVDLegacySparseKVCache if lowrank_cache else FlashSVDV15DenseKVCache
+    kind = FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if lowrank_cache else FlashSVDV15DenseKVCache
     cache = kind(model.config, max_batch_size=int(batch_size), max_cache_len=int(max_cache_len), device=dev, dtype=dtype)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
@@ -319,7 +344,7 @@ def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128,
         "decode_tok_s": float(batch_size * new_tokens / t_decode) if t_decode > 0 else float("inf"),
         "decode_ms_per_token": float(t_decode * 1000.0 / max(1, int(new_tokens))),
         "lowrank_cache": bool(lowrank_cache), "flashsvd_dense_cache": bool(flashsvd_dense_cache),
-        "baseline_dense_kvcache": bool(baseline_dense_kvcache),
+        "baseline_dense_kvcache": bool(baseline_dense_kvcache), "kv8_cache": bool(kv8_cache),
     }
     profile = None
     if profile_decode and pdec is not None:

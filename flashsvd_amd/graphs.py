@@ -8,7 +8,7 @@ memset nodes: scratch comes from torch's capture pool and counters are reset by 
 """
 from __future__ import annotations
 
-from typing import Callable
+from typing import Callable, Optional
 
 import torch
 
@@ -38,17 +38,26 @@ class GraphedCallable:
 class GraphedDecoder:
     """Whole-step greedy decode as one graph: embed -> layers -> norm+lm_head -> argmax, with the
     token id and the write position living on the device and advanced inside the graph, so a
-    run of N tokens is N replays with no host synchronisation in between."""
+    run of N tokens is N replays with no host synchronisation in between.
 
-    def __init__(self, model, cache, batch_size: int, *, nsplit=None, warmup: int = 3):
+    ``sampling`` (the keyword arguments of ``hip_ops.sample_token_``: temperature, top_k, top_p, min_p, numbers or tensors [B]) draws the
+    tokens instead, with uniform numbers that ``generator`` (a generator of the device; None: the default one) gives before each step."""
+
+    def __init__(self, model, cache, batch_size: int, *, nsplit=None, warmup: int = 3, sampling: Optional[dict] = None, generator=None):
         from . import hip_ops
+        from .runtime.cache import FlashSVDKV8Cache
         self.model, self.cache, self.B = model, cache, int(batch_size)
         dev = model.lm_head.weight.device
         cfg = model.config
         H = int(cfg.num_attention_heads)
         Dh = int(getattr(cfg, "head_dim", None) or cfg.hidden_size // H)
-        self.nsplit = nsplit or hip_ops.pick_nsplit(cache.max_cache_len, self.B, H, Dh)
-        self.attn_ws = hip_ops.attn_workspace(self.B, H, Dh, self.nsplit, dev)
+        if isinstance(cache, FlashSVDKV8Cache):             # the call picks its key ranges and has scratch of its own
+            self.nsplit, self.attn_ws = nsplit, None
+        else:
+            self.nsplit = nsplit or hip_ops.pick_nsplit(cache.max_cache_len, self.B, H, Dh)
+            self.attn_ws = hip_ops.attn_workspace(self.B, H, Dh, self.nsplit, dev)
+        self.sampling, self.generator = None if sampling is None else dict(sampling), generator
+        self.uniforms = torch.zeros(self.B, dtype=torch.float32, device=dev)
         self.rope = cache.get_rope_tables(seqlen=cache.max_cache_len, head_dim=Dh, device=dev, dtype=model.lm_head.weight.dtype)
         self.tokens = torch.zeros(self.B, 1, dtype=torch.long, device=dev)
         self.positions = torch.zeros(self.B, dtype=torch.int32, device=dev)
@@ -62,7 +71,9 @@ class GraphedDecoder:
         logits, hidden = self.model.decode_step(self.tokens, self.cache, self.positions, rope=self.rope,
                                                 attn_ws=self.attn_ws, nsplit=self.nsplit, return_hidden=True)
         last = logits[:, -1, :]
-        if last.dtype in (torch.bfloat16, torch.float16) and last.stride(1) == 1:
+        if self.sampling is not None:
+            hip_ops.sample_token_(last, self.uniforms, self.tokens, self.positions, **self.sampling)
+        elif last.dtype in (torch.bfloat16, torch.float16) and last.stride(1) == 1:
             hip_ops.greedy_token_(last, self.tokens, self.positions)
         else:
             self.tokens.copy_(last.argmax(dim=-1, keepdim=True))
@@ -71,9 +82,14 @@ class GraphedDecoder:
 
     def eager_step(self):
         """One un-captured step on the current stream (same kernels, same buffers)."""
+        self._next_uniforms()
         self.logits, self.hidden = self._step()
         self.cache._seen_tokens += 1
         return self.tokens
+
+    def _next_uniforms(self) -> None:
+        if self.sampling is not None:
+            self.uniforms.uniform_(generator=self.generator)
 
     def capture(self) -> None:
         tok0, pos0 = self.tokens.clone(), self.positions.clone()
@@ -111,6 +127,7 @@ class GraphedDecoder:
             self.capture()
         if getattr(self, "_host_pos", 0) + 1 > self.cache.max_cache_len:
             raise IndexError(f"decode position {self._host_pos} outside the cache (max {self.cache.max_cache_len})")
+        self._next_uniforms()
         self.graph.replay()
         self._host_pos = getattr(self, "_host_pos", 0) + 1
         self.cache._seen_tokens += 1

@@ -22,7 +22,7 @@ import torch
 from torch import nn
 
 from . import hip_ops
-from .runtime.cache import FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
+from .runtime.cache import FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
 
 _TRUE = {"1", "true", "yes", "y", "on"}
 # set by api.enable_flashsvd_llama_layer_tail_cuda_graph(); read at call time together with the env flags
@@ -297,24 +297,30 @@ class SVD_LlamaAttention(nn.Module):
         H, Hk, Dh = self.num_heads, self.num_key_value_heads, self.head_dim
         if isinstance(cache, FlashSVDLegacySparseKVCache):
             return self._decode_token_rank(x, cache, positions, norm_weight=norm_weight, eps=eps, residual=residual, rope=rope)
-        if not isinstance(cache, FlashSVDV15DenseKVCache):
-            raise TypeError(f"decode needs a FlashSVDV15DenseKVCache or FlashSVDLegacySparseKVCache, got {type(cache).__name__}")
+        kv8 = isinstance(cache, FlashSVDKV8Cache)
+        if not kv8 and not isinstance(cache, FlashSVDV15DenseKVCache):
+            raise TypeError(f"decode needs a FlashSVDV15DenseKVCache, FlashSVDKV8Cache or FlashSVDLegacySparseKVCache, got {type(cache).__name__}")
         cache._ensure_layer_spec(self.layer_idx, h=Hk, dh=Dh)
         kc, vc = cache.key_cache[self.layer_idx], cache.value_cache[self.layer_idx]
         if rope is None:
             rope = cache.get_rope_tables(seqlen=cache.max_cache_len, head_dim=Dh, device=x.device, dtype=x.dtype)
         from .quant import apply_linear, is_quantized
         quantized = is_quantized(*self._factor_modules())
-        by_module = quantized or self._dense_decode_backend(cache) == "exact"
-        if nsplit is None:
+        by_module = quantized or kv8 or self._dense_decode_backend(cache) == "exact"
+        if nsplit is None and not kv8:
             nsplit = hip_ops.pick_nsplit(cache.max_cache_len, B, H, Dh, own_row=by_module and H == Hk)
         if by_module:
             # module by module: three rank projections, three head expansions, rotary + append inside attention
-            # (the only form for int4 factors, whose bytes cannot be row-packed with their neighbours')
+            # (the only form for int4 factors, whose bytes cannot be row-packed with their neighbours', and for the cache in 8 bits,
+            # whose rows the attention rounds as it writes them)
             pk = getattr(self, "_q4_qkv_v", None) if quantized else None
             if pk is not None and self.q_v_proj.streams_int4(B):
                 rq, rk, rv = self._qkv_rank_tuple()
                 p = hip_ops.linear_q4(x, *pk, group_size=self.q_v_proj.group_size, norm_weight=norm_weight, eps=eps)
+                pq, pkk, pv = p[:, :rq], p[:, rq:rq + rk], p[:, rq + rk:]
+            elif kv8 and not quantized:
+                rq, rk, rv = self._qkv_rank_tuple()
+                p = hip_ops.linear(x, self._packed_qkv_v, norm_weight=norm_weight, eps=eps)
                 pq, pkk, pv = p[:, :rq], p[:, rq:rq + rk], p[:, rq + rk:]
             else:
                 xn = x if norm_weight is None else hip_ops.rmsnorm(x, norm_weight, eps)
@@ -322,8 +328,12 @@ class SVD_LlamaAttention(nn.Module):
             q = apply_linear(self.q_u_proj, pq).view(B, H, Dh)
             k = apply_linear(self.k_u_proj, pkk).view(B, Hk, Dh)
             v = apply_linear(self.v_u_proj, pv).view(B, Hk, Dh)
-            a = hip_ops.attn_decode_densekv(q, kc[:B], vc[:B], positions, k_new=k, v_new=v, cos=rope[0], sin=rope[1],
-                                            nsplit=nsplit, workspace=attn_ws)
+            if kv8:
+                a = hip_ops.attn_decode_kv8(q, *cache.operands(self.layer_idx, B), positions, block=cache.block_size, k_new=k, v_new=v, cos=rope[0],
+                                            sin=rope[1], nsplit=nsplit)
+            else:
+                a = hip_ops.attn_decode_densekv(q, kc[:B], vc[:B], positions, k_new=k, v_new=v, cos=rope[0], sin=rope[1],
+                                                nsplit=nsplit, workspace=attn_ws)
             cache._layer_initialized[self.layer_idx] = True
             po = apply_linear(self.o_v_proj, a.view(B, H * Dh))
             return apply_linear(self.o_u_proj, po, residual=residual)
@@ -424,7 +434,8 @@ class SVD_LlamaAttention(nn.Module):
         quantized = is_quantized(*self._factor_modules())
         mfma_ok = Dh == 128 and T >= 16 \
             and os.getenv("FLASHSVD_AMD_PREFILL", "mfma").strip().lower() != "decode"
-        if mfma_ok and not quantized:
+        kv8 = isinstance(cache, FlashSVDKV8Cache)
+        if mfma_ok and not quantized and not kv8:
             # the matrix-core route below, its launches issued by one native call
             out = hip_ops.lowrank_attn_prefill(
                 x, self._packed_qkv_v, self.q_u_proj.weight, self.k_u_proj.weight, self.v_u_proj.weight, self.o_v_proj.weight,
@@ -444,7 +455,9 @@ class SVD_LlamaAttention(nn.Module):
             wq, wk, wv = self.q_u_proj.weight, self.k_u_proj.weight, self.v_u_proj.weight
         rq, rk, rv = self._qkv_rank_tuple()
         a = torch.empty(B, T, H * Dh, device=x.device, dtype=x.dtype)
-        if mfma_ok:
+        if kv8:
+            self._prefill_kv8(p, wq, wk, wv, cache, start, rope, a.view(B, T, H, Dh))
+        elif mfma_ok:
             # matrix-core route: q/k/v rebuilt once per token with the rotation fused (k, v land in the
             # cache rows start..start+T-1), then causal flash attention over the cache
             pos0 = torch.full((B,), start, device=x.device, dtype=torch.int32)
@@ -467,6 +480,26 @@ class SVD_LlamaAttention(nn.Module):
         cache._note_seen(self.layer_idx, T, cache_position)
         po = apply_linear(self.o_v_proj, a)
         return apply_linear(self.o_u_proj, po, residual=residual)
+
+
+    def _prefill_kv8(self, p: torch.Tensor, wq, wk, wv, cache, start: int, rope, out: torch.Tensor) -> None:
+        """q, k and v of a chunk from its rank coefficients p [B, T, R]; k and v into the cache in 8 bits at start .. start + T - 1, attention over the
+        cache into out [B, T, H, Dh], so that later chunks and tokens see what this one saw."""
+        B, T, H, Dh = out.shape
+        Hk = self.num_key_value_heads
+        rq, rk, rv = self._qkv_rank_tuple()
+        pos0 = torch.full((B,), start, device=p.device, dtype=torch.int32)
+        pq, pk, pv = p[..., :rq], p[..., rq:rq + rk], p[..., rq + rk:]
+        if Dh == 128 and T >= 16:
+            q, k, v = (torch.empty(B, T, n, Dh, device=p.device, dtype=p.dtype) for n in (H, Hk, Hk))
+            hip_ops.lowrank_expand_heads_multi([dict(p=pq, u=wq, num_heads=H, out=q, rotate=True), dict(p=pk, u=wk, num_heads=Hk, out=k, rotate=True),
+                                                dict(p=pv, u=wv, num_heads=Hk, out=v)], head_dim=Dh, cos=rope[0], sin=rope[1], positions=pos0)
+            turn = {}
+        else:
+            q, k, v = (hip_ops.linear(c, w).view(B, T, n, Dh) for c, w, n in ((pq, wq, H), (pk, wk, Hk), (pv, wv, Hk)))
+            turn = dict(cos=rope[0], sin=rope[1])
+        cache.append(self.layer_idx, k, v, pos0, **turn)
+        hip_ops.attn_prefill_kv8(q, *cache.operands(self.layer_idx, B), pos0, block=cache.block_size, out=out, **turn)
 
 
 def _prefill_tokens_rank(self, x, cache, cache_position=None, *, norm_weight=None, eps=1e-6, residual=None):
@@ -800,7 +833,7 @@ def patch_hf_llama_decoder_layer() -> bool:
         if past_key_values is None:
             past_key_values = kwargs.pop("past_key_value", None)
         if isinstance(self.self_attn, SVD_LlamaAttention) and \
-                (past_key_values is None or isinstance(past_key_values, (FlashSVDV15DenseKVCache, FlashSVDLegacySparseKVCache))):
+                (past_key_values is None or isinstance(past_key_values, (FlashSVDV15DenseKVCache, FlashSVDKV8Cache, FlashSVDLegacySparseKVCache))):
             out = decoder_layer_forward(self, hidden_states, past_key_values=past_key_values,
                                         cache_position=kwargs.get("cache_position"))
         else:

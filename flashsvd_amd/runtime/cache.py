@@ -3,7 +3,7 @@
 ``FlashSVDV15DenseKVCache`` keeps post-RoPE K and V per layer as [Bmax, Smax, Hk, Dh]
 (runtime/cache/attn_dense_kv.py:7-357 of the reference); ``FlashSVDLegacySparseKVCache`` keeps
 the pre-RoPE rank coefficients Pk, Pv per layer as [Bmax, Smax, R]
-(runtime/cache/attn_legacy_sparse_kv.py:22-257).  Both are plain Python objects (no dependency
+(runtime/cache/attn_legacy_sparse_kv.py:22-257).  ``FlashSVDKV8Cache`` keeps K and V in 8 bits.  All are plain Python objects (no dependency
 on the transformers ``Cache`` base class) with the method names, return values and error
 behaviour the reference's callers rely on.  Storage is allocated once at full size so that
 decode kernels can write in place and a captured HIP graph keeps valid pointers.
@@ -89,34 +89,14 @@ class _CacheBase:
         self._seen_tokens = 0
 
 
-class FlashSVDV15DenseKVCache(_CacheBase):
-    """Dense KV cache, [B, S, Hk, Dh] per layer, K stored after RoPE."""
+class _HeadCacheBase(_CacheBase):
+    """What the caches of whole heads share: head counts learnt from the first write, the device buffers of the decoded positions."""
 
-    def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device=None,
-                 dtype: torch.dtype = torch.float16, layer_device_map: Optional[dict] = None) -> None:
+    def __init__(self, config, max_batch_size: int, max_cache_len: int, device, dtype, layer_device_map):
         super().__init__(config, max_batch_size, max_cache_len, device, dtype, layer_device_map)
-        for dev in self._layer_device:
-            # shaped lazily: head count / head_dim are learnt from the first write
-            self.key_cache.append(torch.zeros((self._max_batch_size, self._max_cache_len, 0, 0), dtype=dtype, device=dev))
-            self.value_cache.append(torch.zeros((self._max_batch_size, self._max_cache_len, 0, 0), dtype=dtype, device=dev))
         self._layer_heads = [0] * len(self._layer_device)
         self._layer_head_dim = [0] * len(self._layer_device)
         self._seqlens: dict[tuple[int, int], torch.Tensor] = {}
-
-    # -- storage ---------------------------------------------------------------------------
-    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
-        layer_idx, h, dh = int(layer_idx), int(h), int(dh)
-        cur = self.key_cache[layer_idx]
-        if (cur.shape[2], cur.shape[3]) == (h, dh):
-            return
-        if self._layer_initialized[layer_idx]:
-            raise RuntimeError(
-                f"FlashSVDV15DenseKVCache shape changed after init for layer {layer_idx}: "
-                f"old={(int(cur.shape[2]), int(cur.shape[3]))}, new={(h, dh)}")
-        shape = (self._max_batch_size, self._max_cache_len, h, dh)
-        self.key_cache[layer_idx] = torch.zeros(shape, dtype=self._dtype, device=self._layer_device[layer_idx])
-        self.value_cache[layer_idx] = torch.zeros(shape, dtype=self._dtype, device=self._layer_device[layer_idx])
-        self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
 
     def _seqlens_buffer(self, layer_idx: int, batch_size: int) -> torch.Tensor:
         key = (int(layer_idx), int(batch_size))
@@ -142,6 +122,42 @@ class FlashSVDV15DenseKVCache(_CacheBase):
         else:
             cache_seqlens.fill_(int(cache_position))
         return cache_seqlens
+
+    def advance_after_fa2(self, layer_idx: int, *, q_len: int, cache_position) -> None:
+        if int(layer_idx) != 0:
+            return
+        if cache_position is not None and torch.is_tensor(cache_position) and not cache_position.is_cuda \
+                and cache_position.numel() > 0:
+            self._seen_tokens = max(self._seen_tokens, int(cache_position.max()) + 1)
+        else:
+            self._seen_tokens = self._seen_tokens + int(q_len)
+
+
+class FlashSVDV15DenseKVCache(_HeadCacheBase):
+    """Dense KV cache, [B, S, Hk, Dh] per layer, K stored after RoPE."""
+
+    def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device=None,
+                 dtype: torch.dtype = torch.float16, layer_device_map: Optional[dict] = None) -> None:
+        super().__init__(config, max_batch_size, max_cache_len, device, dtype, layer_device_map)
+        for dev in self._layer_device:
+            # shaped lazily: head count / head_dim are learnt from the first write
+            self.key_cache.append(torch.zeros((self._max_batch_size, self._max_cache_len, 0, 0), dtype=dtype, device=dev))
+            self.value_cache.append(torch.zeros((self._max_batch_size, self._max_cache_len, 0, 0), dtype=dtype, device=dev))
+
+    # -- storage ---------------------------------------------------------------------------
+    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
+        layer_idx, h, dh = int(layer_idx), int(h), int(dh)
+        cur = self.key_cache[layer_idx]
+        if (cur.shape[2], cur.shape[3]) == (h, dh):
+            return
+        if self._layer_initialized[layer_idx]:
+            raise RuntimeError(
+                f"FlashSVDV15DenseKVCache shape changed after init for layer {layer_idx}: "
+                f"old={(int(cur.shape[2]), int(cur.shape[3]))}, new={(h, dh)}")
+        shape = (self._max_batch_size, self._max_cache_len, h, dh)
+        self.key_cache[layer_idx] = torch.zeros(shape, dtype=self._dtype, device=self._layer_device[layer_idx])
+        self.value_cache[layer_idx] = torch.zeros(shape, dtype=self._dtype, device=self._layer_device[layer_idx])
+        self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
 
     # -- HF-style update (prefill copy or positional scatter) -------------------------------
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int,
@@ -207,15 +223,6 @@ class FlashSVDV15DenseKVCache(_CacheBase):
         self._layer_initialized[layer_idx] = True
         return kc, vc, kc[:, start:start + q_len], vc[:, start:start + q_len], lens
 
-    def advance_after_fa2(self, layer_idx: int, *, q_len: int, cache_position) -> None:
-        if int(layer_idx) != 0:
-            return
-        if cache_position is not None and torch.is_tensor(cache_position) and not cache_position.is_cuda \
-                and cache_position.numel() > 0:
-            self._seen_tokens = max(self._seen_tokens, int(cache_position.max()) + 1)
-        else:
-            self._seen_tokens = self._seen_tokens + int(q_len)
-
     def clone_for_autotune(self, *, layer_idx: int, batch_size: int) -> "FlashSVDV15DenseKVCache":
         """A scratch copy holding only ``layer_idx``'s first ``batch_size`` rows."""
         layer_idx, batch_size = int(layer_idx), int(batch_size)
@@ -230,6 +237,92 @@ class FlashSVDV15DenseKVCache(_CacheBase):
             other.value_cache[layer_idx][:batch_size].copy_(self.value_cache[layer_idx][:batch_size])
             other._layer_initialized[layer_idx] = self._layer_initialized[layer_idx]
         return other
+
+
+class FlashSVDKV8Cache(_HeadCacheBase):
+    """Dense KV cache in 8 bits: per layer e4m3 codes [B, S, Hk, Dh] of K (after RoPE) and V, and one float32 power of two for each
+    block of ``block_size`` tokens (16, 32, 64 or 128) of a kv head, [B, ceil(S / block_size), Hk]; ``value = code * scale``.
+
+    Half the bytes of :class:`FlashSVDV15DenseKVCache` and its method names where they make sense; rows are written by
+    ``hip_ops.kv8_append`` and read by ``hip_ops.attn_decode_kv8`` / ``attn_prefill_kv8``.  ``dtype`` is that of the activations.  A row's
+    tokens stand side by side for each head in memory (the kernels take any strides).  Writing a position makes it the last valid one
+    of its block, so rows are written in order; going back to an earlier position and continuing from there is fine.  No counterpart in
+    the reference, whose caches are of 16 bits."""
+
+    def __init__(self, config, *, max_batch_size: int, max_cache_len: int, block_size: int = 32, device=None, dtype: torch.dtype = torch.float16,
+                 layer_device_map: Optional[dict] = None) -> None:
+        super().__init__(config, max_batch_size, max_cache_len, device, dtype, layer_device_map)
+        if int(block_size) not in (16, 32, 64, 128):
+            raise ValueError(f"block_size must be 16, 32, 64 or 128 tokens, got {block_size}")
+        self.block_size = int(block_size)
+        self.key_scale: list[torch.Tensor] = []
+        self.value_scale: list[torch.Tensor] = []
+        for dev in self._layer_device:
+            codes, scale = self._storage(0, 0, dev)
+            self.key_cache.append(codes)
+            self.value_cache.append(codes)
+            self.key_scale.append(scale)
+            self.value_scale.append(scale)
+
+    def _storage(self, h: int, dh: int, dev):
+        codes = torch.zeros((self._max_batch_size, h, self._max_cache_len, dh), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
+        scale = torch.zeros((self._max_batch_size, h, -(-self._max_cache_len // self.block_size)), dtype=torch.float32, device=dev)
+        return codes.transpose(1, 2), scale.transpose(1, 2)
+
+    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
+        layer_idx, h, dh = int(layer_idx), int(h), int(dh)
+        cur = self.key_cache[layer_idx]
+        if (cur.shape[2], cur.shape[3]) == (h, dh):
+            return
+        if self._layer_initialized[layer_idx]:
+            raise RuntimeError(f"FlashSVDKV8Cache shape changed after init for layer {layer_idx}: old={(int(cur.shape[2]), int(cur.shape[3]))}, new={(h, dh)}")
+        dev = self._layer_device[layer_idx]
+        self.key_cache[layer_idx], self.key_scale[layer_idx] = self._storage(h, dh, dev)
+        self.value_cache[layer_idx], self.value_scale[layer_idx] = self._storage(h, dh, dev)
+        self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
+
+    def operands(self, layer_idx: int, batch_size: int):
+        """(key codes, value codes, key scales, value scales) of the first ``batch_size`` sequences, as the operators take them."""
+        i, b = int(layer_idx), int(batch_size)
+        return self.key_cache[i][:b], self.value_cache[i][:b], self.key_scale[i][:b], self.value_scale[i][:b]
+
+    def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, *, cos=None, sin=None, rows=None) -> None:
+        """``hip_ops.kv8_append`` of rows k, v [B, T, Hk, Dh] at positions int32 [B] of this layer."""
+        from .. import hip_ops
+        self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
+        hip_ops.kv8_append(k, v, *self.operands(layer_idx, k.shape[0]), positions, block=self.block_size, cos=cos, sin=sin, rows=rows)
+        self._layer_initialized[int(layer_idx)] = True
+
+    def dequantize(self, layer_idx: int, *, batch_size: Optional[int] = None, length: Optional[int] = None):
+        """(K, V) of the first ``length`` positions as ``dtype`` [B, L, Hk, Dh]."""
+        i = int(layer_idx)
+        b = self._max_batch_size if batch_size is None else int(batch_size)
+        n = self._max_cache_len if length is None else int(length)
+        out = []
+        for codes, scale in ((self.key_cache[i], self.key_scale[i]), (self.value_cache[i], self.value_scale[i])):
+            full = scale[:b].repeat_interleave(self.block_size, 1)[:, :n, :, None]
+            out.append((codes[:b, :n].float() * full).to(self._dtype))
+        return out[0], out[1]
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs: Optional[dict[str, Any]] = None):
+        """key/value_states are [B, Hk, T, Dh] (keys rotated) for consecutive positions; returns the held cache prefix as [B, Hk, L, Dh]."""
+        cache_position = (cache_kwargs or {}).get("cache_position")
+        t, start = key_states.shape[2], 0
+        if cache_position is not None:
+            pos = cache_position.reshape(-1).tolist()
+            if pos != list(range(pos[0], pos[0] + t)):
+                raise ValueError("FlashSVDKV8Cache takes consecutive positions: a block's scale is that of the rows up to the last one written")
+            start = pos[0]
+        if start < 0 or start + t > self._max_cache_len:
+            raise IndexError(f"FlashSVDKV8Cache write position out of range: start={start} q_len={t} max={self._max_cache_len}")
+        dev = self._layer_device[int(layer_idx)]
+        k, v = (x.to(device=dev, dtype=self._dtype).transpose(1, 2) for x in (key_states, value_states))
+        k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v))
+        self.append(layer_idx, k, v, torch.full((k.shape[0],), start, dtype=torch.int32, device=dev))
+        self._note_seen(layer_idx, t, cache_position)
+        n = t if cache_position is None else max(int(self.get_seq_length()), start + t)
+        k, v = self.dequantize(layer_idx, batch_size=k.shape[0], length=n)
+        return k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
 
 
 @dataclass

@@ -124,3 +124,26 @@ def test_refusals_of_the_c_abi():
     assert chunk(H=3) == -1 and chunk(M=-1) == -1 and chunk(q=None) == -4 and chunk(M=0) == 0
     draw = lambda x=p, B=1, V=8, dt=0: lib.fsvd_sample_token(x, 8, p, p, 1, None, 1.0, None, 0, None, 1.0, None, 0.0, None, B, V, dt, None)      # noqa: E731
     assert draw(x=None) == -4 and draw(B=0) == -1 and draw(V=0) == -1 and draw(V=(1 << 24) + 1) == -1 and draw(dt=2) == -3 and draw(x=p + 1) == -2
+
+
+def test_the_cache_object_without_a_gpu():
+    from types import SimpleNamespace
+    from flashsvd_amd.runtime import FlashSVDKV8Cache, FlashSVDV15DenseKVCache
+    cfg = SimpleNamespace(num_hidden_layers=2, rope_theta=10000.0)
+    with pytest.raises(ValueError, match="block_size"):
+        FlashSVDKV8Cache(cfg, max_batch_size=1, max_cache_len=8, block_size=24)
+    c = FlashSVDKV8Cache(cfg, max_batch_size=3, max_cache_len=70, block_size=32)
+    assert not isinstance(c, FlashSVDV15DenseKVCache) and len(c) == 2 and c.max_cache_len == 70
+    c._ensure_layer_spec(1, h=4, dh=64)
+    k, v, ks, vs = c.operands(1, 2)
+    assert k.shape == v.shape == (2, 70, 4, 64) and k.dtype == F8 and k.stride(3) == 1 and k.stride(1) == 64
+    assert ks.shape == vs.shape == (2, 3, 4) and ks.dtype == torch.float32
+    assert c.key_cache[0].shape == (3, 70, 0, 0)
+    K, V = c.dequantize(1, length=5)
+    assert K.shape == (3, 5, 4, 64) and not bool(K.any()) and not bool(V.any())
+    with pytest.raises(IndexError):
+        c.update(torch.zeros(1, 4, 3, 64), torch.zeros(1, 4, 3, 64), 1, {"cache_position": torch.arange(68, 71)})
+    with pytest.raises(ValueError, match="consecutive"):
+        c.update(torch.zeros(1, 4, 2, 64), torch.zeros(1, 4, 2, 64), 1, {"cache_position": torch.tensor([4, 6])})
+    with pytest.raises(ValueError, match="GPU tensor"):
+        c.update(torch.zeros(1, 4, 2, 64), torch.zeros(1, 4, 2, 64), 1)
