@@ -1,4 +1,6 @@
 // Attention over the KV cache in 8 bits.
+#include <type_traits>
+
 #include "kv8.hpp"
 
 namespace fsvd {
@@ -366,11 +368,13 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 constexpr int kTile = 64;
+constexpr float kSlack = 8.f;
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
-// four codes as two pairs of bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
-__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, bool hi, float scale, bool power) {
-  if (power) return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
-  const f32x2_t x = hi ? codes_hi(w) : codes_lo(w);
+// a pair of codes as bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
+template <bool HI, bool POWER>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
+  if constexpr (POWER) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+  const f32x2_t x = HI ? codes_hi(w) : codes_lo(w);
   return pack_bf16x2(x[0] * scale, x[1] * scale);
 }
 
@@ -457,18 +461,30 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   u32x4_t kreg[KP];
   uint32_t vreg[VP][4];
   float vscale[VP], kscale[4];
-  const auto request = [&](int n0) {
+  // a tile's first row is the workgroup's, 64 bits; from there on 32 do (and stay the same from tile to tile, but for one that the range ends in)
+  const uint32_t line = (uint32_t)a.c.sc_s;
+  uint32_t koff[KP], voff[VP][4];
+  const auto offsets = [&](int left) {
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
-      const int row = krow + p * (TH / KL);
-      if (kTile * KL % TH == 0 || row < kTile) kreg[p] = *reinterpret_cast<const u32x4_t*>(kb + (int64_t)min(n0 + row, n_end - 1) * a.c.sc_s + kd);
-    }
+    for (int p = 0; p < KP; ++p) koff[p] = (uint32_t)min(krow + p * (TH / KL), left - 1) * line + kd;
+#pragma unroll
+    for (int p = 0; p < VP; ++p)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) voff[p][e] = (uint32_t)min(4 * (vrow + p * (TH / VL)) + e, left - 1) * line + vd;
+  };
+  const auto request = [&](int n0) {
+    if (n0 + kTile > n_end) offsets(n_end - n0);
+    const uint8_t* kt = kb + (int64_t)n0 * a.c.sc_s;
+    const uint8_t* vt = vb + (int64_t)n0 * a.c.sc_s;
+#pragma unroll
+    for (int p = 0; p < KP; ++p)
+      if (kTile * KL % TH == 0 || krow + p * (TH / KL) < kTile) kreg[p] = *reinterpret_cast<const u32x4_t*>(kt + koff[p]);
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       const int row = 4 * (vrow + p * (TH / VL));
       if (kTile / 4 * VL % TH == 0 || row < kTile) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vb + (int64_t)min(n0 + row + e, n_end - 1) * a.c.sc_s + vd);
+        for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vt + voff[p][e]);
         vscale[p] = vsp[(int64_t)(min(n0 + row, n_end - 1) >> shift) * a.c.ss_n];
       }
     }
@@ -495,22 +511,27 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
       const int row4 = vrow + p * (TH / VL);
       if (kTile / 4 * VL % TH == 0 || row4 < kTile / 4) {
         const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
-        const bool power = (__float_as_uint(vscale[p]) & 0x7fffffu) == 0;
+        const auto put = [&](auto power) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
-          const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = vd + 2 * c + e;
-            *reinterpret_cast<u32x2_t*>(vt + d * kTile + (col ^ (8 * v_piece(d)))) = u32x2_t{scaled_pair(lo, e, vscale[p], power), scaled_pair(hi, e, vscale[p], power)};
+          for (int c = 0; c < 2; ++c) {
+            const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
+            const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
+            const int d = vd + 2 * c;
+            *reinterpret_cast<u32x2_t*>(vt + d * kTile + (col ^ (8 * v_piece(d)))) =
+                u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
+            *reinterpret_cast<u32x2_t*>(vt + (d + 1) * kTile + (col ^ (8 * v_piece(d + 1)))) =
+                u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
           }
-        }
+        };
+        if (__all((__float_as_uint(vscale[p]) & 0x7fffffu) == 0)) put(std::true_type{});
+        else put(std::false_type{});
       }
     }
   };
 
+  offsets(kTile);
   if (n_begin < n_end) request(n_begin);
+  const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
   int buf = 0;
   for (int n0 = n_begin; n0 < n_end; n0 += kTile, buf ^= 1) {
     stage(buf);
@@ -522,20 +543,29 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
     if (n0 >= wave_end) continue;
     const uint16_t* ks = Ks + buf * kTile * KSTR;
     const uint16_t* vt = Vt + buf * DH * kTile;
+    // all the fragments of K are asked for before the first product: left to itself the compiler asks for each in front of its use
     f32x4_t s[MI][4];
+    frag_t kf[4][ST];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      frag_t kf[ST];
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int st = 0; st < ST; ++st) kf[st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (16 * j + lr) * KSTR + 32 * st + 8 * lg));
+      for (int st = 0; st < ST; ++st) kf[j][st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (16 * j + lr) * KSTR + 32 * st + 8 * lg));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int mi = 0; mi < MI; ++mi) {
-        s[mi][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int st = 0; st < ST; ++st) s[mi][j] = E::mfma(kf[st], qf[mi][st], s[mi][j]);
-      }
-    }
-    const bool plain = n0 + kTile <= seen_by(w0);                  // every row of the wave sees the whole tile (rows see more from one to the next)
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) s[mi][j] = E::mfma(kf[j][st], qf[mi][st], st ? s[mi][j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+    const auto v_frag = [&](int st, int t) {
+      const int d = 16 * t + lr;
+      return __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + d * kTile + ((32 * st + 8 * lg) ^ (8 * v_piece(d)))));
+    };
+    pfrag_t vf[2][NT];                   // those of V's first half during the softmax, of its second during the products with the first
+#pragma unroll
+    for (int t = 0; t < NT; ++t) vf[0][t] = v_frag(0, t);
+    __builtin_amdgcn_sched_barrier(0);
+    const bool plain = n0 + kTile <= wave_sees;                    // every row of the wave sees the whole tile
     pfrag_t ph[MI][2], pl[MI][2];
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
@@ -553,20 +583,33 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
             top = fmaxf(top, s[mi][j][i]);
           }
       }
-      top = fmaxf(m_run[mi], column_max(top));
-      if (__any(top > m_run[mi])) {
+      top = column_max(top);
+      // The reference of the weights moves only where a score is kSlack over it: until then weights are up to 2^kSlack, which changes no rounding.
+      if (__any(top > m_run[mi] + kSlack)) {
+        top = fmaxf(m_run[mi], top);
         const float keep = top > m_run[mi] ? __builtin_amdgcn_exp2f(m_run[mi] - top) : 1.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[mi][t] *= keep;
         l_run[mi] *= keep;
         m_run[mi] = top;
       }
-      const float base = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet: exp2(-inf - 0)
+      const float base = m_run[mi] == -INFINITY ? 0.f : m_run[mi];  // a row that has seen nothing yet: exp2(-inf - 0)
+      if (plain) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[mi][j][i] = fmaf(s[mi][j][i], f[j], -base);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[mi][j][i] -= base;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[mi][j][i] = __builtin_amdgcn_exp2f(plain ? fmaf(s[mi][j][i], f[j], -base) : s[mi][j][i] - base);
+          s[mi][j][i] = __builtin_amdgcn_exp2f(s[mi][j][i]);
           l_run[mi] += s[mi][j][i];
         }
 #pragma unroll
@@ -583,17 +626,17 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
       }
     }
 #pragma unroll
+    for (int t = 0; t < NT; ++t) vf[1][t] = v_frag(1, t);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
     for (int st = 0; st < 2; ++st)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int d = 16 * t + lr;
-        const pfrag_t vf = __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + d * kTile + ((32 * st + 8 * lg) ^ (8 * v_piece(d)))));
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi) {
-          o[mi][t] = E16<0>::mfma(vf, ph[mi][st], o[mi][t]);
-          if (kRest) o[mi][t] = E16<0>::mfma(vf, pl[mi][st], o[mi][t]);
+          o[mi][t] = E16<0>::mfma(vf[st][t], ph[mi][st], o[mi][t]);
+          if (kRest) o[mi][t] = E16<0>::mfma(vf[st][t], pl[mi][st], o[mi][t]);
         }
-      }
   }
   // element i of tile t is dimension 16 t + 4 lg + i of row lr
   const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
