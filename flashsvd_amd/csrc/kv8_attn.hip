@@ -460,25 +460,30 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   const int krow = tid / KL, kd = tid % KL * 16, vrow = tid / VL, vd = tid % VL * 4;
   u32x4_t kreg[KP];
   uint32_t vreg[VP][4];
-  float vscale[VP], kscale[4];
+  float vscale[VP];
   // a tile's first row is the workgroup's, 64 bits; from there on 32 do (and stay the same from tile to tile, but for one that the range ends in)
   const uint32_t line = (uint32_t)a.c.sc_s;
   uint32_t koff[KP], voff[VP][4];
-  const auto offsets = [&](int left) {
+  const auto k_offset = [&](int p, int left) { return (uint32_t)min(krow + p * (TH / KL), left - 1) * line + kd; };
+  const auto v_offset = [&](int p, int e, int left) { return (uint32_t)min(4 * (vrow + p * (TH / VL)) + e, left - 1) * line + vd; };
+  const auto request_k = [&](int n0) {
+    if (n0 + kTile > n_end) {
 #pragma unroll
-    for (int p = 0; p < KP; ++p) koff[p] = (uint32_t)min(krow + p * (TH / KL), left - 1) * line + kd;
-#pragma unroll
-    for (int p = 0; p < VP; ++p)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) voff[p][e] = (uint32_t)min(4 * (vrow + p * (TH / VL)) + e, left - 1) * line + vd;
-  };
-  const auto request = [&](int n0) {
-    if (n0 + kTile > n_end) offsets(n_end - n0);
+      for (int p = 0; p < KP; ++p) koff[p] = k_offset(p, n_end - n0);
+    }
     const uint8_t* kt = kb + (int64_t)n0 * a.c.sc_s;
-    const uint8_t* vt = vb + (int64_t)n0 * a.c.sc_s;
 #pragma unroll
     for (int p = 0; p < KP; ++p)
       if (kTile * KL % TH == 0 || krow + p * (TH / KL) < kTile) kreg[p] = *reinterpret_cast<const u32x4_t*>(kt + koff[p]);
+  };
+  const auto request_v = [&](int n0) {
+    if (n0 + kTile > n_end) {
+#pragma unroll
+      for (int p = 0; p < VP; ++p)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) voff[p][e] = v_offset(p, e, n_end - n0);
+    }
+    const uint8_t* vt = vb + (int64_t)n0 * a.c.sc_s;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       const int row = 4 * (vrow + p * (TH / VL));
@@ -488,12 +493,14 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
         vscale[p] = vsp[(int64_t)(min(n0 + row, n_end - 1) >> shift) * a.c.ss_n];
       }
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) kscale[j] = ksp[(int64_t)(min(n0 + 16 * j, n_end - 1) >> shift) * a.c.ss_n];
   };
-  const auto stage = [&](int buf) {
+  float fs[4];                           // the key scales of a tile's four blocks of 16 keys
+  const auto request_f = [&](int n0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fs[j] = ksp[(int64_t)(min(n0 + 16 * j, n_end - 1) >> shift) * a.c.ss_n];
+  };
+  const auto stage_k = [&](int buf) {
     uint16_t* ks = Ks + buf * kTile * KSTR;
-    uint16_t* vt = Vt + buf * DH * kTile;
 #pragma unroll
     for (int p = 0; p < KP; ++p) {
       const int row = krow + p * (TH / KL);
@@ -506,21 +513,24 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
         }
       }
     }
+  };
+  const auto stage_v = [&](int buf) {
+    uint16_t* vt = Vt + buf * DH * kTile;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       const int row4 = vrow + p * (TH / VL);
       if (kTile / 4 * VL % TH == 0 || row4 < kTile / 4) {
         const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
+        uint16_t* to = vt + vd * kTile;
+        const uint32_t turned = col ^ (8 * v_piece(vd));          // of rows vd and vd + 1; of the next two the piece two further
         const auto put = [&](auto power) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
             const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
-            const int d = vd + 2 * c;
-            *reinterpret_cast<u32x2_t*>(vt + d * kTile + (col ^ (8 * v_piece(d)))) =
-                u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
-            *reinterpret_cast<u32x2_t*>(vt + (d + 1) * kTile + (col ^ (8 * v_piece(d + 1)))) =
-                u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
+            uint16_t* at = to + (c ? turned ^ 16 : turned) + 2 * c * kTile;
+            *reinterpret_cast<u32x2_t*>(at) = u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
+            *reinterpret_cast<u32x2_t*>(at + kTile) = u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
           }
         };
         if (__all((__float_as_uint(vscale[p]) & 0x7fffffu) == 0)) put(std::true_type{});
@@ -528,45 +538,46 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
       }
     }
   };
-
-  offsets(kTile);
-  if (n_begin < n_end) request(n_begin);
-  const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
-  int buf = 0;
-  for (int n0 = n_begin; n0 < n_end; n0 += kTile, buf ^= 1) {
-    stage(buf);
-    float f[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = kscale[j] * scale;
-    if (n0 + kTile < n_end) request(n0 + kTile);
-    __syncthreads();                     // this buffer is written; the other one is read by nobody any more
-    if (n0 >= wave_end) continue;
+  // Fragments are asked for ahead of the products: left to itself the compiler asks for each in front of its use.
+  const auto k_frags = [&](frag_t (&kf)[2][ST], int buf, int half) {       // of 32 of the tile's keys
     const uint16_t* ks = Ks + buf * kTile * KSTR;
-    const uint16_t* vt = Vt + buf * DH * kTile;
-    // all the fragments of K are asked for before the first product: left to itself the compiler asks for each in front of its use
-    f32x4_t s[MI][4];
-    frag_t kf[4][ST];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int st = 0; st < ST; ++st) kf[j][st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (16 * j + lr) * KSTR + 32 * st + 8 * lg));
-    __builtin_amdgcn_sched_barrier(0);
+      for (int st = 0; st < ST; ++st) kf[j][st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (32 * half + 16 * j + lr) * KSTR + 32 * st + 8 * lg));
+  };
+  const auto scores = [&](f32x4_t (&s)[MI][4], const frag_t (&kf)[2][ST], int half) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int st = 0; st < ST; ++st)
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) s[mi][j] = E::mfma(kf[j][st], qf[mi][st], st ? s[mi][j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
-    const auto v_frag = [&](int st, int t) {
-      const int d = 16 * t + lr;
-      return __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + d * kTile + ((32 * st + 8 * lg) ^ (8 * v_piece(d)))));
-    };
-    pfrag_t vf[2][NT];                   // those of V's first half during the softmax, of its second during the products with the first
+        for (int mi = 0; mi < MI; ++mi)
+          s[mi][2 * half + j] = E::mfma(kf[j][st], qf[mi][st], st ? s[mi][2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+  };
+  // row d = 16 t + lr of V: its piece is turned by (lr / 4) ^ (lr & 6) ^ 4 (t % 2), so two addresses and constants reach all of them
+  const uint32_t vread = lr * kTile + 8 * (lg ^ (lr >> 2) ^ (lr & 6));
+  const auto v_frags = [&](pfrag_t (&vf)[NT], int buf, int st) {
+    const uint16_t* vt = Vt + buf * DH * kTile;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) vf[0][t] = v_frag(0, t);
-    __builtin_amdgcn_sched_barrier(0);
-    const bool plain = n0 + kTile <= wave_sees;                    // every row of the wave sees the whole tile
-    pfrag_t ph[MI][2], pl[MI][2];
+    for (int t = 0; t < NT; ++t) vf[t] = __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + ((st ^ t) & 1 ? vread ^ 32 : vread) + 16 * t * kTile));
+  };
+  pfrag_t ph[MI][2], pl[MI][2];
+  const auto values = [&](const pfrag_t (&vf)[NT], int st) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) {
+        o[mi][t] = E16<0>::mfma(vf[t], ph[mi][st], o[mi][t]);
+        if (kRest) o[mi][t] = E16<0>::mfma(vf[t], pl[mi][st], o[mi][t]);
+      }
+  };
+  const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
+  const auto weights = [&](f32x4_t (&s)[MI][4], int n0, const float (&by)[4]) {
+    float f[4];
+    const bool plain = n0 + kTile <= wave_sees;                      // every row of the wave sees the whole tile
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = by[j] * scale;
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       float top = -INFINITY;
@@ -583,10 +594,10 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
             top = fmaxf(top, s[mi][j][i]);
           }
       }
-      top = column_max(top);
-      // The reference of the weights moves only where a score is kSlack over it: until then weights are up to 2^kSlack, which changes no rounding.
+      // The reference of the weights moves only where a score is kSlack over it: until then weights are up to 2^kSlack, which changes no rounding, and the
+      // lanes of a column need not agree on a maximum.
       if (__any(top > m_run[mi] + kSlack)) {
-        top = fmaxf(m_run[mi], top);
+        top = fmaxf(m_run[mi], column_max(top));
         const float keep = top > m_run[mi] ? __builtin_amdgcn_exp2f(m_run[mi] - top) : 1.f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[mi][t] *= keep;
@@ -625,18 +636,42 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
         if (kRest) pl[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
       }
     }
+  };
+
 #pragma unroll
-    for (int t = 0; t < NT; ++t) vf[1][t] = v_frag(1, t);
+  for (int p = 0; p < KP; ++p) koff[p] = k_offset(p, kTile);
+#pragma unroll
+  for (int p = 0; p < VP; ++p)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) voff[p][e] = v_offset(p, e, kTile);
+  const auto at = [&](int i) { return n_begin + i * kTile; };
+  const int n = n_begin < n_end ? (n_end - n_begin + kTile - 1) / kTile : 0;
+  if (n > 0) { request_k(n_begin); request_v(n_begin); request_f(n_begin); }
+  for (int i = 0; i < n; ++i) {
+    const int buf = i & 1;
+    stage_k(buf);
+    stage_v(buf);
+    float g[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = fs[j];
+    if (i + 1 < n) { request_k(at(i + 1)); request_v(at(i + 1)); request_f(at(i + 1)); }
+    __syncthreads();                   // this buffer is written; the other one is read by nobody any more
+    if (at(i) >= wave_end) continue;
+    f32x4_t s[MI][4];
+    frag_t kf[2][2][ST];
+    k_frags(kf[0], buf, 0);
+    k_frags(kf[1], buf, 1);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-          o[mi][t] = E16<0>::mfma(vf[st][t], ph[mi][st], o[mi][t]);
-          if (kRest) o[mi][t] = E16<0>::mfma(vf[st][t], pl[mi][st], o[mi][t]);
-        }
+    scores(s, kf[0], 0);
+    scores(s, kf[1], 1);
+    pfrag_t vf[2][NT];                 // those of V's first half during the softmax, of its second during the products with the first
+    v_frags(vf[0], buf, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    weights(s, at(i), g);
+    v_frags(vf[1], buf, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    values(vf[0], 0);
+    values(vf[1], 1);
   }
   // element i of tile t is dimension 16 t + 4 lg + i of row lr
   const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
@@ -670,14 +705,13 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   }
 }
 
-// Rows of a workgroup and key ranges of a chunk: 256 rows where they fill the chip, fewer below, and where 64 rows leave part of it idle, the keys in ranges.
+// Rows of a workgroup and key ranges of a chunk: 128 rows where those workgroups are one for each compute unit at least, else 64, and where these leave part of the
+// chip idle, the keys in ranges.
 struct PromptForm { int rows, ranges; };
 static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
   const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
-  const auto groups = [&](int bm) { return (list + bm - 1) / bm * pairs; };
-  if (groups(256) * 2 >= cu * 3) return {256, 1};
-  if (groups(128) >= cu) return {128, 1};
-  const int64_t n = groups(64);
+  if ((list + 127) / 128 * pairs >= cu) return {128, 1};
+  const int64_t n = (list + 63) / 64 * pairs;
   if (n * 2 > cu) return {64, 1};
   return {64, (int)max((int64_t)1, min((2 * cu + n - 1) / n, (int64_t)(S + 4 * kTile - 1) / (4 * kTile)))};
 }
@@ -703,7 +737,6 @@ static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
-  if (f.rows == 256) return prompt_launch<DT, DH, 2, 8>(fn, a, f.ranges, scratch, st);
   if (f.rows == 128) return prompt_launch<DT, DH, 2, 4>(fn, a, f.ranges, scratch, st);
   return prompt_launch<DT, DH, 1, 4>(fn, a, f.ranges, scratch, st);
 }
