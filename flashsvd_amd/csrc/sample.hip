@@ -11,7 +11,7 @@
 namespace fsvd {
 
 constexpr int kDrawThreads = 1024, kDrawWaves = kDrawThreads / kWave, kDrawRow = 1 << 24;
-constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64;      // two 16-bit counts a word; keys of a segment
+constexpr int kHistWords = 32768, kSegs = 1024, kSegBins = 64, kBatch = 8;      // two 16-bit counts a word; keys of a segment; segments of a wave
 constexpr int kMostExtra = kDrawRow / 32768;
 
 struct SampleArgs {
@@ -26,7 +26,6 @@ struct SampleArgs {
 
 // 16-bit patterns as unsigned numbers in the order of their values, two to a word: a negative pattern inverted, a positive one above all of them.  -0 comes
 // out next below +0 (its count is moved there), a NaN beyond the infinity of its sign.
-typedef double f64x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
 constexpr uint32_t kMinusZero = 0x7fffu, kZero = 0x8000u;
@@ -60,16 +59,36 @@ __device__ __forceinline__ double lane_value(double v, int l) {
   const u32x2_t w = __builtin_bit_cast(u32x2_t, v);
   return __builtin_bit_cast(double, u32x2_t{(uint32_t)__builtin_amdgcn_readlane(w.x, l), (uint32_t)__builtin_amdgcn_readlane(w.y, l)});
 }
-// e^x for -746 < x <= 0, to a few 2^-53: x = n ln 2 + r, the series of e^r to r^13 (|r| <= 0.347: the next term is 4e-18)
+// e^x for -746 < x <= 0, to a few 2^-53, by the reduction of Cody and Waite: x = n ln 2 + r with ln 2 in two parts, the first of 41 bits (n has eleven), and
+// the series of e^r to r^13 (|r| <= 0.347: the next term is 4e-18)
 __device__ __forceinline__ double exp_below(double x) {
   const double n = rint(x * 1.4426950408889634074);
-  double r = fma(n, -6.93147180369123816490e-01, x);      // ln 2 in two parts, the first of 32 bits
-  r = fma(n, -1.90821492927058770002e-10, r);
+  double r = fma(n, -0.693147180559663, x);
+  r = fma(n, -2.8235290563031577e-13, r);
   double y = 1. / 6227020800.;
 #pragma unroll
   for (const double c : {1. / 479001600., 1. / 39916800., 1. / 3628800., 1. / 362880., 1. / 40320., 1. / 5040., 1. / 720., 1. / 120., 1. / 24., 1. / 6., .5, 1., 1.})
     y = fma(y, r, c);
   return ldexp(y, (int)n);
+}
+// the halves (or rows of 16 lanes, by pairs) of two values change places and are added
+template <int LANES>
+__device__ __forceinline__ double swap_add(double x, double y) {
+  const u32x2_t a = __builtin_bit_cast(u32x2_t, x), b = __builtin_bit_cast(u32x2_t, y);
+  const uint32_t al = a.x, ah = a.y, bl = b.x, bh = b.y;
+  if constexpr (LANES == 32) {
+    const auto l = __builtin_amdgcn_permlane32_swap(al, bl, false, false), h = __builtin_amdgcn_permlane32_swap(ah, bh, false, false);
+    return __builtin_bit_cast(double, u32x2_t{l[0], h[0]}) + __builtin_bit_cast(double, u32x2_t{l[1], h[1]});
+  } else {
+    const auto l = __builtin_amdgcn_permlane16_swap(al, bl, false, false), h = __builtin_amdgcn_permlane16_swap(ah, bh, false, false);
+    return __builtin_bit_cast(double, u32x2_t{l[0], h[0]}) + __builtin_bit_cast(double, u32x2_t{l[1], h[1]});
+  }
+}
+__device__ __forceinline__ double row_sum(double v) {      // of 16 lanes, in each of them: rotations by 8, 4, 2, 1
+  v = dpp_add<0x128, 0xf>(v);
+  v = dpp_add<0x124, 0xf>(v);
+  v = dpp_add<0x122, 0xf>(v);
+  return dpp_add<0x121, 0xf>(v);
 }
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
 #pragma unroll
@@ -82,8 +101,10 @@ template <int DT, int R>
 __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a) {
   constexpr uint32_t kInf = DT == 1 ? 0x7c00u : 0x7f80u, kNegInf = kMinusZero - kInf, kLowest = kNegInf + 1, kHighest = kZero + kInf - 1;
   extern __shared__ __align__(16) uint32_t hist[];                       // [kHistWords]
-  __shared__ double seg_mass[kSegs], group_mass[kDrawWaves];             // from the largest values down
-  __shared__ uint32_t seg_count[kSegs], group_count[kDrawWaves], wave_a[kDrawWaves], wave_b[kDrawWaves], wave_kept[kDrawWaves], drawn_key, drawn_rank;
+  // the segments that hold something, from the largest values down: which, their masses, their counts with all before them
+  __shared__ __align__(16) uint16_t seg_at[kSegs + kBatch];
+  __shared__ double seg_mass[kSegs], group_mass[kDrawWaves];
+  __shared__ uint32_t seg_count[kSegs], wave_a[kDrawWaves], wave_b[kDrawWaves], wave_kept[kDrawWaves], drawn_key, drawn_rank;
   __shared__ uint16_t extra[kMostExtra];                                  // keys that hold 32768 more than their bin says, once for each
   __shared__ uint32_t n_extra;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -115,7 +136,6 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
     }
   };
   for (int i = tid; i < kHistWords / 4; i += kDrawThreads) reinterpret_cast<u32x4_t*>(hist)[i] = u32x4_t{0u, 0u, 0u, 0u};
-  for (int i = tid; i < kSegs; i += kDrawThreads) { seg_mass[i] = 0.; seg_count[i] = 0; }
   if (tid == 0) n_extra = 0;
   if constexpr (R > 0) {
 #pragma unroll
@@ -177,7 +197,7 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
     all_pieces([&](int, u32x4_t v) { count_up(v); });
     if (R == 0 || R > 8) {
       mine = wave_scan(mine);
-      if (lane == 63) wave_a[wave] = mine;
+      if (lane == 63) wave_kept[wave] = mine;
     }
     __syncthreads();
     constexpr bool kMayRunOver = R == 0 || R > 8;        // rows of more than 65535
@@ -189,25 +209,38 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
     const auto bin = [&](uint32_t k) { return counts(k, (hist[k >> 1] >> (16 * (k & 1))) & 0xffffu); };
     // the count of -0 belongs to 0
     const auto merged = [&](uint32_t s, uint32_t k, uint32_t n) {
-      if (s == kMinusZero / kSegBins) return k == kMinusZero ? 0u : n;
-      if (s == kZero / kSegBins) return k == kZero ? n + bin(kMinusZero) : n;
+      if (s - kMinusZero / kSegBins <= 1) n = k == kMinusZero ? 0u : k == kZero ? n + bin(kMinusZero) : n;
       return n;
     };
     const double per = 1. / fmax(temp, 1e-280);
     const auto weight = [&](uint32_t k) { return exp_below(((double)key_value<DT>(k) - high) * per); };
+    // what a thread's segment holds, read in an order that spreads the lanes over the banks
+    const int last_seg = (int)(most / kSegBins), seg = kSegs - 1 - tid;
+    const bool in_range = kSegs - wave * kWave > (int)(least / kSegBins) && kSegs - wave * kWave - kWave <= last_seg;
+    const auto counted_here = [&] {
+      uint32_t n = 0;
+      if (in_range) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const u32x4_t w = reinterpret_cast<const u32x4_t*>(hist)[seg * 8 + ((j + (seg >> 1)) & 7)];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t x = w[e];
+            n = __builtin_amdgcn_udot2(__builtin_bit_cast(u16x2_t, x), u16x2_t{1, 1}, n, false);
+          }
+        }
+      }
+      return n;
+    };
+    uint32_t here = counted_here();
     if (kMayRunOver) {
       // A 16-bit count runs over where more than 65535 logits are equal, and all of them come to less then than there are.  The row is counted again in
       // steps that cannot, and after each what exceeds 32767 is set aside.
-      uint32_t there = 0, sum = 0, counted = 0;
-#pragma unroll
-      for (int i = 0; i < kHistWords / 4; i += kDrawThreads) {
-        const u32x4_t w = reinterpret_cast<const u32x4_t*>(hist)[i + tid];
-        sum += (w.x & 0xffffu) + (w.x >> 16) + (w.y & 0xffffu) + (w.y >> 16) + (w.z & 0xffffu) + (w.z >> 16) + (w.w & 0xffffu) + (w.w >> 16);
-      }
-      sum = lane_value(wave_scan(sum), 63);
+      const uint32_t sum = lane_value(wave_scan(here), 63);
       if (lane == 0) wave_b[wave] = sum;
       __syncthreads();
-      for (int i = 0; i < kDrawWaves; ++i) { there += wave_b[i]; counted += wave_a[i]; }
+      uint32_t there = 0, counted = 0;
+      for (int i = 0; i < kDrawWaves; ++i) { there += wave_b[i]; counted += wave_kept[i]; }
       if (there != counted) {
         for (int i = tid; i < kHistWords; i += kDrawThreads) hist[i] = 0;
         for (int c0 = 0; c0 < pieces; c0 += 4095) {
@@ -223,94 +256,114 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
         }
         __syncthreads();
         extras = n_extra;
+        here = counted_here();
+        for (uint32_t i = 0; i < extras; ++i) here += extra[i] / kSegBins == seg ? 32768u : 0u;
       }
     }
-    // Sums over segments of 64 keys.  A wave asks for the counts of every 16th of 256 segments at once (those that hold something stand side by side, so
-    // the waves share them); the sums over the lanes come from the matrix cores, in 64 bits: a segment's masses are the rows, and a column of ones puts
-    // their sums into the segment's own column.
+    if (seg == kMinusZero / kSegBins) here -= bin(kMinusZero);
+    if (seg == kZero / kSegBins) here += bin(kMinusZero);
+    const uint64_t some = __ballot(here != 0);
+    const uint32_t run_here = wave_scan(here);
+    if (kMayRunOver) __syncthreads();                     // all have read wave_b
+    if (lane == 63) { wave_a[wave] = __popcll(some); wave_b[wave] = run_here; }
+    __syncthreads();
+    uint32_t segs = 0, run_c = 0, seg_before = 0, c_before = 0;
+#pragma unroll
+    for (int i = 0; i < kDrawWaves; ++i) {
+      if (i == wave) { seg_before = segs; c_before = run_c; }
+      segs += wave_a[i];
+      run_c += wave_b[i];
+    }
+    if (here) {
+      const uint32_t at = seg_before + __popcll(some & ((1ull << lane) - 1));
+      seg_at[at] = (uint16_t)seg;
+      seg_count[at] = c_before + run_here;
+    }
+    if (tid < kBatch) seg_at[segs + tid] = 0;             // a segment that is never counted
+    __syncthreads();
+    // Masses of the segments, eight at a time for a wave.  The values of a segment are evenly spaced, and those of all segments of an exponent alike, so a
+    // key's weight is that of its segment's last one times what the way there makes: one exponential of a wave for its eight segments, and one for the lanes
+    // at each exponent.  (In the segment of the largest, that one stands in for the last: its weight is 1 as it has to be, and nothing runs over.)
     uint32_t kept = 0;
-    constexpr int kAsk = 16, kStep = kAsk * kDrawWaves;
-    const int last_seg = (int)(most / kSegBins);
-    for (int s0 = (int)(least / kSegBins) / kStep * kStep + wave; s0 <= last_seg; s0 += kStep) {
-      const uint16_t* counts16 = reinterpret_cast<const uint16_t*>(hist) + s0 * kSegBins + lane;
-      constexpr int kNext = kDrawWaves * kSegBins;
-      uint32_t raw[kAsk];
+    constexpr int kExponent = (DT == 1 ? 1024 : 128) / kSegBins;
+    const auto below = [&](uint32_t k, double top) { return exp_below(fmin(fmax(((double)key_value<DT>(k) - top) * per, -700.), 0.)); };
+    const auto last_key = [&](int s) { return s == last_seg ? most : (uint32_t)s * kSegBins + kSegBins - 1; };
+    const int my = 2 * (lane >> 4) + (lane & 1);          // whose sum ends in this lane
+    for (uint32_t b0 = wave * kBatch; b0 < segs; b0 += kDrawWaves * kBatch) {
+      const uint16_t* counts16 = reinterpret_cast<const uint16_t*>(hist) + lane;
+      int s[kBatch];
+      uint32_t n[kBatch];
+      const u32x4_t at = *reinterpret_cast<const u32x4_t*>(seg_at + b0);
 #pragma unroll
-      for (int i = 0; i < kAsk; ++i) raw[i] = counts16[i * kNext];
-      uint32_t some = 0;                                  // segments with a count, and those whose counts are not all in their bins
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t w = at[i >> 1];
+        s[i] = __builtin_amdgcn_readfirstlane(i & 1 ? w >> 16 : w & 0xffffu);
+        n[i] = counts16[s[i] * kSegBins];
+      }
+      const double seg_weight = below(last_key(seg_at[b0 + my]), high);
+      double lane_weight = 0., m[kBatch];
+      int exponent = -1;
 #pragma unroll
-      for (int i = 0; i < kAsk; ++i) some |= __any(raw[i] != 0) ? 1u << i : 0u;
-      const auto also = [&](int s) {
-        s -= s0;
-        if (s >= 0 && s < kStep && s % kDrawWaves == 0) some |= 1u << (s / kDrawWaves);
-      };
-      also(kZero / kSegBins);
-      for (uint32_t i = 0; kMayRunOver && i < extras; ++i) also(extra[i] / kSegBins);
-      f64x4_t mass = {0., 0., 0., 0.};
-      f32x4_t count = {0.f, 0.f, 0.f, 0.f};               // whole numbers up to 2^24
-      while (some) {
-        const int i = __builtin_ctz(some), s = s0 + i * kDrawWaves;
-        some &= some - 1;
-        const uint32_t k = s * kSegBins + lane, n = merged(s, k, counts(k, counts16[i * kNext]));
-        const bool own = (lane & 15) == i;
-        const double w = n ? weight(k) : 0.;
-        if (min_p > 0.) kept += w >= min_p ? n : 0;
-        mass = __builtin_amdgcn_mfma_f64_16x16x4f64(n * w, own ? 1. : 0., mass, 0, 0, 0);
-        count = __builtin_amdgcn_mfma_f32_16x16x4f32((float)n, own ? 1.f : 0.f, count, 0, 0, 0);
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t k = s[i] * kSegBins + lane;
+        const int e = s[i] == last_seg ? kSegs : s[i] / kExponent;
+        if (e != exponent) {
+          exponent = e;
+          lane_weight = below(k, (double)key_value<DT>(last_key(s[i])));
+        }
+        const uint32_t c = merged(s[i], k, counts(k, n[i]));
+        if (min_p > 0.) kept += lane_weight * lane_value(seg_weight, (i >> 1) * 16 + (i & 1)) >= min_p ? c : 0;
+        m[i] = c * lane_weight;
       }
-      double m = (mass[0] + mass[1]) + (mass[2] + mass[3]);
-      float c = (count[0] + count[1]) + (count[2] + count[3]);
-      m += __shfl_xor(m, 16); c += __shfl_xor(c, 16);
-      m += __shfl_xor(m, 32); c += __shfl_xor(c, 32);
-      if (lane < kAsk) {
-        const int at = kSegs - 1 - (s0 + lane * kDrawWaves);
-        seg_mass[at] = m;
-        seg_count[at] = (uint32_t)c;
-      }
+      // sums over the lanes: halves, then rows of 16 lanes change places with those of another segment and are added; a row adds up by rotations
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = swap_add<32>(m[i], m[i + 4]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) m[i] = row_sum(swap_add<16>(m[i], m[i + 2]));
+      if ((lane & 15) < 2 && b0 + my < segs) seg_mass[b0 + my] = (lane & 1 ? m[1] : m[0]) * seg_weight;
     }
     kept = wave_scan(kept);
     if (lane == 63) wave_kept[wave] = kept;
     __syncthreads();
     // running sums of groups of 64 segments, a wave each
-    const double gm = wave_scan(seg_mass[tid]);
-    const uint32_t gc = wave_scan(seg_count[tid]);
+    const double gm = wave_scan((uint32_t)tid < segs ? seg_mass[tid] : 0.);
     seg_mass[tid] = gm;
-    seg_count[tid] = gc;
-    if (lane == 63) { group_mass[wave] = gm; group_count[wave] = gc; }
+    if (lane == 63) group_mass[wave] = gm;
     __syncthreads();
     if (wave == 0) {
       double run_m = 0., to_m = 0.;                     // lane i: up to group i
-      uint32_t run_c = 0, to_c = 0, likely = 0;
+      uint32_t likely = 0;
 #pragma unroll
       for (int i = 0; i < kDrawWaves; ++i) {
         run_m += group_mass[i];
-        run_c += group_count[i];
         likely += wave_kept[i];
-        if (lane == i) { to_m = run_m; to_c = run_c; }
+        if (lane == i) to_m = run_m;
       }
+      const bool is_group = lane * kWave < (int)segs;
+      const uint32_t to_c = is_group ? seg_count[min(lane * kWave + kWave, (int)segs) - 1] : 0;
       // The n-th of the order, where n is the smallest with C_n > target (by_mass) or given: its key, how many of its key are up to it, n and C_n.  Where
       // rounding leaves no C above the target, the last that there is.
       uint32_t at_key = 0, at_rank = 0, at_n = 0;
       double at_mass = 0.;
       const auto locate = [&](bool by_mass, double target, uint32_t n) {
-        const auto first = [&](bool in, double m, uint32_t c, uint32_t before) {
-          const uint64_t hit = __ballot(in && (by_mass ? m > target : c >= n)), some = __ballot(in && c > before);
-          return hit ? __builtin_ctzll(hit) : some ? 63 - __builtin_clzll(some) : 0;
+        const auto first = [&](bool in, double m, uint32_t c) {
+          const uint64_t hit = __ballot(in && (by_mass ? m > target : c >= n)), some = __ballot(in);
+          return hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some | 1);
         };
-        const auto shifted = [&](uint32_t c) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)c, 0x138, 0xf, 0xf, false); };      // from the lane before
-        const int g = first(lane < kDrawWaves, to_m, to_c, shifted(to_c));
+        const int g = first(is_group, to_m, to_c);
         const double m0 = g ? lane_value(to_m, g - 1) : 0.;
         const uint32_t c0 = g ? lane_value(to_c, g - 1) : 0;
+        const bool is_seg = (uint32_t)(g * kWave + lane) < segs;
         const double ms = m0 + seg_mass[g * kWave + lane];
-        const uint32_t cs = c0 + seg_count[g * kWave + lane], cp = shifted(cs);
-        const int t = first(true, ms, cs, lane ? cp : c0);
+        const uint32_t cs = is_seg ? seg_count[g * kWave + lane] : 0;
+        const int t = first(is_seg, ms, cs);
         const double m1 = t ? lane_value(ms, t - 1) : m0;
         const uint32_t c1 = t ? lane_value(cs, t - 1) : c0;
-        const uint32_t k = (kSegs - 1 - (g * kWave + t)) * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(k / kSegBins, k, bin(k)) : 0;
+        const uint32_t s = seg_at[g * kWave + t], k = s * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(s, k, bin(k)) : 0;
         const double w = c ? weight(k) : 0., m = c * w, mk = m1 + wave_scan(m);
         const uint32_t ck = c1 + wave_scan(c);
         const bool found = __any(c && (by_mass ? mk > target : ck >= n));
-        const int l = first(c != 0, mk, ck, ck - c);
+        const int l = first(c != 0, mk, ck);
         uint32_t j = c;
         if (found) j = by_mass ? (uint32_t)fmin(fmax(floor((target - (mk - m)) / w), 0.) + 1., (double)c) : n - (ck - c);
         at_key = lane_value(k, l);
