@@ -1,6 +1,8 @@
 // Shared device helpers for the gfx950 kernels: bf16 packing, wave64 reductions,
 // status codes of the C ABI.
 #pragma once
+#include <atomic>
+
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -23,6 +25,18 @@ enum Status : int {
 
 void set_last_error(const char* fmt, ...);
 void set_last_form(const char* name);   // of static storage: what fsvd_last_form() reports
+
+// Dynamic LDS of more than 64 KB, asked for once for a kernel and device (a bit of `granted`; devices from 32 on ask each time).
+inline int grant_lds(const char* fn, const void* kernel, size_t bytes, std::atomic<uint32_t>& granted) {
+  int dev = -1;
+  hipError_t e = hipGetDevice(&dev);
+  const uint32_t bit = e == hipSuccess && dev < 32 ? 1u << dev : 0;
+  if (granted.load(std::memory_order_relaxed) & bit) return kOk;
+  if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != hipSuccess) { set_last_error("%s: cannot reserve %zu bytes of LDS: %s", fn, bytes, hipGetErrorString(e)); return kErrLaunch; }
+  granted.fetch_or(bit, std::memory_order_relaxed);
+  return kOk;
+}
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));

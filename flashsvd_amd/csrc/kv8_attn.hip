@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges
   if (!live || part_of || (a.rows && m >= a.rows[b])) return;
   uint16_t* o = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + lane * D;
 #pragma unroll
-  for (int i = 0; i < D; ++i) o[i] = (uint16_t)E::bits(sum > 0.f ? v[i] / sum : 0.f);
+  for (int i = 0; i < D; ++i) o[i] = (uint16_t)E::bits(sum == 0.f ? 0.f : v[i] / sum);
 }
 template <int DT, int DH>
 static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* scratch, hipStream_t st) {
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8Att
   int id = blockIdx.x - turn * pairs;
   const int gg = id % GG; id /= GG;
   const int b = id / a.c.Hk, hk = id - b * a.c.Hk;
-  const int pos = a.positions[b], keys = max(0, min(pos + a.key_add, a.c.S));
+  const int pos = a.positions[b], keys = (int)max((int64_t)0, min((int64_t)pos + a.key_add, (int64_t)a.c.S));
   const int per = kv8_range(keys, ranges), used = max(1, (keys + per - 1) / per), s = turn < used ? used - 1 - turn : turn;
   const int k0 = min(s * per, keys), k1 = min(k0 + per, keys);
   const int h0 = hk * G + gg * kDecGroup, heads = min(kDecGroup, G - gg * kDecGroup);
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8Att
       v += f * os[(w * heads + q) * (DH + 4) + d];
     }
     if (ranges == 1) {
-      a.out[(int64_t)b * a.so_b + (int64_t)(h0 + q) * a.so_h + d] = (uint16_t)E::bits(sum > 0.f ? v / sum : 0.f);
+      a.out[(int64_t)b * a.so_b + (int64_t)(h0 + q) * a.so_h + d] = (uint16_t)E::bits(sum == 0.f ? 0.f : v / sum);
     } else {
       const int64_t row = (int64_t)b * a.H + h0 + q;
       part.values(row, s)[d] = v;
@@ -390,6 +390,8 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   extern __shared__ __align__(16) unsigned char smem[];
   uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile][KSTR]
   uint16_t* Vt = Ks + 2 * kTile * KSTR;                                     // [2][DH][kTile]
+  __shared__ __align__(16) int nan_at[DH];                                  // the first NaN of a dimension among the values that not every row sees
+  __shared__ int any_nan;
 
   const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
   int mt, hb;
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
   const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
   if (row0 >= rows) return;
-  const int pos = a.positions[b];
+  const int pos = min(a.positions[b], 0x7ffffffe - a.M);
   const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
   const int all_end = seen_by(min(row0 + BM, rows) - 1);
   const int tiles = (all_end + kTile - 1) / kTile, per = (tiles + ranges - 1) / ranges;
@@ -511,6 +513,27 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
           *reinterpret_cast<u32x4_t*>(ks + row * KSTR + kd + 8 * h) = u32x4_t{Code16<DT>::template pair<false>(x), Code16<DT>::template pair<true>(x),
                                                                               Code16<DT>::template pair<false>(y), Code16<DT>::template pair<true>(y)};
         }
+      }
+    }
+  };
+  // A masked key has weight zero, and zero times a NaN is one: where not every row sees the whole tile, a NaN is staged as zero and put into the rows that see
+  // it at the end.
+  const int all_see = seen_by(row0);
+  const auto set_nans_aside = [&](int n0) {
+#pragma unroll
+    for (int p = 0; p < VP; ++p) {
+      const int row = 4 * (vrow + p * (TH / VL));
+      if (kTile / 4 * VL % TH != 0 && row >= kTile) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t nan = ((vreg[p][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        if (nan == 0) continue;
+        any_nan = 1;
+        for (int i = 0; i < 4; ++i)
+          if (nan >> (8 * i + 7) & 1) {
+            atomicMin(&nan_at[vd + i], n0 + row + e);
+            vreg[p][e] &= ~(0xffu << 8 * i);
+          }
       }
     }
   };
@@ -647,9 +670,13 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   const auto at = [&](int i) { return n_begin + i * kTile; };
   const int n = n_begin < n_end ? (n_end - n_begin + kTile - 1) / kTile : 0;
   if (n > 0) { request_k(n_begin); request_v(n_begin); request_f(n_begin); }
+  for (int d = tid; d < DH; d += TH) nan_at[d] = 0x7fffffff;
+  if (tid == 0) any_nan = 0;
+  __syncthreads();
   for (int i = 0; i < n; ++i) {
     const int buf = i & 1;
     stage_k(buf);
+    if (at(i) + kTile > all_see) set_nans_aside(at(i));
     stage_v(buf);
     float g[4];
 #pragma unroll
@@ -680,6 +707,13 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
     const int r = w0 + 16 * mi + lr;
     const float l = column_sum(l_run[mi]);
     if (r >= rows) continue;
+    if (any_nan) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (nan_at[16 * t + 4 * lg + i] < seen[mi]) o[mi][t][i] = __builtin_nanf("");
+    }
     if (ranges > 1) {
       const Kv8Parts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
       const int64_t row = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
@@ -723,12 +757,8 @@ size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
 template <int DT, int DH, int MI, int NW>
 static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   constexpr size_t lds = 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
-  static bool granted = lds <= 65536;
-  if (!granted) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-    if (e != hipSuccess) { set_last_error("%s: cannot reserve %zu bytes of LDS: %s", fn, lds, hipGetErrorString(e)); return kErrLaunch; }
-    granted = true;
-  }
+  static std::atomic<uint32_t> granted{0};
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW>), lds, granted) : kOk) return rc;
   const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * NW - 1) / (16 * MI * NW) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
   hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, NW>), dim3((unsigned)groups, ranges), dim3(NW * kWave), lds, st, a, ranges, scratch);

@@ -440,12 +440,8 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
 
 template <int DT, int R>
 static int launch_sample(const char* fn, const SampleArgs& a, int B, hipStream_t st) {
-  static bool granted = false;
-  if (!granted) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sample_token_kernel<DT, R>), hipFuncAttributeMaxDynamicSharedMemorySize, kHistWords * 4);
-    if (e != hipSuccess) { set_last_error("%s: cannot reserve %d bytes of LDS: %s", fn, kHistWords * 4, hipGetErrorString(e)); return kErrLaunch; }
-    granted = true;
-  }
+  static std::atomic<uint32_t> granted{0};
+  if (const int rc = grant_lds(fn, reinterpret_cast<const void*>(&sample_token_kernel<DT, R>), kHistWords * 4, granted)) return rc;
   hipLaunchKernelGGL((sample_token_kernel<DT, R>), dim3(B), dim3(kDrawThreads), kHistWords * 4, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }

@@ -275,6 +275,79 @@ def test_prompt_attention(dt, Dh, H, Hk, block, layout, M, start, rows):
         assert not bool(zeros[b, n[b]:].any())
 
 
+@pytest.mark.parametrize("Dh,H,Hk,M,start", [
+    (128, 32, 32, 130, [0, 3, 64, 200]),       # 128 rows of a workgroup
+    (64, 64, 32, 70, [0, 1, 31, 77]),
+    (128, 40, 40, 50, [5, 0, 63, 64]),         # 64 rows, no key ranges
+])
+def test_prompt_attention_of_many_heads(Dh, H, Hk, M, start):
+    from flashsvd_amd import hip_ops
+    dt, B = torch.float16, len(start)
+    c = Cache(B, max(start) + M, Hk, Dh, 32, seed=M).finite()
+    g = torch.Generator().manual_seed(14)
+    q = (torch.randn(B, M, H, Dh, generator=g) * 0.7).to(dt)
+    out = hip_ops.attn_prefill_kv8(q.cuda(), *c.t, torch.tensor(start, dtype=torch.int32, device="cuda"), block=32).cpu()
+    picked = [(0, 0), (0, M - 1), (1, 15), (1, 16), (2, 63 if M > 63 else 31), (3, M // 2), (3, M - 1)]
+    _check_rows(c, torch.stack([q[b, m] for b, m in picked]), torch.stack([out[b, m] for b, m in picked]),
+                [(b, start[b] + m + 1) for b, m in picked], Dh ** -0.5, dt, what="prompt")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Dh,H,Hk,M,start,B", [(128, 2, 1, 90, 37, 1), (64, 3, 3, 40, 100, 2), (128, 32, 32, 130, 3, 4), (64, 4, 2, 70, 400, 1)])
+def test_a_nan_stays_in_what_sees_it(dt, Dh, H, Hk, M, start, B):
+    """A NaN among the values of a later token leaves the rows before it as they are, in every dimension; so does one among its keys."""
+    from flashsvd_amd import hip_ops
+    S = start + M
+    clean = Cache(B, S, Hk, Dh, 16, seed=41).finite()
+    g = torch.Generator().manual_seed(42)
+    q = (torch.randn(B, M, H, Dh, generator=g) * 0.7).to(dt)
+    pos = torch.full((B,), start, dtype=torch.int32, device="cuda")
+    marks = [(0, start + 11, 0, 5), (0, start + 30, 0, 0), (0, start + 12, 0, 5), (B - 1, start + M - 1, Hk - 1, Dh - 1), (B - 1, start, Hk - 1, 2)]
+    for b, n, hk, d in marks:                             # the clean cache holds zeros there: what else goes into the sums is alike
+        clean.t[1].view(torch.uint8)[b, n, hk, d] = 0
+    c = Cache(B, S, Hk, Dh, 16, seed=41).finite()
+    for t, u in zip(c.t, clean.t):
+        t.copy_(u) if t.dtype is not F8 else t.view(torch.uint8).copy_(u.view(torch.uint8))
+    for b, n, hk, d in marks:
+        c.t[1].view(torch.uint8)[b, n, hk, d] = 0xff if d else 0x7f
+    want, got = (hip_ops.attn_prefill_kv8(q.cuda(), *x.t, pos, block=16).float().cpu() for x in (clean, c))
+    per = H // Hk
+    for b, n, hk, d in marks:
+        want[b, n - start:, hk * per:(hk + 1) * per, d] = float("nan")
+    assert _same(got.double(), want.double())
+    one, seen = torch.full((B,), start + 12, dtype=torch.int32, device="cuda"), hip_ops.attn_decode_kv8
+    want, got = (seen(q[:, 0].cuda(), *x.t, one, block=16).float().cpu() for x in (clean, c))
+    for b, n, hk, d in marks:
+        if n < start + 12:
+            want[b, hk * per:(hk + 1) * per, d] = float("nan")
+    assert _same(got.double(), want.double())
+
+    base = hip_ops.attn_prefill_kv8(q.cuda(), *clean.t, pos, block=16).float().cpu()
+    clean.t[0].view(torch.uint8)[0, start + 20, 0, 3] = 0x7f
+    got = hip_ops.attn_prefill_kv8(q.cuda(), *clean.t, pos, block=16).float().cpu()
+    assert bool(got[0, 20:, :per].isnan().all())
+    assert torch.equal(got[0, :20], base[0, :20]) and torch.equal(got[0, :, per:], base[0, :, per:]) and torch.equal(got[1:], base[1:])
+    for n, nsplit in ((start + 20, 0), (start + 21, 0), (start + 21, 1)):
+        got = seen(q[:, 0].cuda(), *clean.t, torch.full((B,), n, dtype=torch.int32, device="cuda"), block=16, nsplit=nsplit or None).float().cpu()
+        assert bool(got[0, :per].isnan().all()) == (n > start + 20) and not bool(got[0, per:].isnan().any() or got[1:].isnan().any())
+
+
+def test_positions_at_the_end_of_the_integers():
+    """Lengths and positions far beyond the cache see all of it."""
+    from flashsvd_amd import hip_ops
+    c = Cache(3, 40, 1, 64, 16, seed=51).finite()
+    g = torch.Generator().manual_seed(52)
+    q = (torch.randn(3, 9, 2, 64, generator=g) * 0.7).to(torch.bfloat16).cuda()
+    far, end = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 5], [40, 0, 40]))
+    for add in (0, 1, 100):
+        want = hip_ops.attn_decode_kv8(q[:, 0], *c.t, end, block=16)
+        got = hip_ops.attn_decode_kv8(q[:, 0], *c.t, far, block=16, seqlen_add=add)
+        assert torch.equal(got, want) and not bool(got[1].any())
+    near = torch.tensor([39, -9, 39], dtype=torch.int32, device="cuda")
+    got, want = (hip_ops.attn_prefill_kv8(q, *c.t, n, block=16) for n in (far, near))
+    assert torch.equal(got, want) and not bool(got[1].any()) and bool(got[0].any())
+
+
 # ------------------------------------------------------------------ together
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 def test_a_decode_loop_captured_and_not(dt):
