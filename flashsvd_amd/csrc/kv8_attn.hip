@@ -527,13 +527,12 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t nan = ((vreg[p][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-        if (nan == 0) continue;
+        if (__builtin_expect(!__any(nan != 0), 1)) continue;
         any_nan = 1;
+#pragma unroll 1
         for (int i = 0; i < 4; ++i)
-          if (nan >> (8 * i + 7) & 1) {
-            atomicMin(&nan_at[vd + i], n0 + row + e);
-            vreg[p][e] &= ~(0xffu << 8 * i);
-          }
+          if (nan >> (8 * i + 7) & 1) atomicMin(&nan_at[vd + i], n0 + row + e);
+        vreg[p][e] &= ~((nan >> 7) * 0xffu);
       }
     }
   };
