@@ -378,8 +378,8 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
   return pack_bf16x2(x[0] * scale, x[1] * scale);
 }
 
-template <int DT, int DH, int MI, int NW>
-__global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
+template <int DT, int DH, int MI, int NW, int KG>
+__global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef typename E::frag_t frag_t;
   typedef E16<0>::frag_t pfrag_t;
@@ -388,7 +388,8 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   constexpr int VL = DH / 4, VP = (kTile / 4 * VL + TH - 1) / TH;
   constexpr bool kRest = DT == 1;
   extern __shared__ __align__(16) unsigned char smem[];
-  uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile][KSTR]
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
+  uint16_t* Ks = reinterpret_cast<uint16_t*>(smem) + kg * 2 * kTile * (KSTR + DH);      // [2][kTile][KSTR]
   uint16_t* Vt = Ks + 2 * kTile * KSTR;                                     // [2][DH][kTile]
   __shared__ __align__(16) int nan_at[DH];                                  // the first NaN of a dimension among the values that not every row sees
   __shared__ int any_nan;
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   }
   mt = MT - 1 - mt;
   const int hk = hb / a.B, b = hb - hk * a.B, range = blockIdx.y;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
+  const int tid = threadIdx.x % TH, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
   const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
   if (row0 >= rows) return;
   const int pos = min(a.positions[b], 0x7ffffffe - a.M);
@@ -666,23 +667,25 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   for (int p = 0; p < VP; ++p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) voff[p][e] = v_offset(p, e, kTile);
-  const auto at = [&](int i) { return n_begin + i * kTile; };
-  const int n = n_begin < n_end ? (n_end - n_begin + kTile - 1) / kTile : 0;
-  if (n > 0) { request_k(n_begin); request_v(n_begin); request_f(n_begin); }
+  const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile; };
+  const int all = n_begin < n_end ? (n_end - n_begin + kTile - 1) / kTile : 0, n = (all - kg + KG - 1) / KG;      // of the workgroup, of this half
+  if (n > 0) { request_k(at(0)); request_v(at(0)); request_f(at(0)); }
   for (int d = tid; d < DH; d += TH) nan_at[d] = 0x7fffffff;
   if (tid == 0) any_nan = 0;
   __syncthreads();
-  for (int i = 0; i < n; ++i) {
+  for (int i = 0; i * KG < all; ++i) {
     const int buf = i & 1;
-    stage_k(buf);
-    if (at(i) + kTile > all_see) set_nans_aside(at(i));
-    stage_v(buf);
+    if (KG == 1 || i < n) {
+      stage_k(buf);
+      if (at(i) + kTile > all_see) set_nans_aside(at(i));
+      stage_v(buf);
+    }
     float g[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[j] = fs[j];
     if (i + 1 < n) { request_k(at(i + 1)); request_v(at(i + 1)); request_f(at(i + 1)); }
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
-    if (at(i) >= wave_end) continue;
+    if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
     f32x4_t s[MI][4];
     frag_t kf[2][2][ST];
     k_frags(kf[0], buf, 0);
@@ -698,6 +701,25 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
     __builtin_amdgcn_sched_barrier(0);
     values(vf[0], 0);
     values(vf[1], 1);
+  }
+  if constexpr (KG > 1) {                // the halves' results
+    static_assert(KG == 2 && MI == 1, "one exchange");
+    f32x4_t* part = reinterpret_cast<f32x4_t*>(smem) + wave * (NT + 1) * kWave + lane;
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) part[t * kWave] = o[0][t];
+      part[NT * kWave] = f32x4_t{m_run[0], l_run[0], 0.f, 0.f};
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const f32x4_t other = part[NT * kWave];
+    const float top = fmaxf(m_run[0], other[0]);
+    const float f0 = m_run[0] > -INFINITY ? __builtin_amdgcn_exp2f(m_run[0] - top) : 0.f, f1 = other[0] > -INFINITY ? __builtin_amdgcn_exp2f(other[0] - top) : 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[0][t] = o[0][t] * f0 + part[t * kWave] * f1;
+    l_run[0] = l_run[0] * f0 + other[1] * f1;
+    m_run[0] = top;
   }
   // element i of tile t is dimension 16 t + 4 lg + i of row lr
   const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
@@ -738,36 +760,37 @@ __global__ __launch_bounds__(kWave * NW, 2) void kv8_prompt_kernel(Kv8AttnArgs a
   }
 }
 
-// Rows of a workgroup and key ranges of a chunk: 128 rows where those workgroups are one for each compute unit at least, else 64, and where these leave part of the
-// chip idle, the keys in ranges.
-struct PromptForm { int rows, ranges; };
+// Rows of a workgroup, its halves and key ranges of a chunk: 128 rows where those workgroups are one for each compute unit at least, else 64; where these are no
+// more than the compute units, two halves with every other tile, and where they leave part of the chip idle, the keys in ranges.
+struct PromptForm { int rows, halves, ranges; };
 static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
   const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
-  if ((list + 127) / 128 * pairs >= cu) return {128, 1};
+  if ((list + 127) / 128 * pairs >= cu) return {128, 1, 1};
   const int64_t n = (list + 63) / 64 * pairs;
-  if (n * 2 > cu) return {64, 1};
-  return {64, (int)max((int64_t)1, min((2 * cu + n - 1) / n, (int64_t)(S + 4 * kTile - 1) / (4 * kTile)))};
+  if (n > cu) return {64, 1, 1};
+  return {64, 2, (int)max((int64_t)1, min(cu / n, (int64_t)(S + 4 * kTile - 1) / (4 * kTile)))};
 }
 size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   const PromptForm f = prompt_form(B, M, H, Hk, S);
   return f.ranges > 1 ? Kv8Parts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
-template <int DT, int DH, int MI, int NW>
+template <int DT, int DH, int MI, int NW, int KG>
 static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
-  constexpr size_t lds = 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
+  constexpr size_t lds = KG * 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
   static std::atomic<uint32_t> granted{0};
-  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW>), lds, granted) : kOk) return rc;
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW, KG>), lds, granted) : kOk) return rc;
   const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * NW - 1) / (16 * MI * NW) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
-  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, NW>), dim3((unsigned)groups, ranges), dim3(NW * kWave), lds, st, a, ranges, scratch);
+  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, NW, KG>), dim3((unsigned)groups, ranges), dim3(NW * KG * kWave), lds, st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, false, scratch, st);
   return kOk;
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
-  if (f.rows == 128) return prompt_launch<DT, DH, 2, 4>(fn, a, f.ranges, scratch, st);
-  return prompt_launch<DT, DH, 1, 4>(fn, a, f.ranges, scratch, st);
+  if (f.rows == 128) return prompt_launch<DT, DH, 2, 4, 1>(fn, a, f.ranges, scratch, st);
+  if (f.halves == 1) return prompt_launch<DT, DH, 1, 4, 1>(fn, a, f.ranges, scratch, st);
+  return prompt_launch<DT, DH, 1, 4, 2>(fn, a, f.ranges, scratch, st);
 }
 int launch_kv8_prompt(const char* fn, const Kv8AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
   const PromptForm f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);
