@@ -144,6 +144,18 @@ static int check_call(const char* fn, int B, int dtype, const void* cos, const v
   if ((cos == nullptr) != (sin == nullptr) || (cos != nullptr && rope_len <= 0)) { set_last_error("%s: cos and sin go together, with rope_len rows", fn); return kErrNullPtr; }
   return kOk;
 }
+// rows that a call writes must not lie in each other
+static int check_written(const char* fn, const fsvd_kv8_cache* c, int B) {
+  if ((B > 1 && (c->sc_b == 0 || c->ss_b == 0)) || (c->Hk > 1 && (c->sc_h == 0 || c->ss_h == 0)) || (c->S > c->block && c->ss_n == 0)) {
+    set_last_error("%s: a cache that is written to must not be expanded over its sequences, blocks or heads", fn);
+    return kErrBadShape;
+  }
+  return kOk;
+}
+static int check_out(const char* fn, int B, int M, int H, int64_t so_b, int64_t so_m, int64_t so_h) {
+  if ((B > 1 && so_b == 0) || (M > 1 && so_m == 0) || (H > 1 && so_h == 0)) { set_last_error("%s: out must not be expanded", fn); return kErrBadShape; }
+  return kOk;
+}
 static const uint16_t* in16(const void* p) { return static_cast<const uint16_t*>(p); }
 
 extern "C" {
@@ -156,6 +168,7 @@ int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, in
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
   if (k == nullptr || v == nullptr || positions == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (T < 0) { set_last_error("%s: %d rows", fn, T); return kErrBadShape; }
+  if (const int rc = check_written(fn, cache, B)) return rc;
   const Kv8AppendArgs a{*cache, in16(k), sk_b, sk_t, sk_h, in16(v), sv_b, sv_t, sv_h, positions, rows, in16(cos), in16(sin), rope_len, B, T, dtype};
   return launch_kv8_append(fn, a, static_cast<hipStream_t>(stream));
 }
@@ -174,6 +187,8 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
   if (q == nullptr || out == nullptr || cache_seqlens == nullptr || (k_new == nullptr) != (v_new == nullptr)) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (H <= 0 || H % cache->Hk) { set_last_error("%s: %d query heads over %d", fn, H, cache->Hk); return kErrBadShape; }
+  if (const int rc = k_new ? check_written(fn, cache, B) : kOk) return rc;
+  if (const int rc = check_out(fn, B, 1, H, so_b, 0, so_h)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   const int ranges = kv8_ranges(B, H, cache->Hk, cache->S, nsplit);
   const size_t need = kv8_decode_scratch_bytes(B, H, cache->Dh, ranges);
@@ -200,6 +215,7 @@ int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
   if (q == nullptr || out == nullptr || q_pos0 == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (M < 0 || H <= 0 || H % cache->Hk) { set_last_error("%s: %d rows of %d query heads over %d", fn, M, H, cache->Hk); return kErrBadShape; }
+  if (const int rc = check_out(fn, B, M, H, so_b, so_m, so_h)) return rc;
   const Kv8AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
                       B, M, H, 1, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
   return M == 0 ? kOk : launch_kv8_prompt(fn, a, static_cast<float*>(scratch), scratch_bytes, static_cast<hipStream_t>(stream));

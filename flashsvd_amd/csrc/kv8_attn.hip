@@ -343,12 +343,12 @@ static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStr
 }
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float* scratch, hipStream_t st) {
   Kv8AttnArgs a = args;
+  if ((int64_t)a.B * a.H * ranges > (1 << 23)) { set_last_error("%s: %d sequences of %d heads in %d ranges", fn, a.B, a.H, ranges); return kErrBadShape; }
   if (a.k_new != nullptr && a.H / a.c.Hk > kDecGroup) {    // several workgroups read the keys of a kv head: the rows in a launch before them
     const Kv8AppendArgs n{a.c, a.k_new, a.sk_b, 0, a.sk_h, a.v_new, a.sv_b, 0, a.sv_h, a.positions, nullptr, a.cos, a.sin, a.rope_len, a.B, 1, a.dt};
     if (const int rc = launch_kv8_append(fn, n, st)) return rc;
     a.k_new = nullptr;
   }
-  if ((int64_t)a.B * a.H * ranges > 0x7fffffff) { set_last_error("%s: %d sequences of %d heads in %d ranges", fn, a.B, a.H, ranges); return kErrBadShape; }
   if (a.dt == 1) a.c.Dh == 128 ? decode_form<1, 128>(a, ranges, scratch, st) : decode_form<1, 64>(a, ranges, scratch, st);
   else a.c.Dh == 128 ? decode_form<0, 128>(a, ranges, scratch, st) : decode_form<0, 64>(a, ranges, scratch, st);
   const hipError_t e = hipGetLastError();

@@ -468,6 +468,7 @@ extern "C" int fsvd_sample_token(const void* logits, int64_t ld, const float* un
   const char* fn = "fsvd_sample_token";
   if (logits == nullptr || uniforms == nullptr || tokens == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (B <= 0 || V <= 0 || V > kDrawRow) { set_last_error("%s: B = %d, V = %d (1 to %d logits are served)", fn, B, V, kDrawRow); return kErrBadShape; }
+  if (B > 1 && ldt == 0) { set_last_error("%s: tokens must not be expanded", fn); return kErrBadShape; }
   if (dtype != 0 && dtype != 1) { set_last_error("%s: dtype code %d (bf16 = 0 and fp16 = 1 are served)", fn, dtype); return kErrBadDtype; }
   if ((reinterpret_cast<uintptr_t>(logits) & 1) != 0) { set_last_error("%s: logits must be 2-byte aligned", fn); return kErrBadAlign; }
   const SampleArgs a{static_cast<const uint16_t*>(logits), ld, uniforms, tokens, ldt, positions, temperature, top_p, min_p, top_k,

@@ -555,6 +555,8 @@ def _sample_token_impl(logits, uniforms, tokens, positions, temperature, top_k, 
         if t is not None and (t.dtype is not dt or tuple(t.shape) != (B,) or t.get_device() != dev or not t.is_contiguous()):
             raise ValueError(f"{nm} must be a contiguous {dt} [{B}] tensor on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
         ptrs.append(None if t is None else t.data_ptr())
+    if B == 0:
+        return
     with _on(dev):
         rc = _lib.load().fsvd_sample_token(logits.data_ptr(), logits.stride(0), ptrs[0], tokens.data_ptr(), tokens.stride(0), ptrs[1], temperature, ptrs[2],
                                            top_k, ptrs[3], top_p, ptrs[4], min_p, ptrs[5], B, V, code, _stream())

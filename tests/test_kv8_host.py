@@ -126,6 +126,30 @@ def test_refusals_of_the_c_abi():
     assert draw(x=None) == -4 and draw(B=0) == -1 and draw(V=0) == -1 and draw(V=(1 << 24) + 1) == -1 and draw(dt=2) == -3 and draw(x=p + 1) == -2
 
 
+def test_tensors_that_a_call_writes_are_not_expanded():
+    lib = _lib.load()
+    p = 1 << 20
+    good = dict(k=p, v=p, k_scale=p, v_scale=p, sc_b=40 * 128, sc_s=128, sc_h=64, ss_b=6, ss_n=2, ss_h=1, S=40, Hk=2, Dh=64, block=16)
+    for kw in (dict(sc_b=0), dict(ss_b=0), dict(sc_h=0), dict(ss_h=0), dict(ss_n=0)):
+        c = _lib.Kv8Cache(**(good | kw))
+        assert lib.fsvd_kv8_append(c, p, 64, 64, 64, p, 64, 64, 64, p, None, None, None, 0, 2, 1, 0, None) == -1
+        assert b"expanded" in lib.fsvd_last_error()
+        assert lib.fsvd_attn_decode_kv8(c, p, 128, 64, p, 64, 64, p, 64, 64, p, 0, None, None, 0, p, 128, 64, p, 1 << 30, 2, 2, 0, 0.0, 0, None) == -1
+        assert b"expanded" in lib.fsvd_last_error()
+    c = _lib.Kv8Cache(**good)
+    for so in ((0, 64), (128, 0)):
+        assert lib.fsvd_attn_decode_kv8(c, p, 128, 64, None, 0, 0, None, 0, 0, p, 0, None, None, 0, p, *so, p, 1 << 30, 2, 2, 0, 0.0, 0, None) == -1
+        assert b"out must not" in lib.fsvd_last_error()
+    for so in ((0, 128, 64), (640, 0, 64), (640, 128, 0)):
+        assert lib.fsvd_attn_prefill_kv8(c, p, 640, 128, 64, p, None, None, None, 0, p, *so, p, 1 << 30, 2, 5, 2, 0.0, 0, None) == -1
+        assert b"out must not" in lib.fsvd_last_error()
+    assert lib.fsvd_sample_token(p, 8, p, p, 0, None, 1.0, None, 0, None, 1.0, None, 0.0, None, 2, 8, 0, None) == -1
+    assert b"tokens must not" in lib.fsvd_last_error()
+    with FakeTensorMode():                                 # no rows: nothing to do
+        none = lambda dt, *s: _on(0, dt, *s)      # noqa: E731
+        hip_ops._sample_token_impl(none(BF16, 0, 9), none(torch.float32, 0), none(torch.long, 0, 1), None, 1.0, 0, 1.0, 0.0, None, None, None, None)
+
+
 def test_the_cache_object_without_a_gpu():
     from types import SimpleNamespace
     from flashsvd_amd.runtime import FlashSVDKV8Cache, FlashSVDV15DenseKVCache
