@@ -987,12 +987,15 @@ def _kv8_cache(B, kc, vc, ks, vs, block):
     """Checks of a cache in 8 bits; its descriptor for the C ABI.  One pass over what a good call has, in few lookups (a decode step takes it per layer)."""
     shape, st, ss = kc.shape, kc.stride(), ks.stride()
     dev = kc.get_device()
-    if not (kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and kc.is_cuda and vc.is_cuda and ks.is_cuda and vs.is_cuda
-            and len(shape) == 4 and vc.shape == shape and vc.stride() == st and shape[0] >= B and st[3] == 1 and vs.shape == ks.shape and vs.stride() == ss
-            and block in (16, 32, 64, 128) and tuple(ks.shape) == (shape[0], -(-shape[1] // block), shape[2])
+    if len(shape) != 4 or block not in (16, 32, 64, 128):
+        _refuse_kv8_cache(B, kc, vc, ks, vs, block)
+    n, S, Hk, Dh = shape
+    blocks = (n, -(-S // block), Hk)
+    if not (kc.dtype is _F8 and vc.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32 and vc.shape == shape and vc.stride() == st and n >= B
+            and st[3] == 1 and ks.shape == blocks and vs.shape == blocks and vs.stride() == ss and dev >= 0
             and vc.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
         _refuse_kv8_cache(B, kc, vc, ks, vs, block)
-    return _lib.Kv8Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], shape[1], shape[2], shape[3], block)
+    return _lib.Kv8Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], S, Hk, Dh, block)
 
 
 def _refuse_kv8_cache(B, kc, vc, ks, vs, block):
@@ -1075,7 +1078,7 @@ def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, 
     if k_new is not None and v_new is not None:
         sk, sv = k_new.stride(), v_new.stride()
         new = (B, Hk, Dh)
-        if not (k_new.dtype is dt and v_new.dtype is dt and tuple(k_new.shape) == new and tuple(v_new.shape) == new and sk[2] == 1 and sv[2] == 1
+        if not (k_new.dtype is dt and v_new.dtype is dt and k_new.shape == new and v_new.shape == new and sk[2] == 1 and sv[2] == 1
                 and k_new.get_device() == dev and v_new.get_device() == dev):
             _need(k_new, "k_new", dtype=dt); _need(v_new, "v_new", dtype=dt)
             raise ValueError(f"k_new/v_new must be [B,Hk,Dh] tensors with unit inner stride on cuda:{dev}, got {tuple(k_new.shape)} / {tuple(v_new.shape)}")
@@ -1084,7 +1087,7 @@ def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, 
     elif k_new is not None or v_new is not None:
         raise ValueError("k_new and v_new go together")
     if out is None:
-        out = torch.empty((B, H, Dh), device=q.device, dtype=dt)
+        out = q.new_empty((B, H, Dh))
     elif out.shape != q.shape or out.stride(2) != 1 or out.dtype is not dt or out.get_device() != dev:
         raise ValueError(f"out must be {dt} [B,H,Dh] with unit inner stride on cuda:{dev}")
     if B == 0:
@@ -1093,7 +1096,7 @@ def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, 
     nsplit = 0 if nsplit is None else nsplit
     nbytes, scratch, ptr = lib.fsvd_attn_decode_kv8_scratch_bytes(B, H, Hk, Dh, c.S, nsplit), None, None
     if nbytes:
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # of this call and stream
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)       # of this call and stream
         ptr = scratch.data_ptr()
     with _on(dev):
         rc = lib.fsvd_attn_decode_kv8(c, q.data_ptr(), sq[0], sq[1], kp, sk[0], sk[1], vp, sv[0], sv[1], lens, seqlen_add, cp, sp, rope_len, out.data_ptr(),
@@ -1116,7 +1119,7 @@ def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block,
     cp, sp, rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
     pos, n = _kv8_vector(q_pos0, B, dev, "q_pos0"), _kv8_vector(rows, B, dev, "rows")
     if out is None:
-        out = (torch.empty if rows is None else torch.zeros)((B, M, H, Dh), device=q.device, dtype=dt)
+        out = (q.new_empty if rows is None else q.new_zeros)((B, M, H, Dh))
     elif out.shape != q.shape or out.stride(3) != 1 or out.dtype is not dt or out.get_device() != dev:
         raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on cuda:{dev}")
     if B == 0:
@@ -1124,7 +1127,7 @@ def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block,
     lib, so = _lib.load(), out.stride()
     nbytes, scratch, ptr = lib.fsvd_attn_prefill_kv8_scratch_bytes(B, M, H, c.Hk, Dh, c.S), None, None
     if nbytes:
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # of this call and stream
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)       # of this call and stream
         ptr = scratch.data_ptr()
     with _on(dev):
         rc = lib.fsvd_attn_prefill_kv8(c, q.data_ptr(), sq[0], sq[1], sq[2], pos, n, cp, sp, rope_len, out.data_ptr(), so[0], so[1], so[2], ptr, nbytes, B, M, H,
