@@ -760,15 +760,22 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
   }
 }
 
-// Rows of a workgroup, its halves and key ranges of a chunk: 128 rows where those workgroups are one for each compute unit at least, else 64; where these are no
-// more than the compute units, two halves with every other tile, and where they leave part of the chip idle, the keys in ranges.
+// Rows of a workgroup, its halves and key ranges of a chunk (times in us of chunks without a past, 32 heads of 128, bf16, and of 64 tokens behind cached ones,
+// 32 heads over 8).
+//  - 128 rows share a tile better, 64 fill the chip and end evenly: 128 from two workgroups for each compute unit on (2 x 1024 tokens: 38.0 against 42.3;
+//    8 x 2048: 357 against 490), else 64 (1500 tokens: 41.9 against 50.0).
+//  - Up to one and a half workgroups of 64 rows for each compute unit, two halves of waves with every other tile (700 tokens: 18.3 against 21.2; 512: 13.7
+//    against 15.9; 2 x 512, which are two for each: 20.9 against 18.9).
+//  - Where these leave compute units idle, the keys in as many ranges as fill them once (64 behind 4800: 22.5 against 73.1 in one range and 31.0 in twice as
+//    many), each of four tiles at least (64 behind 600: 13.1 against 15.5; behind 300: 12.2 against 11.1), of eight where the partial results are many (256
+//    tokens without a past in ranges of two tiles and a half: 17.0 against 9.5).
 struct PromptForm { int rows, halves, ranges; };
 static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
   const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
-  if ((list + 127) / 128 * pairs >= cu) return {128, 1, 1};
+  if ((list + 127) / 128 * pairs >= 2 * cu) return {128, 1, 1};
   const int64_t n = (list + 63) / 64 * pairs;
-  if (n > cu) return {64, 1, 1};
-  return {64, 2, (int)max((int64_t)1, min(cu / n, (int64_t)(S + 4 * kTile - 1) / (4 * kTile)))};
+  if (n * 2 > 3 * cu) return {64, 1, 1};
+  return {64, 2, (int)max((int64_t)1, min(cu / n, (int64_t)S / ((n * 4 > cu ? 8 : 4) * kTile)))};
 }
 size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   const PromptForm f = prompt_form(B, M, H, Hk, S);

@@ -245,6 +245,8 @@ def test_decode_attention_appends_its_token(dt, Dh, H, Hk, block, at, S):
     (128, 1, 1, 16, "token", 150, [0], None),
     (64, 3, 1, 16, "head", 64, [64], None),
     (128, 2, 1, 32, "head", 40, [500, 1], None),
+    (128, 4, 2, 32, "head", 9, [900, 3, 650], [9, 9, 0]),      # in ranges of the keys
+    (64, 2, 2, 128, "token", 3, [1500], None),
 ])
 def test_prompt_attention(dt, Dh, H, Hk, block, layout, M, start, rows):
     from flashsvd_amd import hip_ops
@@ -293,7 +295,7 @@ def test_prompt_attention_of_many_heads(Dh, H, Hk, M, start):
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("Dh,H,Hk,M,start,B", [(128, 2, 1, 90, 37, 1), (64, 3, 3, 40, 100, 2), (128, 32, 32, 130, 3, 4), (64, 4, 2, 70, 400, 1)])
+@pytest.mark.parametrize("Dh,H,Hk,M,start,B", [(128, 2, 1, 90, 37, 1), (64, 3, 3, 40, 100, 2), (128, 32, 32, 130, 3, 4), (64, 4, 2, 70, 400, 1), (128, 4, 2, 70, 700, 1)])
 def test_a_nan_stays_in_what_sees_it(dt, Dh, H, Hk, M, start, B):
     """A NaN among the values of a later token leaves the rows before it as they are, in every dimension; so does one among its keys."""
     from flashsvd_amd import hip_ops
