@@ -135,6 +135,10 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
       for (int r = 0; r < rounds; ++r) f(r, ordered(fetch(r * kDrawThreads + tid)));
     }
   };
+  // the row's numbers: asked for here, as a load that is waited for further down costs a round trip to memory
+  const double temp = a.temperatures ? (double)a.temperatures[b] : a.temperature, top_p = a.top_ps ? (double)a.top_ps[b] : a.top_p;
+  const double min_p = a.min_ps ? (double)a.min_ps[b] : a.min_p, u = (double)a.uniforms[b];
+  const int top_k = a.top_ks ? a.top_ks[b] : a.top_k;
   for (int i = tid; i < kHistWords / 4; i += kDrawThreads) reinterpret_cast<u32x4_t*>(hist)[i] = u32x4_t{0u, 0u, 0u, 0u};
   if (tid == 0) n_extra = 0;
   if constexpr (R > 0) {
@@ -163,11 +167,8 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
   const bool nan = most > kHighest + 1 || 0xffffu - deep < kNegInf;
   if (most == kMinusZero) most = kZero;
 
-  const double temp = a.temperatures ? (double)a.temperatures[b] : a.temperature;
   uint32_t key = most, rank = 0;                        // the token: this occurrence of this key
   if (temp > 0. && !nan && most >= kLowest && most <= kHighest) {
-    const double top_p = a.top_ps ? (double)a.top_ps[b] : a.top_p, min_p = a.min_ps ? (double)a.min_ps[b] : a.min_p, u = (double)a.uniforms[b];
-    const int top_k = a.top_ks ? a.top_ks[b] : a.top_k;
     const double high = (double)key_value<DT>(most);
     // what is below e^-80 of the largest changes no sum of 64 bits and is not counted
     const double floor_ = high - 80. * temp;
@@ -194,7 +195,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
         }
       }
     };
-    all_pieces([&](int, u32x4_t v) { count_up(v); });
+    all_pieces([&](int r, u32x4_t v) {
+      if (r * kDrawThreads + wave * kWave < pieces) count_up(v);          // not all behind the row
+    });
     if (R == 0 || R > 8) {
       mine = wave_scan(mine);
       if (lane == 63) wave_kept[wave] = mine;
