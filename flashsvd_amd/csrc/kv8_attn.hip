@@ -28,7 +28,9 @@ __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u3
 }
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 
-constexpr int kMinRange = 256;                            // keys of a decode range, but for the last
+// Keys of a decode range, but for the last.  With 128, 138 keys of one sequence become two ranges and a join: 22.7 us a call against 17.9; 16001 keys of one
+// sequence take the same time either way.
+constexpr int kMinRange = 256;
 __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
   const int per = (keys + ranges - 1) / ranges;
   return per < kMinRange ? kMinRange : (per + 127) / 128 * 128;
@@ -100,6 +102,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges
 template <int DT, int DH>
 static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* scratch, hipStream_t st) {
   const int64_t rows = (int64_t)a.B * a.M * a.H;
+  // 63 ranges of 32 rows: 13.9 us with the attention before it, 15.2 by one wave a row; 8 ranges of 512 rows: 27.5 by one wave, 28.5 by four
   if (ranges > 8) hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ranges, decode, scratch);
   else hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ranges, decode, scratch);
 }
@@ -110,7 +113,10 @@ static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* sc
 //   K: lane (n, g) = (lane % 16, lane / 16) loads 16-byte pieces of key n: the order of the products' k axis is free as long as q is laid out the same.
 //   S^T leaves lane (n, g) the scores of query n and keys 4 g .. 4 g + 3 of the two 16-key tiles: eight weights that are one operand of the second product.
 //   V: lane (n, g) loads those eight keys' dimensions DH / 16 n .. of the row, and byte permutes put two keys of a dimension next to each other.
-// Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.
+// Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.  The weights go
+// into the second product as two bf16 parts, 16 significant bits.
+// Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 97 us, 5.5 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 24 and a
+// join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.5 us).  Four waves a SIMD rather than three: 27.4 against 28.2.
 // ---------------------------------------------------------------------------------------------
 constexpr int kDecWaves = 4, kDecStep = 32, kDecGroup = 16;
 
@@ -328,6 +334,8 @@ int kv8_ranges(int B, int H, int Hk, int S, int nsplit) {
   const int most = (S + kMinRange - 1) / kMinRange;
   if (nsplit <= 0) {
     const int64_t pairs = (int64_t)B * Hk * ((H / Hk + kDecGroup - 1) / kDecGroup);
+    // about four workgroups for each compute unit; with 512 / 1024 / 2048 in all: 27.9 / 27.4 / 28.6 us (16 sequences of up to 4001 keys, 8 kv heads) and
+    // 102.9 / 102.0 / 100.4 (16 of 4090, 32 heads)
     nsplit = (int)((1024 + pairs - 1) / pairs);
   }
   return max(1, min(nsplit, most));
@@ -367,8 +375,11 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
+// Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
+// 8 x 2048 tokens, 32 heads of 128: 357 us, 770 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
+// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.6 us for two of them.
 constexpr int kTile = 64;
-constexpr float kSlack = 8.f;
+constexpr float kSlack = 8.f;                             // 357 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 // a pair of codes as bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
 template <bool HI, bool POWER>

@@ -5,6 +5,8 @@
 // Every filter keeps a prefix of that order, and 16-bit logits have few distinct values, so nothing is sorted: the values of a row are counted in a
 // histogram over their 65536 patterns in LDS, and an exponential is taken for each value that occurs, once, in 64 bits, as the sums are (a boundary between
 // two of 10^5 nearly equal tokens is 10^-5 of the sum wide; with 32-bit sums one draw in a thousand lands on the wrong side of it).
+// A row is one workgroup's, so latency bounds it.  Of the 12.6 us of 32000 logits with every filter on, reading and the largest take 2.2, counting 2.5 (LDS
+// additions), the list of segments 1.1, their masses 2.1, the search by one wave 2.8, the token's place 0.7; 64 rows take 13.5, 16 rows of 128256 logits 27.7.
 #include "common.hpp"
 #include "../../include/flashsvd_hip.h"
 
@@ -96,7 +98,8 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
   return v;
 }
 
-// R: 16-byte pieces of the row that a thread keeps in registers; 0: longer rows, read once for each pass.
+// R: 16-byte pieces of the row that a thread keeps in registers; 0: longer rows, read once for each pass (32000 logits: 13.1 us from registers, 16.3 read again;
+// 128256: 28.1 and 33.3).  The smallest R that holds the row: 32000 logits with R = 16 take 30.8.
 template <int DT, int R>
 __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a) {
   constexpr uint32_t kInf = DT == 1 ? 0x7c00u : 0x7f80u, kNegInf = kMinusZero - kInf, kLowest = kNegInf + 1, kHighest = kZero + kInf - 1;
