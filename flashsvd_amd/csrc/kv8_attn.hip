@@ -16,15 +16,23 @@ struct Kv8Parts {
 };
 
 // eight elements x of a query row in the lower or upper half of the head, rotated with their partners y half a head away, in fp32 and rounded to the type of
-// the products
+// the products; rest: what that rounding leaves
 template <class E>
-__device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper) {
+__device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper, u32x4_t& rest) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float sl = upper ? E::lo(sin[i]) : -E::lo(sin[i]), sh = upper ? E::hi(sin[i]) : -E::hi(sin[i]);
-    x[i] = E::pack2(E::lo(x[i]) * E::lo(cos[i]) + E::lo(y[i]) * sl, E::hi(x[i]) * E::hi(cos[i]) + E::hi(y[i]) * sh);
+    const float l = E::lo(x[i]) * E::lo(cos[i]) + E::lo(y[i]) * sl, h = E::hi(x[i]) * E::hi(cos[i]) + E::hi(y[i]) * sh;
+    const uint32_t w = E::pack2(l, h);
+    x[i] = w;
+    rest[i] = E::pack2(l - E::lo(w), h - E::hi(w));
   }
   return x;
+}
+template <class E>
+__device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper) {
+  u32x4_t rest;
+  return rotated<E>(x, y, cos, sin, upper, rest);
 }
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 
@@ -116,12 +124,14 @@ static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* sc
 // Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.  The weights go
 // into the second product as two bf16 parts, 16 significant bits.
 // Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 97 us, 5.5 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 24 and a
-// join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.5 us).  Four waves a SIMD rather than three: 27.4 against 28.2.
+// join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.5 us).  A rotated q goes into the first product as
+// two parts of its type: one rounding of it would be the largest error of the output (0.0036 of its size against 0.0016 in bf16, the output's own rounding) and
+// saves 2 to 3 % of a call.  Three waves a SIMD hold that; four spill (stress call: 131 us against 102).
 // ---------------------------------------------------------------------------------------------
 constexpr int kDecWaves = 4, kDecStep = 32, kDecGroup = 16;
 
 template <int DT, int DH>
-__global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
+__global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef typename E::frag_t frag_t;
   typedef E16<0>::frag_t pfrag_t;
@@ -187,13 +197,15 @@ __global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8Att
                        b, hk, pos, lane);
   if (c0 < before) { fetch_k(c0); fetch_v(c0); }
 
-  // q: element e of piece (j, h) is dimension 64 j + 16 g + 8 h + e of query n, rotated in fp32 and rounded to the type of the products
-  frag_t qf[ST];
+  // q: element e of piece (j, h) is dimension 64 j + 16 g + 8 h + e of query n, rotated in fp32, as two parts of the type of the products then
+  frag_t qf[ST], qr[ST];
   {
     const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)(h0 + min(n, heads - 1)) * a.sq_h;
     constexpr int HALF = DH / 2;
     const auto dim = [&](int st) { return 64 * (st >> 1) + 16 * g + 8 * (st & 1); };
-    u32x4_t x[ST], y[2], cw[2], sw[2];
+    u32x4_t x[ST], z[ST], y[2], cw[2], sw[2];
+#pragma unroll
+    for (int st = 0; st < ST; ++st) z[st] = u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
     for (int st = 0; st < ST; ++st) x[st] = eight(qp + dim(st));
     if (a.cos) {
@@ -207,16 +219,19 @@ __global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8Att
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if constexpr (DH == 64) {
-          x[h] = rotated<E>(x[h], y[h], cw[h], sw[h], dim(h) >= HALF);
+          x[h] = rotated<E>(x[h], y[h], cw[h], sw[h], dim(h) >= HALF, z[h]);
         } else {
           const u32x4_t low = x[h];
-          x[h] = rotated<E>(low, x[h + 2], cw[h], sw[h], false);
-          x[h + 2] = rotated<E>(x[h + 2], low, cw[h], sw[h], true);
+          x[h] = rotated<E>(low, x[h + 2], cw[h], sw[h], false, z[h]);
+          x[h + 2] = rotated<E>(x[h + 2], low, cw[h], sw[h], true, z[h + 2]);
         }
       }
     }
 #pragma unroll
-    for (int st = 0; st < ST; ++st) qf[st] = __builtin_bit_cast(frag_t, n < heads ? x[st] : u32x4_t{0u, 0u, 0u, 0u});
+    for (int st = 0; st < ST; ++st) {
+      qf[st] = __builtin_bit_cast(frag_t, n < heads ? x[st] : u32x4_t{0u, 0u, 0u, 0u});
+      qr[st] = __builtin_bit_cast(frag_t, n < heads ? z[st] : u32x4_t{0u, 0u, 0u, 0u});
+    }
   }
 
   const float scale = a.scale * 1.4426950408889634f;      // weights are powers of two of the scores' differences
@@ -239,6 +254,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 4) void kv8_decode_kernel(Kv8Att
           const u32x4_t kk{Code16<DT>::template pair<false>(w0), Code16<DT>::template pair<true>(w0), Code16<DT>::template pair<false>(w1),
                            Code16<DT>::template pair<true>(w1)};
           acc = E::mfma(__builtin_bit_cast(frag_t, kk), qf[2 * j + h], acc);
+          acc = E::mfma(__builtin_bit_cast(frag_t, kk), qr[2 * j + h], acc);
         }
       const float by = ks[t] * scale;
 #pragma unroll
@@ -371,7 +387,8 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
 //   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
-//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.
+//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.  A q that the call rotates
+//   is rounded to its type, as one that comes rotated is: the registers of 128 rows are full.
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
