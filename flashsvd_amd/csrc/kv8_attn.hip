@@ -123,8 +123,8 @@ static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* sc
 //   V: lane (n, g) loads those eight keys' dimensions DH / 16 n .. of the row, and byte permutes put two keys of a dimension next to each other.
 // Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.  The weights go
 // into the second product as two bf16 parts, 16 significant bits.
-// Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 97 us, 5.5 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 24 and a
-// join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.5 us).  A rotated q goes into the first product as
+// Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 102 us, 5.3 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 25 and a
+// join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.7 us).  A rotated q goes into the first product as
 // two parts of its type: one rounding of it would be the largest error of the output (0.0036 of its size against 0.0016 in bf16, the output's own rounding) and
 // saves 2 to 3 % of a call.  Three waves a SIMD hold that; four spill (stress call: 131 us against 102).
 // ---------------------------------------------------------------------------------------------
@@ -393,10 +393,10 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 357 us, 770 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
+// 8 x 2048 tokens, 32 heads of 128: 349 us, 790 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
 // LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.6 us for two of them.
 constexpr int kTile = 64;
-constexpr float kSlack = 8.f;                             // 357 us against 372 with a reference that moves with every larger score
+constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 // a pair of codes as bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
 template <bool HI, bool POWER>
@@ -473,11 +473,15 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     for (int st = 0; st < ST; ++st) qf[mi][st] = __builtin_bit_cast(frag_t, x[st]);
   }
   const float scale = a.scale * 1.4426950408889634f;
-  float m_run[MI], l_run[MI];
+  float m_run[MI];
+  // Sums of the weights: as they are rounded, by products with ones (the same in every element; 349 us against 357 for the long call); where the registers hold
+  // the second products' operands, a lane's own, unrounded.
+  typedef std::conditional_t<kRest, float, f32x4_t> sum_t;
+  sum_t l_run[MI];
   f32x4_t o[MI][NT];
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
-    m_run[mi] = -INFINITY; l_run[mi] = 0.f;
+    m_run[mi] = -INFINITY; l_run[mi] = sum_t{};
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[mi][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -614,7 +618,12 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     for (int t = 0; t < NT; ++t) vf[t] = __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + ((st ^ t) & 1 ? vread ^ 32 : vread) + 16 * t * kTile));
   };
   pfrag_t ph[MI][2], pl[MI][2];
+  const pfrag_t ones = __builtin_bit_cast(pfrag_t, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   const auto values = [&](const pfrag_t (&vf)[NT], int st) {
+    if constexpr (!kRest) {
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) l_run[mi] = E16<0>::mfma(ones, ph[mi][st], l_run[mi]);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -672,7 +681,7 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[mi][j][i] = __builtin_amdgcn_exp2f(s[mi][j][i]);
-          l_run[mi] += s[mi][j][i];
+          if constexpr (kRest) l_run[mi] += s[mi][j][i];
         }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -730,6 +739,10 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     values(vf[0], 0);
     values(vf[1], 1);
   }
+  const auto own_sum = [](const sum_t& l) {
+    if constexpr (kRest) return l;
+    else return l[0];
+  };
   if constexpr (KG > 1) {                // the halves' results
     static_assert(KG == 2 && MI == 1, "one exchange");
     f32x4_t* part = reinterpret_cast<f32x4_t*>(smem) + wave * (NT + 1) * kWave + lane;
@@ -737,7 +750,7 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     if (kg == 1) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) part[t * kWave] = o[0][t];
-      part[NT * kWave] = f32x4_t{m_run[0], l_run[0], 0.f, 0.f};
+      part[NT * kWave] = f32x4_t{m_run[0], own_sum(l_run[0]), 0.f, 0.f};
     }
     __syncthreads();
     if (kg == 1) return;
@@ -754,7 +767,7 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
     const int r = w0 + 16 * mi + lr;
-    const float l = column_sum(l_run[mi]);
+    const float l = kRest ? column_sum(own_sum(l_run[mi])) : own_sum(l_run[mi]);
     if (r >= rows) continue;
     if (any_nan) {
 #pragma unroll
