@@ -36,12 +36,11 @@ __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u3
 }
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 
-// Keys of a decode range, but for the last.  With 128, 138 keys of one sequence become two ranges and a join: 22.7 us a call against 17.9; 16001 keys of one
-// sequence take the same time either way.
-constexpr int kMinRange = 256;
+// Keys of a decode range, but for the last: a step of every wave, and whole blocks.
+constexpr int kMinRange = 128;
 __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
   const int per = (keys + ranges - 1) / ranges;
-  return per < kMinRange ? kMinRange : (per + 127) / 128 * 128;
+  return (max(per, 1) + kMinRange - 1) / kMinRange * kMinRange;
 }
 
 // The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
@@ -346,13 +345,17 @@ __global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8Att
   }
 }
 
+// Ranges of a decode call (times in us from a captured graph, 32 heads of 128 over 8).
+//  - About two workgroups for each compute unit: with 512 / 640 / 1024 in all one sequence of 30000 keys takes 20.3 / 22.2 / 23.1, 64 of 2000 49.5 / 52.9 / 52.4;
+//    with 384 one sequence of 16001 takes 16.4 against 14.3.
+//  - Ranges of 2048 keys at most: 16 sequences of 4090 keys with 32 kv heads take 105 in one range, 97 to 102 in three, 114 in six.
+//  - One range below 384 keys (137 keys of 8 heads of 64: 5.7, in two 7.5), else down to 128 keys (one sequence of 400 keys 8.3, with 256 at least 9.5; of 4000
+//    9.5 and 10.9; of 8000 12.4 and 11.4).
 int kv8_ranges(int B, int H, int Hk, int S, int nsplit) {
-  const int most = (S + kMinRange - 1) / kMinRange;
+  const int most = S < 384 ? 1 : (S + kMinRange - 1) / kMinRange;
   if (nsplit <= 0) {
     const int64_t pairs = (int64_t)B * Hk * ((H / Hk + kDecGroup - 1) / kDecGroup);
-    // about four workgroups for each compute unit; with 512 / 1024 / 2048 in all: 27.9 / 27.4 / 28.6 us (16 sequences of up to 4001 keys, 8 kv heads) and
-    // 102.9 / 102.0 / 100.4 (16 of 4090, 32 heads)
-    nsplit = (int)((1024 + pairs - 1) / pairs);
+    nsplit = max((int)((512 + pairs - 1) / pairs), (S + 2047) / 2048);
   }
   return max(1, min(nsplit, most));
 }
