@@ -122,7 +122,7 @@ static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* sc
 //   V: lane (n, g) loads those eight keys' dimensions DH / 16 n .. of the row, and byte permutes put two keys of a dimension next to each other.
 // Codes become 16-bit elements exactly; a scale multiplies what one tile of 16 keys has in common, the scores and the weights.  The weights go
 // into the second product as two bf16 parts, 16 significant bits.
-// Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 102 us, 5.3 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 25 and a
+// Bound by the bytes of the cache: 16 x 4090 keys of 32 heads of 128 (537 MB) in 93 us and a join of 5, 5.5 TB/s, 16 x 1000 to 4001 keys of 8 kv heads (92 MB) in 25 and a
 // join of 4; small calls by the latency of a few dependent loads (137 keys of 8 heads of 64: 5.7 us).  A rotated q goes into the first product as
 // two parts of its type: one rounding of it would be the largest error of the output (0.0036 of its size against 0.0016 in bf16, the output's own rounding) and
 // saves 2 to 3 % of a call.  Three waves a SIMD hold that; four spill (stress call: 131 us against 102).

@@ -187,6 +187,7 @@ def _check_rows(c, q, out, lens, scale, dt, cos=None, sin=None, pos=None, what="
     (128, 34, 2, 16, "token", [300, 7], 301),
     (128, 2, 2, 32, "head", [1500, 3, 700], 1501),
     (128, 8, 1, 64, "head", [4097], 4100),
+    (64, 20, 1, 32, "head", [900, 0, 513], 1000),          # more than 16 heads of a kv head over key ranges
     (128, 1, 1, 16, "head", [500, 0, -4, 9999], 256),      # a negative length, and one beyond the cache
 ])
 def test_decode_attention(dt, Dh, H, Hk, block, layout, lens, S):
@@ -215,6 +216,8 @@ def test_decode_attention(dt, Dh, H, Hk, block, layout, lens, S):
     (64, 8, 8, 16, [137, 0], 144),
     (128, 4, 4, 64, [63, 64, 699], 700),
     (64, 9, 1, 128, [130, 127, 128, 50, 40, 1], 200),
+    (64, 20, 1, 32, [900, 0, 513], 1000),
+    (128, 4, 2, 128, [127, 128, 383, 384, 511, 1151], 1152),      # a new row at the ends of ranges
 ])
 def test_decode_attention_appends_its_token(dt, Dh, H, Hk, block, at, S):
     """The call against an append of its own followed by attention: the same cache, bit for bit, and the output within the bound over it."""
