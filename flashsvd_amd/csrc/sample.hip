@@ -5,8 +5,8 @@
 // Every filter keeps a prefix of that order, and 16-bit logits have few distinct values, so nothing is sorted: the values of a row are counted in a
 // histogram over their 65536 patterns in LDS, and an exponential is taken for each value that occurs, once, in 64 bits, as the sums are (a boundary between
 // two of 10^5 nearly equal tokens is 10^-5 of the sum wide; with 32-bit sums one draw in a thousand lands on the wrong side of it).
-// A row is one workgroup's, so latency bounds it.  Of the 12.6 us of 32000 logits with every filter on, reading and the largest take 2.2, counting 2.5 (LDS
-// additions), the list of segments 1.1, their masses 2.1, the search by one wave 2.8, the token's place 0.7; 64 rows take 13.5, 16 rows of 128256 logits 27.7.
+// A row is one workgroup's, so latency bounds it.  Of the 12.3 us of 32000 logits with every filter on, reading and the largest take 1.9, counting 2.5 (LDS
+// additions), the list of segments 1.1, their masses 2.1, the search by one wave 2.7, the token's place 0.7; 64 rows take 13.2, 16 rows of 128256 logits 28.
 #include "common.hpp"
 #include "../../include/flashsvd_hip.h"
 
@@ -92,10 +92,15 @@ __device__ __forceinline__ double row_sum(double v) {      // of 16 lanes, in ea
   v = dpp_add<0x122, 0xf>(v);
   return dpp_add<0x121, 0xf>(v);
 }
-__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-  return v;
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_most(uint32_t v) { return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false)); }
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {      // the steps of a running sum
+  v = dpp_most<0x111, 0xf>(v);
+  v = dpp_most<0x112, 0xf>(v);
+  v = dpp_most<0x114, 0xf>(v);
+  v = dpp_most<0x118, 0xf>(v);
+  v = dpp_most<0x142, 0xa>(v);
+  return lane_value(dpp_most<0x143, 0xc>(v), 63);
 }
 
 // R: 16-byte pieces of the row that a thread keeps in registers; 0: longer rows, read once for each pass (32000 logits: 13.1 us from registers, 16.3 read again;
@@ -350,7 +355,9 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
       // The n-th of the order, where n is the smallest with C_n > target (by_mass) or given: its key, how many of its key are up to it, n and C_n.  Where
       // rounding leaves no C above the target, the last that there is.
       uint32_t at_key = 0, at_rank = 0, at_n = 0;
-      double at_mass = 0.;
+      double at_mass = 0., w = 0., m = 0., to_mk = 0.;
+      uint32_t k = 0, c = 0, to_ck = 0;
+      int held = -1;
       const auto locate = [&](bool by_mass, double target, uint32_t n) {
         const auto first = [&](bool in, double m, uint32_t c) {
           const uint64_t hit = __ballot(in && (by_mass ? m > target : c >= n)), some = __ballot(in);
@@ -365,9 +372,18 @@ __global__ __launch_bounds__(kDrawThreads) void sample_token_kernel(SampleArgs a
         const int t = first(is_seg, ms, cs);
         const double m1 = t ? lane_value(ms, t - 1) : m0;
         const uint32_t c1 = t ? lane_value(cs, t - 1) : c0;
-        const uint32_t s = seg_at[g * kWave + t], k = s * kSegBins + kSegBins - 1 - lane, c = k >= least ? merged(s, k, bin(k)) : 0;
-        const double w = c ? weight(k) : 0., m = c * w, mk = m1 + wave_scan(m);
-        const uint32_t ck = c1 + wave_scan(c);
+        if (held != g * kWave + t) {                    // its keys from the largest down; the next search often ends in the same segment
+          held = g * kWave + t;
+          const uint32_t s = seg_at[held];
+          k = s * kSegBins + kSegBins - 1 - lane;
+          c = k >= least ? merged(s, k, bin(k)) : 0;
+          w = c ? weight(k) : 0.;
+          m = c * w;
+          to_mk = wave_scan(m);
+          to_ck = wave_scan(c);
+        }
+        const double mk = m1 + to_mk;
+        const uint32_t ck = c1 + to_ck;
         const bool found = __any(c && (by_mass ? mk > target : ck >= n));
         const int l = first(c != 0, mk, ck);
         uint32_t j = c;
