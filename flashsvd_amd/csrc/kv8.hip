@@ -128,7 +128,7 @@ int check_kv8_cache(const char* fn, const fsvd_kv8_cache* c) {
   }
   if (c->S <= 0 || c->Hk <= 0 || (c->Dh != 64 && c->Dh != 128)) { set_last_error("%s: bad cache: S=%d Hk=%d Dh=%d (64 and 128 are served)", fn, c->S, c->Hk, c->Dh); return kErrBadShape; }
   if (c->block != 16 && c->block != 32 && c->block != 64 && c->block != 128) { set_last_error("%s: block of %d tokens (16, 32, 64 and 128 are served)", fn, c->block); return kErrBadShape; }
-  if (c->sc_b < 0 || c->sc_s < c->Dh || c->sc_s > (1 << 26) || c->sc_h < 0 || c->ss_b < 0 || c->ss_n < 0 || c->ss_h < 0) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
+  if (c->sc_b < 0 || c->sc_s < c->Dh || c->sc_s > (1 << 26) || c->sc_h < 0 || c->ss_b < 0 || c->ss_n < 0 || c->ss_n > (1 << 26) || c->ss_h < 0) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15) || ((c->sc_b | c->sc_s | c->sc_h) & 15)) {
     set_last_error("%s: cache pointers and strides must be 16-byte aligned", fn);
     return kErrBadAlign;

@@ -501,9 +501,14 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
   float vscale[VP];
   // a tile's first row is the workgroup's, 64 bits; from there on 32 do (and stay the same from tile to tile, but for one that the range ends in)
   const uint32_t line = (uint32_t)a.c.sc_s;
-  uint32_t koff[KP], voff[VP][4];
+  uint32_t koff[KP], voff[VP][4], kso, vso[VP];
+  const uint32_t step = (uint32_t)a.c.ss_n * 4;
   const auto k_offset = [&](int p, int left) { return (uint32_t)min(krow + p * (TH / KL), left - 1) * line + kd; };
   const auto v_offset = [&](int p, int e, int left) { return (uint32_t)min(4 * (vrow + p * (TH / VL)) + e, left - 1) * line + vd; };
+  const auto s_offset = [&](int row, int left) { return (uint32_t)(min(row, left - 1) >> shift) * step; };      // of a tile's row, tiles begin with blocks or lie in one
+  const auto scale_at = [&](const float* base, int n0, uint32_t off) {
+    return *reinterpret_cast<const float*>(reinterpret_cast<const char*>(base + (int64_t)(n0 >> shift) * a.c.ss_n) + off);
+  };
   const auto request_k = [&](int n0) {
     if (n0 + kTile > n_end) {
 #pragma unroll
@@ -520,6 +525,8 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
       for (int p = 0; p < VP; ++p)
 #pragma unroll
         for (int e = 0; e < 4; ++e) voff[p][e] = v_offset(p, e, n_end - n0);
+#pragma unroll
+      for (int p = 0; p < VP; ++p) vso[p] = s_offset(4 * (vrow + p * (TH / VL)), n_end - n0);
     }
     const uint8_t* vt = vb + (int64_t)n0 * a.c.sc_s;
 #pragma unroll
@@ -528,14 +535,14 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
       if (kTile / 4 * VL % TH == 0 || row < kTile) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vt + voff[p][e]);
-        vscale[p] = vsp[(int64_t)(min(n0 + row, n_end - 1) >> shift) * a.c.ss_n];
+        vscale[p] = scale_at(vsp, n0, vso[p]);
       }
     }
   };
-  float fs[4];                           // the key scales of a tile's four blocks of 16 keys
+  float fs;                              // the key scale of block lane % 4 of a tile's four blocks of 16 keys (by a vector load: a scalar one would be waited for here)
   const auto request_f = [&](int n0) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) fs[j] = ksp[(int64_t)(min(n0 + 16 * j, n_end - 1) >> shift) * a.c.ss_n];
+    if (n0 + kTile > n_end) kso = s_offset(16 * (lane & 3), n_end - n0);
+    fs = scale_at(ksp, n0, kso);
   };
   const auto stage_k = [&](int buf) {
     uint16_t* ks = Ks + buf * kTile * KSTR;
@@ -636,11 +643,12 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
       }
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
-  const auto weights = [&](f32x4_t (&s)[MI][4], int n0, const float (&by)[4]) {
+  const auto weights = [&](f32x4_t (&s)[MI][4], int n0, float by) {
     float f[4];
+    by *= scale;
     const bool plain = n0 + kTile <= wave_sees;                      // every row of the wave sees the whole tile
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = by[j] * scale;
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(by), j));
 #pragma unroll
     for (int mi = 0; mi < MI; ++mi) {
       float top = -INFINITY;
@@ -707,6 +715,9 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
   for (int p = 0; p < VP; ++p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) voff[p][e] = v_offset(p, e, kTile);
+  kso = s_offset(16 * (lane & 3), kTile);
+#pragma unroll
+  for (int p = 0; p < VP; ++p) vso[p] = s_offset(4 * (vrow + p * (TH / VL)), kTile);
   const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile; };
   const int all = n_begin < n_end ? (n_end - n_begin + kTile - 1) / kTile : 0, n = (all - kg + KG - 1) / KG;      // of the workgroup, of this half
   if (n > 0) { request_k(at(0)); request_v(at(0)); request_f(at(0)); }
@@ -720,9 +731,7 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
       if (at(i) + kTile > all_see) set_nans_aside(at(i));
       stage_v(buf);
     }
-    float g[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) g[j] = fs[j];
+    const float g = fs;
     if (i + 1 < n) { request_k(at(i + 1)); request_v(at(i + 1)); request_f(at(i + 1)); }
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
     if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
