@@ -396,8 +396,8 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 349 us, 790 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
-// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.6 us for two of them.
+// 8 x 2048 tokens, 32 heads of 128: 342 us, 805 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
+// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.5 us for two of them.
 constexpr int kTile = 64;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }

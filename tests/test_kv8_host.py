@@ -112,7 +112,7 @@ def test_refusals_of_the_c_abi():
     append = lambda c, B=1, T=1, dt=0, k=p, cos=None, rope=0: lib.fsvd_kv8_append(c, k, 64, 64, 64, p, 64, 64, 64, p, None, cos, cos, rope, B, T, dt, None)      # noqa: E731
     cache = lambda **kw: _lib.Kv8Cache(**(good | kw))      # noqa: E731
     for kw, code in ((dict(k=None), -4), (dict(v_scale=None), -4), (dict(Dh=96), -1), (dict(block=8), -1), (dict(S=0), -1), (dict(k=p + 8), -2),
-                     (dict(sc_s=72), -2), (dict(sc_b=-16), -1)):
+                     (dict(sc_s=72), -2), (dict(sc_b=-16), -1), (dict(ss_n=(1 << 26) + 1), -1), (dict(sc_s=(1 << 26) + 16), -1)):
         assert append(cache(**kw)) == code, kw
         assert b"fsvd_kv8_append" in lib.fsvd_last_error()
     assert append(cache(), B=0) == -1 and append(cache(), T=-1) == -1 and append(cache(), dt=2) == -3 and append(cache(), k=None) == -4
