@@ -385,7 +385,7 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 
 // ---------------------------------------------------------------------------------------------
 // A chunk of a prompt.  The query rows of the heads that share a kv head are one list, row r = query token r / G of head r % G, so that grouped heads share
-// the tiles of keys too.  A workgroup of NW waves takes 16 MI rows for each wave; tiles of 64 keys go through LDS as 16-bit elements, converted once for
+// the tiles of keys too.  A workgroup of four waves takes 16 MI rows for each; tiles of 64 keys go through LDS as 16-bit elements, converted once for
 // the workgroup: K row by row, V transposed (two keys of a dimension next to each other by byte permutes), two buffers and one barrier a tile.
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
@@ -398,7 +398,7 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
 // 8 x 2048 tokens, 32 heads of 128: 342 us, 805 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
 // LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.5 us for two of them.
-constexpr int kTile = 64;
+constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 // a pair of codes as bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
@@ -409,14 +409,14 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
   return pack_bf16x2(x[0] * scale, x[1] * scale);
 }
 
-template <int DT, int DH, int MI, int NW, int KG>
-__global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
+template <int DT, int DH, int MI, int KG>
+__global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef typename E::frag_t frag_t;
   typedef E16<0>::frag_t pfrag_t;
-  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * NW, QW = 16 * MI, BM = QW * NW;
-  constexpr int KL = DH / 16, KP = (kTile * KL + TH - 1) / TH;              // lanes of a key row; passes of the workgroup over the tile's keys
-  constexpr int VL = DH / 4, VP = (kTile / 4 * VL + TH - 1) / TH;
+  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * kPromptWaves, QW = 16 * MI, BM = QW * kPromptWaves;
+  constexpr int KL = DH / 16, KP = kTile * KL / TH;              // lanes of a key row; passes of the workgroup over the tile's keys
+  constexpr int VL = DH / 4, VP = kTile / 4 * VL / TH;
   constexpr bool kRest = DT == 1;
   extern __shared__ __align__(16) unsigned char smem[];
   const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
@@ -516,8 +516,7 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     }
     const uint8_t* kt = kb + (int64_t)n0 * a.c.sc_s;
 #pragma unroll
-    for (int p = 0; p < KP; ++p)
-      if (kTile * KL % TH == 0 || krow + p * (TH / KL) < kTile) kreg[p] = *reinterpret_cast<const u32x4_t*>(kt + koff[p]);
+    for (int p = 0; p < KP; ++p) kreg[p] = *reinterpret_cast<const u32x4_t*>(kt + koff[p]);
   };
   const auto request_v = [&](int n0) {
     if (n0 + kTile > n_end) {
@@ -531,12 +530,9 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
     const uint8_t* vt = vb + (int64_t)n0 * a.c.sc_s;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
-      const int row = 4 * (vrow + p * (TH / VL));
-      if (kTile / 4 * VL % TH == 0 || row < kTile) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vt + voff[p][e]);
-        vscale[p] = scale_at(vsp, n0, vso[p]);
-      }
+      for (int e = 0; e < 4; ++e) vreg[p][e] = *reinterpret_cast<const uint32_t*>(vt + voff[p][e]);
+      vscale[p] = scale_at(vsp, n0, vso[p]);
     }
   };
   float fs;                              // the key scale of block lane % 4 of a tile's four blocks of 16 keys (by a vector load: a scalar one would be waited for here)
@@ -547,17 +543,13 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
   const auto stage_k = [&](int buf) {
     uint16_t* ks = Ks + buf * kTile * KSTR;
 #pragma unroll
-    for (int p = 0; p < KP; ++p) {
-      const int row = krow + p * (TH / KL);
-      if (kTile * KL % TH == 0 || row < kTile) {
+    for (int p = 0; p < KP; ++p)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t x = kreg[p][2 * h], y = kreg[p][2 * h + 1];
-          *reinterpret_cast<u32x4_t*>(ks + row * KSTR + kd + 8 * h) = u32x4_t{Code16<DT>::template pair<false>(x), Code16<DT>::template pair<true>(x),
-                                                                              Code16<DT>::template pair<false>(y), Code16<DT>::template pair<true>(y)};
-        }
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t x = kreg[p][2 * h], y = kreg[p][2 * h + 1];
+        *reinterpret_cast<u32x4_t*>(ks + (krow + p * (TH / KL)) * KSTR + kd + 8 * h) = u32x4_t{
+            Code16<DT>::template pair<false>(x), Code16<DT>::template pair<true>(x), Code16<DT>::template pair<false>(y), Code16<DT>::template pair<true>(y)};
       }
-    }
   };
   // A masked key has weight zero, and zero times a NaN is one: where not every row sees the whole tile, a NaN is staged as zero and put into the rows that see
   // it at the end.
@@ -566,7 +558,6 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       const int row = 4 * (vrow + p * (TH / VL));
-      if (kTile / 4 * VL % TH != 0 && row >= kTile) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t nan = ((vreg[p][e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
@@ -584,23 +575,21 @@ __global__ __launch_bounds__(kWave * NW * KG, 2) void kv8_prompt_kernel(Kv8AttnA
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
       const int row4 = vrow + p * (TH / VL);
-      if (kTile / 4 * VL % TH == 0 || row4 < kTile / 4) {
-        const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
-        uint16_t* to = vt + vd * kTile;
-        const uint32_t turned = col ^ (8 * v_piece(vd));          // of rows vd and vd + 1; of the next two the piece two further
-        const auto put = [&](auto power) {
+      const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
+      uint16_t* to = vt + vd * kTile;
+      const uint32_t turned = col ^ (8 * v_piece(vd));          // of rows vd and vd + 1; of the next two the piece two further
+      const auto put = [&](auto power) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
-            const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
-            uint16_t* at = to + (c ? turned ^ 16 : turned) + 2 * c * kTile;
-            *reinterpret_cast<u32x2_t*>(at) = u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
-            *reinterpret_cast<u32x2_t*>(at + kTile) = u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
-          }
-        };
-        if (__all((__float_as_uint(vscale[p]) & 0x7fffffu) == 0)) put(std::true_type{});
-        else put(std::false_type{});
-      }
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
+          const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
+          uint16_t* at = to + (c ? turned ^ 16 : turned) + 2 * c * kTile;
+          *reinterpret_cast<u32x2_t*>(at) = u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
+          *reinterpret_cast<u32x2_t*>(at + kTile) = u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
+        }
+      };
+      if (__all((__float_as_uint(vscale[p]) & 0x807fffffu) == 0)) put(std::true_type{});
+      else put(std::false_type{});
     }
   };
   // Fragments are asked for ahead of the products: left to itself the compiler asks for each in front of its use.
@@ -835,22 +824,22 @@ size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   return f.ranges > 1 ? Kv8Parts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
-template <int DT, int DH, int MI, int NW, int KG>
+template <int DT, int DH, int MI, int KG>
 static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   constexpr size_t lds = KG * 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
   static std::atomic<uint32_t> granted{0};
-  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, NW, KG>), lds, granted) : kOk) return rc;
-  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * NW - 1) / (16 * MI * NW) * a.B * a.c.Hk;
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, KG>), lds, granted) : kOk) return rc;
+  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * kPromptWaves - 1) / (16 * MI * kPromptWaves) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
-  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, NW, KG>), dim3((unsigned)groups, ranges), dim3(NW * KG * kWave), lds, st, a, ranges, scratch);
+  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, KG>), dim3((unsigned)groups, ranges), dim3(kPromptWaves * KG * kWave), lds, st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, false, scratch, st);
   return kOk;
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
-  if (f.rows == 128) return prompt_launch<DT, DH, 2, 4, 1>(fn, a, f.ranges, scratch, st);
-  if (f.halves == 1) return prompt_launch<DT, DH, 1, 4, 1>(fn, a, f.ranges, scratch, st);
-  return prompt_launch<DT, DH, 1, 4, 2>(fn, a, f.ranges, scratch, st);
+  if (f.rows == 128) return prompt_launch<DT, DH, 2, 1>(fn, a, f.ranges, scratch, st);
+  if (f.halves == 1) return prompt_launch<DT, DH, 1, 1>(fn, a, f.ranges, scratch, st);
+  return prompt_launch<DT, DH, 1, 2>(fn, a, f.ranges, scratch, st);
 }
 int launch_kv8_prompt(const char* fn, const Kv8AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
   const PromptForm f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);
