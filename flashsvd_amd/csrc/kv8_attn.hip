@@ -29,11 +29,6 @@ __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u3
   }
   return x;
 }
-template <class E>
-__device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper) {
-  u32x4_t rest;
-  return rotated<E>(x, y, cos, sin, upper, rest);
-}
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 
 // Keys of a decode range, but for the last: a step of every wave, and whole blocks.
@@ -391,7 +386,8 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
 //   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
 //   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.  A q that the call rotates
-//   is rounded to its type, as one that comes rotated is: the registers of 128 rows are full.
+//   is two parts of its type in workgroups of 64 rows (77 tokens behind 1411: 22.4 us against 21.6, error 0.0002 of the output against 0.0004); in those of 128
+//   it is rounded once, as one that comes rotated is: with the second part their registers spill, 807 us against 347 for 8 x 2048 tokens.
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
@@ -409,7 +405,7 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
   return pack_bf16x2(x[0] * scale, x[1] * scale);
 }
 
-template <int DT, int DH, int MI, int KG>
+template <int DT, int DH, int MI, int KG, bool TURN>
 __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kernel(Kv8AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef typename E::frag_t frag_t;
@@ -450,7 +446,8 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   const int w0 = row0 + wave * QW;
   const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
 
-  frag_t qf[MI][ST];
+  constexpr bool kTwo = TURN && MI == 1;
+  frag_t qf[MI][ST], qr[kTwo ? ST : 1];                                     // qr: what the rounding of a rotated q leaves
   int seen[MI];
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
@@ -461,15 +458,17 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
     u32x4_t x[ST], cw[SH], sw[SH];
 #pragma unroll
     for (int st = 0; st < ST; ++st) x[st] = eight(qp + 32 * st + 8 * lg);
-    if (a.cos) {
+    if constexpr (TURN) {
       const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lg;
 #pragma unroll
       for (int st = 0; st < SH; ++st) { cw[st] = eight(a.cos + tp + 32 * st); sw[st] = eight(a.sin + tp + 32 * st); }
 #pragma unroll
       for (int st = 0; st < SH; ++st) {
         const u32x4_t low = x[st];
-        x[st] = rotated<E>(low, x[st + SH], cw[st], sw[st], false);
-        x[st + SH] = rotated<E>(x[st + SH], low, cw[st], sw[st], true);
+        u32x4_t r0, r1;
+        x[st] = rotated<E>(low, x[st + SH], cw[st], sw[st], false, r0);
+        x[st + SH] = rotated<E>(x[st + SH], low, cw[st], sw[st], true, r1);
+        if constexpr (kTwo) { qr[st] = __builtin_bit_cast(frag_t, r0); qr[st + SH] = __builtin_bit_cast(frag_t, r1); }
       }
     }
 #pragma unroll
@@ -606,8 +605,10 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
 #pragma unroll
       for (int st = 0; st < ST; ++st)
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
+        for (int mi = 0; mi < MI; ++mi) {
           s[mi][2 * half + j] = E::mfma(kf[j][st], qf[mi][st], st ? s[mi][2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+          if constexpr (kTwo) s[mi][2 * half + j] = E::mfma(kf[j][st], qr[st], s[mi][2 * half + j]);
+        }
   };
   // row d = 16 t + lr of V: its piece is turned by (lr / 4) ^ (lr & 6) ^ 4 (t % 2), so two addresses and constants reach all of them
   const uint32_t vread = lr * kTile + 8 * (lg ^ (lr >> 2) ^ (lr & 6));
@@ -824,16 +825,20 @@ size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   return f.ranges > 1 ? Kv8Parts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
-template <int DT, int DH, int MI, int KG>
-static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+template <int DT, int DH, int MI, int KG, bool TURN>
+static int prompt_launch_form(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   constexpr size_t lds = KG * 2 * ((size_t)kTile * (DH + 16) * 2 + (size_t)DH * kTile * 2);
   static std::atomic<uint32_t> granted{0};
-  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, KG>), lds, granted) : kOk) return rc;
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv8_prompt_kernel<DT, DH, MI, KG, TURN>), lds, granted) : kOk) return rc;
   const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * kPromptWaves - 1) / (16 * MI * kPromptWaves) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
-  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, KG>), dim3((unsigned)groups, ranges), dim3(kPromptWaves * KG * kWave), lds, st, a, ranges, scratch);
+  hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, KG, TURN>), dim3((unsigned)groups, ranges), dim3(kPromptWaves * KG * kWave), lds, st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, false, scratch, st);
   return kOk;
+}
+template <int DT, int DH, int MI, int KG>
+static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+  return a.cos ? prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, MI, KG, false>(fn, a, ranges, scratch, st);
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
