@@ -385,15 +385,16 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
 //   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
-//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.  A q that the call rotates
+//   The weights go into the second product as two bf16 parts, 16 significant bits, and into their sums as they are: rounded to one, outputs in bf16 are off by
+//   0.0020 of their size instead of 0.0016 (their own rounding), and 8 x 2048 tokens take 348 us instead of 434.  A q that the call rotates
 //   is two parts of its type in workgroups of 64 rows (77 tokens behind 1411: 22.4 us against 21.6, error 0.0002 of the output against 0.0004); in those of 128
 //   it is rounded once, as one that comes rotated is: with the second part their registers spill, 807 us against 347 for 8 x 2048 tokens.
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 342 us, 805 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
-// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.5 us for two of them.
+// 8 x 2048 tokens, 32 heads of 128: 434 us, 634 TFLOP/s of the formula's operations and half as many again for the second parts, 950 in all, where a large
+// product of the library reaches 1189.  Short chunks are bound by the time of a tile.
 constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
@@ -413,7 +414,6 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * kPromptWaves, QW = 16 * MI, BM = QW * kPromptWaves;
   constexpr int KL = DH / 16, KP = kTile * KL / TH;              // lanes of a key row; passes of the workgroup over the tile's keys
   constexpr int VL = DH / 4, VP = kTile / 4 * VL / TH;
-  constexpr bool kRest = DT == 1;
   extern __shared__ __align__(16) unsigned char smem[];
   const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
   uint16_t* Ks = reinterpret_cast<uint16_t*>(smem) + kg * 2 * kTile * (KSTR + DH);      // [2][kTile][KSTR]
@@ -476,14 +476,11 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   }
   const float scale = a.scale * 1.4426950408889634f;
   float m_run[MI];
-  // Sums of the weights: as they are rounded, by products with ones (the same in every element; 349 us against 357 for the long call); where the registers hold
-  // the second products' operands, a lane's own, unrounded.
-  typedef std::conditional_t<kRest, float, f32x4_t> sum_t;
-  sum_t l_run[MI];
+  float l_run[MI];                                                          // a lane's own sum of the weights, not rounded
   f32x4_t o[MI][NT];
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
-    m_run[mi] = -INFINITY; l_run[mi] = sum_t{};
+    m_run[mi] = -INFINITY; l_run[mi] = 0.f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[mi][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -618,18 +615,13 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
     for (int t = 0; t < NT; ++t) vf[t] = __builtin_bit_cast(pfrag_t, *reinterpret_cast<const u32x4_t*>(vt + ((st ^ t) & 1 ? vread ^ 32 : vread) + 16 * t * kTile));
   };
   pfrag_t ph[MI][2], pl[MI][2];
-  const pfrag_t ones = __builtin_bit_cast(pfrag_t, u32x4_t{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   const auto values = [&](const pfrag_t (&vf)[NT], int st) {
-    if constexpr (!kRest) {
-#pragma unroll
-      for (int mi = 0; mi < MI; ++mi) l_run[mi] = E16<0>::mfma(ones, ph[mi][st], l_run[mi]);
-    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi) {
         o[mi][t] = E16<0>::mfma(vf[t], ph[mi][st], o[mi][t]);
-        if (kRest) o[mi][t] = E16<0>::mfma(vf[t], pl[mi][st], o[mi][t]);
+        o[mi][t] = E16<0>::mfma(vf[t], pl[mi][st], o[mi][t]);
       }
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
@@ -682,7 +674,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s[mi][j][i] = __builtin_amdgcn_exp2f(s[mi][j][i]);
-          if constexpr (kRest) l_run[mi] += s[mi][j][i];
+          l_run[mi] += s[mi][j][i];
         }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -691,10 +683,10 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
         for (int c = 0; c < 4; ++c) {
           const float x0 = s[mi][2 * st + (c >> 1)][2 * (c & 1)], x1 = s[mi][2 * st + (c >> 1)][2 * (c & 1) + 1];
           hw[c] = pack_bf16x2(x0, x1);
-          if (kRest) lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+          lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
         }
         ph[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
-        if (kRest) pl[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+        pl[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
       }
     }
   };
@@ -741,10 +733,6 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
     values(vf[0], 0);
     values(vf[1], 1);
   }
-  const auto own_sum = [](const sum_t& l) {
-    if constexpr (kRest) return l;
-    else return l[0];
-  };
   if constexpr (KG > 1) {                // the halves' results
     static_assert(KG == 2 && MI == 1, "one exchange");
     f32x4_t* part = reinterpret_cast<f32x4_t*>(smem) + wave * (NT + 1) * kWave + lane;
@@ -752,7 +740,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
     if (kg == 1) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) part[t * kWave] = o[0][t];
-      part[NT * kWave] = f32x4_t{m_run[0], own_sum(l_run[0]), 0.f, 0.f};
+      part[NT * kWave] = f32x4_t{m_run[0], l_run[0], 0.f, 0.f};
     }
     __syncthreads();
     if (kg == 1) return;
@@ -769,7 +757,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
     const int r = w0 + 16 * mi + lr;
-    const float l = kRest ? column_sum(own_sum(l_run[mi])) : own_sum(l_run[mi]);
+    const float l = column_sum(l_run[mi]);
     if (r >= rows) continue;
     if (any_nan) {
 #pragma unroll
