@@ -385,16 +385,15 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
 //   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
-//   The weights go into the second product as two bf16 parts, 16 significant bits, and into their sums as they are: rounded to one, outputs in bf16 are off by
-//   0.0020 of their size instead of 0.0016 (their own rounding), and 8 x 2048 tokens take 348 us instead of 434.  A q that the call rotates
-//   is two parts of its type in workgroups of 64 rows (77 tokens behind 1411: 22.4 us against 21.6, error 0.0002 of the output against 0.0004); in those of 128
-//   it is rounded once, as one that comes rotated is: with the second part their registers spill, 807 us against 347 for 8 x 2048 tokens.
+//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.  A q that the call rotates
+//   is two parts of its type (77 tokens behind 1411: 22.4 us against 21.6, float16 outputs off by 0.0002 of their size against 0.0004; 8 x 2048 tokens, whose
+//   workgroups of 128 rows have registers for the fragments of 32 keys at a time only: 505 us against 442).
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 434 us, 634 TFLOP/s of the formula's operations and half as many again for the second parts, 950 in all, where a large
-// product of the library reaches 1189.  Short chunks are bound by the time of a tile.
+// 8 x 2048 tokens, 32 heads of 128: 342 us, 805 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
+// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.5 us for two of them.
 constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
@@ -446,8 +445,8 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   const int w0 = row0 + wave * QW;
   const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
 
-  constexpr bool kTwo = TURN && MI == 1;
-  frag_t qf[MI][ST], qr[kTwo ? ST : 1];                                     // qr: what the rounding of a rotated q leaves
+  constexpr bool kTight = TURN && MI == 2 && DH == 128;                     // fragments of 32 keys at a time: the registers hold no more beside both parts of q
+  frag_t qf[MI][ST], qr[TURN ? MI : 1][ST];                                 // qr: what the rounding of a rotated q leaves
   int seen[MI];
 #pragma unroll
   for (int mi = 0; mi < MI; ++mi) {
@@ -468,7 +467,9 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
         u32x4_t r0, r1;
         x[st] = rotated<E>(low, x[st + SH], cw[st], sw[st], false, r0);
         x[st + SH] = rotated<E>(x[st + SH], low, cw[st], sw[st], true, r1);
-        if constexpr (kTwo) { qr[st] = __builtin_bit_cast(frag_t, r0); qr[st + SH] = __builtin_bit_cast(frag_t, r1); }
+        if constexpr (kTight) asm volatile("" : "+v"(r0), "+v"(r1), "+v"(x[st]), "+v"(x[st + SH]));       // made here: put off, they spill
+        qr[mi][st] = __builtin_bit_cast(frag_t, r0);
+        qr[mi][st + SH] = __builtin_bit_cast(frag_t, r1);
       }
     }
 #pragma unroll
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
 #pragma unroll
         for (int mi = 0; mi < MI; ++mi) {
           s[mi][2 * half + j] = E::mfma(kf[j][st], qf[mi][st], st ? s[mi][2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
-          if constexpr (kTwo) s[mi][2 * half + j] = E::mfma(kf[j][st], qr[st], s[mi][2 * half + j]);
+          if constexpr (TURN) s[mi][2 * half + j] = E::mfma(kf[j][st], qr[mi][st], s[mi][2 * half + j]);
         }
   };
   // row d = 16 t + lr of V: its piece is turned by (lr / 4) ^ (lr & 6) ^ 4 (t % 2), so two addresses and constants reach all of them
@@ -718,20 +719,38 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
     if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
     f32x4_t s[MI][4];
-    frag_t kf[2][2][ST];
-    k_frags(kf[0], buf, 0);
-    k_frags(kf[1], buf, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    scores(s, kf[0], 0);
-    scores(s, kf[1], 1);
-    pfrag_t vf[2][NT];                 // those of V's first half during the softmax, of its second during the products with the first
-    v_frags(vf[0], buf, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    weights(s, at(i), g);
-    v_frags(vf[1], buf, 1);
-    __builtin_amdgcn_sched_barrier(0);
-    values(vf[0], 0);
-    values(vf[1], 1);
+    if constexpr (kTight) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        frag_t kf[2][ST];
+        k_frags(kf, buf, half);
+        scores(s, kf, half);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      weights(s, at(i), g);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        __builtin_amdgcn_sched_barrier(0);
+        pfrag_t vf[NT];
+        v_frags(vf, buf, st);
+        values(vf, st);
+      }
+    } else {
+      frag_t kf[2][2][ST];
+      k_frags(kf[0], buf, 0);
+      k_frags(kf[1], buf, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(s, kf[0], 0);
+      scores(s, kf[1], 1);
+      pfrag_t vf[2][NT];               // those of V's first half during the softmax, of its second during the products with the first
+      v_frags(vf[0], buf, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      weights(s, at(i), g);
+      v_frags(vf[1], buf, 1);
+      __builtin_amdgcn_sched_barrier(0);
+      values(vf[0], 0);
+      values(vf[1], 1);
+    }
   }
   if constexpr (KG > 1) {                // the halves' results
     static_assert(KG == 2 && MI == 1, "one exchange");

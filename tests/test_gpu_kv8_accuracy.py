@@ -1,12 +1,12 @@
-"""How few bits the attention over the KV cache in 8 bits may lose (csrc/kv8_attn.hip): the weights go into the 16-bit products as two parts, so what one
-16-bit rounding of them would leave is over the bounds here.  Inputs are made so that such roundings add up instead of averaging out."""
+"""How few bits the attention over the KV cache in 8 bits may lose (csrc/kv8_attn.hip): weights and a q that the call rotates go into the 16-bit products as
+two parts, so what a 16-bit rounding of either would leave is over the bounds here.  Inputs are made so that such roundings add up instead of averaging out."""
 import math
 
 import pytest
 import torch
 
 from tests import kv8_reference as R
-from tests.test_gpu_kv8 import F8, _close
+from tests.test_gpu_kv8 import F8, _close, half_step, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,75 @@ def test_decode_weights_are_two_parts(Dh, H, Hk, lens, dt):
                 hk = h // (H // Hk)
                 want, room = R.attend(q[b, h].cpu().double(), k[b, :n, hk].double(), v[b, :n, hk].double(), by, 0.0, TWO_PARTS)
                 _close(out[b, h], want, room, dt, f"{n} keys, head {h}, in {nsplit}")
+
+
+SHARP = 4.0                                              # softmax scale of the cases below
+
+
+def _against_rounding(x, cos, sin, pos, dt):
+    """(key, error of q's elements): codes +-1 that follow the signs of what a 16-bit rounding of x, rotated at pos, leaves of its elements, as many as keep the
+    score near 0, and the relative error of an element as two parts: 2^-2p of the rounding, 2^-22 of the rotated pair for the rotation in fp32."""
+    y = R.rotate(x.double(), cos, sin, pos)
+    left = y.to(dt).double() - y
+    part = left.sign() * y                               # of the score
+    up, down = ([d for d in part.abs().argsort().tolist() if part[d] * s > 0 and abs(y[d]) > 0.2] for s in (1, -1))
+    key, run = torch.zeros_like(y), 0.0
+    while up if run <= 0 else down:
+        d = (up if run <= 0 else down).pop()
+        if abs(run + float(part[d])) <= 1.0:
+            key[d], run = left[d].sign(), run + float(part[d])
+    pair = x.double().abs()
+    pair = pair + pair.roll(len(y) // 2)
+    used = key != 0
+    error = half_step(dt) ** 2 + 2.0 ** -22 * float((pair[used] / y[used].abs()).max())
+    shift, bound = SHARP * float((key * left).sum()), SHARP * float(key.abs() @ y.abs()) * (error + len(y) * 2.0 ** -23)
+    assert shift > 3 * bound + 4 * half_step(dt), "the case would not tell one rounding from two"
+    return key, error
+
+
+def _away_from_zero(g, dt, Dh):
+    return ((0.5 + torch.rand(Dh, generator=g)) * torch.where(torch.rand(Dh, generator=g) < 0.5, -1.0, 1.0)).to(dt)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("form", PROMPTS)
+def test_a_rotated_prompt_query_is_two_parts(form, Dh, dt):
+    """One key against the roundings of the row that it is made for; its score would be off by the sum of them all."""
+    from flashsvd_amd import hip_ops
+    p = PROMPTS[form]
+    B, Hk, M, past, H = p["B"], p["Hk"], p["M"], p["past"], p["Hk"] * p["G"]
+    g = torch.Generator().manual_seed(61)
+    cos, sin = tables(past + M, Dh, dt)
+    x = _away_from_zero(g, dt, Dh)
+    q = x.expand(B, M, H, Dh).contiguous().cuda()
+    pos = torch.full((B,), past, dtype=torch.int32, device="cuda")
+    for b, m, h in [(0, 5, 0), (B - 1, M - 1, H - 1)]:
+        k, v, scale = _held(B, past + M, Hk, Dh, 32)
+        hk = h // p["G"]
+        key, error = _against_rounding(x, cos, sin, past + m, dt)
+        k[b, 3, hk] = key.float()
+        v[b, 3, hk] = _varied(Dh)
+        out = hip_ops.attn_prefill_kv8(q, k.to(F8).cuda(), v.to(F8).cuda(), scale.cuda(), scale.cuda(), pos, block=32, cos=cos.cuda(), sin=sin.cuda(),
+                                       softmax_scale=SHARP).cpu()
+        n = past + m + 1
+        want, room = R.attend(R.rotate(x.double(), cos, sin, past + m), k[b, :n, hk].double(), v[b, :n, hk].double(), SHARP, error, TWO_PARTS)
+        _close(out[b, m, h], want, room, dt, f"{form}: row {m} of head {h}")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Dh,H,Hk,n", [(64, 8, 8, 137), (128, 8, 2, 900), (128, 4, 4, 30), (64, 40, 2, 200)])
+def test_a_rotated_decode_query_is_two_parts(Dh, H, Hk, n, dt):
+    from flashsvd_amd import hip_ops
+    g = torch.Generator().manual_seed(62)
+    cos, sin = tables(n + 1, Dh, dt)
+    x = _away_from_zero(g, dt, Dh)
+    key, error = _against_rounding(x, cos, sin, n, dt)
+    k, v, scale = _held(1, n, Hk, Dh, 32)
+    k[0, 3], v[0, 3] = key.float(), _varied(Dh)
+    q = x.expand(1, H, Dh).contiguous().cuda()
+    out = hip_ops.attn_decode_kv8(q, k.to(F8).cuda(), v.to(F8).cuda(), scale.cuda(), scale.cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"), block=32,
+                                  cos=cos.cuda(), sin=sin.cuda(), softmax_scale=SHARP).cpu()
+    for h in (0, H - 1):
+        want, room = R.attend(R.rotate(x.double(), cos, sin, n), k[0, :, 0].double(), v[0, :, 0].double(), SHARP, error, TWO_PARTS)
+        _close(out[0, h], want, room, dt, f"head {h}")
