@@ -385,15 +385,16 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
 //   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
-//   The weights are rounded to 16 bits (2^-8 of each, which averages out); for float16 outputs what that leaves is a second product.  A q that the call rotates
+//   The weights go into the second product as two bf16 parts, 16 significant bits, and into their sums as they are: rounded to one, outputs in bf16 are off by
+//   0.0020 of their size instead of 0.0016 (their own rounding), and 8 x 2048 tokens take 348 us instead of 434.  A q that the call rotates
 //   is two parts of its type (77 tokens behind 1411: 22.4 us against 21.6, float16 outputs off by 0.0002 of their size against 0.0004; 8 x 2048 tokens, whose
 //   workgroups of 128 rows have registers for the fragments of 32 keys at a time only: 505 us against 442).
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 342 us, 805 TFLOP/s where a large product of the library reaches 1189.  The vector unit (conversion, softmax), the reads of
-// LDS and the matrix cores are busy about 40 % of the time each and overlap in part.  Short chunks are bound by the time of a tile, 1.5 us for two of them.
+// 8 x 2048 tokens, 32 heads of 128: 434 us, 634 TFLOP/s of the formula's operations and half as many again for the second parts, 950 in all, where a large
+// product of the library reaches 1189.  Short chunks are bound by the time of a tile.
 constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
