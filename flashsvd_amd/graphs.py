@@ -111,6 +111,7 @@ class GraphedDecoder:
 
     def set_state(self, tokens: torch.Tensor, position: int) -> None:
         from . import hip_ops
+        from .runtime.cache import FlashSVDKV8Cache
         if position < 0 or position >= self.cache.max_cache_len:
             raise IndexError(f"decode position {position} outside the cache (max {self.cache.max_cache_len})")
         ids = tokens.reshape(self.B, 1)
@@ -120,6 +121,8 @@ class GraphedDecoder:
             self.tokens.copy_(ids)
             self.positions.fill_(int(position))
         self._host_pos = int(position)
+        if isinstance(self.cache, FlashSVDKV8Cache):        # rows behind it are given up
+            self.cache._seen_tokens = int(position)
 
     def step(self) -> torch.Tensor:
         """Replay one token; returns the device tensor holding the next token ids [B,1]."""

@@ -246,8 +246,9 @@ class FlashSVDKV8Cache(_HeadCacheBase):
     Half the bytes of :class:`FlashSVDV15DenseKVCache` and its method names where they make sense; rows are written by
     ``hip_ops.kv8_append`` and read by ``hip_ops.attn_decode_kv8`` / ``attn_prefill_kv8``.  ``dtype`` is that of the activations.  A row's
     tokens stand side by side for each head in memory (the kernels take any strides).  Writing a position makes it the last valid one
-    of its block, so rows are written in order; going back to an earlier position and continuing from there is fine.  No counterpart in
-    the reference, whose caches are of 16 bits."""
+    of its block, so rows are written in order: a write at an earlier position gives up the rows behind it, and the held length
+    (``get_seq_length()``) is what it leaves, where the caches of 16 bits keep the largest.  A token whose position is on the device
+    counts as one further.  No counterpart in the reference, whose caches are of 16 bits."""
 
     def __init__(self, config, *, max_batch_size: int, max_cache_len: int, block_size: int = 32, device=None, dtype: torch.dtype = torch.float16,
                  layer_device_map: Optional[dict] = None) -> None:
@@ -281,6 +282,23 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         self.value_cache[layer_idx], self.value_scale[layer_idx] = self._storage(h, dh, dev)
         self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
 
+    def _note_seen(self, layer_idx: int, q_len: int, cache_position) -> None:
+        if int(layer_idx) != 0:
+            return
+        if cache_position is None:
+            self._seen_tokens = int(q_len)
+            return
+        pos = torch.as_tensor(cache_position).reshape(-1)
+        if int(q_len) != 1:                                # a chunk: its first position
+            self._seen_tokens = (int(pos[0]) if pos.numel() else self._seen_tokens) + int(q_len)
+        elif pos.is_cuda:
+            self._seen_tokens += 1
+        else:
+            self._seen_tokens = int(pos.max()) + 1
+
+    def advance_after_fa2(self, layer_idx: int, *, q_len: int, cache_position) -> None:
+        self._note_seen(layer_idx, q_len, self._seen_tokens if cache_position is None else cache_position)
+
     def operands(self, layer_idx: int, batch_size: int):
         """(key codes, value codes, key scales, value scales) of the first ``batch_size`` sequences, as the operators take them."""
         i, b = int(layer_idx), int(batch_size)
@@ -305,12 +323,13 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         return out[0], out[1]
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs: Optional[dict[str, Any]] = None):
-        """key/value_states are [B, Hk, T, Dh] (keys rotated) for consecutive positions; returns the held cache prefix as [B, Hk, L, Dh]."""
+        """key/value_states are [B, Hk, T, Dh] (keys rotated) for consecutive positions; returns what the cache holds then, up to the last row
+        written, as [B, Hk, L, Dh]."""
         cache_position = (cache_kwargs or {}).get("cache_position")
         t, start = key_states.shape[2], 0
         if cache_position is not None:
             pos = cache_position.reshape(-1).tolist()
-            if pos != list(range(pos[0], pos[0] + t)):
+            if not pos or pos != list(range(pos[0], pos[0] + t)):
                 raise ValueError("FlashSVDKV8Cache takes consecutive positions: a block's scale is that of the rows up to the last one written")
             start = pos[0]
         if start < 0 or start + t > self._max_cache_len:
@@ -319,9 +338,8 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         k, v = (x.to(device=dev, dtype=self._dtype).transpose(1, 2) for x in (key_states, value_states))
         k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v))
         self.append(layer_idx, k, v, torch.full((k.shape[0],), start, dtype=torch.int32, device=dev))
-        self._note_seen(layer_idx, t, cache_position)
-        n = t if cache_position is None else max(int(self.get_seq_length()), start + t)
-        k, v = self.dequantize(layer_idx, batch_size=k.shape[0], length=n)
+        self._note_seen(layer_idx, t, torch.tensor([start]))
+        k, v = self.dequantize(layer_idx, batch_size=k.shape[0], length=start + t)
         return k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
 
 
