@@ -168,7 +168,7 @@ int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, in
   const char* fn = "fsvd_kv8_append";
   if (const int rc = check_kv8_cache(fn, cache)) return rc;
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
-  if (k == nullptr || v == nullptr || positions == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (positions == nullptr || (T != 0 && (k == nullptr || v == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (T < 0) { set_last_error("%s: %d rows", fn, T); return kErrBadShape; }
   if (const int rc = check_written(fn, cache, B)) return rc;
   const Kv8AppendArgs a{*cache, in16(k), sk_b, sk_t, sk_h, in16(v), sv_b, sv_t, sv_h, positions, rows, in16(cos), in16(sin), rope_len, B, T, dtype};
@@ -215,7 +215,7 @@ int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq
   const char* fn = "fsvd_attn_prefill_kv8";
   if (const int rc = check_kv8_cache(fn, cache)) return rc;
   if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
-  if (q == nullptr || out == nullptr || q_pos0 == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (q_pos0 == nullptr || (M != 0 && (q == nullptr || out == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (M < 0 || H <= 0 || H % cache->Hk) { set_last_error("%s: %d rows of %d query heads over %d", fn, M, H, cache->Hk); return kErrBadShape; }
   if (const int rc = check_out(fn, B, M, H, so_b, so_m, so_h)) return rc;
   const Kv8AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,

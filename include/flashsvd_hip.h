@@ -205,7 +205,8 @@ typedef struct fsvd_kv8_cache {
 /* Row t < rows[b] (rows NULL: T) of k and v [B, T, Hk, Dh] goes to cache position positions[b] + t of sequence b; k is rotated there (cos and sin
  * [rope_len, Dh / 2], NULL: not; halves of a head are the pairs, fp32) and rounded once.  A block's scale covers its new rows; a block with rows before the
  * first new one keeps the larger of that and its old scale, and those rows move to it.  The rows behind the last written one of a block are not valid
- * from then on.  Rows outside [0, S) are dropped.  A NaN stays one, an infinity becomes the largest code; neither decides a scale. */
+ * from then on.  Rows outside [0, S) are dropped; with T = 0 there are none, and k and v may be NULL.  A NaN stays one, an infinity becomes the
+ * largest code; neither decides a scale. */
 int fsvd_kv8_append(const fsvd_kv8_cache* cache, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t,
                     int64_t sv_h, const int32_t* positions, const int32_t* rows, const void* cos, const void* sin, int rope_len, int B, int T, int dtype,
                     void* stream);
@@ -222,7 +223,7 @@ int fsvd_attn_decode_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_
 
 /* Causal attention of a chunk of a prompt over a cache in 8 bits that holds the chunk's own rows already: q [B, M, H, Dh], row m of sequence b stands
  * at position q_pos0[b] + m (rotated there with cos / sin, NULL: q comes rotated) and sees the keys up to that.  Rows m >= rows[b] (NULL: M) of out
- * [B, M, H, Dh] are left as they were.  Softmax scale 1 / sqrt(Dh) when scale <= 0.  scratch as for fsvd_attn_decode_kv8. */
+ * [B, M, H, Dh] are left as they were; with M = 0 q and out may be NULL.  Softmax scale 1 / sqrt(Dh) when scale <= 0.  scratch as for fsvd_attn_decode_kv8. */
 size_t fsvd_attn_prefill_kv8_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S);
 int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
                           const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
