@@ -92,13 +92,17 @@ class GraphedDecoder:
             self.uniforms.uniform_(generator=self.generator)
 
     def capture(self) -> None:
+        from .runtime.cache import FlashSVDKV8Cache
         tok0, pos0 = self.tokens.clone(), self.positions.clone()
+        if isinstance(self.cache, FlashSVDKV8Cache):        # a row gives up those behind it in its block: the warm-ups' go behind the cache, where they are dropped
+            self.positions.fill_(self.cache.max_cache_len)
+        warm = self.positions.clone()
         side = torch.cuda.Stream(device=self.tokens.device)
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(max(1, self.warmup)):
                 self._step()
-                self.positions.copy_(pos0)   # warm-ups rewrite the same slot
+                self.positions.copy_(warm)   # warm-ups rewrite the same slot
                 self.tokens.copy_(tok0)
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()

@@ -98,3 +98,37 @@ def test_a_model_continues_from_where_it_went_back_to():
     assert torch.equal(out[0][0], out[1][0]) and out[0][1] == out[1][1]
     for a, b in zip(out[0][2], out[1][2]):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sampling", [None, dict(temperature=0.9, top_k=20)])
+def test_a_capture_leaves_the_cache_as_it_was(sampling):
+    """Captured before the first state is set as well as behind it, and again in between: the tokens of a decoder that runs eagerly."""
+    from flashsvd_amd.graphs import GraphedDecoder
+    from tests.test_gpu_kv8_model import _cache, _model
+    model, S = _model(128), 64
+    ids = torch.randint(0, 512, (2, 20), generator=torch.Generator().manual_seed(5)).cuda()
+    out = []
+    for captures in ((), (0,), (1, 4)):
+        c = _cache(model, 2, S)
+        first = model(ids, past_key_values=c, cache_position=torch.arange(20)).logits[:, -1].argmax(-1, keepdim=True)
+        dec = GraphedDecoder(model, c, 2, sampling=sampling, generator=torch.Generator(device="cuda").manual_seed(7))
+
+        def capture():
+            buffers = c.key_cache + c.value_cache + c.key_scale + c.value_scale
+            before = [t.view(torch.uint8).clone() if t.element_size() == 1 else t.clone() for t in buffers]
+            dec.capture()
+            for t, w in zip(buffers, before):
+                assert torch.equal(t.view(torch.uint8) if t.element_size() == 1 else t, w)
+
+        if 0 in captures:
+            capture()
+        dec.set_state(first, 20)
+        got = []
+        for i in range(1, 8):
+            if i in captures:
+                capture()
+            got.append((dec.step() if captures else dec.eager_step()).tolist())
+        assert c.get_seq_length() == 27
+        out.append(got)
+    assert out[0] == out[1] == out[2]
