@@ -14,6 +14,7 @@ from . import _lib
 from .torch_ops import ops as _OPS
 
 _BF16, _F8, _F32, _I32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
+_MOST_INT = 2 ** 31 - 1
 
 
 def _stream() -> int:
@@ -557,6 +558,7 @@ def _sample_token_impl(logits, uniforms, tokens, positions, temperature, top_k, 
         ptrs.append(None if t is None else t.data_ptr())
     if B == 0:
         return
+    top_k = top_k if 0 < top_k <= V else 0                      # the C ABI's int need not hold what keeps all
     with _on(dev):
         rc = _lib.load().fsvd_sample_token(logits.data_ptr(), logits.stride(0), ptrs[0], tokens.data_ptr(), tokens.stride(0), ptrs[1], temperature, ptrs[2],
                                            top_k, ptrs[3], top_p, ptrs[4], min_p, ptrs[5], B, V, code, _stream())
@@ -1093,7 +1095,10 @@ def _attn_decode_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, 
     if B == 0:
         return out
     lib, so = _lib.load(), out.stride()
-    nsplit = 0 if nsplit is None else nsplit
+    # the C ABI takes 32 bits of either; more ranges than keys are none
+    nsplit = 0 if nsplit is None else max(0, min(nsplit, c.S))
+    if not -_MOST_INT <= seqlen_add <= _MOST_INT:
+        raise ValueError(f"seqlen_add must be a 32-bit number, got {seqlen_add}")
     nbytes, scratch, ptr = lib.fsvd_attn_decode_kv8_scratch_bytes(B, H, Hk, Dh, c.S, nsplit), None, None
     if nbytes:
         scratch = q.new_empty(nbytes, dtype=torch.uint8)       # of this call and stream
