@@ -101,11 +101,13 @@ __global__ __launch_bounds__(kWave) void kv8_append_one_kernel(Kv8AppendArgs a) 
 template <int DT, int DH>
 static void append_form(const Kv8AppendArgs& a, hipStream_t st) {
   if (a.T == 1) {
+    set_last_form("kv8 row");
     hipLaunchKernelGGL((kv8_append_one_kernel<DT, DH>), dim3((unsigned)(a.B * a.c.Hk)), dim3(kWave), 0, st, a);
     return;
   }
   constexpr int LPR = DH / 16;
   const int passes = max(1, a.c.block * LPR / 256), rows = passes * 256 / LPR;       // rows of a workgroup: whole blocks
+  set_last_form(passes == 1 ? "kv8 rows 1" : passes == 2 ? "kv8 rows 2" : "kv8 rows 4");
   const dim3 grid(2 * a.c.Hk, (unsigned)((a.T + a.c.block - 1 + (int64_t)rows - 1) / rows), a.B);
   if (passes == 1) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 1>), grid, dim3(256), 0, st, a);
   else if (passes == 2) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 2>), grid, dim3(256), 0, st, a);

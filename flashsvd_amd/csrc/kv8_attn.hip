@@ -362,6 +362,7 @@ static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStr
   hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave),
                      kDecWaves * min(a.H / a.c.Hk, kDecGroup) * (DH + 4) * sizeof(float), st, a, ranges, scratch);
   if (ranges > 1) launch_join<DT, DH>(a, ranges, true, scratch, st);
+  set_last_form(ranges == 1 ? "kv8 decode" : ranges <= 8 ? "kv8 decode ranges" : ranges <= kWave ? "kv8 decode ranges 9" : "kv8 decode ranges 65");
 }
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float* scratch, hipStream_t st) {
   Kv8AttnArgs a = args;
@@ -850,6 +851,7 @@ static int prompt_launch(const char* fn, const Kv8AttnArgs& a, int ranges, float
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv8AttnArgs& a, PromptForm f, float* scratch, hipStream_t st) {
+  set_last_form(f.rows == 128 ? "kv8 prompt 128" : f.halves == 1 ? "kv8 prompt 64" : f.ranges == 1 ? "kv8 prompt 64 halves" : "kv8 prompt 64 halves ranges");
   if (f.rows == 128) return prompt_launch<DT, DH, 2, 1>(fn, a, f.ranges, scratch, st);
   if (f.halves == 1) return prompt_launch<DT, DH, 1, 1>(fn, a, f.ranges, scratch, st);
   return prompt_launch<DT, DH, 1, 2>(fn, a, f.ranges, scratch, st);

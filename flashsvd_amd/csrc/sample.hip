@@ -464,6 +464,7 @@ template <int DT, int R>
 static int launch_sample(const char* fn, const SampleArgs& a, int B, hipStream_t st) {
   static std::atomic<uint32_t> granted{0};
   if (const int rc = grant_lds(fn, reinterpret_cast<const void*>(&sample_token_kernel<DT, R>), kHistWords * 4, granted)) return rc;
+  set_last_form(R == 0 ? "draw" : R == 2 ? "draw 2" : R == 4 ? "draw 4" : R == 8 ? "draw 8" : "draw 16");
   hipLaunchKernelGGL((sample_token_kernel<DT, R>), dim3(B), dim3(kDrawThreads), kHistWords * 4, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }

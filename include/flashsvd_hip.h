@@ -38,8 +38,8 @@ extern "C" {
 
 int fsvd_version(void);
 const char* fsvd_last_error(void);
-/* Which kernel form the last projection, gate / up pair, q / k / v expansion or head expansion that this thread issued took
- * ("256 x 256 pair", "ring 128 x 64", "vector", ...): for tests and measurements; the names are no part of the interface. */
+/* Which kernel form the last projection, gate / up pair, q / k / v expansion, head expansion, call on a cache in 8 bits or draw of a
+ * token that this thread issued took ("256 x 256 pair", "ring 128 x 64", "vector", "kv8 prompt 128", ...): for tests and measurements; the names are no part of the interface. */
 const char* fsvd_last_form(void);
 
 /* Optional scratch for the projections (fsvd_linear, fsvd_swiglu_linear) of 17..127 rows, of 3..16 rows when the matrix has
