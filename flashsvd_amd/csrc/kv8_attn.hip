@@ -1,6 +1,4 @@
 // Attention over the KV cache in 8 bits.
-#include <type_traits>
-
 #include "kv8.hpp"
 
 namespace fsvd {
@@ -399,12 +397,24 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
-// a pair of codes as bf16, times a scale: in the conversion where it is a power of two, as kv8_append leaves it
-template <bool HI, bool POWER>
-__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float scale) {
-  if constexpr (POWER) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-  const f32x2_t x = HI ? codes_hi(w) : codes_lo(w);
-  return pack_bf16x2(x[0] * scale, x[1] * scale);
+// A value scale as a power of two, which goes into the conversion of the codes to bf16 exactly, and the factor that it leaves, which is multiplied to the
+// weights in front of their rounding: 1 for the scales that kv8_append makes (looking for others costs 3 us of 436).  A zero, a subnormal, an infinity and a
+// NaN are all factor.
+__device__ __forceinline__ bool is_power(float scale) {
+  const uint32_t u = __float_as_uint(scale);
+  return (u & 0x807fffffu) == 0 && u != 0 && u != 0x7f800000u;
+}
+__device__ __forceinline__ float power_of(float scale) {
+  const uint32_t e = __float_as_uint(scale) & 0x7f800000u;
+  return e == 0 || e == 0x7f800000u ? 1.f : __uint_as_float(e);
+}
+__device__ __forceinline__ float factor_of(float scale) {
+  const uint32_t u = __float_as_uint(scale), e = u & 0x7f800000u;
+  return e == 0 || e == 0x7f800000u ? scale : __uint_as_float((u & 0x807fffffu) | 0x3f800000u);
+}
+template <bool HI>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t w, float power) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, power, HI));
 }
 
 template <int DT, int DH, int MI, int KG, bool TURN>
@@ -421,6 +431,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   uint16_t* Vt = Ks + 2 * kTile * KSTR;                                     // [2][DH][kTile]
   __shared__ __align__(16) int nan_at[DH];                                  // the first NaN of a dimension among the values that not every row sees
   __shared__ int any_nan;
+  __shared__ int odd_tile[KG][2];                                           // the last tile of a buffer with a value scale that is no power of two
 
   const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
   int mt, hb;
@@ -569,7 +580,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
       }
     }
   };
-  const auto stage_v = [&](int buf) {
+  const auto stage_v = [&](int buf, int tile) {
     uint16_t* vt = Vt + buf * DH * kTile;
 #pragma unroll
     for (int p = 0; p < VP; ++p) {
@@ -577,18 +588,19 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
       const int ko = (4 * row4) & 31, col = ((4 * row4) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
       uint16_t* to = vt + vd * kTile;
       const uint32_t turned = col ^ (8 * v_piece(vd));          // of rows vd and vd + 1; of the next two the piece two further
-      const auto put = [&](auto power) {
+      float power = vscale[p];
+      if (__builtin_expect(!__all(is_power(power)), 0)) {
+        power = power_of(power);
+        odd_tile[kg][buf] = tile;
+      }
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
-          const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
-          uint16_t* at = to + (c ? turned ^ 16 : turned) + 2 * c * kTile;
-          *reinterpret_cast<u32x2_t*>(at) = u32x2_t{scaled_pair<false, power>(lo, vscale[p]), scaled_pair<false, power>(hi, vscale[p])};
-          *reinterpret_cast<u32x2_t*>(at + kTile) = u32x2_t{scaled_pair<true, power>(lo, vscale[p]), scaled_pair<true, power>(hi, vscale[p])};
-        }
-      };
-      if (__all((__float_as_uint(vscale[p]) & 0x807fffffu) == 0)) put(std::true_type{});
-      else put(std::false_type{});
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t lo = __builtin_amdgcn_perm(vreg[p][1], vreg[p][0], c ? 0x07030602u : 0x05010400u);
+        const uint32_t hi = __builtin_amdgcn_perm(vreg[p][3], vreg[p][2], c ? 0x07030602u : 0x05010400u);
+        uint16_t* at = to + (c ? turned ^ 16 : turned) + 2 * c * kTile;
+        *reinterpret_cast<u32x2_t*>(at) = u32x2_t{scaled_pair<false>(lo, power), scaled_pair<false>(hi, power)};
+        *reinterpret_cast<u32x2_t*>(at + kTile) = u32x2_t{scaled_pair<true>(lo, power), scaled_pair<true>(hi, power)};
+      }
     }
   };
   // Fragments are asked for ahead of the products: left to itself the compiler asks for each in front of its use.
@@ -628,7 +640,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
       }
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
-  const auto weights = [&](f32x4_t (&s)[MI][4], int n0, float by) {
+  const auto weights = [&](f32x4_t (&s)[MI][4], int n0, float by, bool odd) {
     float f[4];
     by *= scale;
     const bool plain = n0 + kTile <= wave_sees;                      // every row of the wave sees the whole tile
@@ -679,6 +691,18 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
           s[mi][j][i] = __builtin_amdgcn_exp2f(s[mi][j][i]);
           l_run[mi] += s[mi][j][i];
         }
+    }
+    if (__builtin_expect(odd, 0)) {
+      const float mine = factor_of(scale_at(vsp, n0, s_offset(16 * (lane & 3), n_end - n0)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float left = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(mine), j));
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) s[mi][j] *= left;
+      }
+    }
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         uint32_t hw[4], lw[4];
@@ -691,7 +715,6 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
         ph[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
         pl[mi][st] = __builtin_bit_cast(pfrag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
       }
-    }
   };
 
 #pragma unroll
@@ -708,19 +731,21 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   if (n > 0) { request_k(at(0)); request_v(at(0)); request_f(at(0)); }
   for (int d = tid; d < DH; d += TH) nan_at[d] = 0x7fffffff;
   if (tid == 0) any_nan = 0;
+  if (tid < 2) odd_tile[kg][tid] = -1;
   __syncthreads();
   for (int i = 0; i * KG < all; ++i) {
     const int buf = i & 1;
     if (KG == 1 || i < n) {
       stage_k(buf);
       if (at(i) + kTile > all_see) set_nans_aside(at(i));
-      stage_v(buf);
+      stage_v(buf, i);
     }
     const float g = fs;
     if (i + 1 < n) { request_k(at(i + 1)); request_v(at(i + 1)); request_f(at(i + 1)); }
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
     if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
     f32x4_t s[MI][4];
+    const bool odd = __builtin_amdgcn_readfirstlane(odd_tile[kg][buf]) == i;
     if constexpr (kTight) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -729,7 +754,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
         scores(s, kf, half);
         __builtin_amdgcn_sched_barrier(0);
       }
-      weights(s, at(i), g);
+      weights(s, at(i), g, odd);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         __builtin_amdgcn_sched_barrier(0);
@@ -747,7 +772,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
       pfrag_t vf[2][NT];               // those of V's first half during the softmax, of its second during the products with the first
       v_frags(vf[0], buf, 0);
       __builtin_amdgcn_sched_barrier(0);
-      weights(s, at(i), g);
+      weights(s, at(i), g, odd);
       v_frags(vf[1], buf, 1);
       __builtin_amdgcn_sched_barrier(0);
       values(vf[0], 0);

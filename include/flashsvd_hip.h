@@ -188,7 +188,7 @@ int fsvd_sample_token(const void* logits, int64_t ld, const float* uniforms, int
 
 /* ---------------------------------------------------------------------------------------------
  * KV cache in 8 bits.  Codes [B, S, Hk, Dh] in e4m3 (finite form, largest 448), keys after their rotation; one fp32 scale for each sequence, block of
- * `block` tokens and kv head, value = code * scale.  fsvd_kv8_append makes every scale a power of two, 2^e with the smallest e >= -126 for which
+ * `block` tokens and kv head, value = code * scale, scale >= 0.  fsvd_kv8_append makes every scale a power of two, 2^e with the smallest e >= -126 for which
  * 448 * 2^e covers what is held.  k and v share their strides (elements; multiples of 16, as the addresses of 16 bytes), k_scale and v_scale theirs;
  * those of tokens and blocks at most 2^26.
  * head_dim 64 and 128; blocks of 16, 32, 64 and 128 tokens.  No counterpart in the reference, whose caches are of 16 bits. */

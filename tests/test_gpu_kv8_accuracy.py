@@ -148,3 +148,33 @@ def test_a_rotated_decode_query_is_two_parts(Dh, H, Hk, n, dt):
     for h in (0, H - 1):
         want, room = R.attend(R.rotate(x.double(), cos, sin, n), k[0, :, 0].double(), v[0, :, 0].double(), SHARP, error, TWO_PARTS)
         _close(out[0, h], want, room, dt, f"head {h}")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("form", PROMPTS)
+def test_scales_that_are_no_power_of_two(form, Dh, dt):
+    """value = code * scale for any scale: 0.98 of a half step of bf16 above 1, with powers of two and zeros among the blocks; a value rounded to bf16 would be off
+    by nearly 2^-8 of itself."""
+    from flashsvd_amd import hip_ops
+    p = PROMPTS[form]
+    B, Hk, M, past, H = p["B"], p["Hk"], p["M"], p["past"], p["Hk"] * p["G"]
+    block = 16
+    k, v, scale = _held(B, past + M, Hk, Dh, block)
+    k[:, 5::16, :, 0] = -1.0
+    v[:, 5::16] = torch.exp2((torch.arange(Dh) % 4).float())
+    ks, vs = scale * 1.37, scale * torch.tensor([1 + 0.98 / 256, 1.0, 0.0, 2.0 * (1 + 0.98 / 256)]).repeat(scale.shape[1])[:scale.shape[1], None]
+    by = 5 * math.log(2) / 1.37
+    q = torch.zeros(B, M, H, Dh, dtype=dt, device="cuda")
+    q[..., 0] = 1.0
+    out = hip_ops.attn_prefill_kv8(q, k.to(F8).cuda(), v.to(F8).cuda(), ks.cuda(), vs.cuda(), torch.full((B,), past, dtype=torch.int32, device="cuda"),
+                                   block=block, softmax_scale=by).cpu()
+    b, h = B - 1, H - 1
+    full = lambda s: s[b, :, h // p["G"], None].double().repeat_interleave(block, 0)[:past + M]      # noqa: E731
+    kk, vv = k[b, :, h // p["G"]].double() * full(ks), v[b, :, h // p["G"]].double() * full(vs)
+    for m in range(M):
+        want, room = R.attend(q[b, m, h].cpu().double(), kk[:past + m + 1], vv[:past + m + 1], by, 0.0, TWO_PARTS)
+        _close(out[b, m, h], want, room, dt, f"{form}: row {m}")
+    one = hip_ops.attn_decode_kv8(q[:, M - 1], k.to(F8).cuda(), v.to(F8).cuda(), ks.cuda(), vs.cuda(), torch.full((B,), past + M, dtype=torch.int32, device="cuda"),
+                                  block=block, softmax_scale=by).cpu()
+    _close(one[b, h], want, room, dt, f"{form}: a token behind it")
