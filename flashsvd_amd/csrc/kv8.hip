@@ -111,7 +111,7 @@ static void append_form(const Kv8AppendArgs& a, hipStream_t st) {
   const dim3 grid(2 * a.c.Hk, (unsigned)((a.T + a.c.block - 1 + (int64_t)rows - 1) / rows), a.B);
   if (passes == 1) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 1>), grid, dim3(256), 0, st, a);
   else if (passes == 2) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 2>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 4>), grid, dim3(256), 0, st, a);
+  else if constexpr (DH == 128) hipLaunchKernelGGL((kv8_append_kernel<DT, DH, 4>), grid, dim3(256), 0, st, a);      // blocks of 128
 }
 int launch_kv8_append(const char* fn, const Kv8AppendArgs& a, hipStream_t st) {
   if (a.T == 0) return kOk;
