@@ -338,7 +338,9 @@ __global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8Att
   }
 }
 
-// Ranges of a decode call (times in us from a captured graph, 32 heads of 128 over 8).
+// Ranges of a decode call (times in us from a captured graph, 32 heads of 128 over 8).  S is the room of the cache: what it holds is known on the device only,
+// so short sequences in a long cache are cut too (without an append, 137 keys of 8 heads of 64 in room for 160: 4.5, for 4096: 6.3; 16 sequences of 4090 keys with 32 kv heads in
+// room for 4091: 96, for 32768: 101).
 //  - About two workgroups for each compute unit: with 512 / 640 / 1024 in all one sequence of 30000 keys takes 20.3 / 22.2 / 23.1, 64 of 2000 49.5 / 52.9 / 52.4;
 //    with 384 one sequence of 16001 takes 16.4 against 14.3.
 //  - Ranges of 2048 keys at most: 16 sequences of 4090 keys with 32 kv heads take 105 in one range, 97 to 102 in three, 114 in six.
@@ -383,23 +385,24 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // the workgroup: K row by row, V transposed (two keys of a dimension next to each other by byte permutes), two buffers and one barrier a tile.
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
-//   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the value scale goes into the conversion.
+//   The key scale of a block multiplies its maximum and goes into the multiply-add in front of the exponential; the power of two of the value scale into the
+//   conversion.
 //   The weights go into the second product as two bf16 parts, 16 significant bits, and into their sums as they are: rounded to one, outputs in bf16 are off by
-//   0.0020 of their size instead of 0.0016 (their own rounding), and 8 x 2048 tokens take 348 us instead of 434.  A q that the call rotates
-//   is two parts of its type (77 tokens behind 1411: 22.4 us against 21.6, float16 outputs off by 0.0002 of their size against 0.0004; 8 x 2048 tokens, whose
-//   workgroups of 128 rows have registers for the fragments of 32 keys at a time only: 505 us against 442).
+//   0.0020 of their size instead of 0.0016 (their own rounding), and 8 x 2048 tokens take four fifths of the time.  A q that the call rotates
+//   is two parts of its type: rounded once, float16 outputs are off by 0.0004 of their size instead of 0.0002, 77 tokens behind 1411 take 4 % less and 8 x 2048,
+//   whose workgroups of 128 rows have registers for the fragments of 32 keys at a time only, 12 %.
 // V columns: 16-byte pieces of the 128-byte rows are XOR-ed with (d / 4 % 8) ^ (d & 6), which keeps the fragments' 16-byte reads and the 8-byte transposing
 // writes off each other's banks (found by enumeration).
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
-// 8 x 2048 tokens, 32 heads of 128: 434 us, 634 TFLOP/s of the formula's operations and half as many again for the second parts, 950 in all, where a large
-// product of the library reaches 1189.  Short chunks are bound by the time of a tile.
+// 8 x 2048 tokens, 32 heads of 128: 445 us, 618 TFLOP/s of the formula's operations and half as many again for the second parts, 927 in all, where a large
+// product of the library reaches 1189: the matrix cores bound it.  Short chunks are bound by the time of a tile.
 constexpr int kTile = 64, kPromptWaves = 4;
-constexpr float kSlack = 8.f;                             // 360 us against 372 with a reference that moves with every larger score
+constexpr float kSlack = 8.f;                             // with a reference that moves with every larger score 8 x 2048 tokens take 1.3 % more
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 // A value scale as a power of two, which goes into the conversion of the codes to bf16 exactly, and the factor that it leaves, which is multiplied to the
-// weights in front of their rounding: 1 for the scales that kv8_append makes (looking for others costs 3 us of 436).  A zero, a subnormal, an infinity and a
-// NaN are all factor.
+// weights in front of their rounding: 1 for the scales that kv8_append makes (looking for others costs 1 to 4 %).  A zero, a subnormal, an infinity and a NaN are
+// all factor.
 __device__ __forceinline__ bool is_power(float scale) {
   const uint32_t u = __float_as_uint(scale);
   return (u & 0x807fffffu) == 0 && u != 0 && u != 0x7f800000u;
@@ -837,15 +840,17 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
   }
 }
 
-// Rows of a workgroup, its halves and key ranges of a chunk (times in us of chunks without a past, 32 heads of 128, bf16, and of 64 tokens behind cached ones,
-// 32 heads over 8).
-//  - 128 rows share a tile better, 64 fill the chip and end evenly: 128 from two workgroups for each compute unit on (2 x 1024 tokens: 38.0 against 42.3;
-//    8 x 2048: 357 against 490), else 64 (1500 tokens: 41.9 against 50.0).
-//  - Up to one and a half workgroups of 64 rows for each compute unit, two halves of waves with every other tile (700 tokens: 18.3 against 21.2; 512: 13.7
-//    against 15.9; 2 x 512, which are two for each: 20.9 against 18.9).
-//  - Where these leave compute units idle, the keys in as many ranges as fill them once (64 behind 4800: 22.5 against 73.1 in one range and 31.0 in twice as
-//    many), each of four tiles at least (64 behind 600: 13.1 against 15.5; behind 300: 12.2 against 11.1), of eight where the partial results are many (256
-//    tokens without a past in ranges of two tiles and a half: 17.0 against 9.5).
+// Rows of a workgroup, its halves and key ranges of a chunk (times in us from a captured graph of chunks without a past, 32 heads of 128, bf16, and of 64 tokens
+// behind cached ones, 32 heads over 8).
+//  - 128 rows share a tile better, 64 fill the chip and end evenly: 128 from two workgroups for each compute unit on (2 x 1024 tokens: 46.6 against 47.2;
+//    8 x 2048: 443 against 542), else 64 (1500 tokens: 47.3 against 61.1).
+//  - Up to one and a half workgroups of 64 rows for each compute unit, two halves of waves with every other tile (700 tokens: 17.7 against 21.9; 512: 13.9
+//    against 16.5; 2 x 512, which are two for each: 19.8 against 18.2).
+//  - Where these leave compute units idle, the keys in as many ranges as fill them once (64 behind 4800: 22.4 against 76.5 in one range and 31.5 in twice as
+//    many), each of four tiles at least (64 behind 600: 14.6 against 16.2; behind 300: 12.2 against 11.2), of eight where the partial results are many (256
+//    tokens without a past in ranges of two tiles: 16.8 against 9.6).
+//  - S is the room of the cache, and ranges go by it: what the cache holds is known on the device only.  A chunk without a past in a long cache pays for empty
+//    ranges and the join (256 tokens in room for 256: 9.9, for 1024 and more: 17.0; 64 tokens of 32 heads over 8: 6.7 and 13.3).
 struct PromptForm { int rows, halves, ranges; };
 static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
   const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
