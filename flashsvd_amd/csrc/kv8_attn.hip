@@ -396,7 +396,8 @@ int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float
 // ---------------------------------------------------------------------------------------------
 // Two halves of waves (KG = 2) take every other tile and add up at the end, in a workgroup of its own for a compute unit, where there are few.
 // 8 x 2048 tokens, 32 heads of 128: 445 us, 618 TFLOP/s of the formula's operations and half as many again for the second parts, 927 in all, where a large
-// product of the library reaches 1189: the matrix cores bound it.  Short chunks are bound by the time of a tile.
+// product of the library reaches 1189.  The vector unit (conversion, softmax, parts of the weights) is busy half of the time, the matrix cores 40 %, LDS a third; they
+// overlap in part.  Short chunks are bound by the time of a tile.
 constexpr int kTile = 64, kPromptWaves = 4;
 constexpr float kSlack = 8.f;                             // with a reference that moves with every larger score 8 x 2048 tokens take 1.3 % more
 __device__ __forceinline__ int v_piece(int d) { return ((d >> 2) & 7) ^ (d & 6); }
