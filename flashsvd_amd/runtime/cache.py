@@ -283,7 +283,7 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
 
     def _note_seen(self, layer_idx: int, q_len: int, cache_position) -> None:
-        if int(layer_idx) != 0:
+        if int(layer_idx) != 0 or int(q_len) == 0:
             return
         if cache_position is None:
             self._seen_tokens = int(q_len)

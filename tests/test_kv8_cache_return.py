@@ -66,6 +66,8 @@ def test_length_follows_the_last_write(cache):
         assert cache.get_seq_length() == want
     cache._note_seen(0, 5, torch.arange(2, 7))
     assert cache.get_seq_length() == 7
+    none = cache.update(*_rows(0, 1.0, 4), 0)               # no rows: nothing is written, nothing given up
+    assert none[0].shape == (2, 3, 0, 64) and cache.get_seq_length() == 7
     with pytest.raises(ValueError, match="consecutive"):
         cache.update(*_rows(2, 1.0, 3), 0, {"cache_position": torch.arange(0)})
 
