@@ -14,14 +14,16 @@ struct Kv8Parts {
 };
 
 // eight elements x of a query row in the lower or upper half of the head, rotated with their partners y half a head away, in fp32 and rounded to the type of
-// the products; rest: what that rounding leaves
+// the products; rest: what that rounding leaves.  A pair of large float16 elements may turn to one beyond the type's range (up to 1.42 times its end): the first
+// part stops at the end, the rest has the remainder.
 template <class E>
 __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u32x4_t sin, bool upper, u32x4_t& rest) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float sl = upper ? E::lo(sin[i]) : -E::lo(sin[i]), sh = upper ? E::hi(sin[i]) : -E::hi(sin[i]);
     const float l = E::lo(x[i]) * E::lo(cos[i]) + E::lo(y[i]) * sl, h = E::hi(x[i]) * E::hi(cos[i]) + E::hi(y[i]) * sh;
-    const uint32_t w = E::pack2(l, h);
+    constexpr float kEnd = 65504.f;
+    const uint32_t w = E::code == 1 ? E::pack2(__builtin_amdgcn_fmed3f(l, -kEnd, kEnd), __builtin_amdgcn_fmed3f(h, -kEnd, kEnd)) : E::pack2(l, h);
     x[i] = w;
     rest[i] = E::pack2(l - E::lo(w), h - E::hi(w));
   }

@@ -178,3 +178,33 @@ def test_scales_that_are_no_power_of_two(form, Dh, dt):
     one = hip_ops.attn_decode_kv8(q[:, M - 1], k.to(F8).cuda(), v.to(F8).cuda(), ks.cuda(), vs.cuda(), torch.full((B,), past + M, dtype=torch.int32, device="cuda"),
                                   block=block, softmax_scale=by).cpu()
     _close(one[b, h], want, room, dt, f"{form}: a token behind it")
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("form", PROMPTS)
+def test_a_rotation_beyond_the_range_of_float16(form, Dh):
+    """Pairs of elements near the end of float16 turn to elements of up to 92600, which the first part of q does not hold (65504); the remainder, at most 27100, is
+    rounded by 2^-11 of itself, 2^-12.2 of the element."""
+    from flashsvd_amd import hip_ops
+    p = PROMPTS[form]
+    B, Hk, M, past, H = p["B"], p["Hk"], p["M"], p["past"], p["Hk"] * p["G"]
+    g = torch.Generator().manual_seed(63)
+    cos, sin = tables(past + M, Dh, torch.float16)
+    x = (_away_from_zero(g, torch.float16, Dh).sign() * (65504 - 2000 * torch.rand(Dh, generator=g))).half()
+    k, v, scale = _held(B, past + M, Hk, Dh, 32)
+    k[:] = torch.randn(past + M, Hk, Dh, generator=g).to(F8).float()
+    v[:] = torch.randn(past + M, Hk, Dh, generator=g).to(F8).float()
+    kw = dict(block=32, cos=cos.cuda(), sin=sin.cuda(), softmax_scale=1e-6)
+    c = [k.to(F8).cuda(), v.to(F8).cuda(), scale.cuda(), scale.cuda()]
+    pos = torch.full((B,), past, dtype=torch.int32, device="cuda")
+    out = hip_ops.attn_prefill_kv8(x.expand(B, M, H, Dh).contiguous().cuda(), *c, pos, **kw).cpu()
+    one = hip_ops.attn_decode_kv8(x.expand(B, H, Dh).contiguous().cuda(), *c, pos + M - 1, seqlen_add=1, **kw).cpu()
+    beyond = 0
+    for b, m, h in [(0, 0, 0), (B - 1, M - 1, H - 1), (B // 2, M // 2, 0)]:
+        y, n, hk = R.rotate(x.double(), cos, sin, past + m), past + m + 1, h // p["G"]
+        beyond += int((y.abs() > 65520).sum())
+        want, room = R.attend(y, k[b, :n, hk].double(), v[b, :n, hk].double(), 1e-6, 2.0 ** -12.2, TWO_PARTS)
+        _close(out[b, m, h], want, room, torch.float16, f"{form}: row {m} of head {h}")
+        if m == M - 1:
+            _close(one[b, h], want, room, torch.float16, f"{form}: one token")
+    assert beyond
