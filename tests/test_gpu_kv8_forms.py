@@ -114,7 +114,7 @@ def test_append_forms(name, Dh, Hk, block, T, at, rows, dt):
     (128, 2, 2, [16500, 8300], 16500, {None: 128, 129: 129}),
 ])
 def test_decode_over_many_ranges(Dh, H, Hk, lens, S, splits, dt):
-    """More ranges than a wave has lanes, with one to four in the last round of the join."""
+    """More ranges than a wave has lanes, with one to four in the last pass of the join."""
     from flashsvd_amd import hip_ops
     B = len(lens)
     c = Cache(B, S, Hk, Dh, 32, seed=S).finite()
