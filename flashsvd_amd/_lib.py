@@ -122,6 +122,12 @@ class Kv8Cache(ctypes.Structure):
                 ("block", ctypes.c_int32)]
 
 
+class Kv4Cache(ctypes.Structure):
+    """fsvd_kv4_cache: codes and scales of a KV cache in 4 bits."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("sc_b", c_int64), ("sc_s", c_int64), ("sc_h", c_int64),
+                ("ss_b", c_int64), ("ss_h", c_int64), ("ss_g", c_int64), ("S", ctypes.c_int32), ("Hk", ctypes.c_int32), ("Dh", ctypes.c_int32)]
+
+
 SIGNATURES = {
     "fsvd_version": (c_int, []),
     "fsvd_last_error": (c_char_p, []),
@@ -197,6 +203,16 @@ SIGNATURES = {
     "fsvd_attn_prefill_kv8": (c_int, [ctypes.POINTER(Kv8Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                       c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
     "fsvd_attn_prefill_kv8_scratch_bytes": (c_size_t, [c_int] * 6),
+    "fsvd_kv4_append": (c_int, [ctypes.POINTER(Kv4Cache)] + [c_void_p, c_int64, c_int64, c_int64] * 2 + [c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                c_int, c_int, c_int, c_void_p]),
+    "fsvd_kv4_dequantize": (c_int, [ctypes.POINTER(Kv4Cache), c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_void_p]),
+    "fsvd_attn_decode_kv4_scratch_bytes": (c_size_t, [c_int] * 6),
+    "fsvd_attn_decode_kv4": (c_int, [ctypes.POINTER(Kv4Cache)] + [c_void_p, c_int64, c_int64] * 3 + [c_void_p, c_int, c_void_p, c_void_p, c_int,
+                                     c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "fsvd_attn_prefill_kv4": (c_int, [ctypes.POINTER(Kv4Cache), c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                      c_void_p, c_int64, c_int64, c_int64, c_void_p, c_size_t, c_int, c_int, c_int, c_float, c_int, c_void_p]),
+    "fsvd_attn_prefill_kv4_scratch_bytes": (c_size_t, [c_int] * 6),
+    "fsvd_token_logprobs": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p]),
     "fsvd_set_token_rows": (c_int, [c_void_p, c_void_p, c_void_p, ctypes.c_int32, c_int, c_void_p]),
     "fsvd_mlp_block_scratch_bytes": (c_size_t, [ctypes.POINTER(MlpBlock)]),
     "fsvd_attn_block_scratch_bytes": (c_size_t, [ctypes.POINTER(AttnBlock)]),

@@ -1,0 +1,231 @@
+// The KV cache in 4 bits: rows written to it, what it holds, and its entry points.
+#include "kv4.hpp"
+
+namespace fsvd {
+
+// A lane holds eight dimensions d .. d + 7 of a row and the eight half a head further (the pairs of the rotation), LPR lanes a row; four lanes have a group of 32
+// channels in either half (of 64 dimensions the halves are the groups).
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
+  typedef E16<DT> E;
+  constexpr int HALF = DH / 2, LPR = HALF / 8, GROUPS = DH / kGroup4;
+  const int part = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, lane = threadIdx.x % LPR, t = (int)blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  const int rows = a.rows ? min(a.rows[b], a.T) : a.T;
+  const int64_t pos = (int64_t)a.positions[b] + t;
+  const bool in = t < rows && pos >= 0 && pos < a.c.S;
+  const int64_t r = in ? t : 0;
+  const uint16_t* x = (part ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h + r * a.sv_t : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h + r * a.sk_t) + lane * 8;
+  const u32x4_t lo = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x)), hi = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x + HALF));
+  const bool turn = part == 0 && a.cos != nullptr;
+  u32x4_t cw, sw;
+  if (turn) {
+    const int64_t tp = min(max(pos, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + lane * 8;
+    cw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.cos + tp));
+    sw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.sin + tp));
+  }
+  float y[2][8], amax[2] = {0.f, 0.f};
+  bool nan[2] = {false, false};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t wl = lo[e >> 1], wh = hi[e >> 1];
+    float u = e & 1 ? E::hi(wl) : E::lo(wl), v = e & 1 ? E::hi(wh) : E::lo(wh);
+    if (turn) {
+      const uint32_t wc = cw[e >> 1], ws = sw[e >> 1];
+      const float c = e & 1 ? E::hi(wc) : E::lo(wc), s = e & 1 ? E::hi(ws) : E::lo(ws), y0 = odd_sum(u * c, -(v * s)), y1 = odd_sum(u * s, v * c);
+      u = y0; v = y1;
+    }
+    y[0][e] = u; y[1][e] = v;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      amax[h] = fmaxf(amax[h], finite_mag4(y[h][e]));
+      nan[h] = nan[h] || y[h][e] != y[h][e];
+    }
+  }
+  uint8_t* codes = static_cast<uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s;
+  uint8_t* scales = static_cast<uint8_t*>(part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    amax[h] = fmaxf(amax[h], dpp_f32<0xB1>(amax[h]));                       // over the four lanes of the group
+    amax[h] = fmaxf(amax[h], dpp_f32<0x4E>(amax[h]));
+    float bad = nan[h] ? 1.f : 0.f;
+    bad = fmaxf(bad, dpp_f32<0xB1>(bad));
+    bad = fmaxf(bad, dpp_f32<0x4E>(bad));
+    const int byte = scale_byte(amax[h]);
+    const float scale = scale_of(byte);
+    if (!in) continue;
+    uint32_t w = codes4_of<0>(0u, y[h][0], y[h][1], scale);
+    w = codes4_of<1>(w, y[h][2], y[h][3], scale);
+    w = codes4_of<2>(w, y[h][4], y[h][5], scale);
+    w = codes4_of<3>(w, y[h][6], y[h][7], scale);
+    *reinterpret_cast<uint32_t*>(codes + h * (HALF / 2) + lane * 4) = w;
+    if (lane % 4 == 0) scales[(h * (GROUPS / 2) + lane / 4) * a.c.ss_g] = (uint8_t)(bad > 0.f ? kNanByte : byte);
+  }
+}
+
+int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st) {
+  if (a.T == 0) return kOk;
+  if ((int64_t)a.B * a.c.Hk > 0x7fffffff || a.T > (1 << 20)) { set_last_error("%s: %d rows of %d heads for %d sequences", fn, a.T, a.c.Hk, a.B); return kErrBadShape; }
+  const int per = 256 / (a.c.Dh / 16);
+  const dim3 grid(2 * a.c.Hk, (a.T + per - 1) / per, a.B);
+  if (a.dt == 1) {
+    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_append_kernel<1, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv4_append_kernel<1, 64>), grid, dim3(256), 0, st, a);
+  } else {
+    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_append_kernel<0, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv4_append_kernel<0, 64>), grid, dim3(256), 0, st, a);
+  }
+  set_last_form("kv4 rows");
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
+  return kOk;
+}
+
+// What the first L rows hold, [B, L, Hk, Dh] each: a thread has 16 bytes of codes, the 32 channels of one scale.
+struct Kv4ReadArgs {
+  fsvd_kv4_cache c;
+  uint16_t* k; uint16_t* v;
+  int64_t so_b, so_t, so_h;
+  int L;
+};
+template <int DT, int DH>
+__global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
+  typedef E16<DT> E;
+  constexpr int GROUPS = DH / kGroup4;
+  const int part = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, g = threadIdx.x % GROUPS;
+  const int64_t pos = (int64_t)blockIdx.y * (256 / GROUPS) + threadIdx.x / GROUPS;
+  if (pos >= a.L) return;
+  const uint8_t* codes = static_cast<const uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s + 16 * g;
+  const uint32_t byte = (static_cast<const uint8_t*>(part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos)[g * a.c.ss_g];
+  uint16_t* out = (part ? a.v : a.k) + b * a.so_b + pos * a.so_t + hk * a.so_h + kGroup4 * g;
+  const u32x4_t w = *reinterpret_cast<const u32x4_t*>(codes);
+  const float scale = scale_of(byte);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2_t x[4] = {pair4_f32<0>(w[i], scale), pair4_f32<1>(w[i], scale), pair4_f32<2>(w[i], scale), pair4_f32<3>(w[i], scale)};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) out[8 * i + e] = (uint16_t)E::bits(byte == kNanByte ? __builtin_nanf("") : x[e >> 1][e & 1]);
+  }
+}
+
+static int check_kv4_cache(const char* fn, const fsvd_kv4_cache* c) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr || c->k_scale == nullptr || c->v_scale == nullptr) {
+    set_last_error("%s: a buffer of the cache is NULL", fn);
+    return kErrNullPtr;
+  }
+  if (c->S <= 0 || c->S % 64 || c->Hk <= 0 || (c->Dh != 64 && c->Dh != 128)) {
+    set_last_error("%s: bad cache: S=%d Hk=%d Dh=%d (a multiple of 64 rows; 64 and 128 dimensions are served)", fn, c->S, c->Hk, c->Dh);
+    return kErrBadShape;
+  }
+  if (c->sc_b < 0 || c->sc_s < c->Dh / 2 || c->sc_s > (1 << 24) || c->sc_h < 0 || c->ss_b < 0 || c->ss_h < 0 || c->ss_g < c->S) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
+  if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15) ||
+      ((c->sc_b | c->sc_s | c->sc_h | c->ss_b | c->ss_h | c->ss_g) & 15)) {
+    set_last_error("%s: cache pointers and strides must be 16-byte aligned", fn);
+    return kErrBadAlign;
+  }
+  return kOk;
+}
+
+}  // namespace fsvd
+
+using namespace fsvd;
+
+static int check_call(const char* fn, int B, int dtype, const void* cos, const void* sin, int rope_len) {
+  if (B <= 0 || B > 65535) { set_last_error("%s: batch of %d (1 to 65535 are served)", fn, B); return kErrBadShape; }
+  if (dtype != 0 && dtype != 1) { set_last_error("%s: dtype code %d (bf16 = 0 and fp16 = 1 are served)", fn, dtype); return kErrBadDtype; }
+  if ((cos == nullptr) != (sin == nullptr) || (cos != nullptr && rope_len <= 0)) { set_last_error("%s: cos and sin go together, with rope_len rows", fn); return kErrNullPtr; }
+  return kOk;
+}
+// rows that a call writes must not lie in each other
+static int check_written(const char* fn, const fsvd_kv4_cache* c, int B) {
+  if ((B > 1 && (c->sc_b == 0 || c->ss_b == 0)) || (c->Hk > 1 && (c->sc_h == 0 || c->ss_h == 0))) {
+    set_last_error("%s: a cache that is written to must not be expanded over its sequences or heads", fn);
+    return kErrBadShape;
+  }
+  return kOk;
+}
+static int check_out(const char* fn, int B, int M, int H, int64_t so_b, int64_t so_m, int64_t so_h) {
+  if ((B > 1 && so_b == 0) || (M > 1 && so_m == 0) || (H > 1 && so_h == 0)) { set_last_error("%s: out must not be expanded", fn); return kErrBadShape; }
+  return kOk;
+}
+static const uint16_t* in16(const void* p) { return static_cast<const uint16_t*>(p); }
+
+extern "C" {
+
+int fsvd_kv4_append(const fsvd_kv4_cache* cache, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t,
+                    int64_t sv_h, const int32_t* positions, const int32_t* rows, const void* cos, const void* sin, int rope_len, int B, int T, int dtype,
+                    void* stream) {
+  const char* fn = "fsvd_kv4_append";
+  if (const int rc = check_kv4_cache(fn, cache)) return rc;
+  if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
+  if (positions == nullptr || (T != 0 && (k == nullptr || v == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (T < 0) { set_last_error("%s: %d rows", fn, T); return kErrBadShape; }
+  if (const int rc = check_written(fn, cache, B)) return rc;
+  const Kv4AppendArgs a{*cache, in16(k), sk_b, sk_t, sk_h, in16(v), sv_b, sv_t, sv_h, positions, rows, in16(cos), in16(sin), rope_len, B, T, dtype};
+  return launch_kv4_append(fn, a, static_cast<hipStream_t>(stream));
+}
+
+int fsvd_kv4_dequantize(const fsvd_kv4_cache* cache, void* k, void* v, int64_t so_b, int64_t so_t, int64_t so_h, int B, int L, int dtype, void* stream) {
+  const char* fn = "fsvd_kv4_dequantize";
+  if (const int rc = check_kv4_cache(fn, cache)) return rc;
+  if (const int rc = check_call(fn, B, dtype, nullptr, nullptr, 0)) return rc;
+  if (L < 0 || L > cache->S) { set_last_error("%s: %d rows of a cache of %d", fn, L, cache->S); return kErrBadShape; }
+  if (L == 0) return kOk;
+  if (k == nullptr || v == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (const int rc = check_out(fn, B, L, cache->Hk, so_b, so_t, so_h)) return rc;
+  const Kv4ReadArgs a{*cache, static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), so_b, so_t, so_h, L};
+  const int per = 256 / (cache->Dh / kGroup4);
+  const dim3 grid(2 * cache->Hk, (L + per - 1) / per, B);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == 1) {
+    if (cache->Dh == 128) hipLaunchKernelGGL((kv4_read_kernel<1, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv4_read_kernel<1, 64>), grid, dim3(256), 0, st, a);
+  } else {
+    if (cache->Dh == 128) hipLaunchKernelGGL((kv4_read_kernel<0, 128>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((kv4_read_kernel<0, 64>), grid, dim3(256), 0, st, a);
+  }
+  set_last_form("kv4 read");
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
+  return kOk;
+}
+
+size_t fsvd_attn_decode_kv4_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) { return 0; }
+
+int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
+                         const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
+                         int rope_len, void* out, int64_t so_b, int64_t so_h, void* scratch, size_t scratch_bytes, int B, int H, int nsplit, float scale,
+                         int dtype, void* stream) {
+  const char* fn = "fsvd_attn_decode_kv4";
+  if (const int rc = check_kv4_cache(fn, cache)) return rc;
+  if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
+  if (q == nullptr || out == nullptr || cache_seqlens == nullptr || (k_new == nullptr) != (v_new == nullptr)) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (H <= 0 || H % cache->Hk) { set_last_error("%s: %d query heads over %d", fn, H, cache->Hk); return kErrBadShape; }
+  if (const int rc = k_new ? check_written(fn, cache, B) : kOk) return rc;
+  if (const int rc = check_out(fn, B, 1, H, so_b, 0, so_h)) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (k_new != nullptr) {
+    const Kv4AppendArgs n{*cache, in16(k_new), sk_b, 0, sk_h, in16(v_new), sv_b, 0, sv_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, B, 1, dtype};
+    if (const int rc = launch_kv4_append(fn, n, st)) return rc;
+  }
+  const Kv4AttnArgs a{*cache, in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
+                      B, 1, H, k_new ? 1 : seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
+  return launch_kv4_attend(fn, a, st);
+}
+
+size_t fsvd_attn_prefill_kv4_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) { return 0; }
+
+int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
+                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
+                          size_t scratch_bytes, int B, int M, int H, float scale, int dtype, void* stream) {
+  const char* fn = "fsvd_attn_prefill_kv4";
+  if (const int rc = check_kv4_cache(fn, cache)) return rc;
+  if (const int rc = check_call(fn, B, dtype, cos, sin, rope_len)) return rc;
+  if (q_pos0 == nullptr || (M != 0 && (q == nullptr || out == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
+  if (M < 0 || H <= 0 || H % cache->Hk) { set_last_error("%s: %d rows of %d query heads over %d", fn, M, H, cache->Hk); return kErrBadShape; }
+  if (const int rc = check_out(fn, B, M, H, so_b, so_m, so_h)) return rc;
+  const Kv4AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
+                      B, M, H, 1, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
+  return M == 0 ? kOk : launch_kv4_attend(fn, a, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

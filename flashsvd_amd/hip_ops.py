@@ -13,7 +13,7 @@ import torch
 from . import _lib
 from .torch_ops import ops as _OPS
 
-_BF16, _F8, _F32, _I32 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32
+_BF16, _F8, _F32, _I32, _U8 = torch.bfloat16, torch.float8_e4m3fn, torch.float32, torch.int32, torch.uint8
 _MOST_INT = 2 ** 31 - 1
 
 
@@ -1140,3 +1140,228 @@ def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block,
     if rc:
         _lib.check("fsvd_attn_prefill_kv8", rc)
     return out
+
+
+# ------------------------------------------------------------------ KV cache in 4 bits
+def kv4_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+               positions: torch.Tensor, *, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+               rows: Optional[torch.Tensor] = None) -> None:
+    """Rows of keys and values [B, T, Hk, Dh] into a cache in 4 bits at positions[b] .. positions[b] + T - 1 (``rows`` int32 [B]: that many of sequence
+    b), keys rotated there when ``cos`` / ``sin`` [len, Dh / 2] are given.  Caches uint8 [>=B, S, Hk, Dh / 2], two e2m1 codes a byte with the even channel in
+    the low bits, scales uint8 [>=B, Hk, Dh / 32, S] with unit inner stride, ``value = code * 2 ** (scale - 127)`` for the 32 channels of a token; S a multiple of
+    64, strides multiples of 16.  A row changes no other row; rows outside the cache are dropped.  Custom operator flashsvd_hip::kv4_append (caches
+    and scales are mutated arguments); see fsvd_kv4_append."""
+    _OPS.kv4_append.default(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows)
+
+
+def kv4_dequantize(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *, length: Optional[int] = None,
+                   dtype: torch.dtype = torch.bfloat16):
+    """(K, V) [B, length, Hk, Dh] that the first ``length`` rows (None: all) of a cache in 4 bits (operands as :func:`kv4_append`) hold: exact in bfloat16,
+    rounded to float16.  Custom operator flashsvd_hip::kv4_dequantize."""
+    return _OPS.kv4_dequantize.default(k_cache, v_cache, k_scale, v_scale, None if length is None else int(length), dtype)
+
+
+def attn_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                    cache_seqlens: torch.Tensor, *, k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
+                    cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, seqlen_add: int = 0, nsplit: Optional[int] = None,
+                    out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """:func:`attn_decode_kv8` over a cache in 4 bits (operands as :func:`kv4_append`).  Custom operator flashsvd_hip::attn_decode_kv4."""
+    a = (q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, int(seqlen_add), None if nsplit is None else int(nsplit),
+         None if not softmax_scale else float(softmax_scale))
+    return _OPS.attn_decode_kv4.default(*a) if out is None else _OPS.attn_decode_kv4.out(*a, out=out)
+
+
+def attn_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, q_pos0: torch.Tensor, *,
+                     rows: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
+                     out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
+    """:func:`attn_prefill_kv8` over a cache in 4 bits (operands as :func:`kv4_append`).  Custom operator flashsvd_hip::attn_prefill_kv4."""
+    a = (q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, None if not softmax_scale else float(softmax_scale))
+    return _OPS.attn_prefill_kv4.default(*a) if out is None else _OPS.attn_prefill_kv4.out(*a, out=out)
+
+
+def _kv4_cache(B, kc, vc, ks, vs):
+    """Checks of a cache in 4 bits; its descriptor for the C ABI.  One pass over what a good call has, as :func:`_kv8_cache`."""
+    shape, st, ss = kc.shape, kc.stride(), ks.stride()
+    dev = kc.get_device()
+    if len(shape) != 4:
+        _refuse_kv4_cache(B, kc, vc, ks, vs)
+    n, S, Hk, half = shape
+    Dh = 2 * half
+    scales = (n, Hk, Dh // 32, S)
+    if not (kc.dtype is _U8 and vc.dtype is _U8 and ks.dtype is _U8 and vs.dtype is _U8 and vc.shape == shape and vc.stride() == st and n >= B and st[3] == 1
+            and ks.shape == scales and vs.shape == scales and vs.stride() == ss and ss[3] == 1 and Dh % 32 == 0 and dev >= 0
+            and vc.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
+        _refuse_kv4_cache(B, kc, vc, ks, vs)
+    return _lib.Kv4Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], S, Hk, Dh)
+
+
+def _refuse_kv4_cache(B, kc, vc, ks, vs):
+    for t, nm in ((kc, "k_cache"), (vc, "v_cache"), (ks, "k_scale"), (vs, "v_scale")):
+        _need(t, nm, dtype=_U8)
+    if kc.dim() != 4 or kc.shape != vc.shape or kc.stride() != vc.stride() or kc.shape[0] < B or kc.stride(3) != 1 or kc.shape[3] % 16:
+        raise ValueError(f"caches must be matching [B>={B}, S, Hk, Dh / 2] tensors with unit inner stride, got {tuple(kc.shape)} / {tuple(vc.shape)}")
+    want = (kc.shape[0], kc.shape[2], kc.shape[3] // 16, kc.shape[1])
+    if tuple(ks.shape) != want or ks.shape != vs.shape or ks.stride() != vs.stride() or ks.stride(3) != 1:
+        raise ValueError(f"scales must be matching {want} tensors with unit inner stride, got {tuple(ks.shape)} / {tuple(vs.shape)}")
+    raise ValueError("caches and scales must be on one device")
+
+
+def _apart4(B, c) -> None:
+    """Rows that a call writes must not lie in each other: no caches expanded over their sequences or heads."""
+    if (B > 1 and (c.sc_b == 0 or c.ss_b == 0)) or (c.Hk > 1 and (c.sc_h == 0 or c.ss_h == 0)) or (c.sc_s == 0 and c.S > 1):
+        raise ValueError("a cache that is written to must not be expanded over its sequences, rows or heads")
+
+
+def _kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows):
+    dt, code = _elem(k, "k")
+    shape, st, sv = k.shape, k.stride(), v.stride()
+    B = shape[0]
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    dev = k_cache.get_device()
+    if not (v.dtype is dt and len(shape) == 4 and v.shape == shape and shape[2] == c.Hk and shape[3] == c.Dh and st[3] == 1 and sv[3] == 1
+            and k.get_device() == dev and v.get_device() == dev):
+        _need(v, "v", dtype=dt)
+        raise ValueError(f"k and v must be [B, T, {c.Hk}, {c.Dh}] tensors with unit inner stride on cuda:{dev}, got {tuple(shape)} / {tuple(v.shape)}")
+    _apart4(B, c)
+    cp, sp, rope_len = _kv8_rope(cos, sin, c.Dh, dt, dev)
+    pos, n = _kv8_vector(positions, B, dev, "positions"), _kv8_vector(rows, B, dev, "rows")
+    if B == 0:
+        return
+    with _on(dev):
+        rc = _lib.load().fsvd_kv4_append(c, k.data_ptr(), st[0], st[1], st[2], v.data_ptr(), sv[0], sv[1], sv[2], pos, n, cp, sp, rope_len, B, shape[1], code,
+                                         _stream())
+    if rc:
+        _lib.check("fsvd_kv4_append", rc)
+
+
+def _kv4_dequantize_impl(k_cache, v_cache, k_scale, v_scale, length, dtype):
+    code = _ELEM_CODES.get(dtype)
+    if code is None:
+        raise ValueError(f"dtype must be torch.bfloat16 or torch.float16, got {dtype}")
+    c = _kv4_cache(0, k_cache, v_cache, k_scale, v_scale)
+    B, L = k_cache.shape[0], c.S if length is None else length
+    if not 0 <= L <= c.S:
+        raise ValueError(f"length must be 0 to {c.S}, got {length}")
+    k, v = (torch.empty(B, L, c.Hk, c.Dh, dtype=dtype, device=k_cache.device) for _ in range(2))
+    if B == 0:
+        return k, v
+    st = k.stride()
+    dev = k_cache.get_device()
+    with _on(dev):
+        rc = _lib.load().fsvd_kv4_dequantize(c, k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], B, L, code, _stream())
+    if rc:
+        _lib.check("fsvd_kv4_dequantize", rc)
+    return k, v
+
+
+def _attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out):
+    dt, code = _elem(q, "q")
+    sq = q.stride()
+    if len(sq) != 3 or sq[2] != 1:
+        raise ValueError(f"q must be [B,H,Dh] with unit inner stride, got {tuple(q.shape)}")
+    B, H, Dh = q.shape
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    dev, Hk = k_cache.get_device(), c.Hk
+    if c.Dh != Dh or H % Hk or q.get_device() != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")
+    cp, sp, rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    lens = _kv8_vector(cache_seqlens, B, dev, "cache_seqlens")
+    kp = vp = None
+    sk = sv = (0, 0)
+    if k_new is not None and v_new is not None:
+        sk, sv = k_new.stride(), v_new.stride()
+        new = (B, Hk, Dh)
+        if not (k_new.dtype is dt and v_new.dtype is dt and k_new.shape == new and v_new.shape == new and sk[2] == 1 and sv[2] == 1
+                and k_new.get_device() == dev and v_new.get_device() == dev):
+            _need(k_new, "k_new", dtype=dt); _need(v_new, "v_new", dtype=dt)
+            raise ValueError(f"k_new/v_new must be [B,Hk,Dh] tensors with unit inner stride on cuda:{dev}, got {tuple(k_new.shape)} / {tuple(v_new.shape)}")
+        _apart4(B, c)
+        kp, vp = k_new.data_ptr(), v_new.data_ptr()
+    elif k_new is not None or v_new is not None:
+        raise ValueError("k_new and v_new go together")
+    if out is None:
+        out = q.new_empty((B, H, Dh))
+    elif out.shape != q.shape or out.stride(2) != 1 or out.dtype is not dt or out.get_device() != dev:
+        raise ValueError(f"out must be {dt} [B,H,Dh] with unit inner stride on cuda:{dev}")
+    if B == 0:
+        return out
+    lib, so = _lib.load(), out.stride()
+    # the C ABI takes 32 bits of either; more ranges than keys are none
+    nsplit = 0 if nsplit is None else max(0, min(nsplit, c.S))
+    if not -_MOST_INT <= seqlen_add <= _MOST_INT:
+        raise ValueError(f"seqlen_add must be a 32-bit number, got {seqlen_add}")
+    nbytes, scratch, ptr = lib.fsvd_attn_decode_kv4_scratch_bytes(B, H, Hk, Dh, c.S, nsplit), None, None
+    if nbytes:
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)       # of this call and stream
+        ptr = scratch.data_ptr()
+    with _on(dev):
+        rc = lib.fsvd_attn_decode_kv4(c, q.data_ptr(), sq[0], sq[1], kp, sk[0], sk[1], vp, sv[0], sv[1], lens, seqlen_add, cp, sp, rope_len, out.data_ptr(),
+                                      so[0], so[1], ptr, nbytes, B, H, nsplit, softmax_scale or 0.0, code, _stream())
+    if rc:
+        _lib.check("fsvd_attn_decode_kv4", rc)
+    return out
+
+
+def _attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out):
+    dt, code = _elem(q, "q")
+    sq = q.stride()
+    if len(sq) != 4 or sq[3] != 1:
+        raise ValueError(f"q must be [B,M,H,Dh] with unit inner stride, got {tuple(q.shape)}")
+    B, M, H, Dh = q.shape
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    dev = k_cache.get_device()
+    if c.Dh != Dh or H % c.Hk or q.get_device() != dev:
+        raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")
+    cp, sp, rope_len = _kv8_rope(cos, sin, Dh, dt, dev)
+    pos, n = _kv8_vector(q_pos0, B, dev, "q_pos0"), _kv8_vector(rows, B, dev, "rows")
+    if out is None:
+        out = (q.new_empty if rows is None else q.new_zeros)((B, M, H, Dh))
+    elif out.shape != q.shape or out.stride(3) != 1 or out.dtype is not dt or out.get_device() != dev:
+        raise ValueError(f"out must be {dt} [B,M,H,Dh] with unit inner stride on cuda:{dev}")
+    if B == 0:
+        return out
+    lib, so = _lib.load(), out.stride()
+    nbytes, scratch, ptr = lib.fsvd_attn_prefill_kv4_scratch_bytes(B, M, H, c.Hk, Dh, c.S), None, None
+    if nbytes:
+        scratch = q.new_empty(nbytes, dtype=torch.uint8)       # of this call and stream
+        ptr = scratch.data_ptr()
+    with _on(dev):
+        rc = lib.fsvd_attn_prefill_kv4(c, q.data_ptr(), sq[0], sq[1], sq[2], pos, n, cp, sp, rope_len, out.data_ptr(), so[0], so[1], so[2], ptr, nbytes, B, M, H,
+                                       softmax_scale or 0.0, code, _stream())
+    if rc:
+        _lib.check("fsvd_attn_prefill_kv4", rc)
+    return out
+
+
+# ------------------------------------------------------------------ log probabilities
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0):
+    """(logprobs, entropy, top_tokens, top_logprobs) of every row of logits [N, V] or [B, T, V] with unit inner stride: the log probability of
+    ``tokens`` (int64 [N] or [B, T]; below 0: none, 0.0), the entropy of the distribution in nats, float32 both, and the ``top`` (0 to 64) likeliest tokens, int64,
+    with their log probabilities, float32 [.., top], equal ones by index.  A row whose largest logit is not finite has NaN for numbers.  One launch that
+    reads the logits once.  Custom operator flashsvd_hip::token_logprobs."""
+    return _OPS.token_logprobs.default(logits, tokens, int(top))
+
+
+def _token_logprobs_impl(logits, tokens, top):
+    _, code = _elem(logits, "logits")
+    shape, st = logits.shape, logits.stride()
+    if len(shape) not in (2, 3) or st[-1] != 1 or shape[-1] == 0:
+        raise ValueError(f"logits must be [N, V] or [B, T, V] with unit inner stride, got {tuple(shape)} strides {st}")
+    V, dev = shape[-1], logits.get_device()
+    if tokens.dtype is not torch.long or tokens.shape != shape[:-1] or tokens.get_device() != dev:
+        _need(tokens, "tokens", dtype=torch.long)
+        raise ValueError(f"tokens must be {tuple(shape[:-1])} on cuda:{dev}, got {tuple(tokens.shape)} on {tokens.device}")
+    if not 0 <= top <= min(64, V):
+        raise ValueError(f"top must be 0 to {min(64, V)}, got {top}")
+    tokens = tokens.contiguous()
+    logprobs, entropy = (torch.empty(shape[:-1], dtype=_F32, device=logits.device) for _ in range(2))
+    ids = torch.empty(*shape[:-1], top, dtype=torch.long, device=logits.device)
+    values = torch.empty(*shape[:-1], top, dtype=_F32, device=logits.device)
+    B, T = (shape[0], 1) if len(shape) == 2 else shape[:2]
+    if B and T:
+        with _on(dev):
+            rc = _lib.load().fsvd_token_logprobs(logits.data_ptr(), st[0], 0 if len(shape) == 2 else st[1], tokens.data_ptr(), logprobs.data_ptr(),
+                                                 entropy.data_ptr(), ids.data_ptr() if top else None, values.data_ptr() if top else None, B, T, V, top, code, _stream())
+        if rc:
+            _lib.check("fsvd_token_logprobs", rc)
+    return logprobs, entropy, ids, values

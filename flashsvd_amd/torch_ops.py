@@ -24,6 +24,11 @@ tensors.  ``flashsvd_amd.hip_ops`` and the modules under ``flashsvd_amd.kernels`
   kv8_append                          fsvd_kv8_append                     rows into a KV cache in 8 bits
   attn_decode_kv8 / .out              fsvd_attn_decode_kv8                single-query attention over it, with append
   attn_prefill_kv8 / .out             fsvd_attn_prefill_kv8               a chunk of a prompt over it
+  kv4_append                          fsvd_kv4_append                     rows into a KV cache in 4 bits
+  kv4_dequantize                      fsvd_kv4_dequantize                 what it holds
+  attn_decode_kv4 / .out              fsvd_attn_decode_kv4                single-query attention over it, with append
+  attn_prefill_kv4 / .out             fsvd_attn_prefill_kv4               a chunk of a prompt over it
+  token_logprobs                      fsvd_token_logprobs                 log probabilities, entropy and likeliest alternatives
   reconstruct_qkv_token               fsvd_reconstruct_qkv_token          reference-layout current-token q / k / v
   xw_linear                           fsvd_xw_linear                      reference-layout x @ W
   mlp_dual_split                      fsvd_mlp_dual_split                 reference-layout dual-split MLP
@@ -332,6 +337,61 @@ _define(f"attn_prefill_kv8({_KP_ARGS}) -> Tensor", _prefill_kv8, lambda q, *a, *
 _define(f"attn_prefill_kv8.out({_KP_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_kv8, lambda *a, out, **k: out)
 
 
+def _kv4_append(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos=None, sin=None, rows=None):
+    from . import hip_ops
+    hip_ops._kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows)
+
+
+def _kv4_dequantize(k_cache, v_cache, k_scale, v_scale, length=None, dtype=torch.bfloat16):
+    from . import hip_ops
+    return hip_ops._kv4_dequantize_impl(k_cache, v_cache, k_scale, v_scale, length, dtype)
+
+
+def _kv4_dequantize_fake(k_cache, v_cache, k_scale, v_scale, length=None, dtype=torch.bfloat16):
+    B, S, Hk, half = k_cache.shape
+    shape = (B, S if length is None else length, Hk, 2 * half)
+    return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+
+def _attn_kv4(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new=None, v_new=None, cos=None, sin=None, seqlen_add=0, nsplit=None,
+              softmax_scale=None, *, out=None):
+    from . import hip_ops
+    return hip_ops._attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out)
+
+
+def _prefill_kv4(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows=None, cos=None, sin=None, softmax_scale=None, *, out=None):
+    from . import hip_ops
+    return hip_ops._attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out)
+
+
+_define(f"kv4_append(Tensor k, Tensor v, {_KV8_HELD}, Tensor positions, Tensor? cos=None, Tensor? sin=None, Tensor? rows=None) -> ()", _kv4_append,
+        lambda *a, **k: None)
+_define("kv4_dequantize(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int? length=None, ScalarType dtype=bfloat16) -> (Tensor, Tensor)",
+        _kv4_dequantize, _kv4_dequantize_fake)
+_K4_ARGS = (f"Tensor q, {_KV8_HELD}, Tensor cache_seqlens, Tensor? k_new=None, Tensor? v_new=None, Tensor? cos=None, Tensor? sin=None, "
+            "int seqlen_add=0, int? nsplit=None, float? softmax_scale=None")
+_define(f"attn_decode_kv4({_K4_ARGS}) -> Tensor", _attn_kv4, lambda q, *a, **k: q.new_empty(q.shape))
+_define(f"attn_decode_kv4.out({_K4_ARGS}, *, Tensor(e!) out) -> Tensor(e!)", _attn_kv4, lambda *a, out, **k: out)
+_P4_ARGS = ("Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor q_pos0, Tensor? rows=None, Tensor? cos=None, "
+            "Tensor? sin=None, float? softmax_scale=None")
+_define(f"attn_prefill_kv4({_P4_ARGS}) -> Tensor", _prefill_kv4, lambda q, *a, **k: q.new_empty(q.shape))
+_define(f"attn_prefill_kv4.out({_P4_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_kv4, lambda *a, out, **k: out)
+
+
+# ------------------------------------------------------------------ log probabilities
+def _token_logprobs(logits, tokens, top=0):
+    from . import hip_ops
+    return hip_ops._token_logprobs_impl(logits, tokens, top)
+
+
+def _token_logprobs_fake(logits, tokens, top=0):
+    f = logits.new_empty(tokens.shape, dtype=torch.float32)
+    return f, f.clone(), tokens.new_empty((*tokens.shape, top)), logits.new_empty((*tokens.shape, top), dtype=torch.float32)
+
+
+_define("token_logprobs(Tensor logits, Tensor tokens, int top=0) -> (Tensor, Tensor, Tensor, Tensor)", _token_logprobs, _token_logprobs_fake)
+
+
 # ------------------------------------------------------------------ reference operand layouts
 def _reconstruct(Pq, Pk, Pv, Vq, Vk, Vv, bq=None, bk=None, bv=None):
     from .kernels import densekv_reconstruct as DR
@@ -367,5 +427,5 @@ _define("mlp_dual_split(Tensor PUp, Tensor PGate, Tensor GateU, Tensor UpU, Tens
         PUp.new_empty((PUp.shape[0], DownU.shape[1])))
 
 ops = getattr(torch.ops, NS)
-OP_NAMES = ("linear", "swiglu_linear", "rmsnorm", "greedy_token_", "set_token_rows_", "sample_token_", "kv8_append", "attn_decode_kv8", "attn_prefill_kv8", "lowrank_mlp", "lowrank_attn_prefill", "rope_tables", "rope_tables_mask", "qkv_rope_append", "attn_decode_densekv", "attn_decode_rankkv", "rankkv_append", "rankkv_fill", "linear_rankkv_append",
+OP_NAMES = ("linear", "swiglu_linear", "rmsnorm", "greedy_token_", "set_token_rows_", "sample_token_", "kv8_append", "attn_decode_kv8", "attn_prefill_kv8", "kv4_append", "kv4_dequantize", "attn_decode_kv4", "attn_prefill_kv4", "token_logprobs", "lowrank_mlp", "lowrank_attn_prefill", "rope_tables", "rope_tables_mask", "qkv_rope_append", "attn_decode_densekv", "attn_decode_rankkv", "rankkv_append", "rankkv_fill", "linear_rankkv_append",
             "lowrank_expand_heads", "rope_attn_prefill", "reconstruct_qkv_token", "xw_linear", "mlp_dual_split")

@@ -38,8 +38,8 @@ extern "C" {
 
 int fsvd_version(void);
 const char* fsvd_last_error(void);
-/* Which kernel form the last projection, gate / up pair, q / k / v expansion, head expansion, call on a cache in 8 bits or draw of a
- * token that this thread issued took ("256 x 256 pair", "ring 128 x 64", "vector", "kv8 prompt 128", ...): for tests and measurements; the names are no part of the interface. */
+/* Which kernel form the last projection, gate / up pair, q / k / v expansion, head expansion, call on a cache in 8 or 4 bits, draw of a
+ * token or call for log probabilities that this thread issued took ("256 x 256 pair", "ring 128 x 64", "vector", "kv8 prompt 128", ...): for tests and measurements; the names are no part of the interface. */
 const char* fsvd_last_form(void);
 
 /* Optional scratch for the projections (fsvd_linear, fsvd_swiglu_linear) of 17..127 rows, of 3..16 rows when the matrix has
@@ -228,6 +228,51 @@ size_t fsvd_attn_prefill_kv8_scratch_bytes(int B, int M, int H, int Hk, int Dh, 
 int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
                           const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
                           size_t scratch_bytes, int B, int M, int H, float scale, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * KV cache in 4 bits.  Codes [B, S, Hk, Dh / 2], two e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign bit) a byte with the even channel in the low
+ * bits, keys after their rotation; one byte for each token, kv head and 32 channels [B, Hk, Dh / 32, S] (tokens next to each other), value =
+ * code * 2^(byte - 127), byte 255 a NaN: the microscaling form of 4 bits.  S a multiple of 64.  k and v share their strides, k_scale and v_scale theirs, all in
+ * bytes; addresses and strides are multiples of 16, that of tokens at most 2^24.  head_dim 64 and 128.  No counterpart in the reference, whose caches
+ * are of 16 bits. */
+typedef struct fsvd_kv4_cache {
+  void* k;
+  void* v;
+  void* k_scale;
+  void* v_scale;
+  int64_t sc_b, sc_s, sc_h;              /* codes: sequence, token, head */
+  int64_t ss_b, ss_h, ss_g;              /* scales: sequence, head, group of channels */
+  int32_t S, Hk, Dh;
+} fsvd_kv4_cache;
+
+/* Row t < rows[b] (rows NULL: T) of k and v [B, T, Hk, Dh] goes to cache position positions[b] + t of sequence b; k is rotated there (cos and sin
+ * [rope_len, Dh / 2], NULL: not; halves of a head are the pairs).  The exponent of a group is the smallest from -125 to 125 whose 7-fold power covers the group
+ * (7 lies halfway between 6 and 8), and each value, the exact one where it was rotated, becomes the nearest code, ties to the even one.  A row changes no
+ * other row.  Rows outside [0, S) are dropped; with T = 0 there are none, and k and v may be NULL.  A group with a NaN is NaN as a whole; an infinity becomes the
+ * largest code and decides no exponent. */
+int fsvd_kv4_append(const fsvd_kv4_cache* cache, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t,
+                    int64_t sv_h, const int32_t* positions, const int32_t* rows, const void* cos, const void* sin, int rope_len, int B, int T, int dtype,
+                    void* stream);
+/* What the first L rows of B sequences hold, k and v [B, L, Hk, Dh] (strides so_b, so_t, so_h for both): exact in bf16, rounded to fp16. */
+int fsvd_kv4_dequantize(const fsvd_kv4_cache* cache, void* k, void* v, int64_t so_b, int64_t so_t, int64_t so_h, int B, int L, int dtype, void* stream);
+
+/* fsvd_attn_decode_kv8 and fsvd_attn_prefill_kv8 over a cache in 4 bits, rows that the former appends as fsvd_kv4_append has them. */
+size_t fsvd_attn_decode_kv4_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit);
+int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
+                         const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
+                         int rope_len, void* out, int64_t so_b, int64_t so_h, void* scratch, size_t scratch_bytes, int B, int H, int nsplit, float scale,
+                         int dtype, void* stream);
+size_t fsvd_attn_prefill_kv4_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S);
+int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
+                          const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
+                          size_t scratch_bytes, int B, int M, int H, float scale, int dtype, void* stream);
+
+/* Of every row of logits [B, T, V] (rows at any element's address, unit inner stride): logprobs[b, t] = log softmax at tokens[b, t], entropy[b, t] =
+ * - sum p log p in nats, and the `top` (0 to 64) largest logits, equal ones by index: top_tokens and top_logprobs [B, T, top] (NULL with top = 0).  tokens,
+ * logprobs and entropy are contiguous.  A token below 0 stands for none and has log probability 0, one from V on NaN.  A NaN ranks above everything; a row whose
+ * largest logit is not finite has no distribution, its numbers are NaN.  Logits of -inf have no weight. */
+int fsvd_token_logprobs(const void* logits, int64_t sl_b, int64_t sl_t, const int64_t* tokens, float* logprobs, float* entropy, int64_t* top_tokens,
+                        float* top_logprobs, int B, int T, int V, int top, int dtype, void* stream);
 
 
 
