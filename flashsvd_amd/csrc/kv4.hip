@@ -3,63 +3,27 @@
 
 namespace fsvd {
 
-// A lane holds eight dimensions d .. d + 7 of a row and the eight half a head further (the pairs of the rotation), LPR lanes a row; four lanes have a group of 32
-// channels in either half (of 64 dimensions the halves are the groups).
+// A workgroup has 256 / (Dh / 16) rows of the keys or the values of one kv head.
 template <int DT, int DH>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
-  typedef E16<DT> E;
-  constexpr int HALF = DH / 2, LPR = HALF / 8, GROUPS = DH / kGroup4;
-  const int part = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, lane = threadIdx.x % LPR, t = (int)blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  constexpr int HALF = DH / 2, LPR = DH / 16;
+  const int value = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, part = threadIdx.x % LPR, t = (int)blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
   const int rows = a.rows ? min(a.rows[b], a.T) : a.T;
   const int64_t pos = (int64_t)a.positions[b] + t;
   const bool in = t < rows && pos >= 0 && pos < a.c.S;
   const int64_t r = in ? t : 0;
-  const uint16_t* x = (part ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h + r * a.sv_t : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h + r * a.sk_t) + lane * 8;
-  const u32x4_t lo = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x)), hi = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(x + HALF));
-  const bool turn = part == 0 && a.cos != nullptr;
-  u32x4_t cw, sw;
+  const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h + r * a.sv_t : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h + r * a.sk_t) + 8 * part;
+  const u32x4_t lo = eight4(x), hi = eight4(x + HALF);
+  const bool turn = !value && a.cos != nullptr;
+  u32x4_t cw = {0u, 0u, 0u, 0u}, sw = cw;
   if (turn) {
-    const int64_t tp = min(max(pos, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + lane * 8;
-    cw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.cos + tp));
-    sw = __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(a.sin + tp));
+    const int64_t tp = min(max(pos, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + 8 * part;
+    cw = eight4(a.cos + tp); sw = eight4(a.sin + tp);
   }
-  float y[2][8], amax[2] = {0.f, 0.f};
-  bool nan[2] = {false, false};
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t wl = lo[e >> 1], wh = hi[e >> 1];
-    float u = e & 1 ? E::hi(wl) : E::lo(wl), v = e & 1 ? E::hi(wh) : E::lo(wh);
-    if (turn) {
-      const uint32_t wc = cw[e >> 1], ws = sw[e >> 1];
-      const float c = e & 1 ? E::hi(wc) : E::lo(wc), s = e & 1 ? E::hi(ws) : E::lo(ws), y0 = odd_sum(u * c, -(v * s)), y1 = odd_sum(u * s, v * c);
-      u = y0; v = y1;
-    }
-    y[0][e] = u; y[1][e] = v;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      amax[h] = fmaxf(amax[h], finite_mag4(y[h][e]));
-      nan[h] = nan[h] || y[h][e] != y[h][e];
-    }
-  }
-  uint8_t* codes = static_cast<uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s;
-  uint8_t* scales = static_cast<uint8_t*>(part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    amax[h] = fmaxf(amax[h], dpp_f32<0xB1>(amax[h]));                       // over the four lanes of the group
-    amax[h] = fmaxf(amax[h], dpp_f32<0x4E>(amax[h]));
-    float bad = nan[h] ? 1.f : 0.f;
-    bad = fmaxf(bad, dpp_f32<0xB1>(bad));
-    bad = fmaxf(bad, dpp_f32<0x4E>(bad));
-    const int byte = scale_byte(amax[h]);
-    const float scale = scale_of(byte);
-    if (!in) continue;
-    uint32_t w = codes4_of<0>(0u, y[h][0], y[h][1], scale);
-    w = codes4_of<1>(w, y[h][2], y[h][3], scale);
-    w = codes4_of<2>(w, y[h][4], y[h][5], scale);
-    w = codes4_of<3>(w, y[h][6], y[h][7], scale);
-    *reinterpret_cast<uint32_t*>(codes + h * (HALF / 2) + lane * 4) = w;
-    if (lane % 4 == 0) scales[(h * (GROUPS / 2) + lane / 4) * a.c.ss_g] = (uint8_t)(bad > 0.f ? kNanByte : byte);
-  }
+  float y[2][8];
+  row_numbers<E16<DT>>(lo, hi, turn, cw, sw, y);
+  put_row<DH>(y, static_cast<uint8_t*>(value ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s,
+              static_cast<uint8_t*>(value ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos, a.c.ss_g, part, in);
 }
 
 int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st) {
@@ -116,7 +80,7 @@ static int check_kv4_cache(const char* fn, const fsvd_kv4_cache* c) {
     set_last_error("%s: bad cache: S=%d Hk=%d Dh=%d (a multiple of 64 rows; 64 and 128 dimensions are served)", fn, c->S, c->Hk, c->Dh);
     return kErrBadShape;
   }
-  if (c->sc_b < 0 || c->sc_s < c->Dh / 2 || c->sc_s > (1 << 24) || c->sc_h < 0 || c->ss_b < 0 || c->ss_h < 0 || c->ss_g < c->S) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
+  if (c->sc_b < 0 || c->sc_s < c->Dh / 2 || c->sc_s > (1 << 24) || c->sc_h < 0 || c->ss_b < 0 || c->ss_h < 0 || c->ss_g < c->S || c->ss_g > (1 << 28)) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15) ||
       ((c->sc_b | c->sc_s | c->sc_h | c->ss_b | c->ss_h | c->ss_g) & 15)) {
     set_last_error("%s: cache pointers and strides must be 16-byte aligned", fn);
@@ -189,7 +153,10 @@ int fsvd_kv4_dequantize(const fsvd_kv4_cache* cache, void* k, void* v, int64_t s
   return kOk;
 }
 
-size_t fsvd_attn_decode_kv4_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) { return 0; }
+size_t fsvd_attn_decode_kv4_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0) return 0;
+  return kv4_decode_scratch_bytes(B, H, Dh, kv4_ranges(B, H, Hk, S, nsplit));
+}
 
 int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
                          const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
@@ -203,13 +170,16 @@ int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_
   if (const int rc = k_new ? check_written(fn, cache, B) : kOk) return rc;
   if (const int rc = check_out(fn, B, 1, H, so_b, 0, so_h)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (k_new != nullptr) {
-    const Kv4AppendArgs n{*cache, in16(k_new), sk_b, 0, sk_h, in16(v_new), sv_b, 0, sv_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, B, 1, dtype};
-    if (const int rc = launch_kv4_append(fn, n, st)) return rc;
+  const int ranges = kv4_ranges(B, H, cache->Hk, cache->S, nsplit);
+  const size_t need = kv4_decode_scratch_bytes(B, H, cache->Dh, ranges);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
+    set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, ranges, need);
+    return kErrWorkspace;
   }
   const Kv4AttnArgs a{*cache, in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
-                      B, 1, H, k_new ? 1 : seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
-  return launch_kv4_attend(fn, a, st);
+                      B, 1, H, k_new ? 1 : seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype,
+                      in16(k_new), sk_b, sk_h, in16(v_new), sv_b, sv_h};
+  return launch_kv4_decode(fn, a, ranges, static_cast<float*>(scratch), st);
 }
 
 size_t fsvd_attn_prefill_kv4_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) { return 0; }

@@ -16,8 +16,8 @@ constexpr int kLeastExp4 = -125, kMostExp4 = 125;
 __device__ __forceinline__ float odd_sum(float p, float q) {
   const float s = p + q, t = s - p, r = (p - (s - t)) + (q - t);          // r: what the rounding left
   const uint32_t u = __float_as_uint(s);
-  if ((r > 0.f || r < 0.f) && !(u & 1)) return __uint_as_float((r > 0.f) == (s > 0.f) ? u + 1 : u - 1);
-  return s;
+  const uint32_t off = (r > 0.f || r < 0.f) ? ~u & 1 : 0;                 // of an even neighbour
+  return __uint_as_float((r > 0.f) == (s > 0.f) ? u + off : u - off);
 }
 // magnitude that counts towards a scale: neither a NaN nor an infinity decides it
 __device__ __forceinline__ float finite_mag4(float x) {
@@ -43,6 +43,80 @@ __device__ __forceinline__ uint32_t pair4(uint32_t w, float scale) {
 template <int AT>
 __device__ __forceinline__ f32x2_t pair4_f32(uint32_t w, float scale) { return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, AT); }
 
+// the same with the position known after unrolling only
+__device__ __forceinline__ uint32_t pair4_at(int at, uint32_t w, float scale) { return at == 0 ? pair4<0>(w, scale) : at == 1 ? pair4<1>(w, scale) : at == 2 ? pair4<2>(w, scale) : pair4<3>(w, scale); }
+// Byte i of four scales as a scale: the conversions read the exponent alone, so what stands around it may stay.  Byte 255 makes NaN of every code.
+__device__ __forceinline__ float scale_at(uint32_t four, int i) { return __uint_as_float(i == 0 ? four << 23 : i == 1 ? four << 15 : i == 2 ? four << 7 : four >> 1); }
+
+// A row of a kv head into the cache: the lane has dimensions 8 part .. 8 part + 7 in x[0] and those half a head further in x[1], Dh / 16 lanes a row, four of
+// them a group of 32 channels in either half (of 64 dimensions the halves are the groups).  codes: the row's; scales: its byte of group 0.  All lanes of the wave
+// call it, `in` says which write.
+template <int DH>
+__device__ __forceinline__ void put_row(const float (&x)[2][8], uint8_t* codes, uint8_t* scales, int64_t ss_g, int part, bool in) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float amax = 0.f, bad = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      amax = fmaxf(amax, finite_mag4(x[h][e]));
+      bad = x[h][e] != x[h][e] ? 1.f : bad;
+    }
+    amax = fmaxf(amax, dpp_f32<0xB1>(amax));               // over the four lanes
+    amax = fmaxf(amax, dpp_f32<0x4E>(amax));
+    bad = fmaxf(bad, dpp_f32<0xB1>(bad));
+    bad = fmaxf(bad, dpp_f32<0x4E>(bad));
+    const int byte = scale_byte(amax);
+    const float scale = scale_of(byte);
+    uint32_t w = codes4_of<0>(0u, x[h][0], x[h][1], scale);
+    w = codes4_of<1>(w, x[h][2], x[h][3], scale);
+    w = codes4_of<2>(w, x[h][4], x[h][5], scale);
+    w = codes4_of<3>(w, x[h][6], x[h][7], scale);
+    if (in) {
+      *reinterpret_cast<uint32_t*>(codes + h * (DH / 4) + part * 4) = w;
+      if (part % 4 == 0) scales[(h * (DH / 64) + part / 4) * ss_g] = (uint8_t)(bad > 0.f ? kNanByte : byte);
+    }
+  }
+}
+// eight elements and those half a head further as numbers, rotated exactly
+template <class E>
+__device__ __forceinline__ void row_numbers(u32x4_t lo, u32x4_t hi, bool turn, u32x4_t cw, u32x4_t sw, float (&x)[2][8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t wl = lo[e >> 1], wh = hi[e >> 1];
+    const uint32_t wc = cw[e >> 1], ws = sw[e >> 1];
+    const float u = e & 1 ? E::hi(wl) : E::lo(wl), v = e & 1 ? E::hi(wh) : E::lo(wh), c = e & 1 ? E::hi(wc) : E::lo(wc), s = e & 1 ? E::hi(ws) : E::lo(ws);
+    const float y0 = odd_sum(u * c, -(v * s)), y1 = odd_sum(u * s, v * c);
+    x[0][e] = turn ? y0 : u; x[1][e] = turn ? y1 : v;
+  }
+}
+__device__ __forceinline__ u32x4_t eight4(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
+
+// Loads at a base of the wave's, an offset of the wave's and one of the lane's (each below 2^31): nothing of the address but the lane's offset is in vector registers.
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef __amdgpu_buffer_rsrc_t Rows4;
+constexpr int kOnce = 2;                                  // read once: not kept in the caches
+__device__ __forceinline__ Rows4 rows4(const uint8_t* base) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0xffffffffu, 0x00020000u); }
+template <int BYTES, int AUX>
+__device__ __forceinline__ void load4(Rows4 r, uint32_t lane, uint32_t off, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane, (int)off, AUX);
+    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const u32x2_t v = __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane, (int)off, AUX);
+    w[0] = v.x; w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane, (int)off, AUX);
+  } else {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, (int)lane, (int)off, AUX);
+  }
+}
+#else
+struct Rows4 {};
+constexpr int kOnce = 2;
+__device__ Rows4 rows4(const uint8_t* base);
+template <int BYTES, int AUX> __device__ void load4(Rows4 r, uint32_t lane, uint32_t off, uint32_t* w);
+#endif
+
 struct Kv4AppendArgs {
   fsvd_kv4_cache c;
   const uint16_t* k; int64_t sk_b, sk_t, sk_h;         // [B, T, Hk, Dh]
@@ -63,9 +137,35 @@ struct Kv4AttnArgs {
   int key_add;                                         // query row m sees the keys below positions[b] + m + key_add
   float scale;
   int dt;
+  // decode: the rows [B, Hk, Dh] that the call appends at positions[b], or null
+  const uint16_t* k_new = nullptr; int64_t sk_b = 0, sk_h = 0;
+  const uint16_t* v_new = nullptr; int64_t sv_b = 0, sv_h = 0;
 };
+
+// One row of a kv head (k, v [Dh]) into its place at position pos, 0 <= pos < S, by one wave: the first Dh / 16 lanes hold the key, as many behind them the value.
+template <int DT, int DH>
+__device__ __forceinline__ void append_row4(const fsvd_kv4_cache& c, const uint16_t* k, const uint16_t* v, const uint16_t* cos, const uint16_t* sin, int rope_len,
+                                            int b, int hk, int pos, int lane) {
+  constexpr int LPR = DH / 16, HALF = DH / 2;
+  const int value = lane / LPR & 1, part = lane % LPR;
+  const uint16_t* x = (value ? v : k) + 8 * part;
+  const u32x4_t lo = eight4(x), hi = eight4(x + HALF);
+  u32x4_t cw = {0u, 0u, 0u, 0u}, sw = cw;
+  if (cos != nullptr) {
+    const int64_t tp = (int64_t)min(pos, rope_len - 1) * HALF + 8 * part;
+    cw = eight4(cos + tp); sw = eight4(sin + tp);
+  }
+  float y[2][8];
+  row_numbers<E16<DT>>(lo, hi, cos != nullptr && !value, cw, sw, y);
+  put_row<DH>(y, static_cast<uint8_t*>(value ? c.v : c.k) + b * c.sc_b + hk * c.sc_h + pos * c.sc_s,
+              static_cast<uint8_t*>(value ? c.v_scale : c.k_scale) + b * c.ss_b + hk * c.ss_h + pos, c.ss_g, part, lane < 2 * LPR);
+}
 
 int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st);
 int launch_kv4_attend(const char* fn, const Kv4AttnArgs& a, hipStream_t st);
+// ranges of keys that a sequence may be cut into, and the scratch for their partial results
+int kv4_ranges(int B, int H, int Hk, int S, int nsplit);
+size_t kv4_decode_scratch_bytes(int B, int H, int Dh, int ranges);
+int launch_kv4_decode(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st);
 
 }  // namespace fsvd

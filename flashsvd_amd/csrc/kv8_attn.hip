@@ -1,17 +1,8 @@
 // Attention over the KV cache in 8 bits.
+#include "attn_join.hpp"
 #include "kv8.hpp"
 
 namespace fsvd {
-
-// Partial results of key ranges: values [rows][ranges][Dh], not divided by their sums, and behind them (maximum, sum) [rows][ranges].
-struct Kv8Parts {
-  float* base;
-  int64_t rows;
-  int ranges, dh;
-  static size_t bytes(int64_t rows, int ranges, int dh) { return (size_t)rows * ranges * (dh + 2) * sizeof(float); }
-  __device__ __forceinline__ float* values(int64_t row, int s) const { return base + (row * ranges + s) * dh; }
-  __device__ __forceinline__ f32x2_t* stats(int64_t row, int s) const { return reinterpret_cast<f32x2_t*>(base + rows * ranges * dh) + row * ranges + s; }
-};
 
 // eight elements x of a query row in the lower or upper half of the head, rotated with their partners y half a head away, in fp32 and rounded to the type of
 // the products; rest: what that rounding leaves.  A pair of large float16 elements may turn to one beyond the type's range (up to 1.42 times its end): the first
@@ -30,83 +21,13 @@ __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u3
   return x;
 }
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
+static JoinArgs join_args(const Kv8AttnArgs& a) { return {a.out, a.so_b, a.so_m, a.so_h, a.rows, a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.dt}; }
 
 // Keys of a decode range, but for the last: a step of every wave, and whole blocks.
 constexpr int kMinRange = 128;
 __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
   const int per = (keys + ranges - 1) / ranges;
   return (max(per, 1) + kMinRange - 1) / kMinRange * kMinRange;
-}
-
-// The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
-// token, head of the group).  Nothing that a load needs comes from another load: what it takes is a round trip to memory and its launch.
-template <int DT, int DH, int WPR>
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8AttnArgs a, int ranges, bool decode, float* scratch) {
-  typedef E16<DT> E;
-  constexpr int D = DH / kWave, U = 8;
-  __shared__ float vs[4][DH];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part_of = wave % WPR, G = a.H / a.c.Hk;
-  const int64_t rows = (int64_t)a.B * a.M * a.H, row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR;
-  const bool live = row < rows;
-  const int64_t at = live ? row : rows - 1;
-  const Kv8Parts part{scratch, rows, ranges, DH};
-  float v[D], sum = 0.f, top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < D; ++i) v[i] = 0.f;
-  if (ranges > kWave)
-    for (int s0 = 0; s0 < ranges; s0 += kWave) top = fmaxf(top, s0 + lane < ranges ? (*part.stats(at, s0 + lane))[0] : -INFINITY);
-  for (int s0 = 0; s0 < ranges; s0 += kWave) {
-    const int n = min(kWave, ranges - s0);
-    const f32x2_t st = *part.stats(at, s0 + min(lane, n - 1));
-    float w = 0.f;
-    for (int s = part_of; s < n; s += WPR * U) {
-      float x[U][D];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
-      if (s == part_of) {                                  // the weights, with the first values on their way
-        if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-        w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : 0.f;
-#pragma unroll
-        for (int i = 0; i < D; ++i) v[i] += f > 0.f ? f * x[u][i] : 0.f;        // a range without keys has written no values
-      }
-    }
-    if (part_of >= n) {                                    // more waves than ranges: the sum all the same
-      if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-      w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
-    }
-    sum += w * st[1];
-  }
-  sum = wave_sum(sum);
-  if (WPR > 1) {
-#pragma unroll
-    for (int i = 0; i < D; ++i) vs[wave][lane * D + i] = v[i];
-    __syncthreads();
-    if (part_of == 0) {
-#pragma unroll
-      for (int i = 0; i < D; ++i)
-#pragma unroll
-        for (int w = 1; w < WPR; ++w) v[i] += vs[wave + w][lane * D + i];
-    }
-  }
-  const int b = (int)(at / ((int64_t)a.M * a.H)), in = (int)(at - (int64_t)b * a.M * a.H), hk = in / (a.M * G), r = in - hk * a.M * G;
-  const int m = decode ? 0 : r / G, h = decode ? in : hk * G + r - m * G;
-  if (!live || part_of || (a.rows && m >= a.rows[b])) return;
-  uint16_t* o = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + lane * D;
-#pragma unroll
-  for (int i = 0; i < D; ++i) o[i] = (uint16_t)E::bits(sum == 0.f ? 0.f : v[i] / sum);
-}
-template <int DT, int DH>
-static void launch_join(const Kv8AttnArgs& a, int ranges, bool decode, float* scratch, hipStream_t st) {
-  const int64_t rows = (int64_t)a.B * a.M * a.H;
-  // 63 ranges of 32 rows: 13.9 us with the attention before it, 15.2 by one wave a row; 8 ranges of 512 rows: 27.5 by one wave, 28.5 by four
-  if (ranges > 8) hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 4>), dim3((unsigned)rows), dim3(256), 0, st, a, ranges, decode, scratch);
-  else hipLaunchKernelGGL((kv8_join_kernel<DT, DH, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a, ranges, decode, scratch);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -143,7 +64,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8Att
   const int per = kv8_range(keys, ranges), used = max(1, (keys + per - 1) / per), s = turn < used ? used - 1 - turn : turn;
   const int k0 = min(s * per, keys), k1 = min(k0 + per, keys);
   const int h0 = hk * G + gg * kDecGroup, heads = min(kDecGroup, G - gg * kDecGroup);
-  const Kv8Parts part{scratch, (int64_t)a.B * a.H, ranges, DH};
+  const RangeParts part{scratch, (int64_t)a.B * a.H, ranges, DH};
   if (s >= used) {
     if (tid < heads) *part.stats((int64_t)b * a.H + h0 + tid, s) = f32x2_t{-INFINITY, 0.f};
     return;
@@ -356,14 +277,14 @@ int kv8_ranges(int B, int H, int Hk, int S, int nsplit) {
   }
   return max(1, min(nsplit, most));
 }
-size_t kv8_decode_scratch_bytes(int B, int H, int Dh, int ranges) { return ranges > 1 ? Kv8Parts::bytes((int64_t)B * H, ranges, Dh) : 0; }
+size_t kv8_decode_scratch_bytes(int B, int H, int Dh, int ranges) { return ranges > 1 ? RangeParts::bytes((int64_t)B * H, ranges, Dh) : 0; }
 
 template <int DT, int DH>
 static void decode_form(const Kv8AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   const int groups = (a.H / a.c.Hk + kDecGroup - 1) / kDecGroup;
   hipLaunchKernelGGL((kv8_decode_kernel<DT, DH>), dim3((unsigned)a.B * a.c.Hk * groups * ranges), dim3(kDecWaves * kWave),
                      kDecWaves * min(a.H / a.c.Hk, kDecGroup) * (DH + 4) * sizeof(float), st, a, ranges, scratch);
-  if (ranges > 1) launch_join<DT, DH>(a, ranges, true, scratch, st);
+  if (ranges > 1) launch_join(join_args(a), ranges, true, scratch, st);
   set_last_form(ranges == 1 ? "kv8 decode" : ranges <= 8 ? "kv8 decode ranges" : ranges <= kWave ? "kv8 decode ranges 9" : "kv8 decode ranges 65");
 }
 int launch_kv8_decode(const char* fn, const Kv8AttnArgs& args, int ranges, float* scratch, hipStream_t st) {
@@ -819,7 +740,7 @@ __global__ __launch_bounds__(kWave * kPromptWaves * KG, 2) void kv8_prompt_kerne
           if (nan_at[16 * t + 4 * lg + i] < seen[mi]) o[mi][t][i] = __builtin_nanf("");
     }
     if (ranges > 1) {
-      const Kv8Parts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+      const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
       const int64_t row = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
       if (lg == 0) *part.stats(row, range) = f32x2_t{m_run[mi], l};
       float* v = part.values(row, range) + 4 * lg;
@@ -864,7 +785,7 @@ static PromptForm prompt_form(int B, int M, int H, int Hk, int S) {
 }
 size_t kv8_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   const PromptForm f = prompt_form(B, M, H, Hk, S);
-  return f.ranges > 1 ? Kv8Parts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
+  return f.ranges > 1 ? RangeParts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
 template <int DT, int DH, int MI, int KG, bool TURN>
@@ -875,7 +796,7 @@ static int prompt_launch_form(const char* fn, const Kv8AttnArgs& a, int ranges, 
   const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * kPromptWaves - 1) / (16 * MI * kPromptWaves) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
   hipLaunchKernelGGL((kv8_prompt_kernel<DT, DH, MI, KG, TURN>), dim3((unsigned)groups, ranges), dim3(kPromptWaves * KG * kWave), lds, st, a, ranges, scratch);
-  if (ranges > 1) launch_join<DT, DH>(a, ranges, false, scratch, st);
+  if (ranges > 1) launch_join(join_args(a), ranges, false, scratch, st);
   return kOk;
 }
 template <int DT, int DH, int MI, int KG>
