@@ -127,7 +127,7 @@ __host__ __device__ __forceinline__ int kv4_range(int keys, int ranges) {
 // key are read and their codes and scores replaced.
 // ---------------------------------------------------------------------------------------------
 template <int DT, int DH, bool HALVES>
-__global__ __launch_bounds__(kDec4Waves * kWave, 2) void kv4_decode_kernel(Kv4AttnArgs a, int ranges, float* scratch) {
+__global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef E16<0> P;
   typedef P::frag_t frag_t;
@@ -155,8 +155,9 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 2) void kv4_decode_kernel(Kv4At
   const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
   const uint8_t* ksp = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
   const uint8_t* vsp = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
-  const uint32_t klane = 4 * n * row + CH / 2 * g, vlane = 16 * g * row + NT / 2 * n;
-  const uint32_t kslane = CH * g / kGroup4 * (uint32_t)a.c.ss_g + 4 * n, vslane = NT * n / kGroup4 * (uint32_t)a.c.ss_g + 16 * g;
+  uint32_t klane = 4 * n * row + CH / 2 * g, vlane = 16 * g * row + NT / 2 * n;
+  uint32_t kslane = CH * g / kGroup4 * (uint32_t)a.c.ss_g + 4 * n, vslane = NT * n / kGroup4 * (uint32_t)a.c.ss_g + 16 * g;
+  asm volatile("" : "+v"(klane), "+v"(vlane), "+v"(kslane), "+v"(vslane));      // made by 64-bit products, each would take two registers
   uint32_t kr[4][KW], vr[16], ks, vs[4];
   const auto fetch_k = [&](int c0) {
     const Rows4 r = rows4(kb + (int64_t)c0 * a.c.sc_s);
@@ -212,20 +213,13 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 2) void kv4_decode_kernel(Kv4At
   }
 
   const float scale = a.scale * 1.4426950408889634f;      // weights are powers of two of the scores' differences
+  const float second = n < 8 ? 0.f : -1.f;                // the columns of the second parts take what the first leave
   float m = -INFINITY, l = 0.f;
   f32x4_t o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int stop = before;; c0 += kDec4Waves * kDec4Step) {
-    if (c0 >= stop) {
-      if (!appends || stop == k1) break;
-      wait_stores_acked();
-      __syncthreads();
-      stop = k1;
-      if (c0 >= k1) break;
-      fetch_k(c0); fetch_v(c0);
-    }
-    {
+  const auto walk = [&](int stop) {
+    for (; c0 < stop; c0 += kDec4Waves * kDec4Step) {
       const int next = c0 + kDec4Waves * kDec4Step, left = k1 - c0 - 16 * g;      // of the lane's 16 keys
       float x[4][4];                                      // key 16 g + 4 i + t
 #pragma unroll
@@ -266,21 +260,26 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 2) void kv4_decode_kernel(Kv4At
         m = top;
       }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {                       // the lane's keys 8 u .. 8 u + 7
-        uint32_t ph[4], pl[4];                            // the weights as a 16-bit part and what it leaves
+      for (int t = 0; t < NT; ++t) asm volatile("" : "+v"(o[t]));           // the sums stay in their registers whether they were rescaled or not
+      frag_t hi[2], lo[2];                                // the weights of the lane's keys 8 u .. 8 u + 7 as a 16-bit part and what it leaves
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t ph[4], pl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int c = 2 * u + (i >> 1), t = 2 * (i & 1);
           const float w0 = __builtin_amdgcn_exp2f(x[t][c] - m), w1 = __builtin_amdgcn_exp2f(x[t + 1][c] - m);
           l += w0 + w1;
           ph[i] = pack_bf16x2(w0, w1);
-          pl[i] = pack_bf16x2(w0 - bf16_lo(ph[i]), w1 - bf16_hi(ph[i]));
+          if constexpr (HALVES) ph[i] = pack_bf16x2(fmaf(bf16_lo(ph[i]), second, w0), fmaf(bf16_hi(ph[i]), second, w1));
+          else pl[i] = pack_bf16x2(w0 - bf16_lo(ph[i]), w1 - bf16_hi(ph[i]));
         }
-        if constexpr (HALVES) {
+        hi[u] = __builtin_bit_cast(frag_t, u32x4_t{ph[0], ph[1], ph[2], ph[3]});
+        if constexpr (!HALVES) lo[u] = __builtin_bit_cast(frag_t, u32x4_t{pl[0], pl[1], pl[2], pl[3]});
+      }
+      __builtin_amdgcn_sched_barrier(0);                  // left to itself the compiler converts far ahead, and three waves a SIMD do not fit
 #pragma unroll
-          for (int i = 0; i < 4; ++i) ph[i] = n < 8 ? ph[i] : pl[i];
-        }
-        const frag_t hi = __builtin_bit_cast(frag_t, u32x4_t{ph[0], ph[1], ph[2], ph[3]}), lo = __builtin_bit_cast(frag_t, u32x4_t{pl[0], pl[1], pl[2], pl[3]});
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int c = 0; c < NT / 2; ++c) {               // channels 2 c and 2 c + 1 of the lane's
           uint32_t w[8];
@@ -292,15 +291,22 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 2) void kv4_decode_kernel(Kv4At
             v0[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05040100u);
             v1[i] = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07060302u);
           }
-          o[2 * c] = P::mfma(__builtin_bit_cast(frag_t, v0), hi, o[2 * c]);
-          if constexpr (!HALVES) o[2 * c] = P::mfma(__builtin_bit_cast(frag_t, v0), lo, o[2 * c]);
-          o[2 * c + 1] = P::mfma(__builtin_bit_cast(frag_t, v1), hi, o[2 * c + 1]);
-          if constexpr (!HALVES) o[2 * c + 1] = P::mfma(__builtin_bit_cast(frag_t, v1), lo, o[2 * c + 1]);
+          o[2 * c] = P::mfma(__builtin_bit_cast(frag_t, v0), hi[u], o[2 * c]);
+          if constexpr (!HALVES) o[2 * c] = P::mfma(__builtin_bit_cast(frag_t, v0), lo[u], o[2 * c]);
+          o[2 * c + 1] = P::mfma(__builtin_bit_cast(frag_t, v1), hi[u], o[2 * c + 1]);
+          if constexpr (!HALVES) o[2 * c + 1] = P::mfma(__builtin_bit_cast(frag_t, v1), lo[u], o[2 * c + 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (next < stop) fetch_v(next);
     }
+  };
+  walk(before);
+  if (appends) {
+    wait_stores_acked();
+    __syncthreads();
+    if (c0 < k1) { fetch_k(c0); fetch_v(c0); }
+    walk(k1);
   }
   // the waves' results through LDS: element i of tile t is channel NT (4 g + i) + t of query n.  A sum that is NaN takes the largest reference, so that it is kept.
   if constexpr (HALVES) {
