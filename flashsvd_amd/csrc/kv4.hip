@@ -182,7 +182,10 @@ int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_
   return launch_kv4_decode(fn, a, ranges, static_cast<float*>(scratch), st);
 }
 
-size_t fsvd_attn_prefill_kv4_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) { return 0; }
+size_t fsvd_attn_prefill_kv4_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
+  if (B <= 0 || M <= 0 || H <= 0 || Hk <= 0 || H % Hk || S <= 0) return 0;
+  return kv4_prompt_scratch_bytes(B, M, H, Hk, Dh, S);
+}
 
 int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_m, int64_t sq_h, const int32_t* q_pos0, const int32_t* rows,
                           const void* cos, const void* sin, int rope_len, void* out, int64_t so_b, int64_t so_m, int64_t so_h, void* scratch,
@@ -195,7 +198,7 @@ int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq
   if (const int rc = check_out(fn, B, M, H, so_b, so_m, so_h)) return rc;
   const Kv4AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
                       B, M, H, 1, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
-  return M == 0 ? kOk : launch_kv4_attend(fn, a, static_cast<hipStream_t>(stream));
+  return M == 0 ? kOk : launch_kv4_prompt(fn, a, static_cast<float*>(scratch), scratch_bytes, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -162,10 +162,11 @@ __device__ __forceinline__ void append_row4(const fsvd_kv4_cache& c, const uint1
 }
 
 int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st);
-int launch_kv4_attend(const char* fn, const Kv4AttnArgs& a, hipStream_t st);
 // ranges of keys that a sequence may be cut into, and the scratch for their partial results
 int kv4_ranges(int B, int H, int Hk, int S, int nsplit);
 size_t kv4_decode_scratch_bytes(int B, int H, int Dh, int ranges);
+size_t kv4_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S);
 int launch_kv4_decode(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st);
+int launch_kv4_prompt(const char* fn, const Kv4AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st);
 
 }  // namespace fsvd

@@ -4,95 +4,6 @@
 
 namespace fsvd {
 
-// One query row of a head for a workgroup: scores of 256 keys at a time, one a thread, their weights against a running maximum, and the values of those keys by
-// DH-fold threads.  Everything in fp32.
-template <int DT, int DH>
-__global__ __launch_bounds__(256) void kv4_attend_kernel(Kv4AttnArgs a) {
-  typedef E16<DT> E;
-  constexpr int HALF = DH / 2, GROUPS = DH / kGroup4, PARTS = 256 / DH;
-  __shared__ float qs[DH], ws[256], red[4], os[PARTS][DH];
-  const int tid = threadIdx.x, h = blockIdx.x, m = blockIdx.y, b = blockIdx.z, hk = h / (a.H / a.c.Hk);
-  if (a.rows && m >= a.rows[b]) return;
-  const int64_t at = (int64_t)a.positions[b] + m;
-  const int keys = (int)max((int64_t)0, min(at + a.key_add, (int64_t)a.c.S));
-  const uint16_t* q = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
-  if (tid < DH) {
-    float x = E::val(q[tid]);
-    if (a.cos) {
-      const int64_t tp = min(max(at, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + tid % HALF;
-      const float c = E::val(a.cos[tp]), s = E::val(a.sin[tp]), y = E::val(q[tid < HALF ? tid + HALF : tid - HALF]);
-      x = x * c + (tid < HALF ? -y : y) * s;
-    }
-    qs[tid] = x * a.scale;
-  }
-  __syncthreads();
-  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
-  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
-  const uint8_t* ks = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
-  const uint8_t* vs = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
-  const int d = tid % DH, part = tid / DH;
-  float top = -INFINITY, sum = 0.f, o = 0.f;
-  for (int n0 = 0; n0 < keys; n0 += 256) {
-    const int n = n0 + tid;
-    float s = -INFINITY;
-    if (n < keys) {
-      s = 0.f;
-      for (int g = 0; g < GROUPS; ++g) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(kb + n * a.c.sc_s + 16 * g);
-        const uint32_t byte = ks[g * a.c.ss_g + n];
-        const float f = scale_of(byte);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x2_t x[4] = {pair4_f32<0>(w[i], f), pair4_f32<1>(w[i], f), pair4_f32<2>(w[i], f), pair4_f32<3>(w[i], f)};
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s += x[e >> 1][e & 1] * qs[32 * g + 8 * i + e];
-        }
-        if (byte == kNanByte) s = __builtin_nanf("");
-      }
-    }
-    float most = wave_max(s);
-    if ((tid & 63) == 0) red[tid >> 6] = most;
-    __syncthreads();
-    most = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), top);
-    const float base = most == -INFINITY ? 0.f : most, keep = __expf(top - base);
-    ws[tid] = n < keys ? __expf(s - base) : 0.f;
-    top = most;
-    __syncthreads();
-    o *= keep; sum *= keep;
-    for (int i = part; i < 256 && n0 + i < keys; i += PARTS) {
-      const uint32_t byte = vs[d / kGroup4 * a.c.ss_g + n0 + i], code = vb[(int64_t)(n0 + i) * a.c.sc_s + d / 2];
-      const f32x2_t x = pair4_f32<0>(code, scale_of(byte));
-      o += ws[i] * (byte == kNanByte ? __builtin_nanf("") : d & 1 ? x[1] : x[0]);
-      sum += ws[i];
-    }
-  }
-  os[part][d] = o;
-  __syncthreads();
-  if (d == 0) ws[part] = sum;
-  __syncthreads();
-  if (part == 0) {
-    for (int p = 1; p < PARTS; ++p) { o += os[p][d]; sum += ws[p]; }
-    a.out[(int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + d] = (uint16_t)E::bits(keys == 0 ? 0.f : o / sum);
-  }
-}
-
-int launch_kv4_attend(const char* fn, const Kv4AttnArgs& a, hipStream_t st) {
-  if (a.M > 65535) { set_last_error("%s: %d rows", fn, a.M); return kErrBadShape; }
-  const dim3 grid(a.H, a.M, a.B);
-  if (a.dt == 1) {
-    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_attend_kernel<1, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv4_attend_kernel<1, 64>), grid, dim3(256), 0, st, a);
-  } else {
-    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_attend_kernel<0, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv4_attend_kernel<0, 64>), grid, dim3(256), 0, st, a);
-  }
-  set_last_form("kv4 attend");
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
-  return kOk;
-}
-
-
 static JoinArgs join_args(const Kv4AttnArgs& a) { return {a.out, a.so_b, a.so_m, a.so_h, a.rows, a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.dt}; }
 
 // Eight elements of a query row, rotated in fp32 (y: those half a head away; sign: -1 in the lower half; not rotated: cosines 1, y and sines 0), as two bf16 parts:
@@ -376,6 +287,393 @@ int launch_kv4_decode(const char* fn, const Kv4AttnArgs& args, int ranges, float
   }
   if (a.dt == 1) a.c.Dh == 128 ? decode_form<1, 128>(a, ranges, scratch, st) : decode_form<1, 64>(a, ranges, scratch, st);
   else a.c.Dh == 128 ? decode_form<0, 128>(a, ranges, scratch, st) : decode_form<0, 64>(a, ranges, scratch, st);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
+  return kOk;
+}
+
+// ---------------------------------------------------------------------------------------------
+// A chunk of a prompt.  The query rows of the heads that share a kv head are one list, row r = query token r / G of head r % G, so that grouped heads share
+// the tiles of keys too.  A workgroup of four waves takes 16 MI rows for each; tiles of 64 keys go through LDS as bf16, converted once for the workgroup,
+// scales included: K row by row, V transposed (two keys of a channel next to each other by byte permutes), two buffers and one barrier a tile.
+//   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
+//   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
+//   The weights go into the second product as two bf16 parts, 16 significant bits, and into their sums as they are; a q that the call rotates, or of float16, is
+//   two parts too (TWO).
+// V columns: 16-byte pieces of the 128-byte rows are XOR-ed with a number of the row, which keeps the fragments' 16-byte reads and the 8-byte transposing writes off
+// each other's banks (found by enumeration).
+// ---------------------------------------------------------------------------------------------
+constexpr int kTile4 = 64, kPrompt4Waves = 4;
+constexpr float kSlack4 = 8.f;
+__device__ __forceinline__ int v_piece4(int d) { return ((d >> 2) & 7) ^ (d & 6); }
+
+template <int DT, int DH, int MI, int KG, bool TWO>
+__global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kernel(Kv4AttnArgs a, int ranges, float* scratch) {
+  typedef E16<DT> E;
+  typedef E16<0> P;
+  typedef P::frag_t frag_t;
+  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * kPrompt4Waves, QW = 16 * MI, BM = QW * kPrompt4Waves, HALF = DH / 2;
+  constexpr int KB = DH / 8, VD = DH / 16;               // bytes of a key, channels of four values that a thread stages
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
+  uint16_t* Ks = reinterpret_cast<uint16_t*>(smem) + kg * 2 * kTile4 * (KSTR + DH);      // [2][kTile4][KSTR]
+  uint16_t* Vt = Ks + 2 * kTile4 * KSTR;                                    // [2][DH][kTile4]
+  __shared__ int nan_at[DH / kGroup4];                                      // the first NaN of a group among the values that not every row sees
+  __shared__ int any_nan;
+
+  const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
+  int mt, hb;
+  // the row tiles of a kv head on one XCD, the ones with the most keys first
+  if (HB % 8 == 0) {
+    const int per = HB >> 3, r = blockIdx.x >> 3;
+    mt = r / per;
+    hb = (blockIdx.x & 7) * per + r - mt * per;
+  } else {
+    const int t = xcd_run_index(blockIdx.x, MT * HB);
+    hb = t / MT;
+    mt = t - hb * MT;
+  }
+  mt = MT - 1 - mt;
+  const int hk = hb / a.B, b = hb - hk * a.B, range = blockIdx.y;
+  const int tid = threadIdx.x % TH, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 15, lg = lane >> 4;
+  const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
+  if (row0 >= rows) return;
+  const int pos = min(a.positions[b], 0x7ffffffe - a.M);
+  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
+  const int all_end = seen_by(min(row0 + BM, rows) - 1);
+  const int tiles = (all_end + kTile4 - 1) / kTile4, per = (tiles + ranges - 1) / ranges;
+  const int n_begin = range * per * kTile4, n_end = min(all_end, (range + 1) * per * kTile4);
+  const int w0 = row0 + wave * QW;
+  const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
+
+  frag_t qf[MI][ST], qr[TWO ? MI : 1][ST];                                  // qr: what the first part leaves
+  int seen[MI];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r = min(w0 + 16 * mi + lr, rows - 1), m = r / G, h = hk * G + r - m * G;
+    seen[mi] = seen_by(r);
+    const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
+    u32x4_t x[ST];
+#pragma unroll
+    for (int st = 0; st < ST; ++st) x[st] = eight4(qp + 32 * st + 8 * lg);
+    if constexpr (TWO) {
+      u32x4_t cw[ST / 2], sw[ST / 2];
+      const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lg;
+#pragma unroll
+      for (int st = 0; st < ST / 2; ++st) {
+        cw[st] = a.cos ? eight4(a.cos + tp + 32 * st) : u32x4_t{E::one2, E::one2, E::one2, E::one2};
+        sw[st] = a.cos ? eight4(a.sin + tp + 32 * st) : u32x4_t{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int st = 0; st < ST / 2; ++st) {
+        const u32x4_t none = {0u, 0u, 0u, 0u};
+        u32x4_t h0, r0, h1, r1;
+        query_parts<E>(x[st], a.cos ? x[st + ST / 2] : none, cw[st], sw[st], -1.f, h0, r0);
+        query_parts<E>(x[st + ST / 2], a.cos ? x[st] : none, cw[st], sw[st], 1.f, h1, r1);
+        asm volatile("" : "+v"(r0), "+v"(r1), "+v"(h0), "+v"(h1));         // made here: put off, they spill
+        qf[mi][st] = __builtin_bit_cast(frag_t, h0);
+        qf[mi][st + ST / 2] = __builtin_bit_cast(frag_t, h1);
+        qr[mi][st] = __builtin_bit_cast(frag_t, r0);
+        qr[mi][st + ST / 2] = __builtin_bit_cast(frag_t, r1);
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < ST; ++st) qf[mi][st] = __builtin_bit_cast(frag_t, x[st]);
+    }
+  }
+  const float scale = a.scale * 1.4426950408889634f;
+  float m_run[MI], l_run[MI];                                               // l_run: a lane's own sum of the weights, not rounded
+  f32x4_t o[MI][NT];
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    m_run[mi] = -INFINITY; l_run[mi] = 0.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[mi][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // K: four lanes a row; V: sixteen lanes with VD channels each for four adjacent keys.  The rooms are whole tiles: nothing is clamped.
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* ksp = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const uint8_t* vsp = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const int krow = tid >> 2, kc = tid & 3, vq = tid >> 4, vc = tid & 15;
+  const uint32_t row = (uint32_t)a.c.sc_s;
+  const uint32_t koff = krow * row + KB * kc, voff = 4 * vq * row + VD / 2 * vc;
+  const uint32_t ksoff = 2 * KB * kc / kGroup4 * (uint32_t)a.c.ss_g + krow, vsoff = VD * vc / kGroup4 * (uint32_t)a.c.ss_g + 4 * vq;
+  uint32_t kreg[KB / 4], vreg[4], kbyte, vbyte;
+  const auto request = [&](int n0) {
+    load4<KB, 0>(rows4(kb + (int64_t)n0 * a.c.sc_s), koff, 0, kreg);
+    const Rows4 r = rows4(vb + (int64_t)n0 * a.c.sc_s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(r, voff, e * row, vreg + e);
+    kbyte = ksp[n0 + ksoff];
+    load4<4, 0>(rows4(vsp + n0), vsoff, 0, &vbyte);
+  };
+  const auto stage_k = [&](int buf) {
+    uint16_t* to = Ks + buf * kTile4 * KSTR + krow * KSTR + 2 * KB * kc;
+    const float f = scale_of(kbyte);
+#pragma unroll
+    for (int i = 0; i < KB / 4; ++i)
+      *reinterpret_cast<u32x4_t*>(to + 8 * i) = u32x4_t{pair4<0>(kreg[i], f), pair4<1>(kreg[i], f), pair4<2>(kreg[i], f), pair4<3>(kreg[i], f)};
+  };
+  // A masked key has weight zero, and zero times a NaN is one: where not every row sees the whole tile, a group that is NaN is staged as numbers and put into the
+  // rows that see it at the end; so is what stands behind the last key, whatever its bytes.
+  const int all_see = seen_by(row0);
+  const auto set_nans_aside = [&](int n0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + 4 * vq + e;
+      const bool none = n >= n_end, nan = !none && (vbyte >> (8 * e) & 0xff) == kNanByte;
+      if (nan) {
+        any_nan = 1;
+        atomicMin(&nan_at[VD * vc / kGroup4], n);
+      }
+      if (none || nan) vbyte &= ~(0xffu << (8 * e));
+    }
+  };
+  const auto stage_v = [&](int buf) {
+    const int ko = (4 * vq) & 31, col = ((4 * vq) & 32) + 8 * ((ko & 15) >> 2) + 4 * (ko >> 4);
+    uint16_t* to = Vt + buf * DH * kTile4 + VD * vc * kTile4;
+#pragma unroll
+    for (int c = 0; c < VD / 2; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pair4_at(c, vreg[e], scale_at(vbyte, e));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = 2 * c + i;
+        const uint32_t lohi = i ? 0x07060302u : 0x05040100u;
+        *reinterpret_cast<u32x2_t*>(to + d * kTile4 + (col ^ (8 * v_piece4(VD * vc + d)))) =
+            u32x2_t{__builtin_amdgcn_perm(w[1], w[0], lohi), __builtin_amdgcn_perm(w[3], w[2], lohi)};
+      }
+    }
+  };
+  const auto k_frags = [&](frag_t (&kf)[2][ST], int buf, int half) {       // of 32 of the tile's keys
+    const uint16_t* ks = Ks + buf * kTile4 * KSTR;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) kf[j][st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (32 * half + 16 * j + lr) * KSTR + 32 * st + 8 * lg));
+  };
+  const auto scores = [&](f32x4_t (&s)[MI][4], const frag_t (&kf)[2][ST], int half) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int st = 0; st < ST; ++st)
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi) {
+          s[mi][2 * half + j] = P::mfma(kf[j][st], qf[mi][st], st ? s[mi][2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+          if constexpr (TWO) s[mi][2 * half + j] = P::mfma(kf[j][st], qr[mi][st], s[mi][2 * half + j]);
+        }
+  };
+  // row d = 16 t + lr of V: its piece is turned by (lr / 4) ^ (lr & 6) ^ 4 (t % 2), so two addresses and constants reach all of them
+  const uint32_t vread = lr * kTile4 + 8 * (lg ^ (lr >> 2) ^ (lr & 6));
+  const auto v_frags = [&](frag_t (&vf)[NT], int buf, int st) {
+    const uint16_t* vt = Vt + buf * DH * kTile4;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) vf[t] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(vt + ((st ^ t) & 1 ? vread ^ 32 : vread) + 16 * t * kTile4));
+  };
+  frag_t ph[MI][2], pl[MI][2];
+  const auto values = [&](const frag_t (&vf)[NT], int st) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi) {
+        o[mi][t] = P::mfma(vf[t], ph[mi][st], o[mi][t]);
+        o[mi][t] = P::mfma(vf[t], pl[mi][st], o[mi][t]);
+      }
+  };
+  const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
+  const auto weights = [&](f32x4_t (&s)[MI][4], int n0) {
+    const bool plain = n0 + kTile4 <= wave_sees;                     // every row of the wave sees the whole tile
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      if (!plain) {
+        const int vis = seen[mi] - n0 - 4 * lg;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[mi][j][i] = 16 * j + i < vis ? s[mi][j][i] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[mi][j][0], s[mi][j][1]), fmaxf(s[mi][j][2], s[mi][j][3])));
+      top *= scale;
+      // The reference of the weights moves only where a score is kSlack4 over it: until then weights are up to 2^kSlack4, which changes no rounding, and the
+      // lanes of a column need not agree on a maximum.
+      if (__any(top > m_run[mi] + kSlack4)) {
+        top = fmaxf(m_run[mi], column_max(top));
+        const float keep = top > m_run[mi] ? __builtin_amdgcn_exp2f(m_run[mi] - top) : 1.f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) o[mi][t] *= keep;
+        l_run[mi] *= keep;
+        m_run[mi] = top;
+      }
+      const float base = m_run[mi] == -INFINITY ? 0.f : m_run[mi];  // a row that has seen nothing yet: exp2(-inf - 0)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[mi][j][i] = __builtin_amdgcn_exp2f(fmaf(s[mi][j][i], scale, -base));
+          l_run[mi] += s[mi][j][i];
+        }
+    }
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        uint32_t hw[4], lw[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x0 = s[mi][2 * st + (c >> 1)][2 * (c & 1)], x1 = s[mi][2 * st + (c >> 1)][2 * (c & 1) + 1];
+          hw[c] = pack_bf16x2(x0, x1);
+          lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+        }
+        ph[mi][st] = __builtin_bit_cast(frag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
+        pl[mi][st] = __builtin_bit_cast(frag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+      }
+  };
+
+  const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile4; };
+  const int all = n_begin < n_end ? (n_end - n_begin + kTile4 - 1) / kTile4 : 0, n = (all - kg + KG - 1) / KG;      // of the workgroup, of this half
+  if (n > 0) request(at(0));
+  if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
+  if (tid == 0) any_nan = 0;
+  __syncthreads();
+  for (int i = 0; i * KG < all; ++i) {
+    const int buf = i & 1;
+    if (KG == 1 || i < n) {
+      stage_k(buf);
+      if (at(i) + kTile4 > all_see) set_nans_aside(at(i));
+      stage_v(buf);
+    }
+    if (i + 1 < n) request(at(i + 1));
+    __syncthreads();                   // this buffer is written; the other one is read by nobody any more
+    if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
+    f32x4_t s[MI][4];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      frag_t kf[2][ST];
+      k_frags(kf, buf, half);
+      scores(s, kf, half);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    weights(s, at(i));
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      __builtin_amdgcn_sched_barrier(0);
+      frag_t vf[NT];
+      v_frags(vf, buf, st);
+      values(vf, st);
+    }
+  }
+  if constexpr (KG > 1) {                // the halves' results
+    static_assert(KG == 2 && MI == 1, "one exchange");
+    f32x4_t* part = reinterpret_cast<f32x4_t*>(smem) + wave * (NT + 1) * kWave + lane;
+    __syncthreads();
+    if (kg == 1) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) part[t * kWave] = o[0][t];
+      part[NT * kWave] = f32x4_t{m_run[0], l_run[0], 0.f, 0.f};
+    }
+    __syncthreads();
+    if (kg == 1) return;
+    const f32x4_t other = part[NT * kWave];
+    const float top = fmaxf(m_run[0], other[0]);
+    // a half whose sum is NaN keeps it, whatever its reference
+    const float f0 = m_run[0] > -INFINITY ? __builtin_amdgcn_exp2f(m_run[0] - top) : l_run[0] == 0.f ? 0.f : 1.f;
+    const float f1 = other[0] > -INFINITY ? __builtin_amdgcn_exp2f(other[0] - top) : other[1] == 0.f ? 0.f : 1.f;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[0][t] = o[0][t] * f0 + part[t * kWave] * f1;
+    l_run[0] = l_run[0] * f0 + other[1] * f1;
+    m_run[0] = top;
+  }
+  // element i of tile t is channel 16 t + 4 lg + i of row lr
+  const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
+#pragma unroll
+  for (int mi = 0; mi < MI; ++mi) {
+    const int r = w0 + 16 * mi + lr;
+    const float l = column_sum(l_run[mi]);
+    if (r >= rows) continue;
+    if (any_nan) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        if (nan_at[t / 2] < seen[mi])
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[mi][t][i] = __builtin_nanf("");
+    }
+    if (ranges > 1) {
+      const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+      const int64_t at = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
+      if (lg == 0) *part.stats(at, range) = f32x2_t{l != l ? INFINITY : m_run[mi], l};
+      float* v = part.values(at, range) + 4 * lg;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t*>(v + 16 * t) = o[mi][t];
+      continue;
+    }
+    const int m = r / G, h = hk * G + r - m * G;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + 4 * lg;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const u32x2_t w{E::pack2(o[mi][t][0] * inv, o[mi][t][1] * inv), E::pack2(o[mi][t][2] * inv, o[mi][t][3] * inv)};
+      if (out8) {
+        *reinterpret_cast<u32x2_t*>(op + 16 * t) = w;
+      } else {
+        op[16 * t] = (uint16_t)w.x; op[16 * t + 1] = (uint16_t)(w.x >> 16);
+        op[16 * t + 2] = (uint16_t)w.y; op[16 * t + 3] = (uint16_t)(w.y >> 16);
+      }
+    }
+  }
+}
+
+// Rows of a workgroup, its halves and key ranges.
+struct Prompt4Form { int rows, halves, ranges; };
+static Prompt4Form prompt_form(int B, int M, int H, int Hk, int S) {
+  const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
+  if ((list + 127) / 128 * pairs >= 2 * cu) return {128, 1, 1};
+  const int64_t n = (list + 63) / 64 * pairs;
+  if (n * 2 > 3 * cu) return {64, 1, 1};
+  return {64, 2, (int)max((int64_t)1, min(cu / n, (int64_t)S / ((n * 4 > cu ? 8 : 4) * kTile4)))};
+}
+size_t kv4_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
+  const Prompt4Form f = prompt_form(B, M, H, Hk, S);
+  return f.ranges > 1 ? RangeParts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
+}
+
+template <int DT, int DH, int MI, int KG, bool TWO>
+static int prompt_launch_form(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+  constexpr size_t lds = KG * 2 * ((size_t)kTile4 * (DH + 16) * 2 + (size_t)DH * kTile4 * 2);
+  static std::atomic<uint32_t> granted{0};
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv4_prompt_kernel<DT, DH, MI, KG, TWO>), lds, granted) : kOk) return rc;
+  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * kPrompt4Waves - 1) / (16 * MI * kPrompt4Waves) * a.B * a.c.Hk;
+  if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
+  hipLaunchKernelGGL((kv4_prompt_kernel<DT, DH, MI, KG, TWO>), dim3((unsigned)groups, ranges), dim3(kPrompt4Waves * KG * kWave), lds, st, a, ranges, scratch);
+  if (ranges > 1) launch_join(join_args(a), ranges, false, scratch, st);
+  return kOk;
+}
+template <int DT, int DH, int MI, int KG>
+static int prompt_launch(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
+  if constexpr (DT == 1) return prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st);
+  else return a.cos ? prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, MI, KG, false>(fn, a, ranges, scratch, st);
+}
+template <int DT, int DH>
+static int prompt_launch_rows(const char* fn, const Kv4AttnArgs& a, Prompt4Form f, float* scratch, hipStream_t st) {
+  set_last_form(f.rows == 128 ? "kv4 prompt 128" : f.halves == 1 ? "kv4 prompt 64" : f.ranges == 1 ? "kv4 prompt 64 halves" : "kv4 prompt 64 halves ranges");
+  if (f.rows == 128) return prompt_launch<DT, DH, 2, 1>(fn, a, f.ranges, scratch, st);
+  if (f.halves == 1) return prompt_launch<DT, DH, 1, 1>(fn, a, f.ranges, scratch, st);
+  return prompt_launch<DT, DH, 1, 2>(fn, a, f.ranges, scratch, st);
+}
+int launch_kv4_prompt(const char* fn, const Kv4AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
+  const Prompt4Form f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);
+  const size_t need = kv4_prompt_scratch_bytes(a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.c.S);
+  if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
+    set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, f.ranges, need);
+    return kErrWorkspace;
+  }
+  const int rc = a.dt == 1 ? (a.c.Dh == 128 ? prompt_launch_rows<1, 128>(fn, a, f, scratch, st) : prompt_launch_rows<1, 64>(fn, a, f, scratch, st))
+                           : (a.c.Dh == 128 ? prompt_launch_rows<0, 128>(fn, a, f, scratch, st) : prompt_launch_rows<0, 64>(fn, a, f, scratch, st));
+  if (rc != kOk) return rc;
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
   return kOk;
