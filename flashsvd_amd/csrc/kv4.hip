@@ -3,48 +3,65 @@
 
 namespace fsvd {
 
-// A workgroup has 256 / (Dh / 16) rows of the keys or the values of one kv head.
-template <int DT, int DH>
+// A workgroup has 256 / (Dh / 16) rows of the keys or the values of HEADS kv heads, which share the rows of the rotation tables and have all their loads in
+// flight.  Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (339 MB) take 68 to 74 us, up to 5.0 TB/s, where a copy
+// reaches 5.4; rows that come rotated 60.
+template <int DT, int DH, int HEADS>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
-  constexpr int HALF = DH / 2, LPR = DH / 16;
-  const int value = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, part = threadIdx.x % LPR, t = (int)blockIdx.y * (256 / LPR) + threadIdx.x / LPR;
+  constexpr int HALF = DH / 2, LPR = DH / 16, PER = 256 / LPR;
+  const int value = blockIdx.x & 1, h0 = (blockIdx.x >> 1) * HEADS, b = blockIdx.z, part = threadIdx.x % LPR, t = (int)blockIdx.y * PER + threadIdx.x / LPR;
   const int rows = a.rows ? min(a.rows[b], a.T) : a.T;
-  const int64_t pos = (int64_t)a.positions[b] + t;
-  const bool in = t < rows && pos >= 0 && pos < a.c.S;
-  const int64_t r = in ? t : 0;
-  const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h + r * a.sv_t : a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h + r * a.sk_t) + 8 * part;
-  const u32x4_t lo = eight4(x), hi = eight4(x + HALF);
-  const bool turn = !value && a.cos != nullptr;
-  u32x4_t cw = {0u, 0u, 0u, 0u}, sw = cw;
+  const int64_t pos = (int64_t)a.positions[b] + t, sh = value ? a.sv_h : a.sk_h;
+  const bool in = t < rows && pos >= 0 && pos < a.c.S, turn = !value && a.cos != nullptr;
+  const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (in ? t : 0) * a.sv_t : a.k + (int64_t)b * a.sk_b + (in ? t : 0) * a.sk_t) + h0 * sh + 8 * part;
+  u32x4_t lo[HEADS], hi[HEADS], cw = {0u, 0u, 0u, 0u}, sw = cw;
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) { lo[i] = eight4(x + i * sh); hi[i] = eight4(x + i * sh + HALF); }
   if (turn) {
     const int64_t tp = min(max(pos, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + 8 * part;
     cw = eight4(a.cos + tp); sw = eight4(a.sin + tp);
   }
-  float y[2][8];
-  row_numbers<E16<DT>>(lo, hi, turn, cw, sw, y);
-  put_row<DH>(y, static_cast<uint8_t*>(value ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s,
-              static_cast<uint8_t*>(value ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos, a.c.ss_g, part, in);
+  uint8_t* codes = static_cast<uint8_t*>(value ? a.c.v : a.c.k) + b * a.c.sc_b + h0 * a.c.sc_h + pos * a.c.sc_s;
+  uint8_t* scales = static_cast<uint8_t*>(value ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + h0 * a.c.ss_h + pos;
+#pragma unroll
+  for (int i = 0; i < HEADS; ++i) {
+    float y[2][8];
+    row_numbers<E16<DT>>(lo[i], hi[i], turn, cw, sw, y);
+    put_row<DH>(y, codes + i * a.c.sc_h, scales + i * a.c.ss_h, a.c.ss_g, part, in);
+  }
+}
+// One row for each sequence: a wave for a kv head.  Nothing but latency.
+template <int DT, int DH>
+__global__ __launch_bounds__(kWave) void kv4_append_one_kernel(Kv4AppendArgs a) {
+  const int b = blockIdx.x / a.c.Hk, hk = blockIdx.x % a.c.Hk, pos = a.positions[b];
+  if (pos < 0 || pos >= a.c.S || (a.rows && a.rows[b] <= 0)) return;
+  append_row4<DT, DH>(a.c, a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin, a.rope_len, b, hk, pos,
+                      threadIdx.x);
+}
+template <int DT, int DH>
+static void append_form(const Kv4AppendArgs& a, hipStream_t st) {
+  constexpr int rows = 256 / (DH / 16);
+    // us with one head / with four, rows of 32 heads of 128: 1 x 128 4.1 / 6.3, 1 x 2048 12.8 / 15.0, 2 x 2048 20.6 / 22.0, 4 x 2048 40.6 / 38.5, 8 x 2048 76.1 / 67.7
+  const int64_t tiles = (a.T + rows - 1) / rows;
+  const bool four = a.c.Hk % 4 == 0 && 2 * a.c.Hk * tiles * a.B >= 16384;
+  set_last_form(a.T == 1 ? "kv4 row" : four ? "kv4 rows of 4 heads" : "kv4 rows");
+  if (a.T == 1) hipLaunchKernelGGL((kv4_append_one_kernel<DT, DH>), dim3((unsigned)(a.B * a.c.Hk)), dim3(kWave), 0, st, a);
+  else if (four) hipLaunchKernelGGL((kv4_append_kernel<DT, DH, 4>), dim3(2 * a.c.Hk / 4, (unsigned)tiles, a.B), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((kv4_append_kernel<DT, DH, 1>), dim3(2 * a.c.Hk, (unsigned)tiles, a.B), dim3(256), 0, st, a);
 }
 
 int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st) {
   if (a.T == 0) return kOk;
   if ((int64_t)a.B * a.c.Hk > 0x7fffffff || a.T > (1 << 20)) { set_last_error("%s: %d rows of %d heads for %d sequences", fn, a.T, a.c.Hk, a.B); return kErrBadShape; }
-  const int per = 256 / (a.c.Dh / 16);
-  const dim3 grid(2 * a.c.Hk, (a.T + per - 1) / per, a.B);
-  if (a.dt == 1) {
-    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_append_kernel<1, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv4_append_kernel<1, 64>), grid, dim3(256), 0, st, a);
-  } else {
-    if (a.c.Dh == 128) hipLaunchKernelGGL((kv4_append_kernel<0, 128>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((kv4_append_kernel<0, 64>), grid, dim3(256), 0, st, a);
-  }
-  set_last_form("kv4 rows");
+  if (a.dt == 1) a.c.Dh == 128 ? append_form<1, 128>(a, st) : append_form<1, 64>(a, st);
+  else a.c.Dh == 128 ? append_form<0, 128>(a, st) : append_form<0, 64>(a, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) { set_last_error("%s: launch failed: %s", fn, hipGetErrorString(e)); return kErrLaunch; }
   return kOk;
 }
 
-// What the first L rows hold, [B, L, Hk, Dh] each: a thread has 16 bytes of codes, the 32 channels of one scale.
+// What the first L rows hold, [B, L, Hk, Dh] each: a thread has eight channels of four rows, whose scales are four bytes next to each other.  8 x 2048 rows of 32 heads
+// of 128 (339 MB) take 64 us, 5.3 TB/s, a copy's rate.
 struct Kv4ReadArgs {
   fsvd_kv4_cache c;
   uint16_t* k; uint16_t* v;
@@ -54,20 +71,28 @@ struct Kv4ReadArgs {
 template <int DT, int DH>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   typedef E16<DT> E;
-  constexpr int GROUPS = DH / kGroup4;
-  const int part = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, g = threadIdx.x % GROUPS;
-  const int64_t pos = (int64_t)blockIdx.y * (256 / GROUPS) + threadIdx.x / GROUPS;
+  constexpr int LPR = DH / 8;
+  const int value = blockIdx.x & 1, hk = blockIdx.x >> 1, b = blockIdx.z, part = threadIdx.x % LPR;
+  const int64_t pos = 4 * ((int64_t)blockIdx.y * (256 / LPR) + threadIdx.x / LPR);
   if (pos >= a.L) return;
-  const uint8_t* codes = static_cast<const uint8_t*>(part ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s + 16 * g;
-  const uint32_t byte = (static_cast<const uint8_t*>(part ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + pos)[g * a.c.ss_g];
-  uint16_t* out = (part ? a.v : a.k) + b * a.so_b + pos * a.so_t + hk * a.so_h + kGroup4 * g;
-  const u32x4_t w = *reinterpret_cast<const u32x4_t*>(codes);
-  const float scale = scale_of(byte);
+  const uint8_t* codes = static_cast<const uint8_t*>(value ? a.c.v : a.c.k) + b * a.c.sc_b + hk * a.c.sc_h + pos * a.c.sc_s + 4 * part;
+  const uint8_t* scales = static_cast<const uint8_t*>(value ? a.c.v_scale : a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h + part / 4 * a.c.ss_g + pos;
+  uint16_t* out = (value ? a.v : a.k) + b * a.so_b + pos * a.so_t + hk * a.so_h + 8 * part;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint32_t*>(codes + i * a.c.sc_s);       // rooms are multiples of four rows
+  const uint32_t four = *reinterpret_cast<const uint32_t*>(scales);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const f32x2_t x[4] = {pair4_f32<0>(w[i], scale), pair4_f32<1>(w[i], scale), pair4_f32<2>(w[i], scale), pair4_f32<3>(w[i], scale)};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[8 * i + e] = (uint16_t)E::bits(byte == kNanByte ? __builtin_nanf("") : x[e >> 1][e & 1]);
+    const float f = scale_at(four, i);
+    u32x4_t x;
+    if constexpr (DT == 0) {
+      x = u32x4_t{pair4<0>(w[i], f), pair4<1>(w[i], f), pair4<2>(w[i], f), pair4<3>(w[i], f)};
+    } else {
+      const f32x2_t y[4] = {pair4_f32<0>(w[i], f), pair4_f32<1>(w[i], f), pair4_f32<2>(w[i], f), pair4_f32<3>(w[i], f)};
+      x = u32x4_t{E::pack2(y[0][0], y[0][1]), E::pack2(y[1][0], y[1][1]), E::pack2(y[2][0], y[2][1]), E::pack2(y[3][0], y[3][1])};
+    }
+    if (pos + i < a.L) *reinterpret_cast<u32x4_any_t*>(out + i * a.so_t) = __builtin_bit_cast(u32x4_any_t, x);
   }
 }
 
@@ -137,7 +162,7 @@ int fsvd_kv4_dequantize(const fsvd_kv4_cache* cache, void* k, void* v, int64_t s
   if (k == nullptr || v == nullptr) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (const int rc = check_out(fn, B, L, cache->Hk, so_b, so_t, so_h)) return rc;
   const Kv4ReadArgs a{*cache, static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), so_b, so_t, so_h, L};
-  const int per = 256 / (cache->Dh / kGroup4);
+  const int per = 4 * 256 / (cache->Dh / 8);
   const dim3 grid(2 * cache->Hk, (L + per - 1) / per, B);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == 1) {
