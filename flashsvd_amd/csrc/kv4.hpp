@@ -122,8 +122,10 @@ __device__ __forceinline__ void load4(Rows4 r, uint32_t lane, uint32_t off, uint
     w[0] = v.x; w[1] = v.y;
   } else if constexpr (BYTES == 4) {
     w[0] = __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane, (int)off, AUX);
-  } else {
+  } else if constexpr (BYTES == 2) {
     w[0] = __builtin_amdgcn_raw_buffer_load_b16(r, (int)lane, (int)off, AUX);
+  } else {
+    w[0] = __builtin_amdgcn_raw_buffer_load_b8(r, (int)lane, (int)off, AUX);
   }
 }
 #else

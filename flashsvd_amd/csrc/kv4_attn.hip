@@ -627,6 +627,251 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
   }
 }
 
+// ---------------------------------------------------------------------------------------------
+// The same for long chunks: 128 rows of a workgroup, 32 of a wave, in products of 32 x 32 x 16.  These hold up the vector unit for 14 cycles of their 38, those of
+// 16 x 16 x 32 for 12 of 19 (a loop of both kinds of work with two waves a SIMD; an exponential takes 9 cycles, a conversion of two codes 4.5), and the vector unit is
+// what this path needs most.
+//   S^T = K Q^T leaves lane (n, h) = (lane % 32, lane / 32) keys 8 b + 4 h + j of a 32-key block of query n; O^T = V^T P^T takes keys 16 u + 4 h + j and 16 u + 8 + 4 h + j
+//   of it in product u, and the V columns stand in that order.
+// K rows are an odd number of 16-byte pieces long and V's pieces XOR-ed with a number of the channel, so that 16 lanes read 16 different pieces of 256 bytes.
+// ---------------------------------------------------------------------------------------------
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ int wide_piece(int c) { return ((c >> 1) ^ (c >> 4)) & 7; }
+
+template <int DT, int DH, bool TWO>
+__global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4AttnArgs a) {
+  typedef E16<DT> E;
+  typedef E16<0> P;
+  typedef P::frag_t frag_t;
+  constexpr int SQ = DH / 16, NB = DH / 32, KSTR = DH + 8, BM = 32 * kPrompt4Waves, HALF = DH / 2;      // products of a key block; output blocks
+  constexpr int KB = DH / 8, VD = DH / 16;               // bytes of a key, channels of four values that a thread stages
+  extern __shared__ __align__(16) unsigned char smem[];
+  uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile4][KSTR]
+  uint16_t* Vt = Ks + 2 * kTile4 * KSTR;                                    // [2][DH][kTile4]
+  __shared__ int nan_at[DH / kGroup4];                                      // the first NaN of a group among the values that not every row sees
+  __shared__ int any_nan;
+
+  const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
+  int mt, hb;
+  // the row tiles of a kv head on one XCD, the ones with the most keys first
+  if (HB % 8 == 0) {
+    const int per = HB >> 3, r = blockIdx.x >> 3;
+    mt = r / per;
+    hb = (blockIdx.x & 7) * per + r - mt * per;
+  } else {
+    const int t = xcd_run_index(blockIdx.x, MT * HB);
+    hb = t / MT;
+    mt = t - hb * MT;
+  }
+  mt = MT - 1 - mt;
+  const int hk = hb / a.B, b = hb - hk * a.B;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
+  const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
+  if (row0 >= rows) return;
+  const int pos = min(a.positions[b], 0x7ffffffe - a.M);
+  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
+  const int n_end = seen_by(min(row0 + BM, rows) - 1);
+  const int w0 = row0 + wave * 32;
+  const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + 32, rows) - 1)) : 0;             // keys past it are unseen by the wave
+  const int r = min(w0 + lr, rows - 1), m = r / G, head = hk * G + r - m * G, seen = seen_by(r);
+
+  frag_t qf[SQ], qr[TWO ? SQ : 1];                                          // qr: what the first part leaves
+  {
+    const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)head * a.sq_h + 8 * lh;
+    u32x4_t x[SQ];
+#pragma unroll
+    for (int st = 0; st < SQ; ++st) x[st] = eight4(qp + 16 * st);
+    if constexpr (TWO) {
+      const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lh;
+#pragma unroll
+      for (int st = 0; st < SQ / 2; ++st) {
+        const u32x4_t none = {0u, 0u, 0u, 0u}, cw = a.cos ? eight4(a.cos + tp + 16 * st) : u32x4_t{E::one2, E::one2, E::one2, E::one2};
+        const u32x4_t sw = a.cos ? eight4(a.sin + tp + 16 * st) : none;
+        u32x4_t h0, r0, h1, r1;
+        query_parts<E>(x[st], a.cos ? x[st + SQ / 2] : none, cw, sw, -1.f, h0, r0);
+        query_parts<E>(x[st + SQ / 2], a.cos ? x[st] : none, cw, sw, 1.f, h1, r1);
+        asm volatile("" : "+v"(r0), "+v"(r1), "+v"(h0), "+v"(h1));         // made here: put off, they spill
+        qf[st] = __builtin_bit_cast(frag_t, h0);
+        qf[st + SQ / 2] = __builtin_bit_cast(frag_t, h1);
+        qr[st] = __builtin_bit_cast(frag_t, r0);
+        qr[st + SQ / 2] = __builtin_bit_cast(frag_t, r1);
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < SQ; ++st) qf[st] = __builtin_bit_cast(frag_t, x[st]);
+    }
+  }
+  const float scale = a.scale * 1.4426950408889634f;
+  float m_run = -INFINITY, l_run = 0.f;                                     // l_run: a lane's own sum of the weights, not rounded
+  f32x16_t o[NB];
+#pragma unroll
+  for (int t = 0; t < NB; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[t][i] = 0.f;
+
+  // K: four lanes a row; V: sixteen lanes with VD channels each for four adjacent keys.  The rooms are whole tiles: nothing is clamped.
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* ksp = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const uint8_t* vsp = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const int krow = tid >> 2, kc = tid & 3, vq = tid >> 4, vc = tid & 15;
+  const uint32_t row = (uint32_t)a.c.sc_s;
+  const uint32_t koff = krow * row + KB * kc, voff = 4 * vq * row + VD / 2 * vc;
+  const uint32_t ksoff = 2 * KB * kc / kGroup4 * (uint32_t)a.c.ss_g + krow, vsoff = VD * vc / kGroup4 * (uint32_t)a.c.ss_g + 4 * vq;
+  uint32_t kreg[KB / 4], vreg[4], kbyte, vbyte;
+  const auto request = [&](int n0) {
+    load4<KB, 0>(rows4(kb + (int64_t)n0 * a.c.sc_s), koff, 0, kreg);
+    load4<1, 0>(rows4(ksp + n0), ksoff, 0, &kbyte);
+    const Rows4 v = rows4(vb + (int64_t)n0 * a.c.sc_s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(v, voff, e * row, vreg + e);
+    load4<4, 0>(rows4(vsp + n0), vsoff, 0, &vbyte);
+  };
+  const auto stage_k = [&](int buf) {
+    uint16_t* to = Ks + buf * kTile4 * KSTR + krow * KSTR + 2 * KB * kc;
+    const float f = scale_of(kbyte);
+#pragma unroll
+    for (int i = 0; i < KB / 4; ++i)
+      *reinterpret_cast<u32x4_t*>(to + 8 * i) = u32x4_t{pair4<0>(kreg[i], f), pair4<1>(kreg[i], f), pair4<2>(kreg[i], f), pair4<3>(kreg[i], f)};
+  };
+  // a masked key has weight zero, and zero times a NaN is one: see kv4_prompt_kernel
+  const int all_see = seen_by(row0);
+  const auto set_nans_aside = [&](int n0) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n0 + 4 * vq + e;
+      const bool none = n >= n_end, nan = !none && (vbyte >> (8 * e) & 0xff) == kNanByte;
+      if (nan) {
+        any_nan = 1;
+        atomicMin(&nan_at[VD * vc / kGroup4], n);
+      }
+      if (none || nan) vbyte &= ~(0xffu << (8 * e));
+    }
+  };
+  const auto stage_v = [&](int buf) {
+    const int piece = 2 * (vq >> 2) + (vq & 1), half = vq >> 1 & 1;
+    uint16_t* to = Vt + buf * DH * kTile4 + VD * vc * kTile4 + 4 * half;
+#pragma unroll
+    for (int c = 0; c < VD / 2; ++c) {
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = pair4_at(c, vreg[e], scale_at(vbyte, e));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int d = 2 * c + i;
+        const uint32_t sel = i ? 0x07060302u : 0x05040100u;
+        *reinterpret_cast<u32x2_t*>(to + d * kTile4 + 8 * (piece ^ wide_piece(VD * vc + d))) =
+            u32x2_t{__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel)};
+      }
+    }
+  };
+  const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
+  const int tiles = (n_end + kTile4 - 1) / kTile4;
+  if (tiles > 0) request(0);
+  if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
+  if (tid == 0) any_nan = 0;
+  __syncthreads();
+  const uint16_t* kread = Ks + lr * KSTR + 8 * lh;
+  for (int i = 0; i < tiles; ++i) {
+    const int buf = i & 1, n0 = i * kTile4;
+    stage_k(buf);
+    if (n0 + kTile4 > all_see) set_nans_aside(n0);
+    stage_v(buf);
+    if (i + 1 < tiles) request(n0 + kTile4);
+    __syncthreads();                     // this buffer is written; the other one is read by nobody any more
+    if (n0 >= wave_end) continue;
+    f32x16_t s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int st = 0; st < SQ; ++st) {
+        const frag_t kf = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(kread + buf * kTile4 * KSTR + 32 * k * KSTR + 16 * st));
+        if (st == 0) s[k] = f32x16_t{};
+        s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[st], s[k], 0, 0, 0);
+        if constexpr (TWO) s[k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qr[st], s[k], 0, 0, 0);
+      }
+    if (n0 + kTile4 > wave_sees) {       // not every row of the wave sees the whole tile
+      const int vis = seen - n0 - 4 * lh;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[k][e] = 32 * k + 8 * (e >> 2) + (e & 3) < vis ? s[k][e] : -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[k][e], s[k][e + 1]));
+    top *= scale;
+    // the reference of the weights moves only where a score is kSlack4 over it: until then weights are up to 2^kSlack4, which changes no rounding
+    if (__any(top > m_run + kSlack4)) {
+      const uint32_t u = __float_as_uint(top);
+      const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      top = fmaxf(m_run, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+      const float keep = top > m_run ? __builtin_amdgcn_exp2f(m_run - top) : 1.f;
+#pragma unroll
+      for (int t = 0; t < NB; ++t) o[t] *= keep;
+      l_run *= keep;
+      m_run = top;
+    }
+    const float base = m_run == -INFINITY ? 0.f : m_run;            // a row that has seen nothing yet: exp2(-inf - 0)
+    frag_t ph[4], pl[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      uint32_t hw[4], lw[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float x0 = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + 2 * c], scale, -base));
+        const float x1 = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + 2 * c + 1], scale, -base));
+        l_run += x0 + x1;
+        hw[c] = pack_bf16x2(x0, x1);
+        lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+      }
+      ph[u] = __builtin_bit_cast(frag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
+      pl[u] = __builtin_bit_cast(frag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int t = 0; t < NB; ++t) {
+        const int c = 32 * t + lr;
+        const frag_t vf = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(Vt + buf * DH * kTile4 + c * kTile4 + 8 * ((2 * u + lh) ^ wide_piece(c))));
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, ph[u], o[t], 0, 0, 0);
+        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pl[u], o[t], 0, 0, 0);
+      }
+  }
+  // element i of block t is channel 32 t + 8 (i / 4) + 4 lh + i % 4 of row lr
+  const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
+  {
+    const uint32_t u = __float_as_uint(l_run);
+    const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    l_run = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+  if (w0 + lr >= rows) return;
+  if (any_nan) {
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+      if (nan_at[t] < seen)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[t][i] = __builtin_nanf("");
+  }
+  const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+  uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)head * a.so_h + 4 * lh;
+#pragma unroll
+  for (int t = 0; t < NB; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const u32x2_t w{E::pack2(o[t][i] * inv, o[t][i + 1] * inv), E::pack2(o[t][i + 2] * inv, o[t][i + 3] * inv)};
+      uint16_t* to = op + 32 * t + 2 * i;
+      if (out8) {
+        *reinterpret_cast<u32x2_t*>(to) = w;
+      } else {
+        to[0] = (uint16_t)w.x; to[1] = (uint16_t)(w.x >> 16);
+        to[2] = (uint16_t)w.y; to[3] = (uint16_t)(w.y >> 16);
+      }
+    }
+}
+
 // Rows of a workgroup, its halves and key ranges.
 struct Prompt4Form { int rows, halves, ranges; };
 static Prompt4Form prompt_form(int B, int M, int H, int Hk, int S) {
@@ -657,10 +902,23 @@ static int prompt_launch(const char* fn, const Kv4AttnArgs& a, int ranges, float
   if constexpr (DT == 1) return prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st);
   else return a.cos ? prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, MI, KG, false>(fn, a, ranges, scratch, st);
 }
+template <int DT, int DH, bool TWO>
+static int wide_launch(const char* fn, const Kv4AttnArgs& a, hipStream_t st) {
+  constexpr size_t lds = 2 * ((size_t)kTile4 * (DH + 8) * 2 + (size_t)DH * kTile4 * 2);
+  static std::atomic<uint32_t> granted{0};
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv4_wide_kernel<DT, DH, TWO>), lds, granted) : kOk) return rc;
+  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 32 * kPrompt4Waves - 1) / (32 * kPrompt4Waves) * a.B * a.c.Hk;
+  if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
+  hipLaunchKernelGGL((kv4_wide_kernel<DT, DH, TWO>), dim3((unsigned)groups), dim3(kPrompt4Waves * kWave), lds, st, a);
+  return kOk;
+}
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv4AttnArgs& a, Prompt4Form f, float* scratch, hipStream_t st) {
   set_last_form(f.rows == 128 ? "kv4 prompt 128" : f.halves == 1 ? "kv4 prompt 64" : f.ranges == 1 ? "kv4 prompt 64 halves" : "kv4 prompt 64 halves ranges");
-  if (f.rows == 128) return prompt_launch<DT, DH, 2, 1>(fn, a, f.ranges, scratch, st);
+  if (f.rows == 128) {
+    if constexpr (DT == 1) return wide_launch<DT, DH, true>(fn, a, st);
+    else return a.cos ? wide_launch<DT, DH, true>(fn, a, st) : wide_launch<DT, DH, false>(fn, a, st);
+  }
   if (f.halves == 1) return prompt_launch<DT, DH, 1, 1>(fn, a, f.ranges, scratch, st);
   return prompt_launch<DT, DH, 1, 2>(fn, a, f.ranges, scratch, st);
 }
