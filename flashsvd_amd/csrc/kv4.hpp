@@ -40,6 +40,13 @@ __device__ __forceinline__ f32x2_t pair4_f32(uint32_t w, float scale) { return _
 
 // the same with the position known after unrolling only
 __device__ __forceinline__ uint32_t pair4_at(int at, uint32_t w, float scale) { return at == 0 ? pair4<0>(w, scale) : at == 1 ? pair4<1>(w, scale) : at == 2 ? pair4<2>(w, scale) : pair4<3>(w, scale); }
+// two elements of float16, rounded where it does not hold them
+__device__ __forceinline__ uint32_t pair4_half_at(int at, uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, at == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0)
+                                      : at == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1)
+                                      : at == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2)
+                                                : __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3));
+}
 // Byte i of four scales as a scale: the conversions read the exponent alone, so what stands around it may stay.  Byte 255 makes NaN of every code.
 __device__ __forceinline__ float scale_at(uint32_t four, int i) { return __uint_as_float(i == 0 ? four << 23 : i == 1 ? four << 15 : i == 2 ? four << 7 : four >> 1); }
 

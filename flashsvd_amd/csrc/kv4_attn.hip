@@ -1,4 +1,6 @@
 // Attention over the KV cache in 4 bits.
+#include <type_traits>
+
 #include "attn_join.hpp"
 #include "kv4.hpp"
 
@@ -294,7 +296,7 @@ int launch_kv4_decode(const char* fn, const Kv4AttnArgs& args, int ranges, float
 
 // ---------------------------------------------------------------------------------------------
 // A chunk of a prompt.  The query rows of the heads that share a kv head are one list, row r = query token r / G of head r % G, so that grouped heads share
-// the tiles of keys too.  A workgroup of four waves takes 16 MI rows for each; tiles of 64 keys go through LDS as bf16, converted once for the workgroup,
+// the tiles of keys too.  A workgroup of four waves takes 16 rows for each; tiles of 64 keys go through LDS as bf16, converted once for the workgroup,
 // scales included: K row by row, V transposed (two keys of a channel next to each other by byte permutes), two buffers and one barrier a tile.
 //   S^T = K Q^T leaves a lane four consecutive keys of one query in every 16-key block, O^T = V^T P^T takes them as they stand (the V columns of 32 keys
 //   follow the order 16 (e / 4) + 4 g + e % 4 of the products' k axis).
@@ -307,12 +309,12 @@ constexpr int kTile4 = 64, kPrompt4Waves = 4;
 constexpr float kSlack4 = 8.f;
 __device__ __forceinline__ int v_piece4(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 
-template <int DT, int DH, int MI, int KG, bool TWO>
+template <int DT, int DH, int KG, bool TWO>
 __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kernel(Kv4AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef E16<0> P;
   typedef P::frag_t frag_t;
-  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * kPrompt4Waves, QW = 16 * MI, BM = QW * kPrompt4Waves, HALF = DH / 2;
+  constexpr int ST = DH / 32, NT = DH / 16, KSTR = DH + 16, TH = kWave * kPrompt4Waves, QW = 16, BM = QW * kPrompt4Waves, HALF = DH / 2;
   constexpr int KB = DH / 8, VD = DH / 16;               // bytes of a key, channels of four values that a thread stages
   extern __shared__ __align__(16) unsigned char smem[];
   const int kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / TH) : 0;
@@ -346,50 +348,41 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
   const int w0 = row0 + wave * QW;
   const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
 
-  frag_t qf[MI][ST], qr[TWO ? MI : 1][ST];                                  // qr: what the first part leaves
-  int seen[MI];
+  frag_t qf[ST], qr[ST];                                  // qr: what the first part leaves
+  const int r = min(w0 + lr, rows - 1), m = r / G, h = hk * G + r - m * G, seen = seen_by(r);
+  const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
+  u32x4_t x[ST];
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    const int r = min(w0 + 16 * mi + lr, rows - 1), m = r / G, h = hk * G + r - m * G;
-    seen[mi] = seen_by(r);
-    const uint16_t* qp = a.q + (int64_t)b * a.sq_b + (int64_t)m * a.sq_m + (int64_t)h * a.sq_h;
-    u32x4_t x[ST];
+  for (int st = 0; st < ST; ++st) x[st] = eight4(qp + 32 * st + 8 * lg);
+  if constexpr (TWO) {
+    u32x4_t cw[ST / 2], sw[ST / 2];
+    const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lg;
 #pragma unroll
-    for (int st = 0; st < ST; ++st) x[st] = eight4(qp + 32 * st + 8 * lg);
-    if constexpr (TWO) {
-      u32x4_t cw[ST / 2], sw[ST / 2];
-      const int64_t tp = (int64_t)min(max(pos + m, 0), a.rope_len - 1) * HALF + 8 * lg;
-#pragma unroll
-      for (int st = 0; st < ST / 2; ++st) {
-        cw[st] = a.cos ? eight4(a.cos + tp + 32 * st) : u32x4_t{E::one2, E::one2, E::one2, E::one2};
-        sw[st] = a.cos ? eight4(a.sin + tp + 32 * st) : u32x4_t{0u, 0u, 0u, 0u};
-      }
-#pragma unroll
-      for (int st = 0; st < ST / 2; ++st) {
-        const u32x4_t none = {0u, 0u, 0u, 0u};
-        u32x4_t h0, r0, h1, r1;
-        query_parts<E>(x[st], a.cos ? x[st + ST / 2] : none, cw[st], sw[st], -1.f, h0, r0);
-        query_parts<E>(x[st + ST / 2], a.cos ? x[st] : none, cw[st], sw[st], 1.f, h1, r1);
-        asm volatile("" : "+v"(r0), "+v"(r1), "+v"(h0), "+v"(h1));         // made here: put off, they spill
-        qf[mi][st] = __builtin_bit_cast(frag_t, h0);
-        qf[mi][st + ST / 2] = __builtin_bit_cast(frag_t, h1);
-        qr[mi][st] = __builtin_bit_cast(frag_t, r0);
-        qr[mi][st + ST / 2] = __builtin_bit_cast(frag_t, r1);
-      }
-    } else {
-#pragma unroll
-      for (int st = 0; st < ST; ++st) qf[mi][st] = __builtin_bit_cast(frag_t, x[st]);
+    for (int st = 0; st < ST / 2; ++st) {
+      cw[st] = a.cos ? eight4(a.cos + tp + 32 * st) : u32x4_t{E::one2, E::one2, E::one2, E::one2};
+      sw[st] = a.cos ? eight4(a.sin + tp + 32 * st) : u32x4_t{0u, 0u, 0u, 0u};
     }
+#pragma unroll
+    for (int st = 0; st < ST / 2; ++st) {
+      const u32x4_t none = {0u, 0u, 0u, 0u};
+      u32x4_t h0, r0, h1, r1;
+      query_parts<E>(x[st], a.cos ? x[st + ST / 2] : none, cw[st], sw[st], -1.f, h0, r0);
+      query_parts<E>(x[st + ST / 2], a.cos ? x[st] : none, cw[st], sw[st], 1.f, h1, r1);
+      asm volatile("" : "+v"(r0), "+v"(r1), "+v"(h0), "+v"(h1));         // made here: put off, they spill
+      qf[st] = __builtin_bit_cast(frag_t, h0);
+      qf[st + ST / 2] = __builtin_bit_cast(frag_t, h1);
+      qr[st] = __builtin_bit_cast(frag_t, r0);
+      qr[st + ST / 2] = __builtin_bit_cast(frag_t, r1);
+    }
+  } else {
+#pragma unroll
+    for (int st = 0; st < ST; ++st) qf[st] = __builtin_bit_cast(frag_t, x[st]);
   }
   const float scale = a.scale * 1.4426950408889634f;
-  float m_run[MI], l_run[MI];                                               // l_run: a lane's own sum of the weights, not rounded
-  f32x4_t o[MI][NT];
+  float m_run = -INFINITY, l_run = 0.f;                                     // l_run: a lane's own sum of the weights, not rounded
+  f32x4_t o[NT];
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    m_run[mi] = -INFINITY; l_run[mi] = 0.f;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) o[mi][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   // K: four lanes a row; V: sixteen lanes with VD channels each for four adjacent keys.  The rooms are whole tiles: nothing is clamped.
   const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
@@ -403,9 +396,9 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
   uint32_t kreg[KB / 4], vreg[4], kbyte, vbyte;
   const auto request = [&](int n0) {
     load4<KB, 0>(rows4(kb + (int64_t)n0 * a.c.sc_s), koff, 0, kreg);
-    const Rows4 r = rows4(vb + (int64_t)n0 * a.c.sc_s);
+    const Rows4 v = rows4(vb + (int64_t)n0 * a.c.sc_s);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(r, voff, e * row, vreg + e);
+    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(v, voff, e * row, vreg + e);
     kbyte = ksp[n0 + ksoff];
     load4<4, 0>(rows4(vsp + n0), vsoff, 0, &vbyte);
   };
@@ -455,16 +448,14 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 #pragma unroll
       for (int st = 0; st < ST; ++st) kf[j][st] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(ks + (32 * half + 16 * j + lr) * KSTR + 32 * st + 8 * lg));
   };
-  const auto scores = [&](f32x4_t (&s)[MI][4], const frag_t (&kf)[2][ST], int half) {
+  const auto scores = [&](f32x4_t (&s)[4], const frag_t (&kf)[2][ST], int half) {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int st = 0; st < ST; ++st)
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-          s[mi][2 * half + j] = P::mfma(kf[j][st], qf[mi][st], st ? s[mi][2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
-          if constexpr (TWO) s[mi][2 * half + j] = P::mfma(kf[j][st], qr[mi][st], s[mi][2 * half + j]);
-        }
+      for (int st = 0; st < ST; ++st) {
+        s[2 * half + j] = P::mfma(kf[j][st], qf[st], st ? s[2 * half + j] : f32x4_t{0.f, 0.f, 0.f, 0.f});
+        if constexpr (TWO) s[2 * half + j] = P::mfma(kf[j][st], qr[st], s[2 * half + j]);
+      }
   };
   // row d = 16 t + lr of V: its piece is turned by (lr / 4) ^ (lr & 6) ^ 4 (t % 2), so two addresses and constants reach all of them
   const uint32_t vread = lr * kTile4 + 8 * (lg ^ (lr >> 2) ^ (lr & 6));
@@ -473,65 +464,58 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 #pragma unroll
     for (int t = 0; t < NT; ++t) vf[t] = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(vt + ((st ^ t) & 1 ? vread ^ 32 : vread) + 16 * t * kTile4));
   };
-  frag_t ph[MI][2], pl[MI][2];
+  frag_t ph[2], pl[2];
   const auto values = [&](const frag_t (&vf)[NT], int st) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int mi = 0; mi < MI; ++mi) {
-        o[mi][t] = P::mfma(vf[t], ph[mi][st], o[mi][t]);
-        o[mi][t] = P::mfma(vf[t], pl[mi][st], o[mi][t]);
-      }
+    for (int t = 0; t < NT; ++t) {
+      o[t] = P::mfma(vf[t], ph[st], o[t]);
+      o[t] = P::mfma(vf[t], pl[st], o[t]);
+    }
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
-  const auto weights = [&](f32x4_t (&s)[MI][4], int n0) {
+  const auto weights = [&](f32x4_t (&s)[4], int n0) {
     const bool plain = n0 + kTile4 <= wave_sees;                     // every row of the wave sees the whole tile
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-      if (!plain) {
-        const int vis = seen[mi] - n0 - 4 * lg;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[mi][j][i] = 16 * j + i < vis ? s[mi][j][i] : -INFINITY;
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[mi][j][0], s[mi][j][1]), fmaxf(s[mi][j][2], s[mi][j][3])));
-      top *= scale;
-      // The reference of the weights moves only where a score is kSlack4 over it: until then weights are up to 2^kSlack4, which changes no rounding, and the
-      // lanes of a column need not agree on a maximum.
-      if (__any(top > m_run[mi] + kSlack4)) {
-        top = fmaxf(m_run[mi], column_max(top));
-        const float keep = top > m_run[mi] ? __builtin_amdgcn_exp2f(m_run[mi] - top) : 1.f;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[mi][t] *= keep;
-        l_run[mi] *= keep;
-        m_run[mi] = top;
-      }
-      const float base = m_run[mi] == -INFINITY ? 0.f : m_run[mi];  // a row that has seen nothing yet: exp2(-inf - 0)
+    if (!plain) {
+      const int vis = seen - n0 - 4 * lg;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[mi][j][i] = __builtin_amdgcn_exp2f(fmaf(s[mi][j][i], scale, -base));
-          l_run[mi] += s[mi][j][i];
-        }
+        for (int i = 0; i < 4; ++i) s[j][i] = 16 * j + i < vis ? s[j][i] : -INFINITY;
     }
+    float top = -INFINITY;
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
+    for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
+    top *= scale;
+    // m_run moves only where a score is kSlack4 over it, and the lanes of a column need not agree on a maximum until then; weights are taken 2^-kSlack4 of
+    // what they are over it, at most 1, which changes no rounding, so that no value becomes infinite on its way.
+    if (__any(top > m_run + kSlack4)) {
+      top = fmaxf(m_run, column_max(top));
+      const float keep = top > m_run ? __builtin_amdgcn_exp2f(m_run - top) : 1.f;
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        uint32_t hw[4], lw[4];
+      for (int t = 0; t < NT; ++t) o[t] *= keep;
+      l_run *= keep;
+      m_run = top;
+    }
+    const float base = m_run == -INFINITY ? 0.f : m_run + kSlack4;  // a row that has seen nothing yet: exp2(-inf - 0)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float x0 = s[mi][2 * st + (c >> 1)][2 * (c & 1)], x1 = s[mi][2 * st + (c >> 1)][2 * (c & 1) + 1];
-          hw[c] = pack_bf16x2(x0, x1);
-          lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
-        }
-        ph[mi][st] = __builtin_bit_cast(frag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
-        pl[mi][st] = __builtin_bit_cast(frag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[j][i] = __builtin_amdgcn_exp2f(fmaf(s[j][i], scale, -base));
+        l_run += s[j][i];
       }
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      uint32_t hw[4], lw[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float x0 = s[2 * st + (c >> 1)][2 * (c & 1)], x1 = s[2 * st + (c >> 1)][2 * (c & 1) + 1];
+        hw[c] = pack_bf16x2(x0, x1);
+        lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+      }
+      ph[st] = __builtin_bit_cast(frag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
+      pl[st] = __builtin_bit_cast(frag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
+    }
   };
 
   const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile4; };
@@ -550,7 +534,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     if (i + 1 < n) request(at(i + 1));
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
     if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
-    f32x4_t s[MI][4];
+    f32x4_t s[4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       frag_t kf[2][ST];
@@ -568,61 +552,56 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     }
   }
   if constexpr (KG > 1) {                // the halves' results
-    static_assert(KG == 2 && MI == 1, "one exchange");
+    static_assert(KG == 2, "one exchange");
     f32x4_t* part = reinterpret_cast<f32x4_t*>(smem) + wave * (NT + 1) * kWave + lane;
     __syncthreads();
     if (kg == 1) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) part[t * kWave] = o[0][t];
-      part[NT * kWave] = f32x4_t{m_run[0], l_run[0], 0.f, 0.f};
+      for (int t = 0; t < NT; ++t) part[t * kWave] = o[t];
+      part[NT * kWave] = f32x4_t{m_run, l_run, 0.f, 0.f};
     }
     __syncthreads();
     if (kg == 1) return;
     const f32x4_t other = part[NT * kWave];
-    const float top = fmaxf(m_run[0], other[0]);
+    const float top = fmaxf(m_run, other[0]);
     // a half whose sum is NaN keeps it, whatever its reference
-    const float f0 = m_run[0] > -INFINITY ? __builtin_amdgcn_exp2f(m_run[0] - top) : l_run[0] == 0.f ? 0.f : 1.f;
+    const float f0 = m_run > -INFINITY ? __builtin_amdgcn_exp2f(m_run - top) : l_run == 0.f ? 0.f : 1.f;
     const float f1 = other[0] > -INFINITY ? __builtin_amdgcn_exp2f(other[0] - top) : other[1] == 0.f ? 0.f : 1.f;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) o[0][t] = o[0][t] * f0 + part[t * kWave] * f1;
-    l_run[0] = l_run[0] * f0 + other[1] * f1;
-    m_run[0] = top;
+    for (int t = 0; t < NT; ++t) o[t] = o[t] * f0 + part[t * kWave] * f1;
+    l_run = l_run * f0 + other[1] * f1;
+    m_run = top;
   }
   // element i of tile t is channel 16 t + 4 lg + i of row lr
   const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
+  const float l = column_sum(l_run);
+  if (w0 + lr >= rows) return;
+  if (any_nan) {
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    const int r = w0 + 16 * mi + lr;
-    const float l = column_sum(l_run[mi]);
-    if (r >= rows) continue;
-    if (any_nan) {
+    for (int t = 0; t < NT; ++t)
+      if (nan_at[t / 2] < seen)
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        if (nan_at[t / 2] < seen[mi])
+        for (int i = 0; i < 4; ++i) o[t][i] = __builtin_nanf("");
+  }
+  if (ranges > 1) {
+    const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+    const int64_t at = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
+    if (lg == 0) *part.stats(at, range) = f32x2_t{l != l ? INFINITY : m_run, l};
+    float* v = part.values(at, range) + 4 * lg;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[mi][t][i] = __builtin_nanf("");
-    }
-    if (ranges > 1) {
-      const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
-      const int64_t at = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
-      if (lg == 0) *part.stats(at, range) = f32x2_t{l != l ? INFINITY : m_run[mi], l};
-      float* v = part.values(at, range) + 4 * lg;
+    for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t*>(v + 16 * t) = o[t];
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + 4 * lg;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4_t*>(v + 16 * t) = o[mi][t];
-      continue;
-    }
-    const int m = r / G, h = hk * G + r - m * G;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)h * a.so_h + 4 * lg;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const u32x2_t w{E::pack2(o[mi][t][0] * inv, o[mi][t][1] * inv), E::pack2(o[mi][t][2] * inv, o[mi][t][3] * inv)};
-      if (out8) {
-        *reinterpret_cast<u32x2_t*>(op + 16 * t) = w;
-      } else {
-        op[16 * t] = (uint16_t)w.x; op[16 * t + 1] = (uint16_t)(w.x >> 16);
-        op[16 * t + 2] = (uint16_t)w.y; op[16 * t + 3] = (uint16_t)(w.y >> 16);
-      }
+  for (int t = 0; t < NT; ++t) {
+    const u32x2_t w{E::pack2(o[t][0] * inv, o[t][1] * inv), E::pack2(o[t][2] * inv, o[t][3] * inv)};
+    if (out8) {
+      *reinterpret_cast<u32x2_t*>(op + 16 * t) = w;
+    } else {
+      op[16 * t] = (uint16_t)w.x; op[16 * t + 1] = (uint16_t)(w.x >> 16);
+      op[16 * t + 2] = (uint16_t)w.y; op[16 * t + 3] = (uint16_t)(w.y >> 16);
     }
   }
 }
@@ -633,9 +612,16 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 // what this path needs most.
 //   S^T = K Q^T leaves lane (n, h) = (lane % 32, lane / 32) keys 8 b + 4 h + j of a 32-key block of query n; O^T = V^T P^T takes keys 16 u + 4 h + j and 16 u + 8 + 4 h + j
 //   of it in product u, and the V columns stand in that order.
+// For outputs in bf16 the weights and V are float16 where it holds V exactly (the codes do, their scales nearly always): eleven bits of a weight are eight times
+// finer than the output.  From the first tile on whose scales it does not hold, and for outputs in float16, they are two bf16 parts and V bf16.
 // K rows are an odd number of 16-byte pieces long and V's pieces XOR-ed with a number of the channel, so that 16 lanes read 16 different pieces of 256 bytes.
+// 8 chunks of 2048 tokens, 32 heads of 128, causal: 338 us, 814 TFLOP/s of scores and outputs (with weights in two bf16 parts 412
+// us, 414 in products of 16 x 16 x 32); with rotation, whose q is two parts, 422 us; in float16 487 us.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+constexpr uint16_t kLeastHalf = 127 - 23, kMostHalf = 127 + 13;            // bytes whose values float16 holds, the least of them as subnormals
+constexpr float kLift4 = 7.f;                                               // weights in float16 are taken 2^7 larger: none above 2^-32 of the largest is lost
 __device__ __forceinline__ int wide_piece(int c) { return ((c >> 1) ^ (c >> 4)) & 7; }
 
 template <int DT, int DH, bool TWO>
@@ -649,7 +635,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile4][KSTR]
   uint16_t* Vt = Ks + 2 * kTile4 * KSTR;                                    // [2][DH][kTile4]
   __shared__ int nan_at[DH / kGroup4];                                      // the first NaN of a group among the values that not every row sees
-  __shared__ int any_nan;
+  __shared__ int any_nan, odd_tile;
 
   const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
   int mt, hb;
@@ -748,18 +734,19 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
       if (none || nan) vbyte &= ~(0xffu << (8 * e));
     }
   };
-  const auto stage_v = [&](int buf) {
-    const int piece = 2 * (vq >> 2) + (vq & 1), half = vq >> 1 & 1;
-    uint16_t* to = Vt + buf * DH * kTile4 + VD * vc * kTile4 + 4 * half;
+  // V as bf16, or (half) as float16
+  const auto stage_v = [&](int i, auto half) {
+    const int piece = 2 * (vq >> 2) + (vq & 1), part = vq >> 1 & 1;
+    uint16_t* to = Vt + (i & 1) * DH * kTile4 + VD * vc * kTile4 + 4 * part;
 #pragma unroll
     for (int c = 0; c < VD / 2; ++c) {
       uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = pair4_at(c, vreg[e], scale_at(vbyte, e));
+      for (int e = 0; e < 4; ++e) w[e] = half ? pair4_half_at(c, vreg[e], scale_at(vbyte, e)) : pair4_at(c, vreg[e], scale_at(vbyte, e));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int d = 2 * c + i;
-        const uint32_t sel = i ? 0x07060302u : 0x05040100u;
+      for (int k = 0; k < 2; ++k) {
+        const int d = 2 * c + k;
+        const uint32_t sel = k ? 0x07060302u : 0x05040100u;
         *reinterpret_cast<u32x2_t*>(to + d * kTile4 + 8 * (piece ^ wide_piece(VD * vc + d))) =
             u32x2_t{__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel)};
       }
@@ -767,19 +754,9 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
   const int tiles = (n_end + kTile4 - 1) / kTile4;
-  if (tiles > 0) request(0);
-  if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
-  if (tid == 0) any_nan = 0;
-  __syncthreads();
   const uint16_t* kread = Ks + lr * KSTR + 8 * lh;
-  for (int i = 0; i < tiles; ++i) {
+  const auto attend = [&](int i, auto half) {
     const int buf = i & 1, n0 = i * kTile4;
-    stage_k(buf);
-    if (n0 + kTile4 > all_see) set_nans_aside(n0);
-    stage_v(buf);
-    if (i + 1 < tiles) request(n0 + kTile4);
-    __syncthreads();                     // this buffer is written; the other one is read by nobody any more
-    if (n0 >= wave_end) continue;
     f32x16_t s[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -803,7 +780,8 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
 #pragma unroll
       for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[k][e], s[k][e + 1]));
     top *= scale;
-    // the reference of the weights moves only where a score is kSlack4 over it: until then weights are up to 2^kSlack4, which changes no rounding
+    // m_run moves only where a score is kSlack4 over it.  Weights in bf16 are taken 2^-kSlack4 of what they are over it, at most 1, so that no value becomes
+    // infinite on its way; those in float16, whose values are small, 2^kLift4, at most 2^15.
     if (__any(top > m_run + kSlack4)) {
       const uint32_t u = __float_as_uint(top);
       const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -814,32 +792,94 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
       l_run *= keep;
       m_run = top;
     }
-    const float base = m_run == -INFINITY ? 0.f : m_run;            // a row that has seen nothing yet: exp2(-inf - 0)
-    frag_t ph[4], pl[4];
+    const float base = m_run == -INFINITY ? 0.f : half ? m_run - kLift4 : m_run + kSlack4;       // a row that has seen nothing yet: exp2(-inf - 0)
+    u32x4_t ph[4], pl[half ? 1 : 4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      uint32_t hw[4], lw[4];
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float x0 = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + 2 * c], scale, -base));
         const float x1 = __builtin_amdgcn_exp2f(fmaf(s[u >> 1][8 * (u & 1) + 2 * c + 1], scale, -base));
         l_run += x0 + x1;
-        hw[c] = pack_bf16x2(x0, x1);
-        lw[c] = pack_bf16x2(x0 - bf16_lo(hw[c]), x1 - bf16_hi(hw[c]));
+        if constexpr (half) {
+          ph[u][c] = E16<1>::pack2(x0, x1);
+        } else {
+          const uint32_t w = pack_bf16x2(x0, x1);
+          ph[u][c] = w;
+          pl[u][c] = pack_bf16x2(x0 - bf16_lo(w), x1 - bf16_hi(w));
+        }
       }
-      ph[u] = __builtin_bit_cast(frag_t, u32x4_t{hw[0], hw[1], hw[2], hw[3]});
-      pl[u] = __builtin_bit_cast(frag_t, u32x4_t{lw[0], lw[1], lw[2], lw[3]});
-    }
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
         const int c = 32 * t + lr;
-        const frag_t vf = __builtin_bit_cast(frag_t, *reinterpret_cast<const u32x4_t*>(Vt + buf * DH * kTile4 + c * kTile4 + 8 * ((2 * u + lh) ^ wide_piece(c))));
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, ph[u], o[t], 0, 0, 0);
-        o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pl[u], o[t], 0, 0, 0);
+        const u32x4_t vf = *reinterpret_cast<const u32x4_t*>(Vt + buf * DH * kTile4 + c * kTile4 + 8 * ((2 * u + lh) ^ wide_piece(c)));
+        if constexpr (half) {
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf), __builtin_bit_cast(f16x8_t, ph[u]), o[t], 0, 0, 0);
+        } else {
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag_t, vf), __builtin_bit_cast(frag_t, ph[u]), o[t], 0, 0, 0);
+          o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(frag_t, vf), __builtin_bit_cast(frag_t, pl[u]), o[t], 0, 0, 0);
+        }
       }
+  };
+  if (tiles > 0) request(0);
+  if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
+  if (tid == 0) { any_nan = 0; odd_tile = tiles; }
+  __syncthreads();
+  if constexpr (DT == 0) {               // the first tile that float16 does not hold: waves in turn have the bytes of a group
+    for (int n = 16 * (lane + kWave * (wave / NB)); n < n_end && wave / NB < kPrompt4Waves / NB; n += 16 * kWave * (kPrompt4Waves / NB)) {
+      uint32_t w[4];
+      load4<16, 0>(rows4(vsp), wave % NB * (uint32_t)a.c.ss_g + n, 0, w);
+      u16x2_t far = {0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int left = n_end - n - 4 * e;                                 // bytes of the word that count
+        if (left < 4) w[e] = left <= 0 ? 0x01010101u * kLeastHalf : (w[e] & ~(~0u << (8 * left))) | (0x01010101u * kLeastHalf & (~0u << (8 * left)));
+        const u16x2_t first = {kLeastHalf, kLeastHalf};
+        far = __builtin_elementwise_max(far, (u16x2_t)(__builtin_bit_cast(u16x2_t, w[e] & 0x00ff00ffu) - first));
+        far = __builtin_elementwise_max(far, (u16x2_t)(__builtin_bit_cast(u16x2_t, w[e] >> 8 & 0x00ff00ffu) - first));
+      }
+      if (max((uint32_t)far.x, (uint32_t)far.y) > kMostHalf - kLeastHalf) atomicMin(&odd_tile, n / kTile4);
+    }
+    __syncthreads();
   }
+  // the wave's own tiles; every wave stages and passes every barrier
+  const int halves = DT == 0 ? __builtin_amdgcn_readfirstlane(odd_tile) : 0, own = (wave_end + kTile4 - 1) / kTile4;
+  int i = 0;
+  const auto stage = [&](auto half) {
+    stage_k(i & 1);
+    if constexpr (half) {
+      if ((i + 1) * kTile4 > n_end) {    // what stands behind the last key, whatever its bytes, becomes small numbers
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i * kTile4 + 4 * vq + e >= n_end) vbyte = (vbyte & ~(0xffu << (8 * e))) | (uint32_t)kLeastHalf << (8 * e);
+      }
+    } else if ((i + 1) * kTile4 > all_see) {
+      set_nans_aside(i * kTile4);
+    }
+    stage_v(i, half);
+    if (i + 1 < tiles) request((i + 1) * kTile4);
+    __syncthreads();                     // this buffer is written; the other one is read by nobody any more
+  };
+  if constexpr (DT == 0) {
+    for (; i < min(halves, own); ++i) {
+      stage(std::true_type{});
+      attend(i, std::true_type{});
+    }
+    for (; i < halves; ++i) stage(std::true_type{});
+    if (i < own) {                       // from the reference of float16 weights to the other
+      constexpr float f = 1.f / (1 << (int)(kLift4 + kSlack4));
+#pragma unroll
+      for (int t = 0; t < NB; ++t) o[t] *= f;
+      l_run *= f;
+    }
+  }
+  for (; i < own; ++i) {
+    stage(std::false_type{});
+    attend(i, std::false_type{});
+  }
+  for (; i < tiles; ++i) stage(std::false_type{});
   // element i of block t is channel 32 t + 8 (i / 4) + 4 lh + i % 4 of row lr
   const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
   {
@@ -886,21 +926,21 @@ size_t kv4_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
   return f.ranges > 1 ? RangeParts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
-template <int DT, int DH, int MI, int KG, bool TWO>
+template <int DT, int DH, int KG, bool TWO>
 static int prompt_launch_form(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   constexpr size_t lds = KG * 2 * ((size_t)kTile4 * (DH + 16) * 2 + (size_t)DH * kTile4 * 2);
   static std::atomic<uint32_t> granted{0};
-  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv4_prompt_kernel<DT, DH, MI, KG, TWO>), lds, granted) : kOk) return rc;
-  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * MI * kPrompt4Waves - 1) / (16 * MI * kPrompt4Waves) * a.B * a.c.Hk;
+  if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv4_prompt_kernel<DT, DH, KG, TWO>), lds, granted) : kOk) return rc;
+  const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 16 * kPrompt4Waves - 1) / (16 * kPrompt4Waves) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
-  hipLaunchKernelGGL((kv4_prompt_kernel<DT, DH, MI, KG, TWO>), dim3((unsigned)groups, ranges), dim3(kPrompt4Waves * KG * kWave), lds, st, a, ranges, scratch);
+  hipLaunchKernelGGL((kv4_prompt_kernel<DT, DH, KG, TWO>), dim3((unsigned)groups, ranges), dim3(kPrompt4Waves * KG * kWave), lds, st, a, ranges, scratch);
   if (ranges > 1) launch_join(join_args(a), ranges, false, scratch, st);
   return kOk;
 }
-template <int DT, int DH, int MI, int KG>
+template <int DT, int DH, int KG>
 static int prompt_launch(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
-  if constexpr (DT == 1) return prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st);
-  else return a.cos ? prompt_launch_form<DT, DH, MI, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, MI, KG, false>(fn, a, ranges, scratch, st);
+  if constexpr (DT == 1) return prompt_launch_form<DT, DH, KG, true>(fn, a, ranges, scratch, st);
+  else return a.cos ? prompt_launch_form<DT, DH, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, KG, false>(fn, a, ranges, scratch, st);
 }
 template <int DT, int DH, bool TWO>
 static int wide_launch(const char* fn, const Kv4AttnArgs& a, hipStream_t st) {
@@ -919,8 +959,8 @@ static int prompt_launch_rows(const char* fn, const Kv4AttnArgs& a, Prompt4Form 
     if constexpr (DT == 1) return wide_launch<DT, DH, true>(fn, a, st);
     else return a.cos ? wide_launch<DT, DH, true>(fn, a, st) : wide_launch<DT, DH, false>(fn, a, st);
   }
-  if (f.halves == 1) return prompt_launch<DT, DH, 1, 1>(fn, a, f.ranges, scratch, st);
-  return prompt_launch<DT, DH, 1, 2>(fn, a, f.ranges, scratch, st);
+  if (f.halves == 1) return prompt_launch<DT, DH, 1>(fn, a, f.ranges, scratch, st);
+  return prompt_launch<DT, DH, 2>(fn, a, f.ranges, scratch, st);
 }
 int launch_kv4_prompt(const char* fn, const Kv4AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
   const Prompt4Form f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);

@@ -7,6 +7,7 @@ import torch
 
 from tests import kv4_reference as R
 from tests.test_gpu_kv8 import _same, half_step, tables
+from tests.util import form_taken
 
 pytestmark = pytest.mark.gpu
 
@@ -35,6 +36,7 @@ class Cache:
 
 
 TWO_PARTS = 2.0 ** -16                                   # of two bf16 parts: the second is rounded by at most 2^-8 of the at most 2^-8 that the first leaves
+HALF_PART = 2.0 ** -11                                   # of one float16: half a step
 
 
 def _close(got, want, room, dt, what):
@@ -47,20 +49,24 @@ def _close(got, want, room, dt, what):
     assert float(over.max()) <= 0, f"{what}: {float(over.max()):.3g} over the bound"
 
 
-def _check_rows(c, q, out, lens, scale, dt, cos=None, sin=None, pos=None, what=""):
+def _check_rows(c, q, out, lens, scale, dt, cos=None, sin=None, pos=None, what="", heads=None):
     """q, out [rows, H, Dh] of rows (sequence b, keys n, position): one query each.  A q that the call rotates and the weights are two parts of 8 bits at least,
-    and the rotation in fp32 leaves 2^-22 of the rotated pair."""
+    and the rotation in fp32 leaves 2^-22 of the rotated pair.  The weights of long chunks in bf16 are one float16, smallest number 2^-24 where the largest weight is
+    2^7 at least: they lose 2^-32 of the largest."""
+    one = dt == torch.bfloat16 and form_taken() == "kv4 prompt 128"
     k, v = c.values()
     H, Hk = q.shape[1], k.shape[2]
     for i, (b, n) in enumerate(lens):
-        for h in range(H):
+        for h in range(H) if heads is None else heads:
             x = q[i, h].double()
             y = R.rotate(x, cos, sin, pos[i] if pos else 0)
             hk = h // (H // Hk)
             kk = k[b, :n, hk]
             pair = x.abs() + x.abs().roll(len(x) // 2)
             turned = 2.0 ** -22 * float(((kk.abs() @ pair) / (kk.abs() @ y.abs()).clamp_min(1e-30)).max()) if cos is not None and n else 0.0
-            want, room = R.attend(y, kk, v[b, :n, hk], scale, TWO_PARTS + turned, TWO_PARTS)
+            want, room = R.attend(y, kk, v[b, :n, hk], scale, TWO_PARTS + turned, HALF_PART if one else TWO_PARTS)
+            if one and n:
+                room = room + n * 2.0 ** -32 * v[b, :n, hk].abs().amax(0)
             _close(out[i, h], want, room, dt, f"{what} row {i} head {h} of {n} keys")
 
 
