@@ -8,6 +8,7 @@ decode_kvcache_eval).  Flag semantics are identical: a flag is the string "1" or
 """
 from __future__ import annotations
 
+import math
 import os
 import time
 from types import SimpleNamespace
@@ -182,10 +183,11 @@ def _draw_next_token(logits: torch.Tensor, *, temperature: float, top_k: int, to
     return tokens
 
 
-def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batch_size: int, device, kv8_cache: bool = False):
+def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batch_size: int, device, kv8_cache: bool = False,
+                            kv4_cache: bool = False):
     """(cache, use_manual_decode).  The dense FlashSVD cache is used when the dense-attention decode
     route or the dense-KV baseline is switched on; the package has no other cache for its modules."""
-    from .runtime.cache import FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
+    from .runtime.cache import FlashSVDKV4Cache, FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
     dtype = next(iter(model.parameters())).dtype
     use_flash = _env_truthy("FLASH_SVD_ENABLE_DENSE_ATTN_DECODE") and not _env_truthy("SVDLLM_FLASH_FALLBACK")
     # the rank-space cache when the checkpoint asks for it (config side channel written by the loader,
@@ -194,7 +196,9 @@ def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batc
         and not use_flash
     if kv8_cache and use_rank:
         raise ValueError("kv8_cache and the rank-space cache are mutually exclusive.")
-    kind = FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if use_rank else FlashSVDV15DenseKVCache
+    if kv4_cache and (use_rank or kv8_cache):
+        raise ValueError("kv4_cache and the other caches are mutually exclusive.")
+    kind = FlashSVDKV4Cache if kv4_cache else FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if use_rank else FlashSVDV15DenseKVCache
     cache = kind(model.config, max_batch_size=int(batch_size), max_cache_len=int(prompt_len) + int(max_new_tokens) + 4,
                  device=device, dtype=dtype)
     return cache, bool(use_flash)
@@ -203,12 +207,18 @@ def _build_generation_cache(model, *, prompt_len: int, max_new_tokens: int, batc
 @torch.no_grad()
 def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, device=None, do_sample: bool = False,
                   temperature: float = 0.8, top_p: float = 0.95, use_graph: Optional[bool] = None, top_k: int = 0, min_p: float = 0.0,
-                  seed: Optional[int] = None, kv8_cache: bool = False) -> dict[str, Any]:
+                  seed: Optional[int] = None, kv8_cache: bool = False, kv4_cache: bool = False, logprobs: Optional[int] = None) -> dict[str, Any]:
     """Single-prompt generation; returns text and token ids like the reference's generate_text.
 
     ``top_k`` (0: off), ``min_p`` (0: off) and ``seed`` are additions to its arguments: with any of them sampling takes
     ``hip_ops.sample_token_`` with uniform numbers of a generator of its own (seeded with ``seed``), captured graph included.
-    ``kv8_cache`` keeps keys and values in 8 bits (FlashSVDKV8Cache)."""
+    ``kv8_cache`` keeps keys and values in 8 bits (FlashSVDKV8Cache), ``kv4_cache`` in 4 (FlashSVDKV4Cache).
+
+    ``logprobs`` (0 to 64) adds to the result, one entry for each generated token, by ``hip_ops.token_logprobs`` from the model's logits before temperature and
+    cuts: ``completion_logprobs``, ``completion_entropies`` (nats) and ``completion_top_logprobs``, the ``logprobs`` likeliest tokens as (token id, log probability),
+    likeliest first.  Needs a model in bfloat16 or float16."""
+    if logprobs is not None and not 0 <= int(logprobs) <= 64:
+        raise ValueError(f"logprobs must be 0 to 64, got {logprobs}")
     if device is None:
         try:
             device = next(model.parameters()).device
@@ -228,7 +238,7 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
         raise ValueError("generate_text currently supports batch_size=1 only.")
     prompt_len = int(input_ids.shape[1])
     cache, _ = _build_generation_cache(model, prompt_len=prompt_len, max_new_tokens=int(max_new_tokens), batch_size=1,
-                                       device=device, kv8_cache=bool(kv8_cache))
+                                       device=device, kv8_cache=bool(kv8_cache), kv4_cache=bool(kv4_cache))
     out = model(input_ids=input_ids, past_key_values=cache, cache_position=torch.arange(prompt_len), logits_to_keep=1)
     output_ids = input_ids[0].tolist()
     eos = getattr(tokenizer, "eos_token_id", None)
@@ -240,7 +250,8 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
         generator = torch.Generator(device=out.logits.device)
         generator.seed() if seed is None else generator.manual_seed(int(seed))
         pick = lambda logits: _draw_next_token(logits, generator=generator, **draws)      # noqa: E731
-    next_token = pick(out.logits[:, -1, :])
+    logits = out.logits
+    next_token = pick(logits[:, -1, :])
     if use_graph is None:
         use_graph = _env_truthy("FLASH_SVD_DENSE_DECODE_GRAPH") or _env_truthy("FLASH_SVD_MLP_CUDA_GRAPH")
     dec = None
@@ -248,14 +259,17 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
     if use_graph and (not do_sample or draws is not None) and hasattr(model, "decode_step"):
         from .graphs import GraphedDecoder
         from .step import make_persistent_decoder
-        pdec = make_persistent_decoder(model, cache, 1, max_new_tokens=int(max_new_tokens) + 1) if draws is None else None
+        pdec = make_persistent_decoder(model, cache, 1, max_new_tokens=int(max_new_tokens) + 1) if draws is None and logprobs is None else None
         if pdec is not None:
             pdec.set_state(next_token, prompt_len)
         else:
             dec = GraphedDecoder(model, cache, 1, sampling=draws, generator=generator)
             dec.set_state(next_token, prompt_len)
             dec.capture()
+    scores = []
     for step in range(int(max_new_tokens)):
+        if logprobs is not None:
+            scores.append(_token_scores(logits[:, -1, :], next_token.reshape(1), int(logprobs)))
         tid = int(next_token.item())
         output_ids.append(tid)
         if (eos is not None and tid == int(eos)) or step + 1 >= int(max_new_tokens):
@@ -264,34 +278,71 @@ def generate_text(model, tokenizer, *, prompt: str, max_new_tokens: int = 64, de
             next_token = pdec.step_token()
         elif dec is not None:
             next_token = dec.step()
+            logits = dec.logits
         else:
             out = _manual_llama_decode_step(model, next_token, past_key_values=cache,
                                             cache_position=torch.tensor([prompt_len + step]))
-            next_token = pick(out.logits[:, -1, :])
+            logits = out.logits
+            next_token = pick(logits[:, -1, :])
     if pdec is not None:
         pdec.check()      # a step that gave up waiting leaves stale token ids behind: raise instead of returning them
     completion = output_ids[prompt_len:]
-    return {"prompt_token_count": prompt_len, "generated_token_count": len(completion), "output_ids": output_ids,
-            "completion_ids": completion, "text": tokenizer.decode(output_ids, skip_special_tokens=False),
-            "completion_text": tokenizer.decode(completion, skip_special_tokens=False)}
+    result = {"prompt_token_count": prompt_len, "generated_token_count": len(completion), "output_ids": output_ids,
+              "completion_ids": completion, "text": tokenizer.decode(output_ids, skip_special_tokens=False),
+              "completion_text": tokenizer.decode(completion, skip_special_tokens=False)}
+    if logprobs is not None:
+        taken, entropy, top, top_logprobs = ([x.tolist() for x in column] for column in zip(*scores)) if scores else ([], [], [], [])
+        result |= {"completion_logprobs": [x[0] for x in taken], "completion_entropies": [x[0] for x in entropy],
+                   "completion_top_logprobs": [list(zip(t[0], p[0])) for t, p in zip(top, top_logprobs)]}
+    return result
+
+
+def _token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int):
+    from . import hip_ops
+    return hip_ops.token_logprobs(logits if logits.stride(-1) == 1 else logits.contiguous(), tokens, top=top)
+
+
+@torch.no_grad()
+def score_text(model, tokenizer, *, text: str, device=None, top: int = 0) -> dict[str, Any]:
+    """Log probabilities of a text's tokens after the first, by ``hip_ops.token_logprobs`` from one pass over the text (a model in bfloat16 or float16): ``ids``,
+    ``logprobs`` and ``entropies`` (nats) of ``ids[1:]``, ``top_logprobs`` (the ``top`` likeliest tokens, 0 to 64, as (token id, log probability)), their ``sum`` and
+    ``perplexity`` (exp of minus their mean; NaN for a text of one token).  No counterpart in the reference."""
+    device = torch.device(device) if device is not None else next(model.parameters()).device
+    ids = tokenizer(text, return_tensors="pt", add_special_tokens=False)["input_ids"].to(device)
+    if int(ids.shape[0]) != 1 or int(ids.shape[1]) == 0:
+        raise ValueError("score_text takes one text of at least one token.")
+    n = int(ids.shape[1])
+    if not 0 <= int(top) <= 64:
+        raise ValueError(f"top must be 0 to 64, got {top}")
+    taken = entropy = likely = likely_logprobs = []
+    if n > 1:
+        logits = model(input_ids=ids).logits[:, :-1]
+        taken, entropy, likely, likely_logprobs = (x[0].tolist() for x in _token_scores(logits, ids[:, 1:], int(top)))
+    total = math.fsum(taken)
+    return {"ids": ids[0].tolist(), "logprobs": taken, "entropies": entropy, "top_logprobs": [list(zip(t, p)) for t, p in zip(likely, likely_logprobs)],
+            "sum": total, "perplexity": float(torch.tensor(-total / (n - 1), dtype=torch.float64).exp()) if n > 1 else math.nan}
 
 
 @torch.no_grad()
 def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128, batch_size: int = 1, device: str = "cuda",
                         warmup: int = 5, max_cache_len: Optional[int] = None, lowrank_cache: bool = False,
                         flashsvd_dense_cache: Optional[bool] = None, baseline_dense_kvcache: bool = False, use_graph: bool = True,
-                        profile_decode: bool = False, profile_decode_steps: int = 20, kv8_cache: bool = False) -> dict:
+                        profile_decode: bool = False, profile_decode_steps: int = 20, kv8_cache: bool = False,
+                        kv4_cache: bool = False) -> dict:
     """Prefill a random prompt, run `warmup` untimed decode tokens, then time `new_tokens` tokens
     between two device synchronisations.  Result keys follow the reference's dict.
 
     Cache choice as in utils/evaluator.py:352-388: ``lowrank_cache`` decodes over the rank-space cache
     (FlashSVDLegacySparseKVCache: per-layer, possibly unequal q/k/v ranks, shaped at the first write), otherwise the
     dense cache (the package has no third, HF-static one, so ``flashsvd_dense_cache`` left unset means "dense unless
-    lowrank_cache").  ``kv8_cache`` decodes over keys and values in 8 bits (FlashSVDKV8Cache).  Two modes switched on together raise, as there."""
+    lowrank_cache").  ``kv8_cache`` decodes over keys and values in 8 bits (FlashSVDKV8Cache), ``kv4_cache`` in 4
+    (FlashSVDKV4Cache).  Two modes switched on together raise, as there."""
     from .graphs import GraphedDecoder
-    from .runtime.cache import FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
+    from .runtime.cache import FlashSVDKV4Cache, FlashSVDKV8Cache, FlashSVDLegacySparseKVCache, FlashSVDV15DenseKVCache
     if flashsvd_dense_cache is None:
-        flashsvd_dense_cache = not (lowrank_cache or baseline_dense_kvcache or kv8_cache)
+        flashsvd_dense_cache = not (lowrank_cache or baseline_dense_kvcache or kv8_cache or kv4_cache)
+    if kv4_cache and (kv8_cache or lowrank_cache or flashsvd_dense_cache or baseline_dense_kvcache):
+        raise ValueError("kv4_cache and the other caches are mutually exclusive.")
     if kv8_cache and (lowrank_cache or flashsvd_dense_cache or baseline_dense_kvcache):
         raise ValueError("kv8_cache and the other caches are mutually exclusive.")
     if lowrank_cache and flashsvd_dense_cache:
@@ -307,7 +358,7 @@ def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128,
     dtype = next(iter(model.parameters())).dtype
     vocab = int(getattr(model.config, "vocab_size", 32000))
     input_ids = torch.randint(0, vocab, (int(batch_size), int(prompt_len)), device=dev, dtype=torch.long)
-    kind = FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if lowrank_cache else FlashSVDV15DenseKVCache
+    kind = FlashSVDKV4Cache if kv4_cache else FlashSVDKV8Cache if kv8_cache else FlashSVDLegacySparseKVCache if lowrank_cache else FlashSVDV15DenseKVCache
     cache = kind(model.config, max_batch_size=int(batch_size), max_cache_len=int(max_cache_len), device=dev, dtype=dtype)
     torch.cuda.synchronize()
     t0 = time.perf_counter()
@@ -345,6 +396,7 @@ def decode_kvcache_eval(model, *, prompt_len: int = 2048, new_tokens: int = 128,
         "decode_ms_per_token": float(t_decode * 1000.0 / max(1, int(new_tokens))),
         "lowrank_cache": bool(lowrank_cache), "flashsvd_dense_cache": bool(flashsvd_dense_cache),
         "baseline_dense_kvcache": bool(baseline_dense_kvcache), "kv8_cache": bool(kv8_cache),
+        "kv4_cache": bool(kv4_cache),
     }
     profile = None
     if profile_decode and pdec is not None:
@@ -470,5 +522,5 @@ def enable_flashsvd_llama_layer_tail_cuda_graph() -> None:
     llama.patch_hf_llama_decoder_layer()
 
 
-__all__ = ["cast_model_for_inference", "configure_runtime", "decode_kvcache_eval", "generate_text", "runtime_env_snapshot",
+__all__ = ["cast_model_for_inference", "configure_runtime", "decode_kvcache_eval", "generate_text", "runtime_env_snapshot", "score_text",
            "enable_flashsvd_llama_layer_tail_cuda_graph"]

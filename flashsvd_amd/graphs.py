@@ -45,13 +45,13 @@ class GraphedDecoder:
 
     def __init__(self, model, cache, batch_size: int, *, nsplit=None, warmup: int = 3, sampling: Optional[dict] = None, generator=None):
         from . import hip_ops
-        from .runtime.cache import FlashSVDKV8Cache
+        from .runtime.cache import FlashSVDKV4Cache, FlashSVDKV8Cache
         self.model, self.cache, self.B = model, cache, int(batch_size)
         dev = model.lm_head.weight.device
         cfg = model.config
         H = int(cfg.num_attention_heads)
         Dh = int(getattr(cfg, "head_dim", None) or cfg.hidden_size // H)
-        if isinstance(cache, FlashSVDKV8Cache):             # the call picks its key ranges and has scratch of its own
+        if isinstance(cache, (FlashSVDKV4Cache, FlashSVDKV8Cache)):        # the call picks its key ranges and has scratch of its own
             self.nsplit, self.attn_ws = nsplit, None
         else:
             self.nsplit = nsplit or hip_ops.pick_nsplit(cache.max_cache_len, self.B, H, Dh)

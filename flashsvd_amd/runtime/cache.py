@@ -3,7 +3,7 @@
 ``FlashSVDV15DenseKVCache`` keeps post-RoPE K and V per layer as [Bmax, Smax, Hk, Dh]
 (runtime/cache/attn_dense_kv.py:7-357 of the reference); ``FlashSVDLegacySparseKVCache`` keeps
 the pre-RoPE rank coefficients Pk, Pv per layer as [Bmax, Smax, R]
-(runtime/cache/attn_legacy_sparse_kv.py:22-257).  ``FlashSVDKV8Cache`` keeps K and V in 8 bits.  All are plain Python objects (no dependency
+(runtime/cache/attn_legacy_sparse_kv.py:22-257).  ``FlashSVDKV8Cache`` keeps K and V in 8 bits, ``FlashSVDKV4Cache`` in 4.  All are plain Python objects (no dependency
 on the transformers ``Cache`` base class) with the method names, return values and error
 behaviour the reference's callers rely on.  Storage is allocated once at full size so that
 decode kernels can write in place and a captured HIP graph keeps valid pointers.
@@ -239,7 +239,38 @@ class FlashSVDV15DenseKVCache(_HeadCacheBase):
         return other
 
 
-class FlashSVDKV8Cache(_HeadCacheBase):
+class _CodesCacheBase(_HeadCacheBase):
+    """What the caches of codes and scales share: storage by the head count of the first write, the operands of the operators."""
+
+    def _make_lists(self) -> None:
+        self.key_scale: list[torch.Tensor] = []
+        self.value_scale: list[torch.Tensor] = []
+        for dev in self._layer_device:
+            codes, scale = self._storage(0, 0, dev)
+            self.key_cache.append(codes)
+            self.value_cache.append(codes)
+            self.key_scale.append(scale)
+            self.value_scale.append(scale)
+
+    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
+        layer_idx, h, dh = int(layer_idx), int(h), int(dh)
+        old = (self._layer_heads[layer_idx], self._layer_head_dim[layer_idx])
+        if old == (h, dh):
+            return
+        if self._layer_initialized[layer_idx]:
+            raise RuntimeError(f"{type(self).__name__} shape changed after init for layer {layer_idx}: old={old}, new={(h, dh)}")
+        dev = self._layer_device[layer_idx]
+        self.key_cache[layer_idx], self.key_scale[layer_idx] = self._storage(h, dh, dev)
+        self.value_cache[layer_idx], self.value_scale[layer_idx] = self._storage(h, dh, dev)
+        self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
+
+    def operands(self, layer_idx: int, batch_size: int):
+        """(key codes, value codes, key scales, value scales) of the first ``batch_size`` sequences, as the operators take them."""
+        i, b = int(layer_idx), int(batch_size)
+        return self.key_cache[i][:b], self.value_cache[i][:b], self.key_scale[i][:b], self.value_scale[i][:b]
+
+
+class FlashSVDKV8Cache(_CodesCacheBase):
     """Dense KV cache in 8 bits: per layer e4m3 codes [B, S, Hk, Dh] of K (after RoPE) and V, and one float32 power of two for each
     block of ``block_size`` tokens (16, 32, 64 or 128) of a kv head, [B, ceil(S / block_size), Hk]; ``value = code * scale``.
 
@@ -256,31 +287,12 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         if int(block_size) not in (16, 32, 64, 128):
             raise ValueError(f"block_size must be 16, 32, 64 or 128 tokens, got {block_size}")
         self.block_size = int(block_size)
-        self.key_scale: list[torch.Tensor] = []
-        self.value_scale: list[torch.Tensor] = []
-        for dev in self._layer_device:
-            codes, scale = self._storage(0, 0, dev)
-            self.key_cache.append(codes)
-            self.value_cache.append(codes)
-            self.key_scale.append(scale)
-            self.value_scale.append(scale)
+        self._make_lists()
 
     def _storage(self, h: int, dh: int, dev):
         codes = torch.zeros((self._max_batch_size, h, self._max_cache_len, dh), dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
         scale = torch.zeros((self._max_batch_size, h, -(-self._max_cache_len // self.block_size)), dtype=torch.float32, device=dev)
         return codes.transpose(1, 2), scale.transpose(1, 2)
-
-    def _ensure_layer_spec(self, layer_idx: int, *, h: int, dh: int) -> None:
-        layer_idx, h, dh = int(layer_idx), int(h), int(dh)
-        cur = self.key_cache[layer_idx]
-        if (cur.shape[2], cur.shape[3]) == (h, dh):
-            return
-        if self._layer_initialized[layer_idx]:
-            raise RuntimeError(f"FlashSVDKV8Cache shape changed after init for layer {layer_idx}: old={(int(cur.shape[2]), int(cur.shape[3]))}, new={(h, dh)}")
-        dev = self._layer_device[layer_idx]
-        self.key_cache[layer_idx], self.key_scale[layer_idx] = self._storage(h, dh, dev)
-        self.value_cache[layer_idx], self.value_scale[layer_idx] = self._storage(h, dh, dev)
-        self._layer_heads[layer_idx], self._layer_head_dim[layer_idx] = h, dh
 
     def _note_seen(self, layer_idx: int, q_len: int, cache_position) -> None:
         if int(layer_idx) != 0 or int(q_len) == 0:
@@ -299,17 +311,22 @@ class FlashSVDKV8Cache(_HeadCacheBase):
     def advance_after_fa2(self, layer_idx: int, *, q_len: int, cache_position) -> None:
         self._note_seen(layer_idx, q_len, self._seen_tokens if cache_position is None else cache_position)
 
-    def operands(self, layer_idx: int, batch_size: int):
-        """(key codes, value codes, key scales, value scales) of the first ``batch_size`` sequences, as the operators take them."""
-        i, b = int(layer_idx), int(batch_size)
-        return self.key_cache[i][:b], self.value_cache[i][:b], self.key_scale[i][:b], self.value_scale[i][:b]
-
     def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, *, cos=None, sin=None, rows=None) -> None:
         """``hip_ops.kv8_append`` of rows k, v [B, T, Hk, Dh] at positions int32 [B] of this layer."""
         from .. import hip_ops
         self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
         hip_ops.kv8_append(k, v, *self.operands(layer_idx, k.shape[0]), positions, block=self.block_size, cos=cos, sin=sin, rows=rows)
         self._layer_initialized[int(layer_idx)] = True
+
+    def attend_token(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
+        """``hip_ops.attn_decode_kv8`` of one query token per sequence, q [B, H, Dh], over this layer."""
+        from .. import hip_ops
+        return hip_ops.attn_decode_kv8(q, *self.operands(layer_idx, q.shape[0]), positions, block=self.block_size, **kw)
+
+    def attend_chunk(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
+        """``hip_ops.attn_prefill_kv8`` of a chunk q [B, M, H, Dh] that the cache holds, over this layer."""
+        from .. import hip_ops
+        return hip_ops.attn_prefill_kv8(q, *self.operands(layer_idx, q.shape[0]), positions, block=self.block_size, **kw)
 
     def dequantize(self, layer_idx: int, *, batch_size: Optional[int] = None, length: Optional[int] = None):
         """(K, V) of the first ``length`` positions as ``dtype`` [B, L, Hk, Dh]."""
@@ -340,6 +357,77 @@ class FlashSVDKV8Cache(_HeadCacheBase):
         self.append(layer_idx, k, v, torch.full((k.shape[0],), start, dtype=torch.int32, device=dev))
         self._note_seen(layer_idx, t, torch.tensor([start]))
         k, v = self.dequantize(layer_idx, batch_size=k.shape[0], length=start + t)
+        return k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
+
+
+class FlashSVDKV4Cache(_CodesCacheBase):
+    """Dense KV cache in 4 bits: per layer two e2m1 codes a byte, [B, S, Hk, Dh / 2], of K (after RoPE) and V, and one byte for each 32 channels of a token,
+    [B, Hk, Dh / 32, S]; ``value = code * 2 ** (byte - 127)``: 4.25 bits a number.
+
+    Heads of 64 or 128 dimensions.  A row's codes and scales are its own, so positions are written in any order, again too, and the held length is that of
+    :class:`FlashSVDV15DenseKVCache`.  Rows are written by ``hip_ops.kv4_append`` and read by ``hip_ops.attn_decode_kv4`` / ``attn_prefill_kv4``.  ``dtype`` is that
+    of the activations.  S is ``max_cache_len`` rounded up to 64 tokens, the operators' tile.  No counterpart in the reference, whose caches are of 16 bits."""
+
+    TILE = 64
+
+    def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device=None, dtype: torch.dtype = torch.float16,
+                 layer_device_map: Optional[dict] = None) -> None:
+        super().__init__(config, max_batch_size, max_cache_len, device, dtype, layer_device_map)
+        self._make_lists()
+
+    def _storage(self, h: int, dh: int, dev):
+        if dh not in (0, 64, 128):
+            raise ValueError(f"FlashSVDKV4Cache takes heads of 64 or 128 dimensions, got {dh}")
+        room = -(-self._max_cache_len // self.TILE) * self.TILE
+        codes = torch.zeros((self._max_batch_size, h, room, dh // 2), dtype=torch.uint8, device=dev)
+        return codes.transpose(1, 2), torch.zeros((self._max_batch_size, h, dh // 32, room), dtype=torch.uint8, device=dev)
+
+    def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, *, cos=None, sin=None, rows=None) -> None:
+        """``hip_ops.kv4_append`` of rows k, v [B, T, Hk, Dh] at positions int32 [B] of this layer."""
+        from .. import hip_ops
+        self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
+        hip_ops.kv4_append(k, v, *self.operands(layer_idx, k.shape[0]), positions, cos=cos, sin=sin, rows=rows)
+        self._layer_initialized[int(layer_idx)] = True
+
+    def attend_token(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
+        """``hip_ops.attn_decode_kv4`` of one query token per sequence, q [B, H, Dh], over this layer."""
+        from .. import hip_ops
+        return hip_ops.attn_decode_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, **kw)
+
+    def attend_chunk(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
+        """``hip_ops.attn_prefill_kv4`` of a chunk q [B, M, H, Dh] that the cache holds, over this layer."""
+        from .. import hip_ops
+        return hip_ops.attn_prefill_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, **kw)
+
+    def dequantize(self, layer_idx: int, *, batch_size: Optional[int] = None, length: Optional[int] = None):
+        """(K, V) of the first ``length`` positions as ``dtype`` [B, L, Hk, Dh] (``hip_ops.kv4_dequantize``)."""
+        from .. import hip_ops
+        b = self._max_batch_size if batch_size is None else int(batch_size)
+        n = self._max_cache_len if length is None else int(length)
+        return hip_ops.kv4_dequantize(*self.operands(layer_idx, b), length=n, dtype=self._dtype)
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, cache_kwargs: Optional[dict[str, Any]] = None):
+        """key/value_states are [B, Hk, T, Dh] (keys rotated), row t for position ``cache_position[t]`` (t without it); returns what the cache holds then as
+        [B, Hk, L, Dh]."""
+        cache_position = (cache_kwargs or {}).get("cache_position")
+        t = key_states.shape[2]
+        pos = list(range(t)) if cache_position is None else cache_position.reshape(-1).tolist()
+        if len(pos) != t:
+            raise ValueError(f"FlashSVDKV4Cache needs a position for each of {t} rows, got {len(pos)}")
+        if pos and (min(pos) < 0 or max(pos) >= self._max_cache_len):
+            raise IndexError(f"FlashSVDKV4Cache write position out of range: positions {min(pos)} to {max(pos)} max={self._max_cache_len}")
+        dev = self._layer_device[int(layer_idx)]
+        k, v = (x.to(device=dev, dtype=self._dtype).transpose(1, 2) for x in (key_states, value_states))
+        k, v = (x if x.stride(-1) == 1 else x.contiguous() for x in (k, v))
+        b, first = k.shape[0], 0
+        self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
+        for i in range(1, t + 1):                          # a call for each run of consecutive positions
+            if i == t or pos[i] != pos[i - 1] + 1:
+                self.append(layer_idx, k[:, first:i], v[:, first:i], torch.full((b,), pos[first], dtype=torch.int32, device=dev))
+                first = i
+        self._note_seen(layer_idx, t, cache_position)
+        n = t if cache_position is None else int(self.get_seq_length())
+        k, v = self.dequantize(layer_idx, batch_size=b, length=min(n, self._max_cache_len))
         return k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
 
 
