@@ -1359,9 +1359,14 @@ def _token_logprobs_impl(logits, tokens, top):
     values = torch.empty(*shape[:-1], top, dtype=_F32, device=logits.device)
     B, T = (shape[0], 1) if len(shape) == 2 else shape[:2]
     if B and T:
+        lib = _lib.load()
+        nbytes, scratch, ptr = lib.fsvd_token_logprobs_scratch_bytes(B, T, V, top), None, None
+        if nbytes:
+            scratch = logits.new_empty(nbytes, dtype=torch.uint8)      # of this call and stream
+            ptr = scratch.data_ptr()
         with _on(dev):
-            rc = _lib.load().fsvd_token_logprobs(logits.data_ptr(), st[0], 0 if len(shape) == 2 else st[1], tokens.data_ptr(), logprobs.data_ptr(),
-                                                 entropy.data_ptr(), ids.data_ptr() if top else None, values.data_ptr() if top else None, B, T, V, top, code, _stream())
+            rc = lib.fsvd_token_logprobs(logits.data_ptr(), st[0], 0 if len(shape) == 2 else st[1], tokens.data_ptr(), logprobs.data_ptr(), entropy.data_ptr(),
+                                         ids.data_ptr() if top else None, values.data_ptr() if top else None, ptr, nbytes, B, T, V, top, code, _stream())
         if rc:
             _lib.check("fsvd_token_logprobs", rc)
     return logprobs, entropy, ids, values

@@ -270,9 +270,11 @@ int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq
 /* Of every row of logits [B, T, V] (rows at any element's address, unit inner stride): logprobs[b, t] = log softmax at tokens[b, t], entropy[b, t] =
  * - sum p log p in nats, and the `top` (0 to 64) largest logits, equal ones by index: top_tokens and top_logprobs [B, T, top] (NULL with top = 0).  tokens,
  * logprobs and entropy are contiguous.  A token below 0 stands for none and has log probability 0, one from V on NaN.  A NaN ranks above everything; a row whose
- * largest logit is not finite has no distribution, its numbers are NaN.  Logits of -inf have no weight. */
+ * largest logit is not finite has no distribution, its numbers are NaN.  Logits of -inf have no weight.  scratch: fsvd_token_logprobs_scratch_bytes of
+ * device memory (0: none is needed), aligned to 16 bytes, of this call and stream alone. */
+size_t fsvd_token_logprobs_scratch_bytes(int B, int T, int V, int top);
 int fsvd_token_logprobs(const void* logits, int64_t sl_b, int64_t sl_t, const int64_t* tokens, float* logprobs, float* entropy, int64_t* top_tokens,
-                        float* top_logprobs, int B, int T, int V, int top, int dtype, void* stream);
+                        float* top_logprobs, void* scratch, size_t scratch_bytes, int B, int T, int V, int top, int dtype, void* stream);
 
 
 

@@ -206,8 +206,9 @@ def test_append_forms_are_alike(dt):
         assert form_taken() == "kv4 row"
 
 
-@pytest.mark.parametrize("B,T,V,name", [(600, 1, 2049, "logprobs 256"), (2, 256, 32000, "logprobs 256"), (512, 1, 32769, "logprobs 1024"), (511, 1, 300, "logprobs 1024"),
-                                        (1, 2, 131072, "logprobs 1024"), (1, 2, 131073, "logprobs long")])
+@pytest.mark.parametrize("B,T,V,name", [(600, 1, 2049, "logprobs 256"), (2, 256, 32000, "logprobs 256"), (512, 1, 32769, "logprobs 1024"), (256, 1, 4096, "logprobs 256"), (256, 1, 4097, "logprobs 1024"), (257, 1, 4097, "logprobs 256"),
+                                        (1, 1, 32768, "logprobs 1024"), (1, 1, 32769, "logprobs parts"), (1, 2, 131073, "logprobs parts"),
+                                        (16, 8, 40001, "logprobs parts"), (129, 1, 40001, "logprobs 1024"), (300, 1, 131073, "logprobs parts"), (1, 1, 2500001, "logprobs long parts")])
 def test_logprob_forms(B, T, V, name):
     from flashsvd_amd import hip_ops
     from tests.test_gpu_logprobs import _check
@@ -218,3 +219,32 @@ def test_logprob_forms(B, T, V, name):
     assert form_taken() == name
     pick = sorted({0, B // 2, B - 1})
     _check(x[pick], t[pick], min(9, V), [o[pick] for o in out])
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("top", [0, 1, 20, 33, 64])
+def test_parts_of_rows_with_ties_masks_and_nans(top, dt):
+    """Equal logits across the borders of parts, parts of -inf alone, fewer logits that are not -inf than alternatives, a NaN in one part, an infinity in another."""
+    from flashsvd_amd import hip_ops
+    from tests.test_gpu_logprobs import _check
+    V = 40003
+    g = torch.Generator().manual_seed(top)
+    x = torch.zeros(9, V)
+    x[1] = torch.randn(V, generator=g).mul(2).round()               # many equal ones
+    x[2] = -math.inf
+    x[2, [3, 20000, 20001, V - 1]] = torch.tensor([1.0, 1.0, 2.0, 1.0])
+    x[3] = torch.randn(V, generator=g)
+    x[3, :30000] = -math.inf
+    x[4] = torch.randn(V, generator=g)
+    x[4, 35000] = math.nan
+    x[5] = torch.randn(V, generator=g)
+    x[5, 100] = math.inf
+    x[6] = -math.inf
+    x[7] = -0.0
+    x[7, ::3] = 0.0
+    x[8] = torch.randn(V, generator=g) * 30
+    x = x.to(dt).cuda()
+    t = torch.tensor([V - 1, 0, 20001, 39999, 35000, 100, 5, -1, V], device="cuda")
+    out = hip_ops.token_logprobs(x, t, top=top)
+    assert form_taken() == "logprobs parts"
+    _check(x, t, top, out)

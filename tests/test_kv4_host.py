@@ -137,7 +137,7 @@ def test_refusals_of_the_c_abi():
     assert decode(H=3) == -1 and decode(out=None) == -4 and decode(v=True) == -4 and decode(c=cache(Dh=32)) == -1
     chunk = lambda H=2, M=1, q=p: lib.fsvd_attn_prefill_kv4(cache(), q, 128, 128, 64, p, None, None, None, 0, p, 128, 128, 64, None, 0, 1, M, H, 0.0, 0, None)      # noqa: E731
     assert chunk(H=3) == -1 and chunk(M=-1) == -1 and chunk(q=None) == -4 and chunk(M=0) == 0
-    lp = lambda x=p, B=1, T=1, V=8, top=0, dt=0, ids=None: lib.fsvd_token_logprobs(x, 8, 8, p, p, p, ids, ids, B, T, V, top, dt, None)      # noqa: E731
+    lp = lambda x=p, B=1, T=1, V=8, top=0, dt=0, ids=None: lib.fsvd_token_logprobs(x, 8, 8, p, p, p, ids, ids, None, 0, B, T, V, top, dt, None)      # noqa: E731
     assert lp(x=None) == -4 and lp(B=-1) == -1 and lp(V=0) == -1 and lp(V=(1 << 24) + 1) == -1 and lp(dt=2) == -3 and lp(x=p + 1) == -2
     assert lp(top=1) == -4 and lp(top=9, ids=p) == -1 and lp(V=100, top=65, ids=p) == -1 and lp(top=-1) == -1 and lp(B=0) == 0 and lp(T=0, x=None) == 0
     assert lp(B=1 << 16, T=1 << 16) == -1
