@@ -259,11 +259,15 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4At
   }
 }
 
+// Key ranges: two workgroups for each compute unit, where a range then has 512 keys at least, else one for each and up to 16 ranges of any length.  Times of a call with
+// its join, us: 8 kv heads of 16000 keys in 16 ranges 16.3, 32 12.9 (taken), 63 14.3; 128 kv heads of 4000 in 2 22.8, 4 21.1 (taken), 8 23.9; 32 of 1000 in 2 10.3, 4
+// 9.1 (taken); 512 of 4090 in 1 56.3 (taken), 2 58.0, with lengths down to a quarter 42.1 and 44.2; 384 of 4000 in 1 52.5, 2 46.2 (taken), 3 50.8; 2048 of 1000 in 1
+// 60.2 (taken), 2 71.6.
 int kv4_ranges(int B, int H, int Hk, int S, int nsplit) {
   const int most = S < 384 ? 1 : (S + kMinRange4 - 1) / kMinRange4;
   if (nsplit <= 0) {
     const int64_t pairs = (int64_t)B * Hk * ((H / Hk + kDec4Group - 1) / kDec4Group);
-    nsplit = max((int)((512 + pairs - 1) / pairs), (S + 2047) / 2048);
+    nsplit = (int)min((512 + pairs - 1) / pairs, max(min((256 + pairs - 1) / pairs, (int64_t)16), ((int64_t)S + 511) / 512));
   }
   return max(1, min(nsplit, most));
 }
