@@ -311,6 +311,7 @@ int launch_kv4_decode(const char* fn, const Kv4AttnArgs& args, int ranges, float
 // ---------------------------------------------------------------------------------------------
 constexpr int kTile4 = 64, kPrompt4Waves = 4;
 constexpr float kSlack4 = 8.f;
+constexpr int kLeastTiles = 4;           // of a range: the room may be longer than what it holds, and ranges without keys only say so
 __device__ __forceinline__ int v_piece4(int d) { return ((d >> 2) & 7) ^ (d & 6); }
 
 template <int DT, int DH, int KG, bool TWO>
@@ -347,10 +348,43 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
   const int pos = min(a.positions[b], 0x7ffffffe - a.M);
   const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
   const int all_end = seen_by(min(row0 + BM, rows) - 1);
-  const int tiles = (all_end + kTile4 - 1) / kTile4, per = (tiles + ranges - 1) / ranges;
+  const int tiles = (all_end + kTile4 - 1) / kTile4, per = max((tiles + ranges - 1) / ranges, kLeastTiles);
   const int n_begin = range * per * kTile4, n_end = min(all_end, (range + 1) * per * kTile4);
+  if (range > 0 && n_begin >= all_end) {
+    const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+    if (threadIdx.x < BM && row0 + threadIdx.x < rows) *part.stats((int64_t)(b * a.c.Hk + hk) * a.M * G + row0 + threadIdx.x, range) = f32x2_t{-INFINITY, 0.f};
+    return;
+  }
   const int w0 = row0 + wave * QW;
   const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + QW, rows) - 1)) : 0;             // keys past it are unseen by the wave
+
+  const float scale = a.scale * 1.4426950408889634f;
+  float m_run = -INFINITY, l_run = 0.f;                                     // l_run: a lane's own sum of the weights, not rounded
+  f32x4_t o[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  // K: four lanes a row; V: sixteen lanes with VD channels each for four adjacent keys.  The rooms are whole tiles: nothing is clamped.
+  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
+  const uint8_t* ksp = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const uint8_t* vsp = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
+  const int krow = tid >> 2, kc = tid & 3, vq = tid >> 4, vc = tid & 15;
+  const uint32_t row = (uint32_t)a.c.sc_s;
+  const uint32_t koff = krow * row + KB * kc, voff = 4 * vq * row + VD / 2 * vc;
+  const uint32_t ksoff = 2 * KB * kc / kGroup4 * (uint32_t)a.c.ss_g + krow, vsoff = VD * vc / kGroup4 * (uint32_t)a.c.ss_g + 4 * vq;
+  uint32_t kreg[KB / 4], vreg[4], kbyte, vbyte;
+  const auto request = [&](int n0) {
+    load4<KB, 0>(rows4(kb + (int64_t)n0 * a.c.sc_s), koff, 0, kreg);
+    const Rows4 v = rows4(vb + (int64_t)n0 * a.c.sc_s);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(v, voff, e * row, vreg + e);
+    kbyte = ksp[n0 + ksoff];
+    load4<4, 0>(rows4(vsp + n0), vsoff, 0, &vbyte);
+  };
+  const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile4; };
+  const int all = n_begin < n_end ? (n_end - n_begin + kTile4 - 1) / kTile4 : 0, n = (all - kg + KG - 1) / KG;      // of the workgroup, of this half
+  if (n > 0) request(at(0));             // the first tile is on its way while q is turned
 
   frag_t qf[ST], qr[ST];                                  // qr: what the first part leaves
   const int r = min(w0 + lr, rows - 1), m = r / G, h = hk * G + r - m * G, seen = seen_by(r);
@@ -382,30 +416,6 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 #pragma unroll
     for (int st = 0; st < ST; ++st) qf[st] = __builtin_bit_cast(frag_t, x[st]);
   }
-  const float scale = a.scale * 1.4426950408889634f;
-  float m_run = -INFINITY, l_run = 0.f;                                     // l_run: a lane's own sum of the weights, not rounded
-  f32x4_t o[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  // K: four lanes a row; V: sixteen lanes with VD channels each for four adjacent keys.  The rooms are whole tiles: nothing is clamped.
-  const uint8_t* kb = static_cast<const uint8_t*>(a.c.k) + b * a.c.sc_b + hk * a.c.sc_h;
-  const uint8_t* vb = static_cast<const uint8_t*>(a.c.v) + b * a.c.sc_b + hk * a.c.sc_h;
-  const uint8_t* ksp = static_cast<const uint8_t*>(a.c.k_scale) + b * a.c.ss_b + hk * a.c.ss_h;
-  const uint8_t* vsp = static_cast<const uint8_t*>(a.c.v_scale) + b * a.c.ss_b + hk * a.c.ss_h;
-  const int krow = tid >> 2, kc = tid & 3, vq = tid >> 4, vc = tid & 15;
-  const uint32_t row = (uint32_t)a.c.sc_s;
-  const uint32_t koff = krow * row + KB * kc, voff = 4 * vq * row + VD / 2 * vc;
-  const uint32_t ksoff = 2 * KB * kc / kGroup4 * (uint32_t)a.c.ss_g + krow, vsoff = VD * vc / kGroup4 * (uint32_t)a.c.ss_g + 4 * vq;
-  uint32_t kreg[KB / 4], vreg[4], kbyte, vbyte;
-  const auto request = [&](int n0) {
-    load4<KB, 0>(rows4(kb + (int64_t)n0 * a.c.sc_s), koff, 0, kreg);
-    const Rows4 v = rows4(vb + (int64_t)n0 * a.c.sc_s);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) load4<VD / 2, 0>(v, voff, e * row, vreg + e);
-    kbyte = ksp[n0 + ksoff];
-    load4<4, 0>(rows4(vsp + n0), vsoff, 0, &vbyte);
-  };
   const auto stage_k = [&](int buf) {
     uint16_t* to = Ks + buf * kTile4 * KSTR + krow * KSTR + 2 * KB * kc;
     const float f = scale_of(kbyte);
@@ -522,9 +532,6 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     }
   };
 
-  const auto at = [&](int i) { return n_begin + (i * KG + kg) * kTile4; };
-  const int all = n_begin < n_end ? (n_end - n_begin + kTile4 - 1) / kTile4 : 0, n = (all - kg + KG - 1) / KG;      // of the workgroup, of this half
-  if (n > 0) request(at(0));
   if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
   if (tid == 0) any_nan = 0;
   __syncthreads();
@@ -629,7 +636,7 @@ constexpr float kLift4 = 7.f;                                               // w
 __device__ __forceinline__ int wide_piece(int c) { return ((c >> 1) ^ (c >> 4)) & 7; }
 
 template <int DT, int DH, bool TWO>
-__global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4AttnArgs a, int ranges, float* scratch) {
   typedef E16<DT> E;
   typedef E16<0> P;
   typedef P::frag_t frag_t;
@@ -639,7 +646,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   uint16_t* Ks = reinterpret_cast<uint16_t*>(smem);                         // [2][kTile4][KSTR]
   uint16_t* Vt = Ks + 2 * kTile4 * KSTR;                                    // [2][DH][kTile4]
   __shared__ int nan_at[DH / kGroup4];                                      // the first NaN of a group among the values that not every row sees
-  __shared__ int any_nan, odd_tile;
+  __shared__ int any_nan, odd_tile, has_nan;
 
   const int G = a.H / a.c.Hk, HB = a.c.Hk * a.B, MT = gridDim.x / HB;
   int mt, hb;
@@ -654,13 +661,19 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     mt = t - hb * MT;
   }
   mt = MT - 1 - mt;
-  const int hk = hb / a.B, b = hb - hk * a.B;
+  const int hk = hb / a.B, b = hb - hk * a.B, range = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lr = lane & 31, lh = lane >> 5;
   const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
   if (row0 >= rows) return;
   const int pos = min(a.positions[b], 0x7ffffffe - a.M);
   const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
-  const int n_end = seen_by(min(row0 + BM, rows) - 1);
+  const int all_end = seen_by(min(row0 + BM, rows) - 1), all_tiles = (all_end + kTile4 - 1) / kTile4, per = max((all_tiles + ranges - 1) / ranges, kLeastTiles);
+  const int t0 = range * per, tiles = min(all_tiles, t0 + per), n_end = min(all_end, tiles * kTile4);        // the range: tiles t0 .. tiles - 1
+  if (range > 0 && t0 >= all_tiles) {
+    const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+    if (tid < BM && row0 + tid < rows) *part.stats((int64_t)(b * a.c.Hk + hk) * a.M * G + row0 + tid, range) = f32x2_t{-INFINITY, 0.f};
+    return;
+  }
   const int w0 = row0 + wave * 32;
   const int wave_end = w0 < rows ? min(n_end, seen_by(min(w0 + 32, rows) - 1)) : 0;             // keys past it are unseen by the wave
   const int r = min(w0 + lr, rows - 1), m = r / G, head = hk * G + r - m * G, seen = seen_by(r);
@@ -724,9 +737,9 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     for (int i = 0; i < KB / 4; ++i)
       *reinterpret_cast<u32x4_t*>(to + 8 * i) = u32x4_t{pair4<0>(kreg[i], f), pair4<1>(kreg[i], f), pair4<2>(kreg[i], f), pair4<3>(kreg[i], f)};
   };
-  // a masked key has weight zero, and zero times a NaN is one: see kv4_prompt_kernel
+  // a masked key has weight zero, and zero times a NaN is one: see kv4_prompt_kernel; a NaN among values in float16 is set aside wherever it stands
   const int all_see = seen_by(row0);
-  const auto set_nans_aside = [&](int n0) {
+  const auto set_nans_aside = [&](int n0, uint32_t to) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int n = n0 + 4 * vq + e;
@@ -735,7 +748,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
         any_nan = 1;
         atomicMin(&nan_at[VD * vc / kGroup4], n);
       }
-      if (none || nan) vbyte &= ~(0xffu << (8 * e));
+      if (none || nan) vbyte = (vbyte & ~(0xffu << (8 * e))) | to << (8 * e);
     }
   };
   // V as bf16, or (half) as float16
@@ -757,7 +770,6 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     }
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
-  const int tiles = (n_end + kTile4 - 1) / kTile4;
   const uint16_t* kread = Ks + lr * KSTR + 8 * lh;
   const auto attend = [&](int i, auto half) {
     const int buf = i & 1, n0 = i * kTile4;
@@ -827,18 +839,27 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
         }
       }
   };
-  if (tiles > 0) request(0);
+  if (t0 < tiles) request(t0 * kTile4);
   if (tid < DH / kGroup4) nan_at[tid] = 0x7fffffff;
-  if (tid == 0) { any_nan = 0; odd_tile = tiles; }
+  if (tid == 0) { any_nan = has_nan = 0; odd_tile = tiles; }
   __syncthreads();
   if constexpr (DT == 0) {               // the first tile that float16 does not hold: waves in turn have the bytes of a group
-    for (int n = 16 * (lane + kWave * (wave / NB)); n < n_end && wave / NB < kPrompt4Waves / NB; n += 16 * kWave * (kPrompt4Waves / NB)) {
+    for (int n = t0 * kTile4 + 16 * (lane + kWave * (wave / NB)); n < n_end && wave / NB < kPrompt4Waves / NB; n += 16 * kWave * (kPrompt4Waves / NB)) {
       uint32_t w[4];
       load4<16, 0>(rows4(vsp), wave % NB * (uint32_t)a.c.ss_g + n, 0, w);
       u16x2_t far = {0, 0};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int left = n_end - n - 4 * e;                                 // bytes of the word that count
+        const uint32_t inv = ~w[e];                                         // a byte of 0 is that of a NaN
+        if ((inv - 0x01010101u) & ~inv & 0x80808080u) {                     // which moves no tile to the other form
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((w[e] >> (8 * i) & 0xff) == kNanByte) {
+              w[e] = (w[e] & ~(0xffu << (8 * i))) | (uint32_t)kLeastHalf << (8 * i);
+              if (i < left) has_nan = 1;
+            }
+        }
         if (left < 4) w[e] = left <= 0 ? 0x01010101u * kLeastHalf : (w[e] & ~(~0u << (8 * left))) | (0x01010101u * kLeastHalf & (~0u << (8 * left)));
         const u16x2_t first = {kLeastHalf, kLeastHalf};
         far = __builtin_elementwise_max(far, (u16x2_t)(__builtin_bit_cast(u16x2_t, w[e] & 0x00ff00ffu) - first));
@@ -849,19 +870,11 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     __syncthreads();
   }
   // the wave's own tiles; every wave stages and passes every barrier
-  const int halves = DT == 0 ? __builtin_amdgcn_readfirstlane(odd_tile) : 0, own = (wave_end + kTile4 - 1) / kTile4;
-  int i = 0;
+  const int halves = DT == 0 ? __builtin_amdgcn_readfirstlane(odd_tile) : 0, nans = __builtin_amdgcn_readfirstlane(has_nan), own = (wave_end + kTile4 - 1) / kTile4;
+  int i = t0;
   const auto stage = [&](auto half) {
     stage_k(i & 1);
-    if constexpr (half) {
-      if ((i + 1) * kTile4 > n_end) {    // what stands behind the last key, whatever its bytes, becomes small numbers
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (i * kTile4 + 4 * vq + e >= n_end) vbyte = (vbyte & ~(0xffu << (8 * e))) | (uint32_t)kLeastHalf << (8 * e);
-      }
-    } else if ((i + 1) * kTile4 > all_see) {
-      set_nans_aside(i * kTile4);
-    }
+    if ((i + 1) * kTile4 > all_see || (half && nans)) set_nans_aside(i * kTile4, half ? kLeastHalf : 0);
     stage_v(i, half);
     if (i + 1 < tiles) request((i + 1) * kTile4);
     __syncthreads();                     // this buffer is written; the other one is read by nobody any more
@@ -899,6 +912,18 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[t][i] = __builtin_nanf("");
   }
+  if (ranges > 1) {
+    const RangeParts part{scratch, (int64_t)HB * a.M * G, ranges, DH};
+    const int64_t at = (int64_t)(b * a.c.Hk + hk) * a.M * G + r;
+    // the reference that the weights were taken to in the end
+    if (lh == 0) *part.stats(at, range) = f32x2_t{l_run != l_run ? INFINITY : DT == 0 && own <= halves ? m_run - kLift4 : m_run + kSlack4, l_run};
+    float* v = part.values(at, range) + 4 * lh;
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) *reinterpret_cast<f32x4_t*>(v + 32 * t + 2 * i) = f32x4_t{o[t][i], o[t][i + 1], o[t][i + 2], o[t][i + 3]};
+    return;
+  }
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
   uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)head * a.so_h + 4 * lh;
 #pragma unroll
@@ -916,17 +941,28 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     }
 }
 
-// Rows of a workgroup, its halves and key ranges.
+// Rows of a workgroup, its halves and key ranges, by the room's length S, as what it holds is known to the device alone.  Times are of bf16 without a rotation, in us.
+//   128 rows where they make up 3/2 workgroups for each compute unit (heads of 64: two), and 3/4 where the room is twice the chunk or more: what a workgroup of a chunk at
+// the start sees varies, and more of them level it out.  32 heads of 1500 tokens 41 (64 rows 43); 16 heads of 1500, with a rotation, 48 (35, therefore 64 rows); 32 of 1024
+// behind 2000 others 72 (81); 8 chunks of 128 tokens, groups of 4, behind 2000 54 (67); 6 of 32 heads 54 (75); heads of 64: 32 of 1500 29.3 (28.1, therefore 64).  In two
+// key ranges where each has 32 tiles: 1024 tokens, groups of 4, behind 16000 310 (364), but 32 heads behind 2000 76 (72).
+//   128 rows in more key ranges where these make up a workgroup for each compute unit, up to two, and have 6 tiles each (heads of 64: 12, as ranges of 10 took 35.1 for
+// 29.1): 128 tokens, groups of 4, behind 16000 in 16 ranges 56 (64 rows 78); 512 behind 8000 in 4 92 (134); 300 behind 2000 in 6 35 (40); but 500 tokens of 8 heads on
+// one behind 3000 in 16 33.7 (26).
+//   64 rows else: 2 of 512 tokens, groups of 4, 18.4 (with halves 20.2); 32 heads of 768 in halves 19.8 (22.9); 77 tokens behind 1411 in halves and 3 ranges 21.3
+// (without ranges 28.4, without halves in 3 22.2, halves in 4 29.8).
 struct Prompt4Form { int rows, halves, ranges; };
-static Prompt4Form prompt_form(int B, int M, int H, int Hk, int S) {
-  const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256;
-  if ((list + 127) / 128 * pairs >= 2 * cu) return {128, 1, 1};
+static Prompt4Form prompt_form(int B, int M, int H, int Hk, int Dh, int S) {
+  const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256, wide = (list + 127) / 128 * pairs, tiles = S / kTile4;
+  const int64_t ranges = max((int64_t)1, min(2 * cu / wide, (int64_t)16)), least = 4 * wide >= 3 * cu ? 32 : Dh == 128 ? 6 : 12;
+  if (ranges > 1 && ranges * wide >= cu && tiles >= least * ranges) return {128, 1, (int)ranges};
+  if (Dh == 64 ? wide >= 2 * cu : (S >= 2 * (int64_t)M ? 4 : 2) * wide >= 3 * cu) return {128, 1, 1};
   const int64_t n = (list + 63) / 64 * pairs;
   if (n * 2 > 3 * cu) return {64, 1, 1};
   return {64, 2, (int)max((int64_t)1, min(cu / n, (int64_t)S / ((n * 4 > cu ? 8 : 4) * kTile4)))};
 }
 size_t kv4_prompt_scratch_bytes(int B, int M, int H, int Hk, int Dh, int S) {
-  const Prompt4Form f = prompt_form(B, M, H, Hk, S);
+  const Prompt4Form f = prompt_form(B, M, H, Hk, Dh, S);
   return f.ranges > 1 ? RangeParts::bytes((int64_t)B * M * H, f.ranges, Dh) : 0;
 }
 
@@ -947,27 +983,28 @@ static int prompt_launch(const char* fn, const Kv4AttnArgs& a, int ranges, float
   else return a.cos ? prompt_launch_form<DT, DH, KG, true>(fn, a, ranges, scratch, st) : prompt_launch_form<DT, DH, KG, false>(fn, a, ranges, scratch, st);
 }
 template <int DT, int DH, bool TWO>
-static int wide_launch(const char* fn, const Kv4AttnArgs& a, hipStream_t st) {
+static int wide_launch(const char* fn, const Kv4AttnArgs& a, int ranges, float* scratch, hipStream_t st) {
   constexpr size_t lds = 2 * ((size_t)kTile4 * (DH + 8) * 2 + (size_t)DH * kTile4 * 2);
   static std::atomic<uint32_t> granted{0};
   if (const int rc = lds > 65536 ? grant_lds(fn, reinterpret_cast<const void*>(&kv4_wide_kernel<DT, DH, TWO>), lds, granted) : kOk) return rc;
   const int64_t list = (int64_t)a.M * (a.H / a.c.Hk), groups = (list + 32 * kPrompt4Waves - 1) / (32 * kPrompt4Waves) * a.B * a.c.Hk;
   if (list > 0x7fffffff - 256 || groups > 0x7fffffff) { set_last_error("%s: %d rows of %d heads", fn, a.M, a.H); return kErrBadShape; }
-  hipLaunchKernelGGL((kv4_wide_kernel<DT, DH, TWO>), dim3((unsigned)groups), dim3(kPrompt4Waves * kWave), lds, st, a);
+  hipLaunchKernelGGL((kv4_wide_kernel<DT, DH, TWO>), dim3((unsigned)groups, ranges), dim3(kPrompt4Waves * kWave), lds, st, a, ranges, scratch);
+  if (ranges > 1) launch_join(join_args(a), ranges, false, scratch, st);
   return kOk;
 }
 template <int DT, int DH>
 static int prompt_launch_rows(const char* fn, const Kv4AttnArgs& a, Prompt4Form f, float* scratch, hipStream_t st) {
-  set_last_form(f.rows == 128 ? "kv4 prompt 128" : f.halves == 1 ? "kv4 prompt 64" : f.ranges == 1 ? "kv4 prompt 64 halves" : "kv4 prompt 64 halves ranges");
+  set_last_form(f.rows == 128 ? (f.ranges == 1 ? "kv4 prompt 128" : "kv4 prompt 128 ranges") : f.halves == 1 ? "kv4 prompt 64" : f.ranges == 1 ? "kv4 prompt 64 halves" : "kv4 prompt 64 halves ranges");
   if (f.rows == 128) {
-    if constexpr (DT == 1) return wide_launch<DT, DH, true>(fn, a, st);
-    else return a.cos ? wide_launch<DT, DH, true>(fn, a, st) : wide_launch<DT, DH, false>(fn, a, st);
+    if constexpr (DT == 1) return wide_launch<DT, DH, true>(fn, a, f.ranges, scratch, st);
+    else return a.cos ? wide_launch<DT, DH, true>(fn, a, f.ranges, scratch, st) : wide_launch<DT, DH, false>(fn, a, f.ranges, scratch, st);
   }
   if (f.halves == 1) return prompt_launch<DT, DH, 1>(fn, a, f.ranges, scratch, st);
   return prompt_launch<DT, DH, 2>(fn, a, f.ranges, scratch, st);
 }
 int launch_kv4_prompt(const char* fn, const Kv4AttnArgs& a, float* scratch, size_t scratch_bytes, hipStream_t st) {
-  const Prompt4Form f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.S);
+  const Prompt4Form f = prompt_form(a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.c.S);
   const size_t need = kv4_prompt_scratch_bytes(a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.c.S);
   if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
     set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, f.ranges, need);

@@ -53,7 +53,7 @@ def _check_rows(c, q, out, lens, scale, dt, cos=None, sin=None, pos=None, what="
     """q, out [rows, H, Dh] of rows (sequence b, keys n, position): one query each.  A q that the call rotates and the weights are two parts of 8 bits at least,
     and the rotation in fp32 leaves 2^-22 of the rotated pair.  The weights of long chunks in bf16 are one float16, smallest number 2^-24 where the largest weight is
     2^7 at least: they lose 2^-32 of the largest."""
-    one = dt == torch.bfloat16 and form_taken() == "kv4 prompt 128"
+    one = dt == torch.bfloat16 and form_taken().startswith("kv4 prompt 128")
     k, v = c.values()
     H, Hk = q.shape[1], k.shape[2]
     for i, (b, n) in enumerate(lens):

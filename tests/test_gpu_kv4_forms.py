@@ -12,24 +12,28 @@ from tests.util import form_taken
 
 pytestmark = pytest.mark.gpu
 
-# the name of the form, what a call takes, and rows of a sequence that are real (of M)
-PROMPTS = [
-    ("kv4 prompt 128", dict(B=8, Hk=32, G=1, M=130, past=7, rows=[130, 129, 128, 65, 64, 1, 0, 130])),
-    ("kv4 prompt 128", dict(B=16, Hk=16, G=2, M=70, past=40, rows=None)),
-    ("kv4 prompt 128", dict(B=1, Hk=8, G=6, M=1400, past=300, rows=None)),
-    ("kv4 prompt 64", dict(B=8, Hk=25, G=1, M=70, past=33, rows=[70, 64, 63, 17, 16, 1, 0, 70])),
-    ("kv4 prompt 64", dict(B=2, Hk=5, G=3, M=850, past=0, rows=None)),
-    ("kv4 prompt 64 halves", dict(B=2, Hk=2, G=2, M=40, past=90, rows=[39, 40])),
-    ("kv4 prompt 64 halves", dict(B=3, Hk=32, G=1, M=256, past=0, rows=None)),
-    ("kv4 prompt 64 halves ranges", dict(B=1, Hk=2, G=3, M=21, past=1200, rows=None)),
-    ("kv4 prompt 64 halves ranges", dict(B=3, Hk=1, G=1, M=64, past=700, rows=[64, 2, 0])),
+# the name of the form, the heads' dimensions that take it, what a call takes, and rows of a sequence that are real (of M)
+SHAPES = [
+    ("kv4 prompt 128", (64, 128), dict(B=8, Hk=32, G=1, M=130, past=7, rows=[130, 129, 128, 65, 64, 1, 0, 130])),
+    ("kv4 prompt 128", (64, 128), dict(B=16, Hk=16, G=2, M=70, past=40, rows=None)),
+    ("kv4 prompt 128", (64, 128), dict(B=1, Hk=8, G=6, M=1400, past=300, rows=None)),
+    ("kv4 prompt 128", (128,), dict(B=8, Hk=25, G=1, M=70, past=133, rows=[70, 64, 63, 17, 16, 1, 0, 70])),
+    ("kv4 prompt 128 ranges", (64, 128), dict(B=1, Hk=8, G=4, M=300, past=4400, rows=None)),
+    ("kv4 prompt 128 ranges", (64, 128), dict(B=2, Hk=4, G=4, M=300, past=4400, rows=[299, 3])),
+    ("kv4 prompt 128 ranges", (64, 128), dict(B=1, Hk=8, G=8, M=400, past=3800, rows=None)),
+    ("kv4 prompt 64", (64, 128), dict(B=8, Hk=25, G=1, M=70, past=33, rows=[70, 64, 63, 17, 16, 1, 0, 70])),
+    ("kv4 prompt 64", (64, 128), dict(B=2, Hk=5, G=3, M=850, past=0, rows=None)),
+    ("kv4 prompt 64 halves", (64, 128), dict(B=2, Hk=2, G=2, M=40, past=90, rows=[39, 40])),
+    ("kv4 prompt 64 halves", (64, 128), dict(B=3, Hk=29, G=1, M=256, past=0, rows=None)),
+    ("kv4 prompt 64 halves ranges", (64, 128), dict(B=1, Hk=2, G=3, M=21, past=1200, rows=None)),
+    ("kv4 prompt 64 halves ranges", (64, 128), dict(B=3, Hk=1, G=1, M=64, past=700, rows=[64, 2, 0])),
 ]
+PROMPTS = [(name, p, Dh) for name, dims, p in SHAPES for Dh in dims]
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("Dh", [64, 128])
 @pytest.mark.parametrize("turn", [False, True])
-@pytest.mark.parametrize("name,p", PROMPTS)
+@pytest.mark.parametrize("name,p,Dh", PROMPTS)
 def test_prompt_forms(name, p, turn, Dh, dt):
     """Rows of unequal numbers, NaN in every row that none sees, an out whose rows stand at odd elements, scores with and without a rotation."""
     from flashsvd_amd import hip_ops
@@ -75,8 +79,7 @@ def test_values_that_float16_does_not_hold(byte, where, Dh):
                 what=f"byte {byte}", heads=[6, 7, 31])
 
 
-@pytest.mark.parametrize("Dh", [64, 128])
-@pytest.mark.parametrize("name,p", PROMPTS[2::2])
+@pytest.mark.parametrize("name,p,Dh", PROMPTS[4:])
 def test_the_largest_values_do_not_become_infinite(name, p, Dh):
     """A value near the largest number of float32 at a key whose score is well above the scores before it."""
     from flashsvd_amd import hip_ops
@@ -92,6 +95,48 @@ def test_the_largest_values_do_not_become_infinite(name, p, Dh):
     picked = [(b, m) for b in {0, B - 1} for m in (0, M // 2, M - 1)]
     _check_rows(c, torch.stack([q[b, m] for b, m in picked]), torch.stack([out[b, m] for b, m in picked]), [(b, past + m + 1) for b, m in picked], Dh ** -0.5, dt,
                 what=name, heads=[0, H - 1])
+
+
+@pytest.mark.parametrize("byte", [1, 103, 141, 252])
+@pytest.mark.parametrize("name,p,Dh", PROMPTS[7:])
+def test_values_far_apart_in_the_other_forms(name, p, byte, Dh):
+    """A value of another size in the first tile, in a middle one and in the last: halves and ranges with and without it are joined."""
+    from flashsvd_amd import hip_ops
+    B, Hk, M, past, H, dt = p["B"], p["Hk"], p["M"], p["past"], p["Hk"] * p["G"], torch.bfloat16
+    for at in (2, past + M // 2, past + M - 2):
+        c = Cache(B, past + M, Hk, Dh, seed=6)
+        c.t[3][:, Hk // 2, 1, at] = byte
+        g = torch.Generator().manual_seed(75)
+        q = (torch.randn(B, M, H, Dh, generator=g) * 0.7).to(dt)
+        out = hip_ops.attn_prefill_kv4(q.cuda(), *c.t, torch.full((B,), past, dtype=torch.int32, device="cuda")).cpu()
+        assert form_taken() == name
+        picked = [(b, m) for b in {0, B - 1} for m in (0, M // 2, M - 1)]
+        _check_rows(c, torch.stack([q[b, m] for b, m in picked]), torch.stack([out[b, m] for b, m in picked]), [(b, past + m + 1) for b, m in picked], Dh ** -0.5, dt,
+                    what=name, heads=sorted({0, H // 2, H - 1}))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_a_room_that_is_nearly_empty(Dh, dt):
+    """Key ranges by the room's length where sequences hold little of it or nothing: ranges without keys, rows that see none."""
+    from flashsvd_amd import hip_ops
+    for name, B, Hk, G, M, starts in (("kv4 prompt 128 ranges", 2, 4, 4, 300, [0, 77]), ("kv4 prompt 64 halves ranges", 3, 1, 2, 40, [0, 300, 5])):
+        room = 4800
+        c = Cache(B, room, Hk, Dh, seed=3)
+        c.spoil([s + M for s in starts])
+        g = torch.Generator().manual_seed(77)
+        q = (torch.randn(B, M, Hk * G, Dh, generator=g) * 0.7).to(dt)
+        rows = [M, M - 7, 0][:B]
+        out = hip_ops.attn_prefill_kv4(q.cuda(), *c.t, torch.tensor(starts, dtype=torch.int32, device="cuda"), rows=torch.tensor(rows, dtype=torch.int32, device="cuda"))
+        assert form_taken() == name
+        out = out.cpu()
+        for b in range(B):
+            assert not bool(out[b, rows[b]:].any())
+        picked = [(b, m) for b in range(B) for m in (0, 1, 31, 63, 64, 200, rows[b] - 1) if 0 <= m < rows[b]]
+        _check_rows(c, torch.stack([q[b, m] for b, m in picked]), torch.stack([out[b, m] for b, m in picked]), [(b, starts[b] + m + 1) for b, m in picked], Dh ** -0.5, dt,
+                    what=name, heads=sorted({0, Hk * G - 1}))
+        before = hip_ops.attn_prefill_kv4(q.cuda(), *c.t, torch.tensor([-M - 3] * B, dtype=torch.int32, device="cuda"))       # in front of the cache: no key
+        assert not bool(before.any())
 
 
 def test_small_weights_of_many_keys_are_kept():
@@ -127,13 +172,15 @@ def _weights_case(B, S, Hk, Dh):
     return c, -math.log((1 + 0.98 / 256) * 2.0 ** -5)
 
 
-ACCURATE = [("kv4 prompt 128", dict(B=8, Hk=32, G=1, M=130, past=7)), ("kv4 prompt 64", dict(B=8, Hk=25, G=1, M=70, past=33)),
-            ("kv4 prompt 64 halves", dict(B=2, Hk=2, G=2, M=40, past=90)), ("kv4 prompt 64 halves ranges", dict(B=1, Hk=2, G=3, M=21, past=1200))]
+ACCURATE = [("kv4 prompt 128", dict(B=8, Hk=32, G=1, M=130, past=7), 64), ("kv4 prompt 128", dict(B=8, Hk=32, G=1, M=130, past=7), 128),
+            ("kv4 prompt 128 ranges", dict(B=1, Hk=8, G=4, M=300, past=4400), 64), ("kv4 prompt 128 ranges", dict(B=1, Hk=8, G=4, M=300, past=4400), 128),
+            ("kv4 prompt 64", dict(B=8, Hk=25, G=1, M=70, past=33), 64), ("kv4 prompt 64", dict(B=8, Hk=25, G=1, M=70, past=33), 128),
+            ("kv4 prompt 64 halves", dict(B=2, Hk=2, G=2, M=40, past=90), 64), ("kv4 prompt 64 halves", dict(B=2, Hk=2, G=2, M=40, past=90), 128),
+            ("kv4 prompt 64 halves ranges", dict(B=1, Hk=2, G=3, M=21, past=1200), 64), ("kv4 prompt 64 halves ranges", dict(B=1, Hk=2, G=3, M=21, past=1200), 128)]
 
 
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("Dh", [64, 128])
-@pytest.mark.parametrize("name,p", ACCURATE)
+@pytest.mark.parametrize("name,p,Dh", ACCURATE)
 def test_prompt_weights_keep_their_bits(name, p, Dh, dt):
     from flashsvd_amd import hip_ops
     B, Hk, M, past, H = p["B"], p["Hk"], p["M"], p["past"], p["Hk"] * p["G"]
