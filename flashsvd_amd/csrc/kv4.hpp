@@ -109,6 +109,11 @@ __device__ __forceinline__ void row_numbers(u32x4_t lo, u32x4_t hi, bool turn, u
       const uint32_t wl = lo[e >> 1], wh = hi[e >> 1];
       const float u = e & 1 ? E::hi(wl) : E::lo(wl), v = e & 1 ? E::hi(wh) : E::lo(wh);
       x[0][e] = odd_sum(u * c[e], -(v * s[e])); x[1][e] = odd_sum(u * s[e], v * c[e]);
+      // beyond fp32, but no infinity (which has no bit behind the first either, so it comes here): decides the scale as the largest number
+      const bool numbers = fabsf(u) < INFINITY && fabsf(v) < INFINITY && fabsf(c[e]) < INFINITY && fabsf(s[e]) < INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (numbers && fabsf(x[h][e]) == INFINITY) x[h][e] = copysignf(__FLT_MAX__, x[h][e]);
     }
   }
 }

@@ -133,6 +133,30 @@ def test_append_at_the_ends_of_the_numbers(dt, T):
         assert _same(got, want) if got.is_floating_point() else torch.equal(got, want)
 
 
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_rotated_keys_at_the_ends_of_the_numbers(dt, T):
+    """A rotated pair of the largest bf16 numbers is beyond 32 bits and still a number that decides the scale; infinities of the input do not."""
+    from flashsvd_amd import hip_ops
+    Dh, S = 64, 64
+    big = float(torch.finfo(dt).max)
+    cos, sin = tables(S, Dh, dt)
+    g = torch.Generator().manual_seed(12)
+    k = torch.rand(1, 20, 1, Dh, generator=g).sub(0.5).to(dt)
+    for t in range(20):                                              # channels 3 and 35 are a pair, 9 and 41 too
+        k[0, t, 0, 3], k[0, t, 0, 35] = big * (-1) ** (t // 2), big * (-1) ** t
+        if t % 5 == 4:
+            k[0, t, 0, 9], k[0, t, 0, 41] = (math.inf, 0.5) if t % 2 else (1.0, -math.inf)
+    c = Cache(1, S, 1, Dh, seed=9, zero=True)
+    values, bytes_ = c.values(), [t.cpu().clone() for t in c.t[2:]]
+    R.append(values[0][0], bytes_[0][0], k[0], 3, 20, cos, sin)
+    R.append(values[1][0], bytes_[1][0], k[0], 3, 20)
+    for i in range(0, 20, T):
+        hip_ops.kv4_append(k[:, i:i + T].cuda(), k[:, i:i + T].cuda(), *c.t, torch.tensor([3 + i], dtype=torch.int32, device="cuda"), cos=cos.cuda(), sin=sin.cuda())
+    for got, want in zip((*c.values(), *(t.cpu() for t in c.t[2:])), (*values, *bytes_)):
+        assert _same(got, want) if got.is_floating_point() else torch.equal(got, want)
+
+
 def test_appends_row_by_row_and_at_once_are_alike():
     from flashsvd_amd import hip_ops
     B, T, Hk, Dh, S = 2, 70, 2, 128, 128
