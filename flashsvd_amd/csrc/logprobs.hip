@@ -393,6 +393,10 @@ extern "C" int fsvd_token_logprobs(const void* logits, int64_t sl_b, int64_t sl_
   if (reinterpret_cast<uintptr_t>(logits) & 1) { set_last_error("%s: logits at an odd address", fn); return kErrBadAlign; }
   const int64_t rows = (int64_t)B * T;
   const int pieces = (V + 7) / 8, want = row_parts(rows, V), part = (pieces + want - 1) / want, parts = (pieces + part - 1) / part;
+  if (rows * parts >= 1 << 22) {                           // 2^32 threads of a launch
+    set_last_error("%s: %lld rows in %d parts (fewer than 4194304 of both are served)", fn, (long long)rows, parts);
+    return kErrBadShape;
+  }
   const size_t need = part_bytes(rows, parts, top);
   if (need > 0 && (scratch == nullptr || scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15))) {
     set_last_error("%s: %zu bytes of scratch for %d parts of a row, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, parts, need);

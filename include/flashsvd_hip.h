@@ -232,7 +232,8 @@ int fsvd_attn_prefill_kv8(const fsvd_kv8_cache* cache, const void* q, int64_t sq
 /* ---------------------------------------------------------------------------------------------
  * KV cache in 4 bits.  Codes [B, S, Hk, Dh / 2], two e2m1 codes (0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign bit) a byte with the even channel in the low
  * bits, keys after their rotation; one byte for each token, kv head and 32 channels [B, Hk, Dh / 32, S] (tokens next to each other), value =
- * code * 2^(byte - 127), byte 255 a NaN: the microscaling form of 4 bits.  S a multiple of 64.  k and v share their strides, k_scale and v_scale theirs, all in
+ * code * 2^(byte - 127), byte 255 a NaN: the microscaling form of 4 bits.  Appends write bytes 2 to 252 and 255; others
+ * may come from elsewhere, but 253 and 254 hold numbers that 16 bits do not and must not be among the values of a prompt's rows.  S a multiple of 64.  k and v share their strides, k_scale and v_scale theirs, all in
  * bytes; addresses and strides are multiples of 16, that of tokens at most 2^24.  head_dim 64 and 128.  No counterpart in the reference, whose caches
  * are of 16 bits. */
 typedef struct fsvd_kv4_cache {
@@ -269,7 +270,7 @@ int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq
 
 /* Of every row of logits [B, T, V] (rows at any element's address, unit inner stride): logprobs[b, t] = log softmax at tokens[b, t], entropy[b, t] =
  * - sum p log p in nats, and the `top` (0 to 64) largest logits, equal ones by index: top_tokens and top_logprobs [B, T, top] (NULL with top = 0).  tokens,
- * logprobs and entropy are contiguous.  A token below 0 stands for none and has log probability 0, one from V on NaN.  A NaN ranks above everything; a row whose
+ * logprobs and entropy are contiguous.  Fewer than 2^22 rows, of more than 2^17 logits fewer by their parts (up to 16).  A token below 0 stands for none and has log probability 0, one from V on NaN.  A NaN ranks above everything; a row whose
  * largest logit is not finite has no distribution, its numbers are NaN.  Logits of -inf have no weight.  scratch: fsvd_token_logprobs_scratch_bytes of
  * device memory (0: none is needed), aligned to 16 bytes, of this call and stream alone. */
 size_t fsvd_token_logprobs_scratch_bytes(int B, int T, int V, int top);

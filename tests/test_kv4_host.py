@@ -141,6 +141,7 @@ def test_refusals_of_the_c_abi():
     assert lp(x=None) == -4 and lp(B=-1) == -1 and lp(V=0) == -1 and lp(V=(1 << 24) + 1) == -1 and lp(dt=2) == -3 and lp(x=p + 1) == -2
     assert lp(top=1) == -4 and lp(top=9, ids=p) == -1 and lp(V=100, top=65, ids=p) == -1 and lp(top=-1) == -1 and lp(B=0) == 0 and lp(T=0, x=None) == 0
     assert lp(B=1 << 16, T=1 << 16) == -1
+    assert lp(B=1 << 11, T=1 << 11) == -1 and b"rows" in lib.fsvd_last_error()      # more workgroups than a launch has
 
 
 def test_tensors_that_a_call_writes_are_not_expanded():
