@@ -3,6 +3,10 @@
 
 namespace fsvd {
 
+// Weight of a range, above zero if it has keys, so that a NaN among its values stays one however small they weigh: at the least 2^-149, which is nothing of a number.
+__device__ __forceinline__ float range_weight(float reference, float top) {
+  return reference > -INFINITY ? fmaxf(__builtin_amdgcn_exp2f(reference - top), 1.4e-45f) : 0.f;
+}
 // The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
 // token, head of the group).  Nothing that a load needs comes from another load: what it takes is a round trip to memory and its launch.
 template <int DT, int DH, int WPR>
@@ -32,7 +36,7 @@ __global__ __launch_bounds__(256) void join_ranges_kernel(JoinArgs a, int ranges
         for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
       if (s == part_of) {                                  // the weights, with the first values on their way
         if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-        w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
+        w = lane < n ? range_weight(st[0], top) : 0.f;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -43,7 +47,7 @@ __global__ __launch_bounds__(256) void join_ranges_kernel(JoinArgs a, int ranges
     }
     if (part_of >= n) {                                    // more waves than ranges: the sum all the same
       if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-      w = lane < n && st[0] > -INFINITY ? __builtin_amdgcn_exp2f(st[0] - top) : 0.f;
+      w = lane < n ? range_weight(st[0], top) : 0.f;
     }
     sum += w * st[1];
   }

@@ -232,6 +232,21 @@ def test_a_range_of_nans_alone():
         assert bool(out.isnan().all())
 
 
+def test_a_nan_of_a_value_that_weighs_nothing():
+    """A weight that 32 bits do not hold is above zero, so a NaN among the values that it stands before is one of the output, in how many ranges of keys ever."""
+    from flashsvd_amd import hip_ops
+    Dh, S = 128, 2048
+    c = Cache(1, S, 1, Dh, seed=8)
+    c.t[0].zero_()
+    c.t[0][:, :256], c.t[2][..., :256] = 0x77, 130                  # the first 256 keys 48, the others 0: scores of 543 and 0
+    c.t[3][:, :, 1, 1500] = 255
+    q = torch.ones(1, 4, Dh, dtype=torch.bfloat16, device="cuda")
+    n = torch.tensor([S], dtype=torch.int32, device="cuda")
+    for out in [hip_ops.attn_decode_kv4(q, *c.t, n, nsplit=nsplit) for nsplit in (None, 1, 3, 8)] + [hip_ops.attn_prefill_kv4(q[:, None], *c.t, n - 1)[:, 0]]:
+        nan = out.isnan()
+        assert bool(nan[..., 32:64].all()) and not bool(nan[..., :32].any()) and not bool(nan[..., 64:].any())
+
+
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
 def test_append_forms_are_alike(dt):
     """Many rows at once, four heads of a workgroup, against the same rows in shorter calls."""
