@@ -92,10 +92,10 @@ class GraphedDecoder:
             self.uniforms.uniform_(generator=self.generator)
 
     def capture(self) -> None:
-        from .runtime.cache import FlashSVDKV8Cache
+        from .runtime.cache import FlashSVDKV4Cache, FlashSVDKV8Cache
         tok0, pos0 = self.tokens.clone(), self.positions.clone()
-        if isinstance(self.cache, FlashSVDKV8Cache):        # a row gives up those behind it in its block: the warm-ups' go behind the cache, where they are dropped
-            self.positions.fill_(self.cache.max_cache_len)
+        if isinstance(self.cache, (FlashSVDKV4Cache, FlashSVDKV8Cache)):        # the warm-ups' rows go behind the cache, where they are dropped: in 8 bits a row
+            self.positions.fill_(self.cache.key_cache[0].shape[1])              # gives up those behind it in its block, and the state may not be set yet
         warm = self.positions.clone()
         side = torch.cuda.Stream(device=self.tokens.device)
         side.wait_stream(torch.cuda.current_stream())

@@ -72,6 +72,24 @@ def test_decode_captured_is_decode_eager(Dh, B):
             assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("S", [64, 100])
+def test_a_capture_before_the_state_is_set_leaves_the_cache_as_it_was(S):
+    from flashsvd_amd.graphs import GraphedDecoder
+    model, T = _model(128), 21
+    ids = torch.randint(0, 512, (2, T), generator=torch.Generator().manual_seed(2)).cuda()
+    c = _cache(model, 2, S)
+    first = model(ids, past_key_values=c, cache_position=torch.arange(T)).logits[:, -1].argmax(-1, keepdim=True)
+    held = [t.clone() for name in ("key_cache", "value_cache", "key_scale", "value_scale") for t in getattr(c, name)]
+    dec = GraphedDecoder(model, c, 2)
+    dec.capture()
+    assert all(torch.equal(a, b) for a, b in zip(held, [t for name in ("key_cache", "value_cache", "key_scale", "value_scale") for t in getattr(c, name)]))
+    dec.set_state(first, T)
+    got = [dec.step().clone() for _ in range(3)]
+    other = GraphedDecoder(model, c, 2)
+    other.set_state(first, T)
+    assert all(torch.equal(a, other.eager_step()) for a in got)
+
+
 def test_decode_sees_the_dense_rows_rounded():
     """One layer, a prompt and one token: the attention's output over the 4-bit cache against the formula in 64 bits over what the cache holds."""
     from flashsvd_amd import hip_ops
