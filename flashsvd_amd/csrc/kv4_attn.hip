@@ -21,6 +21,13 @@ __device__ __forceinline__ void query_parts(u32x4_t x, u32x4_t y, u32x4_t cos, u
   }
 }
 
+// The largest of three numbers, in one instruction: what fmaxf compiles to first makes quiet NaNs of each product's result, which has no others.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "v"(c));
+  return d;
+}
+
 // Keys of a decode range, but for the last: a step of every wave.
 constexpr int kDec4Waves = 4, kDec4Step = 64, kDec4Group = 16, kMinRange4 = kDec4Waves * kDec4Step;
 __host__ __device__ __forceinline__ int kv4_range(int keys, int ranges) {
@@ -162,10 +169,10 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4At
             if (j >= left) vs[i] &= ~(0x80u << (8 * t));   // no byte of a row behind the last key is that of a NaN or beyond the numbers: zeros stay zeros
           }
       }
-      float top = x[0][0];
+      float top = m;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) top = fmaxf(top, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
-      top = fmaxf(m, column_max(top));
+      for (int t = 0; t < 4; ++t) top = max3(max3(top, x[t][0], x[t][1]), x[t][2], x[t][3]);
+      top = column_max(top);
       if (__any(top > m)) {
         const float keep = __builtin_amdgcn_exp2f(m - top);                // 0 in front of the first step
 #pragma unroll
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(fmaxf(s[j][0], s[j][1]), fmaxf(s[j][2], s[j][3])));
+    for (int j = 0; j < 4; ++j) top = max3(max3(top, s[j][0], s[j][1]), s[j][2], s[j][3]);
     top *= scale;
     // m_run moves only where a score is kSlack4 over it, and the lanes of a column need not agree on a maximum until then; weights are taken 2^-kSlack4 of
     // what they are over it, at most 1, which changes no rounding, so that no value becomes infinite on its way.
@@ -772,6 +779,8 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   };
   const int wave_sees = seen_by(min(w0, rows - 1));                  // keys of the wave's first row; the others see more from one to the next
   const uint16_t* kread = Ks + lr * KSTR + 8 * lh;
+  // channel 32 d + lr of V: its piece 2 u + lh is turned by (lr / 2) ^ (lr / 16) ^ 2 d, so four addresses and constants reach all of them
+  const uint32_t vread = lr * kTile4 + 8 * ((lh ^ (lr >> 1) ^ (lr >> 4)) & 7);
   const auto attend = [&](int i, auto half) {
     const int buf = i & 1, n0 = i * kTile4;
     f32x16_t s[2];
@@ -795,7 +804,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) top = fmaxf(top, fmaxf(s[k][e], s[k][e + 1]));
+      for (int e = 0; e < 16; e += 2) top = max3(top, s[k][e], s[k][e + 1]);
     top *= scale;
     // m_run moves only where a score is kSlack4 over it.  Weights in bf16 are taken 2^-kSlack4 of what they are over it, at most 1, so that no value becomes
     // infinite on its way; those in float16, whose values are small, 2^kLift4, at most 2^15.
@@ -830,8 +839,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int t = 0; t < NB; ++t) {
-        const int c = 32 * t + lr;
-        const u32x4_t vf = *reinterpret_cast<const u32x4_t*>(Vt + buf * DH * kTile4 + c * kTile4 + 8 * ((2 * u + lh) ^ wide_piece(c)));
+        const u32x4_t vf = *reinterpret_cast<const u32x4_t*>(Vt + buf * DH * kTile4 + (vread ^ (16 * (u ^ t))) + 32 * t * kTile4);
         if constexpr (half) {
           o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf), __builtin_bit_cast(f16x8_t, ph[u]), o[t], 0, 0, 0);
         } else {
