@@ -553,22 +553,23 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     if (i + 1 < n) request(at(i + 1));
     __syncthreads();                   // this buffer is written; the other one is read by nobody any more
     if (at(i) >= wave_end || (KG > 1 && i >= n)) continue;
+    // All fragments of K are read at once, those of V before and behind the weights, so that no product waits for one: 512 tokens of 32 heads 13.9 us (14.5 with a half of
+    // K's and of V's at a time), 2 x 512 in groups of 4 18.5 (19.8).
     f32x4_t s[4];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      frag_t kf[2][ST];
-      k_frags(kf, buf, half);
-      scores(s, kf, half);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    frag_t kf0[2][ST], kf1[2][ST], vf0[NT], vf1[NT];
+    k_frags(kf0, buf, 0);
+    k_frags(kf1, buf, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    scores(s, kf0, 0);
+    scores(s, kf1, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    v_frags(vf0, buf, 0);
+    __builtin_amdgcn_sched_barrier(0);
     weights(s, at(i));
-#pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      __builtin_amdgcn_sched_barrier(0);
-      frag_t vf[NT];
-      v_frags(vf, buf, st);
-      values(vf, st);
-    }
+    v_frags(vf1, buf, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    values(vf0, 0);
+    values(vf1, 1);
   }
   if constexpr (KG > 1) {                // the halves' results
     static_assert(KG == 2, "one exchange");
