@@ -635,8 +635,8 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 // For outputs in bf16 the weights and V are float16 where it holds V exactly (the codes do, their scales nearly always): eleven bits of a weight are eight times
 // finer than the output.  From the first tile on whose scales it does not hold, and for outputs in float16, they are two bf16 parts and V bf16.
 // K rows are an odd number of 16-byte pieces long and V's pieces XOR-ed with a number of the channel, so that 16 lanes read 16 different pieces of 256 bytes.
-// 8 chunks of 2048 tokens, 32 heads of 128, causal: 338 us, 814 TFLOP/s of scores and outputs (with weights in two bf16 parts 412
-// us, 414 in products of 16 x 16 x 32); with rotation, whose q is two parts, 422 us; in float16 487 us.
+// 8 chunks of 2048 tokens, 32 heads of 128, causal: 330 us, 833 TFLOP/s of scores and outputs (before the maxima and the order of
+// its reads were what they are now 344; with weights in two bf16 parts then 412, 414 in products of 16 x 16 x 32); with rotation, whose q is two parts, 413 us; in float16 478 us.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
@@ -966,14 +966,14 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
 
 // Rows of a workgroup, its halves and key ranges, by the room's length S, as what it holds is known to the device alone.  Times are of bf16 without a rotation, in us.
 //   128 rows where they make up 3/2 workgroups for each compute unit (heads of 64: two), and 3/4 where the room is twice the chunk or more: what a workgroup of a chunk at
-// the start sees varies, and more of them level it out.  32 heads of 1500 tokens 41 (64 rows 43); 16 heads of 1500, with a rotation, 48 (35, therefore 64 rows); 32 of 1024
-// behind 2000 others 72 (81); 8 chunks of 128 tokens, groups of 4, behind 2000 54 (67); 6 of 32 heads 54 (75); heads of 64: 32 of 1500 29.3 (28.1, therefore 64).  In two
-// key ranges where each has 32 tiles: 1024 tokens, groups of 4, behind 16000 310 (364), but 32 heads behind 2000 76 (72).
+// the start sees varies, and more of them level it out.  32 heads of 1500 tokens 43 (64 rows 47); 16 heads of 1500, with a rotation, 45 (35, therefore 64 rows); 32 of 1024
+// behind 2000 others 70 (82); 8 chunks of 128 tokens, groups of 4, behind 2000 56 (72); 6 of 32 heads 54 (67); heads of 64: 32 of 1500 28.7 (28.1, therefore 64).  In two
+// key ranges where each has 32 tiles: 1024 tokens, groups of 4, behind 16000 301 (341), but 32 heads behind 2000 75 (70).
 //   128 rows in more key ranges where these make up a workgroup for each compute unit, up to two, and have 6 tiles each (heads of 64: 12, as ranges of 10 took 35.1 for
-// 29.1): 128 tokens, groups of 4, behind 16000 in 16 ranges 56 (64 rows 78); 512 behind 8000 in 4 92 (134); 300 behind 2000 in 6 35 (40); but 500 tokens of 8 heads on
-// one behind 3000 in 16 33.7 (26).
-//   64 rows else: 2 of 512 tokens, groups of 4, 18.4 (with halves 20.2); 32 heads of 768 in halves 19.8 (22.9); 77 tokens behind 1411 in halves and 3 ranges 21.3
-// (without ranges 28.4, without halves in 3 22.2, halves in 4 29.8).
+// 29.1): 128 tokens, groups of 4, behind 16000 in 16 ranges 56 (64 rows 68); 512 behind 8000 in 4 92 (118); 300 behind 2000 in 6 36 (38); but 500 tokens of 8 heads on
+// one behind 3000 in 16 33 (26).
+//   64 rows else: 2 of 512 tokens, groups of 4, 18.0 (with halves 20.9); 32 heads of 768 in halves 21.0 (23.1); 77 tokens behind 1411 in halves and 3 ranges 21.6
+// (without ranges 26.9, without halves in 3 22.9, halves in 4 29.7).
 struct Prompt4Form { int rows, halves, ranges; };
 static Prompt4Form prompt_form(int B, int M, int H, int Hk, int Dh, int S) {
   const int64_t pairs = (int64_t)B * Hk, list = (int64_t)M * (H / Hk), cu = 256, wide = (list + 127) / 128 * pairs, tiles = S / kTile4;
