@@ -465,3 +465,24 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for g_, w in zip(got, want):
         assert all(torch.equal(x, w) for x in g_)
+
+
+def test_opcheck_of_the_operators():
+    """Schemas and fake tensors against what the kernels do."""
+    from flashsvd_amd import hip_ops      # noqa: F401  (registers them)
+    ops, checks = torch.ops.flashsvd_hip, ("test_schema", "test_faketensor")
+    c = Cache(2, 700, 2, 64, seed=51).t
+    g = torch.Generator().manual_seed(52)
+    rand = lambda *shape: torch.randn(*shape, generator=g).to(torch.bfloat16).cuda()      # noqa: E731
+    n = torch.tensor([600, 5], dtype=torch.int32, device="cuda")
+    torch.library.opcheck(ops.kv4_append.default, (rand(2, 9, 2, 64), rand(2, 9, 2, 64), *c, n), test_utils=checks)
+    torch.library.opcheck(ops.kv4_dequantize.default, (*c, 70, torch.float16), test_utils=checks)
+    q, out = rand(2, 4, 64), rand(2, 4, 64)
+    torch.library.opcheck(ops.attn_decode_kv4.default, (q, *c, n), dict(k_new=rand(2, 2, 64), v_new=rand(2, 2, 64)), test_utils=checks)
+    torch.library.opcheck(ops.attn_decode_kv4.out, (q, *c, n), dict(out=out), test_utils=checks)
+    q, out = rand(2, 9, 4, 64), rand(2, 9, 4, 64)
+    torch.library.opcheck(ops.attn_prefill_kv4.default, (q, *c, n), test_utils=checks)
+    torch.library.opcheck(ops.attn_prefill_kv4.out, (q, *c, n), dict(rows=torch.tensor([3, 9], dtype=torch.int32, device="cuda"), out=out), test_utils=checks)
+    x, t = rand(3, 5, 40000), torch.randint(0, 40000, (3, 5), generator=g).cuda()
+    for top in (0, 4):
+        torch.library.opcheck(ops.token_logprobs.default, (x, t, top), test_utils=checks)

@@ -135,3 +135,27 @@ def test_many_rows():
     assert float((ent.double() + (ref.exp() * ref).sum(1)).abs().max()) < 5.2e-5
     order = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :3]
     assert torch.equal(ids, order) and float((best.double() - ref.gather(1, order)).abs().max()) < 9e-6
+
+
+@pytest.mark.parametrize("V,top", [(1000, 5), (70000, 20)])
+def test_captured_and_replayed(V, top):
+    """One workgroup a row and rows in parts, whose scratch is the graph's; other calls of the program between the replays."""
+    from flashsvd_amd import hip_ops
+    g = torch.Generator().manual_seed(V)
+    rows = [(torch.randn(3, V, generator=g) * 3).to(torch.bfloat16).cuda() for _ in range(4)]
+    ids = [torch.randint(-1, V, (3,), generator=g).cuda() for _ in range(4)]
+    x, t = rows[0].clone(), ids[0].clone()
+    hip_ops.token_logprobs(x, t, top=top)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = hip_ops.token_logprobs(x, t, top=top)
+    for a, b in zip(rows, ids):
+        x.copy_(a)
+        t.copy_(b)
+        graph.replay()
+        other = hip_ops.token_logprobs(a.flip(0).contiguous(), b.flip(0), top=top)
+        torch.cuda.synchronize()
+        want = hip_ops.token_logprobs(a, b, top=top)
+        for got, w, o in zip(out, want, other):
+            assert torch.equal(got, w) and torch.equal(o.flip(0), w)
