@@ -15,8 +15,13 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   const bool in = t < rows && pos >= 0 && pos < a.c.S, turn = !value && a.cos != nullptr;
   const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (in ? t : 0) * a.sv_t : a.k + (int64_t)b * a.sk_b + (in ? t : 0) * a.sk_t) + h0 * sh + 8 * part;
   u32x4_t lo[HEADS], hi[HEADS], cw = {0u, 0u, 0u, 0u}, sw = cw;
+  // Many rows are read past the caches, which they would only empty; of few it costs more than it gives (2 x 2048 rows of 32 heads 24.2 us, 26.6 so).
+  const auto once = [](const uint16_t* p) {
+    if constexpr (HEADS == 1) return eight4(p);
+    else return __builtin_bit_cast(u32x4_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any_t*>(p)));
+  };
 #pragma unroll
-  for (int i = 0; i < HEADS; ++i) { lo[i] = eight4(x + i * sh); hi[i] = eight4(x + i * sh + HALF); }
+  for (int i = 0; i < HEADS; ++i) { lo[i] = once(x + i * sh); hi[i] = once(x + i * sh + HALF); }
   if (turn) {
     const int64_t tp = min(max(pos, (int64_t)0), (int64_t)a.rope_len - 1) * HALF + 8 * part;
     cw = eight4(a.cos + tp); sw = eight4(a.sin + tp);
@@ -60,8 +65,8 @@ int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st) {
   return kOk;
 }
 
-// What the first L rows hold, [B, L, Hk, Dh] each: a thread has eight channels of four rows, whose scales are four bytes next to each other.  8 x 2048 rows of 32 heads
-// of 128 (339 MB) take 64 us, 5.3 TB/s, a copy's rate.
+// What the first L rows hold, [B, L, Hk, Dh] each: a thread has eight channels of four rows, whose scales are four bytes next to each other.  What it makes goes past
+// the caches: 8 x 2048 rows of 32 heads of 128 (339 MB) take 49.5 us, 6.9 TB/s (65 through them), 512 rows 4.1 (4.5).
 struct Kv4ReadArgs {
   fsvd_kv4_cache c;
   uint16_t* k; uint16_t* v;
@@ -92,7 +97,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
       const f32x2_t y[4] = {pair4_f32<0>(w[i], f), pair4_f32<1>(w[i], f), pair4_f32<2>(w[i], f), pair4_f32<3>(w[i], f)};
       x = u32x4_t{E::pack2(y[0][0], y[0][1]), E::pack2(y[1][0], y[1][1]), E::pack2(y[2][0], y[2][1]), E::pack2(y[3][0], y[3][1])};
     }
-    if (pos + i < a.L) *reinterpret_cast<u32x4_any_t*>(out + i * a.so_t) = __builtin_bit_cast(u32x4_any_t, x);
+    if (pos + i < a.L) __builtin_nontemporal_store(__builtin_bit_cast(u32x4_any_t, x), reinterpret_cast<u32x4_any_t*>(out + i * a.so_t));
   }
 }
 
