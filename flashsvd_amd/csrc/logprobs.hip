@@ -3,7 +3,7 @@
 // A row is read once, into the registers of a workgroup.  Each thread sums against the largest of its own logits, so that the sums need no maximum of the row;
 // one exchange joins them and gives, as the k-th largest of the maxima of groups of the row's logits, a bound below which no alternative lies.  What is not below it is
 // collected and ranked by counting.  Rows in which that is much (many equal logits, most of them masked) or that hold a NaN are gone over again, see below.
-// 4096 rows of 32000 logits in bf16: 60 us, 4.4 TB/s of the 5.3 that a copy reaches; 64 rows of 128256, in parts, 13.2 us; 1 row of 32000 8.5 us (12.6 of the 17 us of
+// 4096 rows of 32000 logits in bf16: 56 us, 4.7 TB/s of the 5.4 that a copy reaches; 64 rows of 128256, in parts, 13.2 us; 1 row of 32000 8.5 us (12.6 of the 17 us of
 // a row of 128256 in one workgroup are the sums, the rest the alternatives).
 #include "common.hpp"
 #include "../../include/flashsvd_hip.h"
@@ -94,7 +94,10 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobArgs a) 
   const uint16_t* row = a.logits + r / a.T * a.sl_b + r % a.T * a.sl_t + first;
   // eight logits; behind the row's end stands -inf
   const auto fetch = [&](int c) {
-    if (c * 8 + 8 <= V) return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(row + (int64_t)c * 8));
+    if (c * 8 + 8 <= V) {
+      const u32x4_any_t* p = reinterpret_cast<const u32x4_any_t*>(row + (int64_t)c * 8);
+      return __builtin_bit_cast(u32x4_t, R > 0 ? __builtin_nontemporal_load(p) : *p);       // read once: past the caches (4096 rows of 32000 61.5 us, 64.8 through them)
+    }
     uint32_t w[4] = {kNegInf2, kNegInf2, kNegInf2, kNegInf2};
 #pragma unroll
     for (int e = 0; e < 8; ++e)
