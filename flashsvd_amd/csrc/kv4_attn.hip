@@ -6,6 +6,7 @@
 
 namespace fsvd {
 
+typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(2)));
 static JoinArgs join_args(const Kv4AttnArgs& a) { return {a.out, a.so_b, a.so_m, a.so_h, a.rows, a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.dt}; }
 
 // Eight elements of a query row, rotated in fp32 (y: those half a head away; sign: -1 in the lower half; not rotated: cosines 1, y and sines 0), as two bf16 parts:
@@ -593,7 +594,6 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
     m_run = top;
   }
   // element i of tile t is channel 16 t + 4 lg + i of row lr
-  const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
   const float l = column_sum(l_run);
   if (w0 + lr >= rows) return;
   if (any_nan) {
@@ -617,12 +617,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const u32x2_t w{E::pack2(o[t][0] * inv, o[t][1] * inv), E::pack2(o[t][2] * inv, o[t][3] * inv)};
-    if (out8) {
-      *reinterpret_cast<u32x2_t*>(op + 16 * t) = w;
-    } else {
-      op[16 * t] = (uint16_t)w.x; op[16 * t + 1] = (uint16_t)(w.x >> 16);
-      op[16 * t + 2] = (uint16_t)w.y; op[16 * t + 3] = (uint16_t)(w.y >> 16);
-    }
+    *reinterpret_cast<u32x2_any_t*>(op + 16 * t) = w;      // at any element's address: of a row's bits nothing depends on where it goes
   }
 }
 
@@ -921,7 +916,6 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   }
   for (; i < tiles; ++i) stage(std::false_type{});
   // element i of block t is channel 32 t + 8 (i / 4) + 4 lh + i % 4 of row lr
-  const bool out8 = (reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && (a.so_b % 4) == 0 && (a.so_m % 4) == 0 && (a.so_h % 4) == 0;
   {
     const uint32_t u = __float_as_uint(l_run);
     const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
@@ -948,19 +942,15 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
     return;
   }
   const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-  uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)head * a.so_h + 4 * lh;
+  // the two lanes of a row change words, so that either has eight channels next to each other (stores of four: 8 x 2048 tokens 325 us)
+  uint16_t* op = a.out + (int64_t)b * a.so_b + (int64_t)m * a.so_m + (int64_t)head * a.so_h + 8 * lh;
 #pragma unroll
   for (int t = 0; t < NB; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const u32x2_t w{E::pack2(o[t][i] * inv, o[t][i + 1] * inv), E::pack2(o[t][i + 2] * inv, o[t][i + 3] * inv)};
-      uint16_t* to = op + 32 * t + 2 * i;
-      if (out8) {
-        *reinterpret_cast<u32x2_t*>(to) = w;
-      } else {
-        to[0] = (uint16_t)w.x; to[1] = (uint16_t)(w.x >> 16);
-        to[2] = (uint16_t)w.y; to[3] = (uint16_t)(w.y >> 16);
-      }
+    for (int i = 0; i < 16; i += 8) {
+      const auto x = __builtin_amdgcn_permlane32_swap(E::pack2(o[t][i] * inv, o[t][i + 1] * inv), E::pack2(o[t][i + 4] * inv, o[t][i + 5] * inv), false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(E::pack2(o[t][i + 2] * inv, o[t][i + 3] * inv), E::pack2(o[t][i + 6] * inv, o[t][i + 7] * inv), false, false);
+      *reinterpret_cast<u32x4_any_t*>(op + 32 * t + 2 * i) = u32x4_any_t{x[0], y[0], x[1], y[1]};
     }
 }
 

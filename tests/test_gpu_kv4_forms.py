@@ -310,3 +310,24 @@ def test_parts_of_rows_with_ties_masks_and_nans(top, dt):
     out = hip_ops.token_logprobs(x, t, top=top)
     assert form_taken() == "logprobs parts"
     _check(x, t, top, out)
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_rows_of_the_output_at_odd_elements(dt, Dh):
+    """Every form of a prompt writes rows of any distance at any element; what stands between them is left as it was."""
+    from flashsvd_amd import hip_ops
+    B, M, H, Hk = 8, 200, 32, 32
+    c = Cache(B, 256, Hk, Dh, seed=61)
+    g = torch.Generator(device="cuda").manual_seed(62)
+    q = (torch.randn(B, M, H, Dh, generator=g, device="cuda") * 0.7).to(dt)
+    names = set()
+    for n, rows in ((8, 200), (4, 200), (4, 70), (1, 70), (1, 9)):
+        pos = torch.arange(n, dtype=torch.int32, device="cuda") * 3
+        args = (q[:n, :rows], *(t[:n] for t in c.t), pos)
+        want = hip_ops.attn_prefill_kv4(*args)
+        names.add(form_taken())
+        into = torch.full((n, rows, H, Dh + 3), 7.0, dtype=dt, device="cuda")
+        hip_ops.attn_prefill_kv4(*args, out=into[..., 1:Dh + 1])
+        assert torch.equal(into[..., 1:Dh + 1], want) and bool((into[..., 0] == 7).all()) and bool((into[..., Dh + 1:] == 7).all())
+    assert names >= {"kv4 prompt 128", "kv4 prompt 64", "kv4 prompt 64 halves"}
