@@ -4,7 +4,7 @@
 namespace fsvd {
 
 // A workgroup has 256 / (Dh / 16) rows of the keys or the values of HEADS kv heads, which share the rows of the rotation tables and have all their loads in
-// flight.  Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (339 MB) take 68 to 74 us, up to 5.0 TB/s, where a copy
+// flight.  Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (339 MB) take 72 to 77 us, up to 4.7 TB/s, where a copy
 // reaches 5.4; rows that come rotated 60.
 template <int DT, int DH, int HEADS>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {

@@ -630,8 +630,9 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
 // For outputs in bf16 the weights and V are float16 where it holds V exactly (the codes do, their scales nearly always): eleven bits of a weight are eight times
 // finer than the output.  From the first tile on whose scales it does not hold, and for outputs in float16, they are two bf16 parts and V bf16.
 // K rows are an odd number of 16-byte pieces long and V's pieces XOR-ed with a number of the channel, so that 16 lanes read 16 different pieces of 256 bytes.
-// 8 chunks of 2048 tokens, 32 heads of 128, causal: 330 us, 833 TFLOP/s of scores and outputs (before the maxima and the order of
-// its reads were what they are now 344; with weights in two bf16 parts then 412, 414 in products of 16 x 16 x 32); with rotation, whose q is two parts, 413 us; in float16 478 us.
+// 8 chunks of 2048 tokens, 32 heads of 128, causal: 320 to 337 us on different machines, up to 855 TFLOP/s of scores and outputs
+// (before the maxima, its reads and its stores were what they are now 344; with weights in two bf16 parts then 412, 414 in products of 16 x 16 x 32); with rotation, whose q is two parts, 403
+// us; in float16 464 us.
 // ---------------------------------------------------------------------------------------------
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
