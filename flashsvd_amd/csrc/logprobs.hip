@@ -37,7 +37,8 @@ __device__ __forceinline__ uint32_t rank_key(uint32_t k) {
   return k > kZero + inf || k < kMinusZero - inf ? 0xffffu : k == kMinusZero ? kZero : k;
 }
 
-// sums of a part against its own largest, m, as sums against another
+// Sums against their own largest, m, as sums against another.  Where the distance is beyond the numbers (logits at the type's lowest value, the usual mask, below others)
+// it counts as 200, whose power is nothing already: 0 times its product with z would be a NaN.
 __device__ __forceinline__ void move_sums(float m, float& z, float& zx, float to) {
   constexpr float kLog2e = 1.4426950408889634f;
   const float d = fmaxf(m - to, -200.f), f = __builtin_amdgcn_exp2f(d * kLog2e);        // a NaN of m, or of m - to at infinity, is in z too
@@ -142,11 +143,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobArgs a) 
       const uint32_t k = largest(v);
       if (k > most) {
         const float to = key_value<DT>(k);
-        if (m > -INFINITY) {                              // the sums move to the new largest
-          const float d = m - to, f = __builtin_amdgcn_exp2f(d * kLog2e);
-          zx = f * fmaf(d, z, zx);
-          z *= f;
-        }
+        if (m > -INFINITY) move_sums(m, z, zx, to);
         most = k;
         m = to;
       }
