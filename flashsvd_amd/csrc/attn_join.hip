@@ -3,10 +3,9 @@
 
 namespace fsvd {
 
-// Weight of a range, above zero if it has keys, so that a NaN among its values stays one however small they weigh: at the least 2^-149, which is nothing of a number.
-__device__ __forceinline__ float range_weight(float reference, float top) {
-  return reference > -INFINITY ? fmaxf(__builtin_amdgcn_exp2f(reference - top), 1.4e-45f) : 0.f;
-}
+// Weight of a range, below zero where it has no keys and so has written no values.  One that fp32 does not hold is 0: nothing of a number, and a NaN among the values stays one.
+constexpr float kNoKeys = -1.f;
+__device__ __forceinline__ float range_weight(float reference, float top) { return reference > -INFINITY ? __builtin_amdgcn_exp2f(reference - top) : kNoKeys; }
 // The ranges of a row joined in their order, WPR waves for a row, each with every WPR-th range.  Rows of a decode call are (b, h), those of a chunk (b, kv head,
 // token, head of the group).  Nothing that a load needs comes from another load: what it takes is a round trip to memory and its launch.
 template <int DT, int DH, int WPR>
@@ -27,7 +26,7 @@ __global__ __launch_bounds__(256) void join_ranges_kernel(JoinArgs a, int ranges
   for (int s0 = 0; s0 < ranges; s0 += kWave) {
     const int n = min(kWave, ranges - s0);
     const f32x2_t st = *part.stats(at, s0 + min(lane, n - 1));
-    float w = 0.f;
+    float w = kNoKeys;
     for (int s = part_of; s < n; s += WPR * U) {
       float x[U][D];
 #pragma unroll
@@ -36,20 +35,20 @@ __global__ __launch_bounds__(256) void join_ranges_kernel(JoinArgs a, int ranges
         for (int i = 0; i < D; ++i) x[u][i] = part.values(at, s0 + min(s + u * WPR, n - 1))[lane * D + i];
       if (s == part_of) {                                  // the weights, with the first values on their way
         if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-        w = lane < n ? range_weight(st[0], top) : 0.f;
+        w = lane < n ? range_weight(st[0], top) : kNoKeys;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : 0.f;
+        const float f = s + u * WPR < n ? __shfl(w, s + u * WPR) : kNoKeys;
 #pragma unroll
-        for (int i = 0; i < D; ++i) v[i] += f > 0.f ? f * x[u][i] : 0.f;        // a range without keys has written no values
+        for (int i = 0; i < D; ++i) v[i] += f >= 0.f ? f * x[u][i] : 0.f;
       }
     }
     if (part_of >= n) {                                    // more waves than ranges: the sum all the same
       if (s0 == 0) top = wave_max(fmaxf(top, lane < n ? st[0] : -INFINITY));
-      w = lane < n ? range_weight(st[0], top) : 0.f;
+      w = lane < n ? range_weight(st[0], top) : kNoKeys;
     }
-    sum += w * st[1];
+    sum += fmaxf(w, 0.f) * st[1];
   }
   sum = wave_sum(sum);
   if (WPR > 1) {
