@@ -29,6 +29,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return d;
 }
 
+// The maximum of a row that has seen no score yet.  A score may be -infinity where fp32 does not hold it, and has no weight against this, where its distance from
+// another -infinity is no number.
+constexpr float kLowest4 = -__FLT_MAX__;
+
 // Keys of a decode range, but for the last: a step of every wave.
 constexpr int kDec4Waves = 4, kDec4Step = 64, kDec4Group = 16, kMinRange4 = kDec4Waves * kDec4Step;
 __host__ __device__ __forceinline__ int kv4_range(int keys, int ranges) {
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4At
 
   const float scale = a.scale * 1.4426950408889634f;      // weights are powers of two of the scores' differences
   const float second = n < 8 ? 0.f : -1.f;                // the columns of the second parts take what the first leave
-  float m = -INFINITY, l = 0.f;
+  float m = kLowest4, l = 0.f;
   f32x4_t o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -238,7 +242,7 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4At
       for (int i = 0; i < 4; ++i) o[t][i] += dpp_f32<0x128>(o[t][i]);
   }
   l = column_sum(l);
-  if (g == 0) { ms[wave][n] = l != l ? INFINITY : m; ls[wave][n] = l; }
+  if (g == 0) { ms[wave][n] = l != l ? INFINITY : m == kLowest4 ? -INFINITY : m; ls[wave][n] = l; }
   if (n < heads) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
