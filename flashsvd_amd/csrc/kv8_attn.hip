@@ -23,6 +23,10 @@ __device__ __forceinline__ u32x4_t rotated(u32x4_t x, u32x4_t y, u32x4_t cos, u3
 __device__ __forceinline__ u32x4_t eight(const uint16_t* p) { return __builtin_bit_cast(u32x4_t, *reinterpret_cast<const u32x4_any_t*>(p)); }
 static JoinArgs join_args(const Kv8AttnArgs& a) { return {a.out, a.so_b, a.so_m, a.so_h, a.rows, a.B, a.M, a.H, a.c.Hk, a.c.Dh, a.dt}; }
 
+// The maximum of a row that has seen no score yet.  A score may be -infinity where fp32 does not hold it, and has no weight against this, where its distance from
+// another -infinity is no number.
+constexpr float kLowest8 = -__FLT_MAX__;
+
 // Keys of a decode range, but for the last: a step of every wave, and whole blocks.
 constexpr int kMinRange = 128;
 __host__ __device__ __forceinline__ int kv8_range(int keys, int ranges) {
@@ -150,7 +154,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8Att
   }
 
   const float scale = a.scale * 1.4426950408889634f;      // weights are powers of two of the scores' differences
-  float m = -INFINITY, l = 0.f;
+  float m = kLowest8, l = 0.f;
   f32x4_t o[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -231,7 +235,7 @@ __global__ __launch_bounds__(kDecWaves * kWave, 3) void kv8_decode_kernel(Kv8Att
   }
   // the waves' results through LDS: element i of tile t is dimension NT (4 g + i) + t of query n
   l = column_sum(l);
-  if (g == 0) { ms[wave][n] = m; ls[wave][n] = l; }
+  if (g == 0) { ms[wave][n] = l != l ? INFINITY : m == kLowest8 ? -INFINITY : m; ls[wave][n] = l; }
   if (n < heads) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
