@@ -425,7 +425,7 @@ class FlashSVDKV4Cache(_CodesCacheBase):
             if i == t or pos[i] != pos[i - 1] + 1:
                 self.append(layer_idx, k[:, first:i], v[:, first:i], torch.full((b,), pos[first], dtype=torch.int32, device=dev))
                 first = i
-        self._note_seen(layer_idx, t, cache_position)
+        self._note_seen(layer_idx, t, None if cache_position is None else torch.tensor(pos, dtype=torch.long))      # on the host, where they have been read
         n = t if cache_position is None else int(self.get_seq_length())
         k, v = self.dequantize(layer_idx, batch_size=b, length=min(n, self._max_cache_len))
         return k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous()
