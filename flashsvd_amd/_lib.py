@@ -125,7 +125,8 @@ class Kv8Cache(ctypes.Structure):
 class Kv4Cache(ctypes.Structure):
     """fsvd_kv4_cache: codes and scales of a KV cache in 4 bits."""
     _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("sc_b", c_int64), ("sc_s", c_int64), ("sc_h", c_int64),
-                ("ss_b", c_int64), ("ss_h", c_int64), ("ss_g", c_int64), ("S", ctypes.c_int32), ("Hk", ctypes.c_int32), ("Dh", ctypes.c_int32)]
+                ("ss_b", c_int64), ("ss_h", c_int64), ("ss_g", c_int64), ("S", ctypes.c_int32), ("Hk", ctypes.c_int32), ("Dh", ctypes.c_int32),
+                ("limit", ctypes.c_int32)]
 
 
 SIGNATURES = {

@@ -12,7 +12,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   const int value = blockIdx.x & 1, h0 = (blockIdx.x >> 1) * HEADS, b = blockIdx.z, part = threadIdx.x % LPR, t = (int)blockIdx.y * PER + threadIdx.x / LPR;
   const int rows = a.rows ? min(a.rows[b], a.T) : a.T;
   const int64_t pos = (int64_t)a.positions[b] + t, sh = value ? a.sv_h : a.sk_h;
-  const bool in = t < rows && pos >= 0 && pos < a.c.S, turn = !value && a.cos != nullptr;
+  const bool in = t < rows && pos >= 0 && pos < a.c.limit, turn = !value && a.cos != nullptr;
   const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (in ? t : 0) * a.sv_t : a.k + (int64_t)b * a.sk_b + (in ? t : 0) * a.sk_t) + h0 * sh + 8 * part;
   u32x4_t lo[HEADS], hi[HEADS], cw = {0u, 0u, 0u, 0u}, sw = cw;
   // Many rows are read past the caches, which they would only empty; of few it costs more than it gives (2 x 2048 rows of 32 heads 24.2 us, 26.6 so).
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
 template <int DT, int DH>
 __global__ __launch_bounds__(kWave) void kv4_append_one_kernel(Kv4AppendArgs a) {
   const int b = blockIdx.x / a.c.Hk, hk = blockIdx.x % a.c.Hk, pos = a.positions[b];
-  if (pos < 0 || pos >= a.c.S || (a.rows && a.rows[b] <= 0)) return;
+  if (pos < 0 || pos >= a.c.limit || (a.rows && a.rows[b] <= 0)) return;
   append_row4<DT, DH>(a.c, a.k + (int64_t)b * a.sk_b + (int64_t)hk * a.sk_h, a.v + (int64_t)b * a.sv_b + (int64_t)hk * a.sv_h, a.cos, a.sin, a.rope_len, b, hk, pos,
                       threadIdx.x);
 }
@@ -110,6 +110,7 @@ static int check_kv4_cache(const char* fn, const fsvd_kv4_cache* c) {
     set_last_error("%s: bad cache: S=%d Hk=%d Dh=%d (a multiple of 64 rows; 64 and 128 dimensions are served)", fn, c->S, c->Hk, c->Dh);
     return kErrBadShape;
   }
+  if (c->limit < 0 || c->limit > c->S) { set_last_error("%s: limit of %d rows of a cache of %d", fn, c->limit, c->S); return kErrBadShape; }
   if (c->sc_b < 0 || c->sc_s < c->Dh / 2 || c->sc_s > (1 << 24) || c->sc_h < 0 || c->ss_b < 0 || c->ss_h < 0 || c->ss_g < c->S || c->ss_g > (1 << 28)) { set_last_error("%s: bad cache strides", fn); return kErrBadShape; }
   if (((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) | reinterpret_cast<uintptr_t>(c->k_scale) | reinterpret_cast<uintptr_t>(c->v_scale)) & 15) ||
       ((c->sc_b | c->sc_s | c->sc_h | c->ss_b | c->ss_h | c->ss_g) & 15)) {
@@ -141,6 +142,11 @@ static int check_out(const char* fn, int B, int M, int H, int64_t so_b, int64_t 
   if ((B > 1 && so_b == 0) || (M > 1 && so_m == 0) || (H > 1 && so_h == 0)) { set_last_error("%s: out must not be expanded", fn); return kErrBadShape; }
   return kOk;
 }
+static fsvd_kv4_cache with_limit(const fsvd_kv4_cache* c) {
+  fsvd_kv4_cache r = *c;
+  if (r.limit == 0) r.limit = r.S;
+  return r;
+}
 static const uint16_t* in16(const void* p) { return static_cast<const uint16_t*>(p); }
 
 extern "C" {
@@ -154,7 +160,7 @@ int fsvd_kv4_append(const fsvd_kv4_cache* cache, const void* k, int64_t sk_b, in
   if (positions == nullptr || (T != 0 && (k == nullptr || v == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (T < 0) { set_last_error("%s: %d rows", fn, T); return kErrBadShape; }
   if (const int rc = check_written(fn, cache, B)) return rc;
-  const Kv4AppendArgs a{*cache, in16(k), sk_b, sk_t, sk_h, in16(v), sv_b, sv_t, sv_h, positions, rows, in16(cos), in16(sin), rope_len, B, T, dtype};
+  const Kv4AppendArgs a{with_limit(cache), in16(k), sk_b, sk_t, sk_h, in16(v), sv_b, sv_t, sv_h, positions, rows, in16(cos), in16(sin), rope_len, B, T, dtype};
   return launch_kv4_append(fn, a, static_cast<hipStream_t>(stream));
 }
 
@@ -206,7 +212,7 @@ int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_
     set_last_error("%s: %zu bytes of scratch for %d key ranges, %zu needed", fn, scratch ? scratch_bytes : (size_t)0, ranges, need);
     return kErrWorkspace;
   }
-  const Kv4AttnArgs a{*cache, in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
+  const Kv4AttnArgs a{with_limit(cache), in16(q), sq_b, 0, sq_h, cache_seqlens, nullptr, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, 0, so_h,
                       B, 1, H, k_new ? 1 : seqlen_add, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype,
                       in16(k_new), sk_b, sk_h, in16(v_new), sv_b, sv_h};
   return launch_kv4_decode(fn, a, ranges, static_cast<float*>(scratch), st);
@@ -226,7 +232,7 @@ int fsvd_attn_prefill_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq
   if (q_pos0 == nullptr || (M != 0 && (q == nullptr || out == nullptr))) { set_last_error("%s: a buffer is NULL", fn); return kErrNullPtr; }
   if (M < 0 || H <= 0 || H % cache->Hk) { set_last_error("%s: %d rows of %d query heads over %d", fn, M, H, cache->Hk); return kErrBadShape; }
   if (const int rc = check_out(fn, B, M, H, so_b, so_m, so_h)) return rc;
-  const Kv4AttnArgs a{*cache, in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
+  const Kv4AttnArgs a{with_limit(cache), in16(q), sq_b, sq_m, sq_h, q_pos0, rows, in16(cos), in16(sin), rope_len, static_cast<uint16_t*>(out), so_b, so_m, so_h,
                       B, M, H, 1, scale > 0.f ? scale : 1.f / sqrtf((float)cache->Dh), dtype};
   return M == 0 ? kOk : launch_kv4_prompt(fn, a, static_cast<float*>(scratch), scratch_bytes, static_cast<hipStream_t>(stream));
 }

@@ -148,7 +148,7 @@ template <int BYTES, int AUX> __device__ void load4(Rows4 r, uint32_t lane, uint
 #endif
 
 struct Kv4AppendArgs {
-  fsvd_kv4_cache c;
+  fsvd_kv4_cache c;                                    // limit: 1 to S
   const uint16_t* k; int64_t sk_b, sk_t, sk_h;         // [B, T, Hk, Dh]
   const uint16_t* v; int64_t sv_b, sv_t, sv_h;
   const int32_t* positions;                            // [B]
@@ -157,7 +157,7 @@ struct Kv4AppendArgs {
   int B, T, dt;
 };
 struct Kv4AttnArgs {
-  fsvd_kv4_cache c;
+  fsvd_kv4_cache c;                                    // limit: 1 to S
   const uint16_t* q; int64_t sq_b, sq_m, sq_h;         // [B, M, H, Dh]
   const int32_t* positions;                            // [B]: position of a sequence's first query row
   const int32_t* rows;                                 // [B] or null: M query rows each
@@ -172,7 +172,7 @@ struct Kv4AttnArgs {
   const uint16_t* v_new = nullptr; int64_t sv_b = 0, sv_h = 0;
 };
 
-// One row of a kv head (k, v [Dh]) into its place at position pos, 0 <= pos < S, by one wave: the first Dh / 16 lanes hold the key, as many behind them the value.
+// One row of a kv head (k, v [Dh]) into its place at position pos, 0 <= pos < limit, by one wave: the first Dh / 16 lanes hold the key, as many behind them the value.
 template <int DT, int DH>
 __device__ __forceinline__ void append_row4(const fsvd_kv4_cache& c, const uint16_t* k, const uint16_t* v, const uint16_t* cos, const uint16_t* sin, int rope_len,
                                             int b, int hk, int pos, int lane) {

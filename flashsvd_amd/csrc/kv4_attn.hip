@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kDec4Waves * kWave, 3) void kv4_decode_kernel(Kv4At
   // the heads of a sequence, whose ranges are alike, on different XCDs; the last range of every sequence, which may hold the new row, first
   const int pairs = a.B * a.c.Hk * GG, turn = __builtin_amdgcn_readfirstlane(blockIdx.x / pairs), of = blockIdx.x - turn * pairs;
   const int id = __builtin_amdgcn_readfirstlane(of / GG), gg = of - id * GG, b = __builtin_amdgcn_readfirstlane(id / a.c.Hk), hk = id - b * a.c.Hk;
-  const int pos = a.positions[b], keys = (int)max((int64_t)0, min((int64_t)pos + a.key_add, (int64_t)a.c.S));
+  const int pos = a.positions[b], keys = (int)max((int64_t)0, min((int64_t)pos + a.key_add, (int64_t)a.c.limit));
   const int per = __builtin_amdgcn_readfirstlane(kv4_range(keys, ranges)), used = __builtin_amdgcn_readfirstlane(max(1, (keys + per - 1) / per)), s = turn < used ? used - 1 - turn : turn;
   const int k0 = min(s * per, keys), k1 = min(k0 + per, keys);
   const int h0 = hk * G + gg * kDec4Group, heads = min(kDec4Group, G - gg * kDec4Group);
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves * KG, 2) void kv4_prompt_kern
   const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
   if (row0 >= rows) return;
   const int pos = min(a.positions[b], 0x7ffffffe - a.M);
-  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
+  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.limit)); };     // keys of row r
   const int all_end = seen_by(min(row0 + BM, rows) - 1);
   const int tiles = (all_end + kTile4 - 1) / kTile4, per = max((tiles + ranges - 1) / ranges, kLeastTiles);
   const int n_begin = range * per * kTile4, n_end = min(all_end, (range + 1) * per * kTile4);
@@ -676,7 +676,7 @@ __global__ __launch_bounds__(kWave * kPrompt4Waves, 2) void kv4_wide_kernel(Kv4A
   const int M = a.rows ? max(0, min(a.rows[b], a.M)) : a.M, rows = M * G, row0 = mt * BM;
   if (row0 >= rows) return;
   const int pos = min(a.positions[b], 0x7ffffffe - a.M);
-  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.S)); };     // keys of row r
+  const auto seen_by = [&](int r) { return max(0, min(pos + r / G + a.key_add, a.c.limit)); };     // keys of row r
   const int all_end = seen_by(min(row0 + BM, rows) - 1), all_tiles = (all_end + kTile4 - 1) / kTile4, per = max((all_tiles + ranges - 1) / ranges, kLeastTiles);
   const int t0 = range * per, tiles = min(all_tiles, t0 + per), n_end = min(all_end, tiles * kTile4);        // the range: tiles t0 .. tiles - 1
   if (range > 0 && t0 >= all_tiles) {

@@ -1145,13 +1145,13 @@ def _attn_prefill_kv8_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, block,
 # ------------------------------------------------------------------ KV cache in 4 bits
 def kv4_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                positions: torch.Tensor, *, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
-               rows: Optional[torch.Tensor] = None) -> None:
+               rows: Optional[torch.Tensor] = None, limit: Optional[int] = None) -> None:
     """Rows of keys and values [B, T, Hk, Dh] into a cache in 4 bits at positions[b] .. positions[b] + T - 1 (``rows`` int32 [B]: that many of sequence
     b), keys rotated there when ``cos`` / ``sin`` [len, Dh / 2] are given.  Caches uint8 [>=B, S, Hk, Dh / 2], two e2m1 codes a byte with the even channel in
     the low bits, scales uint8 [>=B, Hk, Dh / 32, S] with unit inner stride, ``value = code * 2 ** (scale - 127)`` for the 32 channels of a token; S a multiple of
-    64, strides multiples of 16.  A row changes no other row; rows outside the cache are dropped.  Custom operator flashsvd_hip::kv4_append (caches
-    and scales are mutated arguments); see fsvd_kv4_append."""
-    _OPS.kv4_append.default(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows)
+    64, strides multiples of 16.  A row changes no other row; rows outside the cache are dropped, and with ``limit`` (1 to S) those from it on.  Custom operator
+    flashsvd_hip::kv4_append (caches and scales are mutated arguments); see fsvd_kv4_append."""
+    _OPS.kv4_append.default(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows, limit)
 
 
 def kv4_dequantize(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, *, length: Optional[int] = None,
@@ -1164,22 +1164,24 @@ def kv4_dequantize(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.
 def attn_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                     cache_seqlens: torch.Tensor, *, k_new: Optional[torch.Tensor] = None, v_new: Optional[torch.Tensor] = None,
                     cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, seqlen_add: int = 0, nsplit: Optional[int] = None,
-                    out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
-    """:func:`attn_decode_kv8` over a cache in 4 bits (operands as :func:`kv4_append`).  Custom operator flashsvd_hip::attn_decode_kv4."""
+                    out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None, limit: Optional[int] = None) -> torch.Tensor:
+    """:func:`attn_decode_kv8` over a cache in 4 bits (operands as :func:`kv4_append`, rows from ``limit`` on neither written nor seen).  Custom operator
+    flashsvd_hip::attn_decode_kv4."""
     a = (q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, int(seqlen_add), None if nsplit is None else int(nsplit),
-         None if not softmax_scale else float(softmax_scale))
+         None if not softmax_scale else float(softmax_scale), limit)
     return _OPS.attn_decode_kv4.default(*a) if out is None else _OPS.attn_decode_kv4.out(*a, out=out)
 
 
 def attn_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, q_pos0: torch.Tensor, *,
                      rows: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
-                     out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None) -> torch.Tensor:
-    """:func:`attn_prefill_kv8` over a cache in 4 bits (operands as :func:`kv4_append`).  Custom operator flashsvd_hip::attn_prefill_kv4."""
-    a = (q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, None if not softmax_scale else float(softmax_scale))
+                     out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None, limit: Optional[int] = None) -> torch.Tensor:
+    """:func:`attn_prefill_kv8` over a cache in 4 bits (operands as :func:`kv4_append`, rows from ``limit`` on not seen).  Custom operator
+    flashsvd_hip::attn_prefill_kv4."""
+    a = (q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, None if not softmax_scale else float(softmax_scale), limit)
     return _OPS.attn_prefill_kv4.default(*a) if out is None else _OPS.attn_prefill_kv4.out(*a, out=out)
 
 
-def _kv4_cache(B, kc, vc, ks, vs):
+def _kv4_cache(B, kc, vc, ks, vs, limit=None):
     """Checks of a cache in 4 bits; its descriptor for the C ABI.  One pass over what a good call has, as :func:`_kv8_cache`."""
     shape, st, ss = kc.shape, kc.stride(), ks.stride()
     dev = kc.get_device()
@@ -1192,7 +1194,9 @@ def _kv4_cache(B, kc, vc, ks, vs):
             and ks.shape == scales and vs.shape == scales and vs.stride() == ss and ss[3] == 1 and Dh % 32 == 0 and dev >= 0
             and vc.get_device() == dev and ks.get_device() == dev and vs.get_device() == dev):
         _refuse_kv4_cache(B, kc, vc, ks, vs)
-    return _lib.Kv4Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], S, Hk, Dh)
+    if limit is not None and not 1 <= limit <= S:
+        raise ValueError(f"limit must be 1 to {S}, got {limit}")
+    return _lib.Kv4Cache(kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), st[0], st[1], st[2], ss[0], ss[1], ss[2], S, Hk, Dh, limit or 0)
 
 
 def _refuse_kv4_cache(B, kc, vc, ks, vs):
@@ -1212,11 +1216,11 @@ def _apart4(B, c) -> None:
         raise ValueError("a cache that is written to must not be expanded over its sequences, rows or heads")
 
 
-def _kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows):
+def _kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows, limit=None):
     dt, code = _elem(k, "k")
     shape, st, sv = k.shape, k.stride(), v.stride()
     B = shape[0]
-    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale, limit)
     dev = k_cache.get_device()
     if not (v.dtype is dt and len(shape) == 4 and v.shape == shape and shape[2] == c.Hk and shape[3] == c.Dh and st[3] == 1 and sv[3] == 1
             and k.get_device() == dev and v.get_device() == dev):
@@ -1255,13 +1259,13 @@ def _kv4_dequantize_impl(k_cache, v_cache, k_scale, v_scale, length, dtype):
     return k, v
 
 
-def _attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out):
+def _attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out, limit=None):
     dt, code = _elem(q, "q")
     sq = q.stride()
     if len(sq) != 3 or sq[2] != 1:
         raise ValueError(f"q must be [B,H,Dh] with unit inner stride, got {tuple(q.shape)}")
     B, H, Dh = q.shape
-    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale, limit)
     dev, Hk = k_cache.get_device(), c.Hk
     if c.Dh != Dh or H % Hk or q.get_device() != dev:
         raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")
@@ -1303,13 +1307,13 @@ def _attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, 
     return out
 
 
-def _attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out):
+def _attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out, limit=None):
     dt, code = _elem(q, "q")
     sq = q.stride()
     if len(sq) != 4 or sq[3] != 1:
         raise ValueError(f"q must be [B,M,H,Dh] with unit inner stride, got {tuple(q.shape)}")
     B, M, H, Dh = q.shape
-    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale)
+    c = _kv4_cache(B, k_cache, v_cache, k_scale, v_scale, limit)
     dev = k_cache.get_device()
     if c.Dh != Dh or H % c.Hk or q.get_device() != dev:
         raise ValueError(f"q {tuple(q.shape)} on {q.device} does not match caches {tuple(k_cache.shape)} on {k_cache.device}")

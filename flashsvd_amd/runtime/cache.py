@@ -366,13 +366,15 @@ class FlashSVDKV4Cache(_CodesCacheBase):
 
     Heads of 64 or 128 dimensions.  A row's codes and scales are its own, so positions are written in any order, again too, and the held length is that of
     :class:`FlashSVDV15DenseKVCache`.  Rows are written by ``hip_ops.kv4_append`` and read by ``hip_ops.attn_decode_kv4`` / ``attn_prefill_kv4``.  ``dtype`` is that
-    of the activations.  S is ``max_cache_len`` rounded up to 64 tokens, the operators' tile.  No counterpart in the reference, whose caches are of 16 bits."""
+    of the activations.  S is ``max_cache_len`` rounded up to 64 tokens, the operators' tile; rows behind ``max_cache_len`` are dropped and not seen.  No counterpart in
+    the reference, whose caches are of 16 bits."""
 
     TILE = 64
 
     def __init__(self, config, *, max_batch_size: int, max_cache_len: int, device=None, dtype: torch.dtype = torch.float16,
                  layer_device_map: Optional[dict] = None) -> None:
         super().__init__(config, max_batch_size, max_cache_len, device, dtype, layer_device_map)
+        self._limit = self._max_cache_len if self._max_cache_len % self.TILE else None      # for the operators, of the room
         self._make_lists()
 
     def _storage(self, h: int, dh: int, dev):
@@ -384,20 +386,23 @@ class FlashSVDKV4Cache(_CodesCacheBase):
 
     def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, *, cos=None, sin=None, rows=None) -> None:
         """``hip_ops.kv4_append`` of rows k, v [B, T, Hk, Dh] at positions int32 [B] of this layer."""
+        self._write(layer_idx, k, v, positions, cos=cos, sin=sin, rows=rows, limit=self._limit)
+
+    def _write(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, **kw) -> None:
         from .. import hip_ops
         self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
-        hip_ops.kv4_append(k, v, *self.operands(layer_idx, k.shape[0]), positions, cos=cos, sin=sin, rows=rows)
+        hip_ops.kv4_append(k, v, *self.operands(layer_idx, k.shape[0]), positions, **kw)
         self._layer_initialized[int(layer_idx)] = True
 
     def attend_token(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
         """``hip_ops.attn_decode_kv4`` of one query token per sequence, q [B, H, Dh], over this layer."""
         from .. import hip_ops
-        return hip_ops.attn_decode_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, **kw)
+        return hip_ops.attn_decode_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, limit=self._limit, **kw)
 
     def attend_chunk(self, layer_idx: int, q: torch.Tensor, positions: torch.Tensor, **kw) -> torch.Tensor:
         """``hip_ops.attn_prefill_kv4`` of a chunk q [B, M, H, Dh] that the cache holds, over this layer."""
         from .. import hip_ops
-        return hip_ops.attn_prefill_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, **kw)
+        return hip_ops.attn_prefill_kv4(q, *self.operands(layer_idx, q.shape[0]), positions, limit=self._limit, **kw)
 
     def dequantize(self, layer_idx: int, *, batch_size: Optional[int] = None, length: Optional[int] = None):
         """(K, V) of the first ``length`` positions as ``dtype`` [B, L, Hk, Dh] (``hip_ops.kv4_dequantize``)."""
@@ -423,7 +428,7 @@ class FlashSVDKV4Cache(_CodesCacheBase):
         self._ensure_layer_spec(layer_idx, h=k.shape[2], dh=k.shape[3])
         for i in range(1, t + 1):                          # a call for each run of consecutive positions
             if i == t or pos[i] != pos[i - 1] + 1:
-                self.append(layer_idx, k[:, first:i], v[:, first:i], torch.full((b,), pos[first], dtype=torch.int32, device=dev))
+                self._write(layer_idx, k[:, first:i], v[:, first:i], torch.full((b,), pos[first], dtype=torch.int32, device=dev))      # inside: checked above
                 first = i
         self._note_seen(layer_idx, t, None if cache_position is None else torch.tensor(pos, dtype=torch.long))      # on the host, where they have been read
         n = t if cache_position is None else int(self.get_seq_length())

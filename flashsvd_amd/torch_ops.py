@@ -337,9 +337,9 @@ _define(f"attn_prefill_kv8({_KP_ARGS}) -> Tensor", _prefill_kv8, lambda q, *a, *
 _define(f"attn_prefill_kv8.out({_KP_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_kv8, lambda *a, out, **k: out)
 
 
-def _kv4_append(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos=None, sin=None, rows=None):
+def _kv4_append(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos=None, sin=None, rows=None, limit=None):
     from . import hip_ops
-    hip_ops._kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows)
+    hip_ops._kv4_append_impl(k, v, k_cache, v_cache, k_scale, v_scale, positions, cos, sin, rows, limit)
 
 
 def _kv4_dequantize(k_cache, v_cache, k_scale, v_scale, length=None, dtype=torch.bfloat16):
@@ -354,26 +354,26 @@ def _kv4_dequantize_fake(k_cache, v_cache, k_scale, v_scale, length=None, dtype=
 
 
 def _attn_kv4(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new=None, v_new=None, cos=None, sin=None, seqlen_add=0, nsplit=None,
-              softmax_scale=None, *, out=None):
+              softmax_scale=None, limit=None, *, out=None):
     from . import hip_ops
-    return hip_ops._attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out)
+    return hip_ops._attn_decode_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, cache_seqlens, k_new, v_new, cos, sin, seqlen_add, nsplit, softmax_scale, out, limit)
 
 
-def _prefill_kv4(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows=None, cos=None, sin=None, softmax_scale=None, *, out=None):
+def _prefill_kv4(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows=None, cos=None, sin=None, softmax_scale=None, limit=None, *, out=None):
     from . import hip_ops
-    return hip_ops._attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out)
+    return hip_ops._attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, softmax_scale, out, limit)
 
 
-_define(f"kv4_append(Tensor k, Tensor v, {_KV8_HELD}, Tensor positions, Tensor? cos=None, Tensor? sin=None, Tensor? rows=None) -> ()", _kv4_append,
+_define(f"kv4_append(Tensor k, Tensor v, {_KV8_HELD}, Tensor positions, Tensor? cos=None, Tensor? sin=None, Tensor? rows=None, int? limit=None) -> ()", _kv4_append,
         lambda *a, **k: None)
 _define("kv4_dequantize(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, int? length=None, ScalarType dtype=bfloat16) -> (Tensor, Tensor)",
         _kv4_dequantize, _kv4_dequantize_fake)
 _K4_ARGS = (f"Tensor q, {_KV8_HELD}, Tensor cache_seqlens, Tensor? k_new=None, Tensor? v_new=None, Tensor? cos=None, Tensor? sin=None, "
-            "int seqlen_add=0, int? nsplit=None, float? softmax_scale=None")
+            "int seqlen_add=0, int? nsplit=None, float? softmax_scale=None, int? limit=None")
 _define(f"attn_decode_kv4({_K4_ARGS}) -> Tensor", _attn_kv4, lambda q, *a, **k: q.new_empty(q.shape))
 _define(f"attn_decode_kv4.out({_K4_ARGS}, *, Tensor(e!) out) -> Tensor(e!)", _attn_kv4, lambda *a, out, **k: out)
 _P4_ARGS = ("Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor q_pos0, Tensor? rows=None, Tensor? cos=None, "
-            "Tensor? sin=None, float? softmax_scale=None")
+            "Tensor? sin=None, float? softmax_scale=None, int? limit=None")
 _define(f"attn_prefill_kv4({_P4_ARGS}) -> Tensor", _prefill_kv4, lambda q, *a, **k: q.new_empty(q.shape))
 _define(f"attn_prefill_kv4.out({_P4_ARGS}, *, Tensor(a!) out) -> Tensor(a!)", _prefill_kv4, lambda *a, out, **k: out)
 

@@ -244,12 +244,13 @@ typedef struct fsvd_kv4_cache {
   int64_t sc_b, sc_s, sc_h;              /* codes: sequence, token, head */
   int64_t ss_b, ss_h, ss_g;              /* scales: sequence, head, group of channels */
   int32_t S, Hk, Dh;
+  int32_t limit;                         /* 0: S; else rows from this one on are dropped and seen by no query, as if they lay outside [0, S) */
 } fsvd_kv4_cache;
 
 /* Row t < rows[b] (rows NULL: T) of k and v [B, T, Hk, Dh] goes to cache position positions[b] + t of sequence b; k is rotated there (cos and sin
  * [rope_len, Dh / 2], NULL: not; halves of a head are the pairs).  The exponent of a group is the smallest from -125 to 125 whose 7-fold power covers the group
  * (7 lies halfway between 6 and 8), and each value, the exact one where it was rotated, becomes the nearest code, ties to the even one.  A row changes no
- * other row.  Rows outside [0, S) are dropped; with T = 0 there are none, and k and v may be NULL.  A group with a NaN is NaN as a whole; an infinity becomes the
+ * other row.  Rows outside [0, limit) are dropped; with T = 0 there are none, and k and v may be NULL.  A group with a NaN is NaN as a whole; an infinity becomes the
  * largest code and decides no exponent. */
 int fsvd_kv4_append(const fsvd_kv4_cache* cache, const void* k, int64_t sk_b, int64_t sk_t, int64_t sk_h, const void* v, int64_t sv_b, int64_t sv_t,
                     int64_t sv_h, const int32_t* positions, const int32_t* rows, const void* cos, const void* sin, int rope_len, int B, int T, int dtype,
