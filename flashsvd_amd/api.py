@@ -303,10 +303,11 @@ def _token_scores(logits: torch.Tensor, tokens: torch.Tensor, top: int):
 
 
 @torch.no_grad()
-def score_text(model, tokenizer, *, text: str, device=None, top: int = 0) -> dict[str, Any]:
+def score_text(model, tokenizer, *, text: str, device=None, top: int = 0, kv8_cache: bool = False, kv4_cache: bool = False) -> dict[str, Any]:
     """Log probabilities of a text's tokens after the first, by ``hip_ops.token_logprobs`` from one pass over the text (a model in bfloat16 or float16): ``ids``,
     ``logprobs`` and ``entropies`` (nats) of ``ids[1:]``, ``top_logprobs`` (the ``top`` likeliest tokens, 0 to 64, as (token id, log probability)), their ``sum`` and
-    ``perplexity`` (exp of minus their mean; NaN for a text of one token).  No counterpart in the reference."""
+    ``perplexity`` (exp of minus their mean; NaN for a text of one token).  ``kv8_cache`` and ``kv4_cache`` attend over keys and values in 8 or 4 bits, as
+    ``generate_text`` does with them: what the lost bits cost is the difference.  No counterpart in the reference."""
     device = torch.device(device) if device is not None else next(model.parameters()).device
     ids = tokenizer(text, return_tensors="pt", add_special_tokens=False)["input_ids"].to(device)
     if int(ids.shape[0]) != 1 or int(ids.shape[1]) == 0:
@@ -314,9 +315,13 @@ def score_text(model, tokenizer, *, text: str, device=None, top: int = 0) -> dic
     n = int(ids.shape[1])
     if not 0 <= int(top) <= 64:
         raise ValueError(f"top must be 0 to 64, got {top}")
+    over = {}
+    if kv8_cache or kv4_cache:
+        cache, _ = _build_generation_cache(model, prompt_len=n, max_new_tokens=0, batch_size=1, device=device, kv8_cache=bool(kv8_cache), kv4_cache=bool(kv4_cache))
+        over = dict(past_key_values=cache, cache_position=torch.arange(n))
     taken = entropy = likely = likely_logprobs = []
     if n > 1:
-        logits = model(input_ids=ids).logits[:, :-1]
+        logits = model(input_ids=ids, **over).logits[:, :-1]
         taken, entropy, likely, likely_logprobs = (x[0].tolist() for x in _token_scores(logits, ids[:, 1:], int(top)))
     total = math.fsum(taken)
     return {"ids": ids[0].tolist(), "logprobs": taken, "entropies": entropy, "top_logprobs": [list(zip(t, p)) for t, p in zip(likely, likely_logprobs)],
