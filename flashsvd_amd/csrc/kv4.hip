@@ -4,8 +4,8 @@
 namespace fsvd {
 
 // A workgroup has 256 / (Dh / 16) rows of the keys or the values of HEADS kv heads, which share the rows of the rotation tables and have all their loads in
-// flight.  Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (339 MB) take 72 to 77 us, up to 4.7 TB/s, where a copy
-// reaches 5.4; rows that come rotated 60.
+// flight.  Bound by its bytes: every row is read once and written once.  8 x 2048 rows of 32 heads of 128 (339 MB) take 73 to 75 us, 4.6 TB/s, where a copy reaches
+// 5.4; rows that come rotated 59 to 60.  Times are of a call in a captured graph of six over three sets of inputs.
 template <int DT, int DH, int HEADS>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   constexpr int HALF = DH / 2, LPR = DH / 16, PER = 256 / LPR;
@@ -15,7 +15,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   const bool in = t < rows && pos >= 0 && pos < a.c.limit, turn = !value && a.cos != nullptr;
   const uint16_t* x = (value ? a.v + (int64_t)b * a.sv_b + (in ? t : 0) * a.sv_t : a.k + (int64_t)b * a.sk_b + (in ? t : 0) * a.sk_t) + h0 * sh + 8 * part;
   u32x4_t lo[HEADS], hi[HEADS], cw = {0u, 0u, 0u, 0u}, sw = cw;
-  // Many rows are read past the caches, which they would only empty; of few it costs more than it gives (2 x 2048 rows of 32 heads 24.2 us, 26.6 so).
+  // Many rows are read past the caches, which they would only empty (8 x 2048 rows of 32 heads that come rotated 60.3 us, 63.3 through them; to be rotated 75 either
+  // way); of few it costs more than it gives (2 x 2048 rows 24.2 us, 26.6 so).
   const auto once = [](const uint16_t* p) {
     if constexpr (HEADS == 1) return eight4(p);
     else return __builtin_bit_cast(u32x4_t, __builtin_nontemporal_load(reinterpret_cast<const u32x4_any_t*>(p)));
@@ -46,7 +47,7 @@ __global__ __launch_bounds__(kWave) void kv4_append_one_kernel(Kv4AppendArgs a) 
 template <int DT, int DH>
 static void append_form(const Kv4AppendArgs& a, hipStream_t st) {
   constexpr int rows = 256 / (DH / 16);
-    // us with one head / with four, rows of 32 heads of 128: 1 x 128 4.1 / 6.3, 1 x 2048 12.8 / 15.0, 2 x 2048 20.6 / 22.0, 4 x 2048 40.6 / 38.5, 8 x 2048 76.1 / 67.7
+  // us with one head / with four, rows of 32 heads of 128: 1 x 128 4.4 / 7.5, 1 x 2048 14.5 / 16.4, 2 x 2048 23.9 / 24.8, 4 x 2048 47.6 / 41.5, 8 x 2048 87.3 / 75.2
   const int64_t tiles = (a.T + rows - 1) / rows;
   const bool four = a.c.Hk % 4 == 0 && 2 * a.c.Hk * tiles * a.B >= 16384;
   set_last_form(a.T == 1 ? "kv4 row" : four ? "kv4 rows of 4 heads" : "kv4 rows");
@@ -66,7 +67,7 @@ int launch_kv4_append(const char* fn, const Kv4AppendArgs& a, hipStream_t st) {
 }
 
 // What the first L rows hold, [B, L, Hk, Dh] each: a thread has eight channels of four rows, whose scales are four bytes next to each other.  What it makes goes past
-// the caches: 8 x 2048 rows of 32 heads of 128 (339 MB) take 49.5 us, 6.9 TB/s (65 through them), 512 rows 4.1 (4.5).
+// the caches: 8 x 2048 rows of 32 heads of 128 (339 MB) take 49 us, 6.9 TB/s (64 through them), 512 rows 4.0 (4.6).
 struct Kv4ReadArgs {
   fsvd_kv4_cache c;
   uint16_t* k; uint16_t* v;

@@ -1,10 +1,10 @@
 // Log probabilities of given tokens, the entropy of their distributions and the likeliest alternatives: with x_i = l_i - max l and Z = sum e^(x_i),
 //   log p_t = x_t - log Z,  H = log Z - sum e^(x_i) x_i / Z,  and the `top` largest logits, equal ones by index.
-// A row is read once, into the registers of a workgroup.  Each thread sums against the largest of its own logits, so that the sums need no maximum of the row;
+// A row is read once, into the registers of a workgroup (from 2097153 logits on twice, by parts that no registers hold).  Each thread sums against the largest of its own logits, so that the sums need no maximum of the row;
 // one exchange joins them and gives, as the k-th largest of the maxima of groups of the row's logits, a bound below which no alternative lies.  What is not below it is
 // collected and ranked by counting.  Rows in which that is much (many equal logits, most of them masked) or that hold a NaN are gone over again, see below.
-// 4096 rows of 32000 logits in bf16: 56 us, 4.7 TB/s of the 5.4 that a copy reaches; 64 rows of 128256, in parts, 13.2 us; 1 row of 32000 8.5 us (12.6 of the 17 us of
-// a row of 128256 in one workgroup are the sums, the rest the alternatives).
+// All times here are of a call in a captured graph of six over three sets of inputs.  4096 rows of 32000 logits in bf16: 56 to 61 us on different machines, 4.3 to 4.7
+// TB/s of the 5.4 that a copy reaches; 64 rows of 128256, in parts, 12.4 us; 1 row of 32000 with 20 alternatives 8.9 us, with 5 8.0.
 #include "common.hpp"
 #include "../../include/flashsvd_hip.h"
 
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobArgs a) 
   const auto fetch = [&](int c) {
     if (c * 8 + 8 <= V) {
       const u32x4_any_t* p = reinterpret_cast<const u32x4_any_t*>(row + (int64_t)c * 8);
-      return __builtin_bit_cast(u32x4_t, R > 0 ? __builtin_nontemporal_load(p) : *p);       // read once: past the caches (4096 rows of 32000 61.5 us, 64.8 through them)
+      return __builtin_bit_cast(u32x4_t, R > 0 ? __builtin_nontemporal_load(p) : *p);       // read once: past the caches (64 rows of 128256 12.4 us, 13.0 through them; 4096 of 32000 and 300 of 6000 within 4 % either way)
     }
     uint32_t w[4] = {kNegInf2, kNegInf2, kNegInf2, kNegInf2};
 #pragma unroll
@@ -344,8 +344,8 @@ static void launch_rows(const LogprobArgs& a, int pieces, hipStream_t st) {
   else if constexpr (PART) hipLaunchKernelGGL((token_logprobs_kernel<DT, THREADS, 0, true>), grid, dim3(THREADS), 0, st, a);
 }
 // Workgroups of a row.  A row of more than 4 pieces a thread has more work than one compute unit should do while others are idle: up to one workgroup for each, of
-// 2000 pieces at least, whose join is a launch of its own (64 rows of 128256 logits: 17.9 us in one, 12.7 in 4; 1 row 17.5 and 11.0 in 8; 1 of 50000 11.6 and 10.2 in
-// 3; of 32000, four a thread, 8.5 and 9.6 in 2).  And so many that a part stays in registers (200 rows of 500000: 89 us in one, 75 in 4).
+// 2000 pieces at least, whose join is a launch of its own (64 rows of 128256 logits: 19.1 us in one, 12.4 in 4; 1 row 16.3 and 9.1 in 8; 1 of 50000 10.6 and 10.1 in
+// 3; of 32000, four a thread, 8.9 and 9.8 in 2, 64 of them 9.0 and 10.3).  And so many that a part stays in registers (200 rows of 500000 in 4: 73 us, 89 read twice).
 static int row_parts(int64_t rows, int V) {
   const int pieces = (V + 7) / 8;
   if (pieces <= 4 * 1024) return 1;
@@ -361,8 +361,8 @@ static void launch_logprobs(const LogprobArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((logprobs_join_kernel<DT>), dim3((unsigned)(a.B * a.T)), dim3(256), 0, st, a);
     return;
   }
-  // More rows than compute units: workgroups of four waves, several to a unit, whose phases overlap (4096 rows of 32000 logits 58 us, in sixteen waves 107; 300 of 6000
-  // 6.9 and 9.8; but 256 of 32000 11.0 and 10.1).  So few logits that four waves hold them in two pieces a thread: less to join (8 rows of 1000: 5.0 and 5.8 us).
+  // More rows than compute units: workgroups of four waves, several to a unit, whose phases overlap (4096 rows of 32000 logits 61 us, in sixteen waves 105; 300 of 6000
+  // 7.2 and 9.8; but 256 of 32000 11.0 and 10.1).  So few logits that four waves hold them in two pieces a thread: less to join (8 rows of 1000: 5.0 and 5.8 us).
   const bool narrow = ((int64_t)a.B * a.T > 256 || a.part <= 512) && a.part <= kMostHeld * 256;
   set_last_form(narrow ? "logprobs 256" : "logprobs 1024");
   narrow ? launch_rows<DT, 256, false>(a, a.part, st) : launch_rows<DT, 1024, false>(a, a.part, st);

@@ -1175,8 +1175,8 @@ def attn_decode_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def attn_prefill_kv4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor, q_pos0: torch.Tensor, *,
                      rows: Optional[torch.Tensor] = None, cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None,
                      out: Optional[torch.Tensor] = None, softmax_scale: Optional[float] = None, limit: Optional[int] = None) -> torch.Tensor:
-    """:func:`attn_prefill_kv8` over a cache in 4 bits (operands as :func:`kv4_append`, rows from ``limit`` on not seen).  Custom operator
-    flashsvd_hip::attn_prefill_kv4."""
+    """:func:`attn_prefill_kv8` over a cache in 4 bits (operands as :func:`kv4_append`, rows from ``limit`` on not seen).  The softmax weights of long chunks in
+    bfloat16 are rounded to 11 bits (their sums are not), 16 bits elsewhere.  Custom operator flashsvd_hip::attn_prefill_kv4."""
     a = (q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, cos, sin, None if not softmax_scale else float(softmax_scale), limit)
     return _OPS.attn_prefill_kv4.default(*a) if out is None else _OPS.attn_prefill_kv4.out(*a, out=out)
 
@@ -1342,8 +1342,9 @@ def _attn_prefill_kv4_impl(q, k_cache, v_cache, k_scale, v_scale, q_pos0, rows, 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0):
     """(logprobs, entropy, top_tokens, top_logprobs) of every row of logits [N, V] or [B, T, V] with unit inner stride: the log probability of
     ``tokens`` (int64 [N] or [B, T]; below 0: none, 0.0), the entropy of the distribution in nats, float32 both, and the ``top`` (0 to 64) likeliest tokens, int64,
-    with their log probabilities, float32 [.., top], equal ones by index.  A row whose largest logit is not finite has NaN for numbers.  One launch that
-    reads the logits once.  Custom operator flashsvd_hip::token_logprobs."""
+    with their log probabilities, float32 [.., top], equal ones by index.  A row whose largest logit is not finite has NaN for numbers.  The logits are read once,
+    in one launch; few rows of more than 32768 logits, and all of more than 131072, are cut into parts and joined by a second one, parts of rows of more than 2^21 are read
+    twice, and rows with more than 512 logits at the border of the alternatives, or a NaN, are gone over again.  Custom operator flashsvd_hip::token_logprobs."""
     return _OPS.token_logprobs.default(logits, tokens, int(top))
 
 

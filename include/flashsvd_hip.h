@@ -258,7 +258,8 @@ int fsvd_kv4_append(const fsvd_kv4_cache* cache, const void* k, int64_t sk_b, in
 /* What the first L rows of B sequences hold, k and v [B, L, Hk, Dh] (strides so_b, so_t, so_h for both): exact in bf16, rounded to fp16. */
 int fsvd_kv4_dequantize(const fsvd_kv4_cache* cache, void* k, void* v, int64_t so_b, int64_t so_t, int64_t so_h, int B, int L, int dtype, void* stream);
 
-/* fsvd_attn_decode_kv8 and fsvd_attn_prefill_kv8 over a cache in 4 bits, rows that the former appends as fsvd_kv4_append has them. */
+/* fsvd_attn_decode_kv8 and fsvd_attn_prefill_kv8 over a cache in 4 bits, rows that the former appends as fsvd_kv4_append has them.  Softmax weights go into the products with
+ * 16 bits, those of long chunks in bf16 with 11 (where float16 holds the values), their sums are fp32.  Values are summed before they are divided: up to 2^128 / S in size. */
 size_t fsvd_attn_decode_kv4_scratch_bytes(int B, int H, int Hk, int Dh, int S, int nsplit);
 int fsvd_attn_decode_kv4(const fsvd_kv4_cache* cache, const void* q, int64_t sq_b, int64_t sq_h, const void* k_new, int64_t sk_b, int64_t sk_h,
                          const void* v_new, int64_t sv_b, int64_t sv_h, const int32_t* cache_seqlens, int seqlen_add, const void* cos, const void* sin,
